@@ -436,6 +436,106 @@ lq4_status lq4_block_rot_signs_from_seed(uint64_t seed, uint32_t n, uint32_t blo
  * (crates/inference/src/quant/quarot/hadamard.rs:114-139). */
 lq4_status lq4_rot_signs_from_seed(uint64_t seed, uint32_t dim, float* signs, void* stream);
 
+/* ---- rotary positions and the key/value cache ------------------------------------------------- */
+
+/* What lies between the q/k/v projections and o_proj of a decode or prefill step.  The calls below take a
+ * context like the projections do, run on the context's device whichever one is current, and are
+ * asynchronous on `stream` (a stream of that device).  None of them synchronises; where a workspace has to
+ * grow the call that grows it does, as lq4_ctx_reserve describes.  Values that the host cannot see (page
+ * ids, lengths, parents, path entries) are checked by the kernels: what is out of range is skipped, and
+ * lq4_ctx_check reports it as LQ4_ERR_DEVICE with bit 8 of the status set. */
+
+enum { LQ4_ROPE_HALF = 0, LQ4_ROPE_INTERLEAVED = 1 };
+enum { LQ4_ROPE_PLAIN = 0, LQ4_ROPE_LINEAR = 1, LQ4_ROPE_NTK = 2, LQ4_ROPE_YARN = 3, LQ4_ROPE_BANDS = 4 };
+
+/* Rotary positions: pair i < rot_dim / 2 of a head turns by positions[row] * freq[i] radians,
+ *   (x1, x2) -> scale * (x1 cos - x2 sin, x1 sin + x2 cos),
+ * where the pair is (x[i], x[i + rot_dim / 2]) for LQ4_ROPE_HALF and (x[2i], x[2i + 1]) for
+ * LQ4_ROPE_INTERLEAVED; entries from rot_dim on are copied.  Frequencies are f64: at position 10^6 an f32
+ * frequency is off by a twentieth of a radian. */
+typedef struct {
+    const double* freq;    /* rot_dim / 2 entries on the device */
+    uint32_t rot_dim;      /* even, 2 .. head_dim */
+    int32_t layout;        /* LQ4_ROPE_HALF / LQ4_ROPE_INTERLEAVED */
+    float scale;           /* factor of the rotated entries; 1 for unscaled positions */
+} lq4_rope_desc;
+
+/* One tensor [rows, heads, head_dim] of a rotary call.  Strides are in elements, the innermost one is 1. */
+typedef struct {
+    const void* x;
+    void* out;                        /* may be x itself with equal type and strides; no other overlap */
+    int32_t x_dtype, out_dtype;       /* F32 or BF16 each; one rounding, at the store */
+    uint32_t heads;
+    int32_t turn;                     /* 1: rotate; -1: the transpose (rotates back, same scale: the backward
+                                         pass, and with scale 1 the inverse); 0: copy / convert */
+    uint64_t x_row, x_head, out_row, out_head;
+} lq4_rope_part;
+
+#define LQ4_MAX_ROPE_PARTS 4
+typedef struct {
+    const lq4_rope_part* parts;       /* q, k and v of a fused projection row, say: one launch for all */
+    uint32_t n_parts, rows, head_dim;
+    const int32_t* positions;         /* [rows] on the device, any int32 */
+    const lq4_rope_desc* rope;        /* may be NULL when no part rotates */
+} lq4_rope_args;
+
+/* rows == 0 or no heads: no-op.  LQ4_ERR_ROT for a rot_dim that is odd, 0 or above head_dim, an unknown
+ * layout or turn, a non-finite scale; LQ4_ERR_DTYPE; LQ4_ERR_SHAPE for head_dim 0 or above 1024, more than
+ * LQ4_MAX_ROPE_PARTS parts; LQ4_ERR_ALIGN for pointers not aligned to their element type.  The head
+ * rotation of the reference's step is partial_rope_interleaved (forward/shaders/qwen35.metal:286). */
+lq4_status lq4_rope_rows(lq4_ctx* ctx, const lq4_rope_args* args, void* stream);
+
+/* Host-side helper: h_freq[i] (rot_dim / 2 entries, host memory) and the matching `scale` of lq4_rope_desc.
+ *   PLAIN   theta^(-2i / rot_dim)
+ *   LINEAR  the same over `factor` (positions interpolated)
+ *   NTK     theta replaced by theta * factor^(rot_dim / (rot_dim - 2)): the slowest pair as LINEAR, the fastest unchanged
+ *   YARN    pairs that turn at least beta_fast times in original_len positions keep their frequency, pairs that
+ *           turn at most beta_slow times get it over factor, a linear ramp over the pair index between;
+ *           scale = 0.1 ln(factor) + 1 (Peng et al. 2023)
+ *   BANDS   as YARN, but the ramp runs over the number of turns in original_len, from beta_slow to beta_fast; scale 1
+ * LQ4_ERR_ROT for an odd or zero rot_dim (NTK: rot_dim 2 too), theta <= 1 or a factor below 1, or unordered betas. */
+typedef struct {
+    int32_t kind;                     /* LQ4_ROPE_PLAIN .. LQ4_ROPE_BANDS */
+    uint32_t rot_dim;
+    double theta, factor, original_len, beta_fast, beta_slow;
+} lq4_rope_scaling;
+lq4_status lq4_rope_frequencies(const lq4_rope_scaling* scaling, double* h_freq, float* h_scale);
+
+/* A paged cache of one layer: slot s of sequence b lies in page page_table[b * max_pages + s / page_size], at
+ * slot s % page_size of it.  Element (page, slot, head, d) is at page * page_stride + slot * slot_stride +
+ * head * head_stride + d of `k` and of `v`; the strides are elements and 0 means dense [pages, page_size,
+ * kv_heads, head_dim].  bf16.  An unpaged cache is one page per sequence with page_table[b] = b. */
+typedef struct {
+    void* k;
+    void* v;
+    uint32_t pages, page_size, kv_heads, head_dim;    /* head_dim a multiple of 8, 8 .. 256 */
+    uint64_t page_stride, slot_stride, head_stride;   /* multiples of 8; k and v 16-byte aligned */
+    const int32_t* page_table;                        /* [batch, max_pages] on the device */
+    uint32_t batch, max_pages;
+} lq4_kv_cache;
+
+/* Appends rows to the sequences: row index[b, j] (index NULL: row j) of k[b] and v[b] goes to slot
+ * kv_lens[b] + j, for j < counts[b] (counts NULL: all `rows`); f32 rows are rounded to bf16 once.  Slots
+ * that are not written keep what they held.  kv_lens[b] < 0 marks a sequence to leave alone.  new_lens[b]
+ * (may be NULL; must not be kv_lens) receives kv_lens[b] + counts[b], or the capacity max_pages * page_size
+ * where that is less (the rows beyond it are skipped and reported).  With `index` = the path and `counts` = the
+ * path length of lq4_verify_draft the call commits what a verification accepted; without, a prompt's rows or
+ * the one row of a plain decode step.  The reference's counterpart is copy_kv_cache_batch
+ * (forward/shaders/qwen35.metal:2493). */
+typedef struct {
+    const lq4_kv_cache* cache;
+    const void* k;                    /* [batch, rows, kv_heads, head_dim] */
+    const void* v;
+    int32_t dtype;                    /* F32 or BF16, both */
+    uint32_t rows;
+    uint64_t batch_stride, row_stride, head_stride;   /* elements, of k and v; multiples of 8; k, v 16-byte aligned */
+    const int32_t* kv_lens;           /* [batch] */
+    const int32_t* counts;            /* [batch] or NULL */
+    const int32_t* index;             /* [batch, rows] or NULL */
+    int32_t* new_lens;                /* [batch] or NULL */
+} lq4_kv_append_args;
+lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* stream);
+
 /* ---- resident objects ---------------------------------------------------- */
 
 /* Validates every block (scale finite and > 0, bias finite) on the host and only

@@ -6,6 +6,7 @@ call sites.  PyTorch is used for device memory and streams only.
 """
 from . import _lib
 from ._lib import Lq4Error
+from .attention import KvCache, RopeTable, rope_frequencies
 from .backend import CudaQ4Backend, LoraLayerData, Q4WeightBuf
 
-__all__ = ["CudaQ4Backend", "LoraLayerData", "Q4WeightBuf", "Lq4Error", "_lib"]
+__all__ = ["CudaQ4Backend", "KvCache", "LoraLayerData", "Q4WeightBuf", "RopeTable", "Lq4Error", "rope_frequencies", "_lib"]

@@ -72,6 +72,45 @@ class MlpArgs(C.Structure):
                 ("rot_down", C.POINTER(RotDesc))]
 
 
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
+MAX_ROPE_PARTS = 4
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("rot_dim", C.c_uint32), ("layout", C.c_int32), ("scale", C.c_float)]
+
+
+class RopePart(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("x_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("heads", C.c_uint32), ("turn", C.c_int32), ("x_row", C.c_uint64), ("x_head", C.c_uint64),
+                ("out_row", C.c_uint64), ("out_head", C.c_uint64)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [("parts", C.POINTER(RopePart)), ("n_parts", C.c_uint32), ("rows", C.c_uint32), ("head_dim", C.c_uint32),
+                ("positions", C.c_void_p), ("rope", C.POINTER(RopeDesc))]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("rot_dim", C.c_uint32), ("theta", C.c_double), ("factor", C.c_double),
+                ("original_len", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_stride", C.c_uint64),
+                ("slot_stride", C.c_uint64), ("head_stride", C.c_uint64), ("page_table", C.c_void_p),
+                ("batch", C.c_uint32), ("max_pages", C.c_uint32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("cache", C.POINTER(KvCacheDesc)), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32),
+                ("rows", C.c_uint32), ("batch_stride", C.c_uint64), ("row_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("kv_lens", C.c_void_p), ("counts", C.c_void_p), ("index", C.c_void_p),
+                ("new_lens", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "lq4_ctx_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
@@ -116,6 +155,9 @@ SIGNATURES = {
     "lq4_block_hadamard_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.POINTER(RotDesc), C.c_void_p]),
     "lq4_cross_head_hadamard_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
     "lq4_block_rot_signs_from_seed": (C.c_int32, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "lq4_rope_rows": (C.c_int32, [C.c_void_p, C.POINTER(RopeArgs), C.c_void_p]),
+    "lq4_rope_frequencies": (C.c_int32, [C.POINTER(RopeScaling), C.c_void_p, C.c_void_p]),
+    "lq4_kv_append": (C.c_int32, [C.c_void_p, C.POINTER(KvAppendArgs), C.c_void_p]),
     "lq4_weights_upload": (C.c_int32, [C.c_void_p, C.c_uint64, C.c_uint64, C.POINTER(C.c_void_p)]),
     "lq4_weights_load_q4_file": (C.c_int32, [C.c_char_p, C.POINTER(C.c_uint64), C.c_uint32, C.POINTER(C.c_void_p)]),
     "lq4_weights_payload": (C.c_void_p, [C.c_void_p]),

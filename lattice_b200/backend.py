@@ -26,7 +26,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import GatherDesc, LinearArgs, LoraDesc, Lq4Error, RotDesc, check
+from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, check
+from .attention import KvCache, RopeTable
 
 
 def _stream() -> int:
@@ -495,6 +496,84 @@ class CudaQ4Backend:
                        C.pointer(rot_down) if rot_down is not None else None)
         check(_lib.lib().lq4_mlp_block(self._ctx, C.byref(args), _stream()))
         return y
+
+    # ---- rotary positions and the key/value cache --------------------------------------------
+    def _own_stream(self) -> int:
+        """The current stream of this backend's device, whichever device is current."""
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _int32(self, name: str, t: Optional[torch.Tensor], *shape: int) -> Optional[int]:
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != self.device:
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on cuda:{self.device}")
+        return t.data_ptr()
+
+    def rope_rows(self, parts, positions: torch.Tensor, rope: Optional[RopeTable] = None, *,
+                  out_dtype: Optional[torch.dtype] = None, outs: Optional[List[torch.Tensor]] = None) -> List[torch.Tensor]:
+        """Rotary positions of several tensors in one launch.  ``parts`` is a list of ``(x, turn)`` with ``x``
+        ``[rows, heads, head_dim]`` (f32 or bf16, any row and head stride: slices of a fused q|k|v row) and
+        ``turn`` 1 (rotate), -1 (the transpose: the backward pass) or 0 (convert only, for v); ``positions``
+        is ``[rows]`` int32.  Returns new dense tensors of ``out_dtype`` (default: each input's), or fills
+        ``outs`` (which may be the inputs themselves)."""
+        n = len(parts)
+        if n == 0:
+            return []
+        if n > _lib.MAX_ROPE_PARTS:
+            raise ValueError(f"rope_rows takes at most {_lib.MAX_ROPE_PARTS} tensors, got {n}")
+        rows, _, dim = parts[0][0].shape
+        arr, ys = (RopePart * n)(), []
+        for i, (x, turn) in enumerate(parts):
+            if x.dim() != 3 or x.shape[0] != rows or x.shape[2] != dim or x.get_device() != self.device:
+                raise ValueError(f"rope_rows: tensors must be [rows, heads, head_dim] on cuda:{self.device}, of equal rows and head_dim")
+            if x.stride(2) != 1:
+                x = x.contiguous()
+            if outs is None:
+                y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+            else:
+                y = outs[i]
+                if y.shape != x.shape or y.get_device() != self.device or y.stride(2) != 1:
+                    raise ValueError("rope_rows: an output must have its input's shape and device and unit stride along head_dim")
+            ys.append(y)
+            xs, yst = x.stride(), y.stride()
+            arr[i] = RopePart(x.data_ptr(), y.data_ptr(), self._dtype_of(x), self._dtype_of(y), x.shape[1], turn, xs[0], xs[1], yst[0], yst[1])
+        if rope is not None and rope.freq.get_device() != self.device:
+            raise ValueError(f"rope_rows: the frequencies must lie on cuda:{self.device}")
+        args = RopeArgs(arr, n, rows, dim, self._int32("positions", positions, rows), C.pointer(rope.desc) if rope is not None else None)
+        check(_lib.lib().lq4_rope_rows(self._ctx, C.byref(args), self._own_stream()))
+        return ys
+
+    def _cache_rows(self, what: str, cache: KvCache, k: torch.Tensor, v: torch.Tensor):
+        """Checks ``[batch, rows, kv_heads, head_dim]`` rows against a cache; returns (k, v) the kernels can read."""
+        d = cache.desc
+        if cache.device != self.device:
+            raise ValueError(f"{what}: the cache lies on cuda:{cache.device}, this backend on cuda:{self.device}")
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != d.batch or k.shape[2] != d.kv_heads or k.shape[3] != d.head_dim:
+            raise ValueError(f"{what}: k and v must be [{d.batch}, rows, {d.kv_heads}, {d.head_dim}], got {list(k.shape)} and {list(v.shape)}")
+        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device:
+            raise ValueError(f"{what}: k and v must have one type and lie on cuda:{self.device}")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            k, v = k.contiguous(), v.contiguous()
+        return k, v
+
+    def kv_append(self, cache: KvCache, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor, *,
+                  counts: Optional[torch.Tensor] = None, index: Optional[torch.Tensor] = None,
+                  new_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Writes rows of ``k`` and ``v`` (``[batch, rows, kv_heads, head_dim]``, f32 or bf16) behind the
+        ``kv_lens[b]`` cached ones: all of them, the first ``counts[b]``, or the rows ``index[b, :counts[b]]``
+        (what ``verify_draft`` accepted).  Returns the new lengths (a new int32 tensor, or ``new_lens``)."""
+        k, v = self._cache_rows("kv_append", cache, k, v)
+        b, rows = k.shape[:2]
+        if new_lens is None:
+            new_lens = torch.empty_like(kv_lens)
+        ks = k.stride()
+        args = KvAppendArgs(C.pointer(cache.desc), k.data_ptr(), v.data_ptr(), self._dtype_of(k), rows, ks[0], ks[1], ks[2],
+                            self._int32("kv_lens", kv_lens, b), self._int32("counts", counts, b),
+                            self._int32("index", index, b, rows), self._int32("new_lens", new_lens, b))
+        check(_lib.lib().lq4_kv_append(self._ctx, C.byref(args), self._own_stream()))
+        if rows == 0 and b:
+            new_lens.copy_(kv_lens)
+        return new_lens
 
     # ---- lm_head: vocabulary projection + exact top-k --------------------------------------
     @staticmethod

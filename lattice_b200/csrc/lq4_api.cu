@@ -14,6 +14,7 @@
 
 #include <map>
 
+#include "lq4_attend.cuh"
 #include "lq4_gemm.cuh"
 #include "lq4_kernels.cuh"
 #include "lq4_step.cuh"
@@ -393,7 +394,9 @@ lq4_status lq4_ctx_check(lq4_ctx* ctx, void* stream) {
     if (h != 0) {
         cudaMemsetAsync(ctx->status, 0, 4, s);
         cudaStreamSynchronize(s);
-        return fail(LQ4_ERR_DEVICE, "kernel reported a failed bounded wait, status bits " + std::to_string(h));
+        const char* what = h == kDevErrBadIndex ? "kernel skipped an index out of range (page, length, count, parent or path entry), status bits "
+                                                : "kernel reported a failed bounded wait, status bits ";
+        return fail(LQ4_ERR_DEVICE, what + std::to_string(h));
     }
     return LQ4_OK;
 }
@@ -1537,6 +1540,148 @@ lq4_status lq4_rot_signs_from_seed(uint64_t seed, uint32_t dim, float* signs, vo
 }
 
 // ---- resident objects ---------------------------------------------------------
+
+// ---- rotary positions, cache append -----------------------------------------------------------------
+
+namespace {
+
+// Makes the context's device current for one call and puts the caller's back.
+struct DeviceScope {
+    int prev = -1;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceScope(int device) {
+        int cur = 0;
+        err = cudaGetDevice(&cur);
+        if (err == cudaSuccess && cur != device) {
+            err = cudaSetDevice(device);
+            if (err == cudaSuccess) prev = cur;
+        }
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+#define LQ4_ON_DEVICE(ctx)             \
+    DeviceScope on_device((ctx)->device); \
+    if (on_device.err != cudaSuccess) return cuda_fail(on_device.err, "selecting the context's device")
+
+bool act_dtype(int32_t t) { return t == LQ4_DTYPE_F32 || t == LQ4_DTYPE_BF16; }
+size_t act_size(int32_t t) { return t == LQ4_DTYPE_F32 ? 4 : 2; }
+
+lq4_status check_cache(const lq4_kv_cache* c) {
+    if (!c) return fail(LQ4_ERR_NULL, "cache is NULL");
+    if (c->head_dim == 0 || c->head_dim > 256 || c->head_dim % 8) return fail(LQ4_ERR_SHAPE, "head_dim must be a multiple of 8, at most 256");
+    if (c->kv_heads == 0 || c->kv_heads > 4096) return fail(LQ4_ERR_SHAPE, "kv_heads must be in 1..4096");
+    if (c->page_size == 0 || c->page_size > 0x40000000u) return fail(LQ4_ERR_SHAPE, "page_size must be in 1..2^30");
+    if (c->pages > 0x7fffffffu) return fail(LQ4_ERR_OVERFLOW, "more than 2^31 - 1 pages");
+    if ((uint64_t)c->max_pages * c->page_size > 0x7fffffffull) return fail(LQ4_ERR_OVERFLOW, "a sequence's capacity does not fit 31 bits");
+    if (c->batch == 0) return LQ4_OK;
+    if (c->pages && (!c->k || !c->v)) return fail(LQ4_ERR_NULL, "cache k and v must be non-NULL");
+    if (c->max_pages && !c->page_table) return fail(LQ4_ERR_NULL, "page_table is NULL");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->page_table, 4)) return fail(LQ4_ERR_ALIGN, "cache k and v must be 16-byte aligned");
+    if (c->page_stride % 8 || c->slot_stride % 8 || c->head_stride % 8) return fail(LQ4_ERR_ALIGN, "cache strides must be multiples of 8 elements");
+    return LQ4_OK;
+}
+
+}  // namespace
+
+lq4_status lq4_rope_rows(lq4_ctx* ctx, const lq4_rope_args* a, void* stream) {
+    if (!a) return fail(LQ4_ERR_NULL, "args is NULL");
+    if (a->n_parts > LQ4_MAX_ROPE_PARTS) return fail(LQ4_ERR_SHAPE, "at most 4 parts");
+    if (a->n_parts && !a->parts) return fail(LQ4_ERR_NULL, "parts is NULL");
+    if (a->head_dim == 0 || a->head_dim > 1024) return fail(LQ4_ERR_SHAPE, "head_dim must be in 1..1024");
+    if (a->rows > 0x7fffffffu) return fail(LQ4_ERR_OVERFLOW, "more than 2^31 - 1 rows");
+    uint64_t heads = 0;
+    bool turns = false;
+    for (uint32_t i = 0; i < a->n_parts; ++i) {
+        const lq4_rope_part& t = a->parts[i];
+        if (!act_dtype(t.x_dtype) || !act_dtype(t.out_dtype)) return fail(LQ4_ERR_DTYPE, "a part's types must be F32 or BF16");
+        if (t.turn < -1 || t.turn > 1) return fail(LQ4_ERR_ROT, "turn must be 1, -1 or 0");
+        if (!t.heads) continue;
+        heads += t.heads;
+        turns |= t.turn != 0;
+        if (a->rows == 0) continue;
+        if (!t.x || !t.out) return fail(LQ4_ERR_NULL, "a part's x and out must be non-NULL");
+        if (!aligned(t.x, act_size(t.x_dtype)) || !aligned(t.out, act_size(t.out_dtype))) return fail(LQ4_ERR_ALIGN, "a part is not aligned to its element type");
+        if (t.x == t.out && (t.x_dtype != t.out_dtype || t.x_row != t.out_row || t.x_head != t.out_head))
+            return fail(LQ4_ERR_SHAPE, "a part that works in place needs equal types and strides");
+        if (mul_overflows(t.x_row, a->rows, 1ull << 60) || mul_overflows(t.out_row, a->rows, 1ull << 60) || mul_overflows(t.x_head, t.heads, 1ull << 60) ||
+            mul_overflows(t.out_head, t.heads, 1ull << 60))
+            return fail(LQ4_ERR_OVERFLOW, "a part's strides do not fit");
+    }
+    if (heads > 4096) return fail(LQ4_ERR_SHAPE, "more than 4096 heads");
+    if (turns && !a->rope) return fail(LQ4_ERR_NULL, "rope is NULL but a part rotates");
+    if (a->rope) {
+        const lq4_rope_desc& r = *a->rope;
+        if (r.rot_dim == 0 || r.rot_dim % 2 || r.rot_dim > a->head_dim) return fail(LQ4_ERR_ROT, "rot_dim must be even and in 2..head_dim");
+        if (r.layout != LQ4_ROPE_HALF && r.layout != LQ4_ROPE_INTERLEAVED) return fail(LQ4_ERR_ROT, "unknown rotary layout");
+        if (!std::isfinite(r.scale)) return fail(LQ4_ERR_ROT, "the rotary scale must be finite");
+    }
+    if (a->rows && heads && a->rope && (!a->rope->freq || !a->positions)) return fail(LQ4_ERR_NULL, "freq and positions must be non-NULL");
+    if (a->rope && (!aligned(a->rope->freq, 8) || !aligned(a->positions, 4))) return fail(LQ4_ERR_ALIGN, "freq or positions is misaligned");
+    if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
+    if (a->rows == 0 || heads == 0) return LQ4_OK;
+    LQ4_ON_DEVICE(ctx);
+    LQ4_CUDA(launch_rope_rows(*a, ctx->sm_count, ctx->pdl, (cudaStream_t)stream));
+    ctx->launches += 1;
+    return LQ4_OK;
+}
+
+lq4_status lq4_rope_frequencies(const lq4_rope_scaling* c, double* h_freq, float* h_scale) {
+    if (!c || !h_freq || !h_scale) return fail(LQ4_ERR_NULL, "scaling, h_freq and h_scale must be non-NULL");
+    if (c->rot_dim == 0 || c->rot_dim % 2 || c->rot_dim > 1024) return fail(LQ4_ERR_ROT, "rot_dim must be even and in 2..1024");
+    if (!(c->theta > 1.0) || !std::isfinite(c->theta)) return fail(LQ4_ERR_ROT, "theta must be above 1");
+    if (c->kind < LQ4_ROPE_PLAIN || c->kind > LQ4_ROPE_BANDS) return fail(LQ4_ERR_ROT, "unknown kind of rotary scaling");
+    const bool ramped = c->kind == LQ4_ROPE_YARN || c->kind == LQ4_ROPE_BANDS;
+    if (c->kind != LQ4_ROPE_PLAIN && (!(c->factor >= 1.0) || !std::isfinite(c->factor))) return fail(LQ4_ERR_ROT, "factor must be at least 1");
+    if (c->kind == LQ4_ROPE_NTK && c->rot_dim == 2) return fail(LQ4_ERR_ROT, "NTK scaling needs more than one pair");
+    if (ramped && (!(c->original_len >= 1.0) || !(c->beta_slow > 0.0) || !(c->beta_fast > c->beta_slow) || !std::isfinite(c->beta_fast) || !std::isfinite(c->original_len)))
+        return fail(LQ4_ERR_ROT, "ramped scaling needs original_len >= 1 and beta_fast > beta_slow > 0");
+    const double pi = 3.14159265358979323846;
+    const uint32_t half = c->rot_dim / 2;
+    const double theta = c->kind == LQ4_ROPE_NTK ? c->theta * std::pow(c->factor, (double)c->rot_dim / (c->rot_dim - 2)) : c->theta;
+    // the pair index (a real number) that turns `n` times in original_len positions
+    auto pair_of = [&](double n) { return half * std::log(c->original_len / (n * 2 * pi)) / std::log(theta); };
+    double low = 0, high = 0;
+    if (c->kind == LQ4_ROPE_YARN) {
+        low = std::fmax(std::floor(pair_of(c->beta_fast)), 0.0);
+        high = std::fmin(std::ceil(pair_of(c->beta_slow)), half - 1.0);
+    }
+    *h_scale = c->kind == LQ4_ROPE_YARN ? (float)(0.1 * std::log(c->factor) + 1.0) : 1.0f;
+    for (uint32_t i = 0; i < half; ++i) {
+        const double f = std::pow(theta, -(double)i / half);
+        double keep = 1.0;                      // share of the unscaled frequency
+        if (c->kind == LQ4_ROPE_LINEAR) keep = 0.0;
+        if (c->kind == LQ4_ROPE_YARN) keep = 1.0 - std::fmin(std::fmax((i - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
+        if (c->kind == LQ4_ROPE_BANDS) keep = std::fmin(std::fmax((c->original_len * f / (2 * pi) - c->beta_slow) / (c->beta_fast - c->beta_slow), 0.0), 1.0);
+        h_freq[i] = c->kind == LQ4_ROPE_PLAIN || c->kind == LQ4_ROPE_NTK ? f : f / c->factor * (1.0 - keep) + f * keep;
+    }
+    return LQ4_OK;
+}
+
+lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* a, void* stream) {
+    if (!a) return fail(LQ4_ERR_NULL, "args is NULL");
+    lq4_status st;
+    if ((st = check_cache(a->cache))) return st;
+    if (!act_dtype(a->dtype)) return fail(LQ4_ERR_DTYPE, "rows must be F32 or BF16");
+    if (a->rows > 0x7fffffffu || (uint64_t)a->cache->batch * a->rows > 0x7fffffffull * 8) return fail(LQ4_ERR_OVERFLOW, "batch * rows does not fit");
+    if (a->cache->batch && a->rows) {
+        if (!a->k || !a->v || !a->kv_lens) return fail(LQ4_ERR_NULL, "k, v and kv_lens must be non-NULL");
+        if (!aligned(a->k, 16) || !aligned(a->v, 16)) return fail(LQ4_ERR_ALIGN, "k and v must be 16-byte aligned");
+        if (a->batch_stride % 8 || a->row_stride % 8 || a->head_stride % 8) return fail(LQ4_ERR_ALIGN, "row strides must be multiples of 8 elements");
+        if (!aligned(a->kv_lens, 4) || !aligned(a->counts, 4) || !aligned(a->index, 4) || !aligned(a->new_lens, 4))
+            return fail(LQ4_ERR_ALIGN, "an int32 array is misaligned");
+        if (a->new_lens && a->new_lens == a->kv_lens) return fail(LQ4_ERR_SHAPE, "new_lens must not be kv_lens: the lengths are read while it is written");
+        if (mul_overflows(a->batch_stride, a->cache->batch, 1ull << 60) || mul_overflows(a->row_stride, a->rows, 1ull << 60))
+            return fail(LQ4_ERR_OVERFLOW, "row strides do not fit");
+    }
+    if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
+    if (a->cache->batch == 0 || a->rows == 0) return LQ4_OK;
+    LQ4_ON_DEVICE(ctx);
+    LQ4_CUDA(launch_kv_append(*a, ctx->status, ctx->pdl, (cudaStream_t)stream));
+    ctx->launches += 1;
+    return LQ4_OK;
+}
 
 static float f16_bits_to_f32_host(uint16_t h) {
     const uint32_t sign = (uint32_t)(h >> 15) << 31, e = (h >> 10) & 0x1f, f = h & 0x3ff;

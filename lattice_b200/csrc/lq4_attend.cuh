@@ -1,0 +1,38 @@
+// Host-callable launchers of the kernels between the q/k/v projections and o_proj (rotary positions, cache
+// append, attention over the cache) and behind lm_head (verification of drafted tokens).
+#pragma once
+
+#include "lq4_kernels.cuh"
+
+namespace lq4 {
+
+constexpr int kDevErrBadIndex = 8;      // a page id, length, count, parent or path entry outside its range
+
+// ---- lq4_rope.cu ----------------------------------------------------------------
+// Arguments are validated by the caller (lq4_api.cu).
+cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, cudaStream_t s);
+cudaError_t launch_kv_append(const lq4_kv_append_args& a, int32_t* status, int use_pdl, cudaStream_t s);
+
+// A cache descriptor with its strides filled in.
+struct CacheView {
+    uint16_t* k;
+    uint16_t* v;
+    uint64_t page_stride, slot_stride, head_stride;
+    const int32_t* table;
+    uint32_t pages, page_size, max_pages;
+};
+inline CacheView cache_view(const lq4_kv_cache& c) {
+    CacheView w;
+    w.k = static_cast<uint16_t*>(c.k);
+    w.v = static_cast<uint16_t*>(c.v);
+    w.head_stride = c.head_stride ? c.head_stride : c.head_dim;
+    w.slot_stride = c.slot_stride ? c.slot_stride : (uint64_t)c.kv_heads * c.head_dim;
+    w.page_stride = c.page_stride ? c.page_stride : (uint64_t)c.page_size * c.kv_heads * c.head_dim;
+    w.table = c.page_table;
+    w.pages = c.pages;
+    w.page_size = c.page_size;
+    w.max_pages = c.max_pages;
+    return w;
+}
+
+}  // namespace lq4

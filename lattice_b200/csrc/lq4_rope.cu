@@ -1,0 +1,312 @@
+// Rotary positions of q / k (with v converted in the same launch) and the append of rows to a paged cache.
+//
+// Both are passes over memory: every element is read once and written once.
+//
+// rope_kernel: pair i of a head is a complex number turned by the angle pos * freq[i].  The angle of a far
+// position does not fit f32 (10^6 radians leave 2^-4 of a turn), so it is formed in f64 as a number of
+// TURNS, its whole part is dropped there, and only the remainder in [-1/2, 1/2] goes to f32 and sincospi:
+// three f64 operations per (row, pair), shared by all heads of the row through shared memory.  A CTA takes a
+// few rows (256 angles, one per thread) and all heads, or a slice of the heads when the rows alone would not
+// fill the GPU; a thread moves 2V elements per step (V pairs: both halves are in its registers before it
+// stores, so the call may work in place).
+#include "lq4_attend.cuh"
+
+#include <cuda_bf16.h>
+
+namespace lq4 {
+
+namespace {
+
+constexpr uint32_t kRopeThreads = 256;
+constexpr uint32_t kRopeMaxPairs = 512;        // head_dim <= 1024
+
+struct RopeParams {
+    lq4_rope_part part[LQ4_MAX_ROPE_PARTS];
+    uint32_t n_parts, rows, head_dim, half;    // half = rot_dim / 2
+    uint32_t heads;                            // of all parts together
+    uint32_t rows_per_cta, heads_per_cta;
+    const int32_t* positions;
+    const double* freq;
+    int32_t interleaved;
+    float scale;
+};
+
+// V consecutive elements, f32 or bf16 in memory, f32 in registers.
+template <int V>
+__device__ __forceinline__ void load_vec(const void* base, int dtype, uint64_t at, float (&v)[V]) {
+    if (dtype == LQ4_DTYPE_F32) {
+        const float* p = static_cast<const float*>(base) + at;
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                const float4 t = reinterpret_cast<const float4*>(p)[i];
+                v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
+            }
+        } else {
+            v[0] = p[0];
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+        if constexpr (V >= 4) {
+            uint32_t w[V / 2];
+            if constexpr (V == 8) {
+                const uint4 t = *reinterpret_cast<const uint4*>(p);
+                w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+            } else {
+                const uint2 t = *reinterpret_cast<const uint2*>(p);
+                w[0] = t.x, w[1] = t.y;
+            }
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+            v[0] = bf16_to_f32(p[0]);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+template <int V>
+__device__ __forceinline__ void store_vec(void* base, int dtype, uint64_t at, const float (&v)[V]) {
+    if (dtype == LQ4_DTYPE_F32) {
+        float* p = static_cast<float*>(base) + at;
+        if constexpr (V >= 4) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i)
+                reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+            p[0] = v[0];
+        }
+    } else {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(base) + at;
+        if constexpr (V == 8)
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        else if constexpr (V == 4)
+            *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        else
+            p[0] = __float2bfloat16_rn(v[0]);
+    }
+}
+
+template <int V>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeParams p) {
+    extern __shared__ float2 cs[];                                        // [rows_per_cta][half] (cos, sin), times scale
+    const uint32_t tid = threadIdx.x;
+    const uint32_t row0 = blockIdx.x * p.rows_per_cta;
+    const uint32_t nrows = min(p.rows_per_cta, p.rows - row0);
+    const uint32_t head0 = blockIdx.y * p.heads_per_cta;
+    const uint32_t nheads = min(p.heads_per_cta, p.heads - head0);
+    pdl_wait_prior_grids();
+    for (uint32_t i = tid; i < nrows * p.half; i += kRopeThreads) {
+        const uint32_t r = i / p.half, pair = i - r * p.half;
+        double turns = (double)p.positions[row0 + r] * p.freq[pair] * 0.15915494309189533577;      // over 2 pi
+        turns -= rint(turns);
+        float sn, cn;
+        sincospif(2.0f * (float)turns, &sn, &cn);
+        cs[i] = make_float2(cn * p.scale, sn * p.scale);
+    }
+    __syncthreads();
+    // units of a head: half / V pair units of 2V elements, then the copied tail in units of V
+    const uint32_t pair_units = p.half / V, units = pair_units + (p.head_dim - 2 * p.half) / V;
+    const uint32_t copy_units = p.head_dim / V;                           // of a part that does not turn (>= units)
+    const uint32_t per_row = nheads * copy_units, total = nrows * per_row;
+    for (uint32_t i = tid; i < total; i += kRopeThreads) {
+        const uint32_t r = i / per_row, rest = i - r * per_row;
+        uint32_t h = rest / copy_units;
+        const uint32_t u = rest - h * copy_units;
+        h += head0;
+        uint32_t part = 0;
+        while (h >= p.part[part].heads) h -= p.part[part++].heads;
+        const lq4_rope_part& t = p.part[part];
+        const uint64_t src = (uint64_t)(row0 + r) * t.x_row + (uint64_t)h * t.x_head;
+        const uint64_t dst = (uint64_t)(row0 + r) * t.out_row + (uint64_t)h * t.out_head;
+        if (t.turn == 0 || (u >= pair_units && u < units)) {
+            const uint32_t e = t.turn == 0 ? u * V : 2 * p.half + (u - pair_units) * V;
+            float v[V];
+            load_vec<V>(t.x, t.x_dtype, src + e, v);
+            store_vec<V>(t.out, t.out_dtype, dst + e, v);
+        } else if (u < pair_units) {
+            const uint32_t e0 = p.interleaved ? 2 * u * V : u * V, e1 = p.interleaved ? e0 + V : e0 + p.half;
+            float a[V], b[V];
+            load_vec<V>(t.x, t.x_dtype, src + e0, a);
+            load_vec<V>(t.x, t.x_dtype, src + e1, b);
+            const float2* c = cs + r * p.half + u * V;
+            const float sign = t.turn < 0 ? -1.0f : 1.0f;
+            if (p.interleaved) {
+                // pairs (v[2i], v[2i + 1]) over the 2V consecutive elements a | b
+                float v[2 * V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = a[j], v[V + j] = b[j];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float cn = c[j].x, sn = c[j].y * sign, x1 = v[2 * j], x2 = v[2 * j + 1];
+                    v[2 * j] = x1 * cn - x2 * sn;
+                    v[2 * j + 1] = x1 * sn + x2 * cn;
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) a[j] = v[j], b[j] = v[V + j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float cn = c[j].x, sn = c[j].y * sign, x1 = a[j], x2 = b[j];
+                    a[j] = x1 * cn - x2 * sn;
+                    b[j] = x1 * sn + x2 * cn;
+                }
+            }
+            store_vec<V>(t.out, t.out_dtype, dst + e0, a);
+            store_vec<V>(t.out, t.out_dtype, dst + e1, b);
+        }
+    }
+    pdl_launch_dependents();
+}
+
+// One warp per (sequence, row): the page is looked up once, the lanes move K then V in 8-element pieces.
+struct AppendParams {
+    CacheView c;
+    const void* k;
+    const void* v;
+    int32_t dtype;
+    uint32_t batch, rows, kv_heads, head_dim;
+    uint64_t batch_stride, row_stride, head_stride;
+    const int32_t* kv_lens;
+    const int32_t* counts;
+    const int32_t* index;
+    int32_t* new_lens;
+    int32_t* status;
+};
+
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ AppendParams p) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t item = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    pdl_wait_prior_grids();
+    pdl_launch_dependents();
+    if (item >= (uint64_t)p.batch * p.rows) return;
+    const uint32_t b = (uint32_t)(item / p.rows), j = (uint32_t)(item - (uint64_t)b * p.rows);
+    const int32_t len = p.kv_lens[b];
+    int32_t count = p.counts ? p.counts[b] : (int32_t)p.rows;
+    const int64_t capacity = (int64_t)p.c.max_pages * p.c.page_size;
+    bool bad = false;
+    if (count > (int32_t)p.rows) count = (int32_t)p.rows, bad = true;
+    if (count < 0 || len < 0) count = 0;
+    if (j == 0 && lane == 0 && p.new_lens)
+        p.new_lens[b] = len < 0 ? len : (int32_t)min((int64_t)len + count, min(capacity, (int64_t)0x7fffffff));
+    if ((int32_t)j < count) {
+        const int64_t slot = (int64_t)len + j;
+        const int32_t src = p.index ? p.index[item] : (int32_t)j;
+        int32_t page = -1;
+        if (slot < capacity) page = p.c.table[(uint64_t)b * p.c.max_pages + slot / p.c.page_size];
+        if (page < 0 || (uint32_t)page >= p.c.pages || src < 0 || (uint32_t)src >= p.rows) {
+            bad = true;
+        } else {
+            const uint64_t to = (uint64_t)page * p.c.page_stride + (uint64_t)(slot % p.c.page_size) * p.c.slot_stride;
+            const uint64_t from = b * p.batch_stride + src * p.row_stride;
+            const uint32_t vecs = p.head_dim / 8, total = p.kv_heads * vecs;
+            for (uint32_t i = lane; i < total; i += 32) {
+                const uint32_t h = i / vecs, e = (i - h * vecs) * 8;
+                const uint64_t at = from + h * p.head_stride + e, dst = to + h * p.c.head_stride + e;
+                float kx[8], vx[8];
+                load_vec<8>(p.k, p.dtype, at, kx);
+                load_vec<8>(p.v, p.dtype, at, vx);
+                store_vec<8>(p.c.k, LQ4_DTYPE_BF16, dst, kx);
+                store_vec<8>(p.c.v, LQ4_DTYPE_BF16, dst, vx);
+            }
+        }
+    }
+    if (bad && lane == 0) atomicOr(p.status, kDevErrBadIndex);
+}
+
+template <typename... Args>
+cudaError_t launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size_t smem, int use_pdl, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    if (use_pdl) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
+// Whether every part can be moved `vec` elements at a time.
+bool vec_fits(const lq4_rope_args& a, uint32_t half, uint32_t vec) {
+    if (half % vec || (a.head_dim - 2 * half) % vec || a.head_dim % vec) return false;
+    for (uint32_t i = 0; i < a.n_parts; ++i) {
+        const lq4_rope_part& t = a.parts[i];
+        if (!t.heads) continue;
+        if (t.x_row % vec || t.x_head % vec || t.out_row % vec || t.out_head % vec) return false;
+        const uintptr_t xa = t.x_dtype == LQ4_DTYPE_F32 ? 16 : vec * 2, oa = t.out_dtype == LQ4_DTYPE_F32 ? 16 : vec * 2;
+        if (reinterpret_cast<uintptr_t>(t.x) % xa || reinterpret_cast<uintptr_t>(t.out) % oa) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, cudaStream_t s) {
+    RopeParams p{};
+    for (uint32_t i = 0; i < a.n_parts; ++i) {
+        if (!a.parts[i].heads) continue;
+        p.part[p.n_parts++] = a.parts[i];
+        p.heads += a.parts[i].heads;
+    }
+    p.rows = a.rows;
+    p.head_dim = a.head_dim;
+    p.positions = a.positions;
+    if (a.rope) {
+        p.half = a.rope->rot_dim / 2;
+        p.freq = a.rope->freq;
+        p.interleaved = a.rope->layout == LQ4_ROPE_INTERLEAVED;
+        p.scale = a.rope->scale;
+    }
+    const uint32_t vec = vec_fits(a, p.half, 8) ? 8 : vec_fits(a, p.half, 4) ? 4 : 1;
+    // one angle per thread, at most as many rows as there are; heads are split while the CTAs do not fill
+    // the GPU twice and a CTA still has a unit for every thread
+    p.rows_per_cta = p.half ? kRopeThreads / p.half : 4;
+    if (p.rows_per_cta == 0) p.rows_per_cta = 1;
+    if (p.rows_per_cta > p.rows) p.rows_per_cta = p.rows;
+    const uint32_t row_ctas = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
+    uint32_t splits = (2u * sm_count + row_ctas - 1) / row_ctas;
+    const uint32_t units = p.rows_per_cta * p.heads * (p.head_dim / vec), most = (units + kRopeThreads - 1) / kRopeThreads;
+    if (splits > most) splits = most;
+    if (splits > p.heads) splits = p.heads;
+    p.heads_per_cta = (p.heads + splits - 1) / splits;
+    const dim3 grid(row_ctas, (p.heads + p.heads_per_cta - 1) / p.heads_per_cta);
+    const size_t smem = (size_t)p.rows_per_cta * p.half * sizeof(float2);
+    auto fn = vec == 8 ? rope_kernel<8> : vec == 4 ? rope_kernel<4> : rope_kernel<1>;
+    return launch(fn, grid, kRopeThreads, smem, use_pdl, s, p);
+}
+
+cudaError_t launch_kv_append(const lq4_kv_append_args& a, int32_t* status, int use_pdl, cudaStream_t s) {
+    AppendParams p{};
+    p.c = cache_view(*a.cache);
+    p.k = a.k;
+    p.v = a.v;
+    p.dtype = a.dtype;
+    p.batch = a.cache->batch;
+    p.rows = a.rows;
+    p.kv_heads = a.cache->kv_heads;
+    p.head_dim = a.cache->head_dim;
+    p.batch_stride = a.batch_stride;
+    p.row_stride = a.row_stride;
+    p.head_stride = a.head_stride;
+    p.kv_lens = a.kv_lens;
+    p.counts = a.counts;
+    p.index = a.index;
+    p.new_lens = a.new_lens;
+    p.status = status;
+    const uint64_t items = (uint64_t)p.batch * p.rows;
+    return launch(kv_append_kernel, dim3((unsigned)((items + 7) / 8)), 256, 0, use_pdl, s, p);
+}
+
+}  // namespace lq4
