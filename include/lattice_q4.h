@@ -536,6 +536,41 @@ typedef struct {
 } lq4_kv_append_args;
 lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* stream);
 
+/* Attention of `nodes` drafted tokens per sequence over its kv_lens[b] cached rows and the nodes' own rows, which
+ * are not in the cache yet:  out[b, t, h] = softmax over j of (scale * q . k_j) weighted v_j, j over the cached
+ * slots [0, kv_lens[b]) and over node t and its ancestors.  parents[b, t] is a node before t, or -1 for a root
+ * (it hangs on the cached sequence); parents NULL: a chain.  nodes == 1 is an ordinary decode step, whose row
+ * lq4_kv_append then adds.  Query head h reads kv head h / (q_heads / kv_heads).
+ *   q and out   [batch, nodes, q_heads, head_dim] of one type, F32 or BF16
+ *   k and v     [batch, nodes, kv_heads, head_dim] bf16
+ * A key that a node may not see contributes nothing whatever it holds (NaN and infinities included).  Nodes from
+ * node_counts[b] on (NULL: all live) and sequences with kv_lens[b] < 0 or no live node are left as they were in
+ * `out`.  Softmax and sums are f32; with f32 activations the products are too (three bf16 terms each).  Pages out
+ * of range are not seen; they, a length above the capacity and a parent that does not come before its node (it
+ * counts as a root) are reported through lq4_ctx_check.  Results depend on the lengths and the device only, not
+ * on timing.  The workspace (at most 40 MB, independent of the lengths) grows on the first call with a larger
+ * row count per kv head: make one plain call before capturing one into a CUDA graph.
+ * Stands between lq4_kv_append and the o_proj call, where the reference encodes decode_attention
+ * (forward/shaders/qwen35.metal:466-663). */
+#define LQ4_MAX_TREE_NODES 64
+typedef struct {
+    const void* q;
+    void* out;
+    int32_t dtype;
+    const void* k;
+    const void* v;
+    const lq4_kv_cache* cache;
+    uint32_t nodes, q_heads;          /* nodes 1..64; q_heads a multiple of cache->kv_heads */
+    uint64_t q_batch, q_node, q_head;            /* strides in elements */
+    uint64_t out_batch, out_node, out_head;
+    uint64_t kv_batch, kv_node, kv_head;         /* of k and v: multiples of 8; k and v 16-byte aligned */
+    const int32_t* kv_lens;           /* [batch] */
+    const int32_t* node_counts;       /* [batch] or NULL */
+    const int32_t* parents;           /* [batch, nodes] or NULL */
+    float scale;                      /* finite; 1 / sqrt(head_dim) as a rule */
+} lq4_tree_attention_args;
+lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args, void* stream);
+
 /* ---- resident objects ---------------------------------------------------- */
 
 /* Validates every block (scale finite and > 0, bias finite) on the host and only

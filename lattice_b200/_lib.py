@@ -111,6 +111,17 @@ class KvAppendArgs(C.Structure):
                 ("new_lens", C.c_void_p)]
 
 
+MAX_TREE_NODES = 64
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("cache", C.POINTER(KvCacheDesc)), ("nodes", C.c_uint32), ("q_heads", C.c_uint32)] + \
+               [(n, C.c_uint64) for n in ("q_batch", "q_node", "q_head", "out_batch", "out_node", "out_head", "kv_batch",
+                                          "kv_node", "kv_head")] + \
+               [("kv_lens", C.c_void_p), ("node_counts", C.c_void_p), ("parents", C.c_void_p), ("scale", C.c_float)]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "lq4_ctx_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
@@ -158,6 +169,7 @@ SIGNATURES = {
     "lq4_rope_rows": (C.c_int32, [C.c_void_p, C.POINTER(RopeArgs), C.c_void_p]),
     "lq4_rope_frequencies": (C.c_int32, [C.POINTER(RopeScaling), C.c_void_p, C.c_void_p]),
     "lq4_kv_append": (C.c_int32, [C.c_void_p, C.POINTER(KvAppendArgs), C.c_void_p]),
+    "lq4_tree_attention": (C.c_int32, [C.c_void_p, C.POINTER(TreeAttentionArgs), C.c_void_p]),
     "lq4_weights_upload": (C.c_int32, [C.c_void_p, C.c_uint64, C.c_uint64, C.POINTER(C.c_void_p)]),
     "lq4_weights_load_q4_file": (C.c_int32, [C.c_char_p, C.POINTER(C.c_uint64), C.c_uint32, C.POINTER(C.c_void_p)]),
     "lq4_weights_payload": (C.c_void_p, [C.c_void_p]),

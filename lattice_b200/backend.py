@@ -26,7 +26,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, check
+from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, TreeAttentionArgs, check
 from .attention import KvCache, RopeTable
 
 
@@ -574,6 +574,35 @@ class CudaQ4Backend:
         if rows == 0 and b:
             new_lens.copy_(kv_lens)
         return new_lens
+
+    def tree_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KvCache, kv_lens: torch.Tensor, *,
+                       parents: Optional[torch.Tensor] = None, node_counts: Optional[torch.Tensor] = None,
+                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of up to 64 drafted tokens per sequence (1: an ordinary decode step) over the ``kv_lens[b]``
+        cached rows and the nodes' own rows ``k`` and ``v`` (``[batch, nodes, kv_heads, head_dim]`` bf16, not in
+        the cache yet).  ``q`` is ``[batch, nodes, q_heads, head_dim]``, f32 or bf16, and the result has its type;
+        ``parents[b, t]`` is the node that ``t`` follows (-1: the cached sequence; None: a chain), ``node_counts``
+        how many nodes of a sequence are live (the others' rows of ``out`` are left as they were), ``scale``
+        defaults to ``head_dim ** -0.5``."""
+        k, v = self._cache_rows("tree_attention", cache, k, v)
+        if k.dtype != torch.bfloat16:
+            raise TypeError(f"tree_attention: the nodes' k and v must be bfloat16, got {k.dtype}")
+        b, t, heads, dim = q.shape
+        if b != k.shape[0] or t != k.shape[1] or dim != k.shape[3] or q.get_device() != self.device:
+            raise ValueError(f"tree_attention: q must be [{k.shape[0]}, {k.shape[1]}, q_heads, {k.shape[3]}] on cuda:{self.device}, got {list(q.shape)}")
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        if out is None:
+            out = torch.empty((b, t, heads, dim), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or out.get_device() != self.device:
+            raise ValueError("tree_attention: out must have q's shape, type and device and unit stride along head_dim")
+        qs, os_, ks = q.stride(), out.stride(), k.stride()
+        args = TreeAttentionArgs(q.data_ptr(), out.data_ptr(), self._dtype_of(q), k.data_ptr(), v.data_ptr(), C.pointer(cache.desc),
+                                 t, heads, qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], ks[0], ks[1], ks[2],
+                                 self._int32("kv_lens", kv_lens, b), self._int32("node_counts", node_counts, b),
+                                 self._int32("parents", parents, b, t), dim ** -0.5 if scale is None else scale)
+        check(_lib.lib().lq4_tree_attention(self._ctx, C.byref(args), self._own_stream()))
+        return out
 
     # ---- lm_head: vocabulary projection + exact top-k --------------------------------------
     @staticmethod

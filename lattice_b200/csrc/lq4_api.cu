@@ -58,6 +58,7 @@ struct lq4_ctx {
     uint32_t* tsync = nullptr;    // 64-bit launch counter of the decode kernels
     Buf xrot, xs, t, tmsg, partials, hx, hy, gemm, logits, topk, topk_ctr, mlp, mlp_h;   // xs: activation limb records of the dense decode kernel
     lq4_peer_buf* mlp_step = nullptr;   // step buffer of lq4_mlp_block's one-launch form (gate||up row + mailbox)
+    Buf attend;                   // lq4_tree_attention: partials of the items that are cut between CTAs
     Buf shard_send, shard_recv;   // staging of lq4_linear_sharded: local slices, NCCL's rank-major blocks
     cudaStream_t comm_stream = nullptr;      // second stream of lq4_linear_sharded (created on first use)
     cudaEvent_t ev_block[4] = {nullptr, nullptr, nullptr, nullptr}, ev_comm = nullptr;
@@ -349,7 +350,7 @@ void lq4_ctx_destroy(lq4_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaDeviceSynchronize();
     free_step_plan(ctx->step_plan);
-    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv})
+    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv, &ctx->attend})
         if (b->p) cudaFree(b->p);
     if (ctx->mlp_step) lq4_peer_buf_free(ctx->mlp_step);
     for (cudaEvent_t e : ctx->ev_block)
@@ -1680,6 +1681,44 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* a, void* stream
     LQ4_ON_DEVICE(ctx);
     LQ4_CUDA(launch_kv_append(*a, ctx->status, ctx->pdl, (cudaStream_t)stream));
     ctx->launches += 1;
+    return LQ4_OK;
+}
+
+lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* a, void* stream) {
+    if (!a) return fail(LQ4_ERR_NULL, "args is NULL");
+    lq4_status st;
+    if ((st = check_cache(a->cache))) return st;
+    const lq4_kv_cache& c = *a->cache;
+    if (!act_dtype(a->dtype)) return fail(LQ4_ERR_DTYPE, "q and out must be F32 or BF16");
+    if (a->nodes > LQ4_MAX_TREE_NODES) return fail(LQ4_ERR_SHAPE, "at most 64 nodes");
+    if (a->q_heads == 0 || a->q_heads % c.kv_heads) return fail(LQ4_ERR_SHAPE, "q_heads must be a multiple of kv_heads");
+    if (a->q_heads / c.kv_heads > 1024) return fail(LQ4_ERR_SHAPE, "more than 1024 query heads per kv head");
+    if (!std::isfinite(a->scale)) return fail(LQ4_ERR_SHAPE, "scale must be finite");
+    if ((uint64_t)c.batch * a->q_heads * a->nodes > 0x7fffffffull) return fail(LQ4_ERR_OVERFLOW, "batch * nodes * q_heads does not fit");
+    if (c.batch && a->nodes) {
+        if (!a->q || !a->out || !a->k || !a->v || !a->kv_lens) return fail(LQ4_ERR_NULL, "q, out, k, v and kv_lens must be non-NULL");
+        if (!aligned(a->q, act_size(a->dtype)) || !aligned(a->out, act_size(a->dtype))) return fail(LQ4_ERR_ALIGN, "q or out is not aligned to its element type");
+        if (!aligned(a->k, 16) || !aligned(a->v, 16)) return fail(LQ4_ERR_ALIGN, "k and v must be 16-byte aligned");
+        if (a->kv_batch % 8 || a->kv_node % 8 || a->kv_head % 8) return fail(LQ4_ERR_ALIGN, "strides of k and v must be multiples of 8 elements");
+        if (!aligned(a->kv_lens, 4) || !aligned(a->node_counts, 4) || !aligned(a->parents, 4)) return fail(LQ4_ERR_ALIGN, "an int32 array is misaligned");
+        const uint64_t most = 1ull << 58;
+        for (uint64_t x : {a->q_batch, a->out_batch, a->kv_batch})
+            if (mul_overflows(x, c.batch, most)) return fail(LQ4_ERR_OVERFLOW, "batch strides do not fit");
+        for (uint64_t x : {a->q_node, a->out_node, a->kv_node, a->q_head, a->out_head, a->kv_head})
+            if (x > (1ull << 40)) return fail(LQ4_ERR_OVERFLOW, "node or head strides do not fit");
+    }
+    if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
+    if (c.batch == 0 || a->nodes == 0) return LQ4_OK;
+    LQ4_ON_DEVICE(ctx);
+    cudaStream_t s = (cudaStream_t)stream;
+    AttendWorkspace ws{ctx->attend.p, ctx->attend.cap, 0, 0};
+    LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
+    if (ws.need) {
+        if ((st = ensure(ctx, ctx->attend, ws.need, false, s))) return st;
+        ws = {ctx->attend.p, ctx->attend.cap, 0, 0};
+        LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
+    }
+    ctx->launches += ws.launches;
     return LQ4_OK;
 }
 

@@ -35,4 +35,15 @@ inline CacheView cache_view(const lq4_kv_cache& c) {
     return w;
 }
 
+// ---- lq4_attend.cu --------------------------------------------------------------
+// Partials of the items that are cut between CTAs.  A launch that needs more than `bytes` does nothing and sets
+// `need`; its size depends on the device and the number of rows per kv head, not on the lengths.
+struct AttendWorkspace {
+    void* p;
+    size_t bytes, need;
+    int launches;
+};
+cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorkspace& ws, int32_t* status, int sm_count,
+                                  int use_pdl, cudaStream_t s);
+
 }  // namespace lq4

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lattice_b200 import KvCache, Lq4Error, RopeTable, _lib, build as lq4_build, rope_frequencies
-from lattice_b200._lib import KvAppendArgs, KvCacheDesc, RopeArgs, RopeDesc, RopePart, RopeScaling
+from lattice_b200._lib import KvAppendArgs, KvCacheDesc, RopeArgs, RopeDesc, RopePart, RopeScaling, TreeAttentionArgs
 
 
 @pytest.fixture(scope="module")
@@ -171,3 +171,30 @@ def test_python_objects_refuse():
         KvCache(k, k[:, :2], table)
     with pytest.raises(ValueError):
         KvCache(k, k.clone(), table)                                           # not on a GPU
+
+
+def attend_args(cache=None, **change):
+    fields = dict(q=P, out=2 * P, dtype=1, k=P, v=P, nodes=3, q_heads=4, q_batch=768, q_node=256, q_head=64, out_batch=768, out_node=256,
+                  out_head=64, kv_batch=384, kv_node=128, kv_head=64, kv_lens=P, node_counts=None, parents=None, scale=0.125)
+    fields.update(change)
+    return TreeAttentionArgs(cache=C.pointer(cache if cache is not None else cache_desc()), **fields)
+
+
+@pytest.mark.parametrize("change, status", CACHE_REFUSALS)
+def test_attention_refuses_bad_caches(L, change, status):
+    a = attend_args(cache_desc(**change))
+    assert L.lq4_tree_attention(None, C.byref(a), None) == status
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(), _lib.ERR_NULL), (dict(dtype=2), _lib.ERR_DTYPE), (dict(nodes=65), _lib.ERR_SHAPE), (dict(q_heads=0), _lib.ERR_SHAPE),
+    (dict(q_heads=5), _lib.ERR_SHAPE), (dict(q_heads=2 * 1025), _lib.ERR_SHAPE), (dict(scale=math.inf), _lib.ERR_SHAPE), (dict(scale=math.nan), _lib.ERR_SHAPE),
+    (dict(q=None), _lib.ERR_NULL), (dict(out=None), _lib.ERR_NULL), (dict(k=None), _lib.ERR_NULL), (dict(v=None), _lib.ERR_NULL),
+    (dict(kv_lens=None), _lib.ERR_NULL), (dict(q=P + 1), _lib.ERR_ALIGN), (dict(dtype=0, out=P + 2), _lib.ERR_ALIGN), (dict(k=P + 8), _lib.ERR_ALIGN),
+    (dict(kv_node=4), _lib.ERR_ALIGN), (dict(kv_head=2), _lib.ERR_ALIGN), (dict(kv_batch=1), _lib.ERR_ALIGN), (dict(parents=P + 2), _lib.ERR_ALIGN),
+    (dict(q_batch=1 << 58), _lib.ERR_OVERFLOW), (dict(out_head=1 << 41), _lib.ERR_OVERFLOW),
+])
+def test_attention_refusals(L, change, status):
+    a = attend_args(**change)
+    assert L.lq4_tree_attention(None, C.byref(a), None) == status
+    assert L.lq4_tree_attention(None, None, None) == _lib.ERR_NULL

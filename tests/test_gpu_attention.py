@@ -229,3 +229,249 @@ def test_append_python_refusals(be):
             a = dict(k=k, v=k, kv_lens=lens)
             a.update(bad)
             be.kv_append(cache, a.pop("k"), a.pop("v"), a.pop("kv_lens"), **a)
+
+
+# ---- tree attention ------------------------------------------------------------------------------------------------
+
+def random_tree(seed, batch, nodes, width):
+    """[batch, nodes] parents: each node hangs on one of the `width` nodes before it, or on the cached sequence."""
+    at = torch.arange(nodes)
+    back = (torch.rand(batch, nodes, generator=rng(seed)) * (at + 1).clamp(max=width)).long()
+    return (at - 1 - back).clamp(min=-1).to(torch.int32)
+
+
+def paths_of(parents, n):
+    """Per node the nodes it sees: itself and its ancestors."""
+    out = []
+    for t in range(n):
+        at, path = t, []
+        while at >= 0:
+            path.append(at)
+            at = int(parents[at]) if parents is not None else at - 1
+        out.append(path)
+    return out
+
+
+def attend_ref(q, k, v, cache_k, cache_v, table, lens, parents, counts, scale):
+    """64-bit attention by the definition, one sequence after the other; also the weighted magnitudes of v and the
+    size of the scores, for the tolerances.  Rows of dead nodes are NaN."""
+    batch, nodes, heads, dim = q.shape
+    hk, page = k.shape[2], cache_k.shape[1]
+    out = torch.full(q.shape, math.nan, dtype=torch.float64)
+    mag, size = torch.zeros_like(out), torch.zeros(batch, nodes, heads, 1, dtype=torch.float64)
+    for b in range(batch):
+        n = lens[b]
+        live = nodes if counts is None else counts[b]
+        if n < 0:
+            continue
+        at = [(int(table[b, s // page]), s % page) for s in range(n)]
+        idx = torch.tensor(at, dtype=torch.long).view(-1, 2)
+        kk = torch.cat([cache_k[idx[:, 0], idx[:, 1]], k[b]]).double().repeat_interleave(heads // hk, 1)
+        vv = torch.cat([cache_v[idx[:, 0], idx[:, 1]], v[b]]).double().repeat_interleave(heads // hk, 1)
+        for t, path in enumerate(paths_of(parents[b] if parents is not None else None, live)):
+            keys = torch.tensor(list(range(n)) + [n + j for j in sorted(path)])
+            s = torch.einsum("hd,nhd->hn", q[b, t].double(), kk[keys]) * scale
+            w = torch.softmax(s, -1)
+            out[b, t] = torch.einsum("hn,nhd->hd", w, vv[keys])
+            mag[b, t] = torch.einsum("hn,nhd->hd", w, vv[keys].abs())
+            size[b, t, :, 0] = (q[b, t].double().norm(dim=-1) * kk[keys].norm(dim=-1).amax(0)) * abs(scale)
+    return out, mag, size
+
+
+def assert_attention(got, ref, mag, size, keys):
+    """Scores: products are exact, about 16 roundings of 2^-23 of at most |q| |k| scale lie in a sum, two more in the
+    exponent and 2^-22 in exp2; each error counts twice (numerator and sum).  bf16 activations: probabilities and result
+    are rounded by half a step of 2^-8.  The running sums round once a tile of 64 keys, and at the joins."""
+    e = 2 * (16 * 2.0 ** -23 * size + 2.0 ** -21) + (keys / 64 + 200) * 2.0 ** -23
+    if got.dtype == BF16:
+        e = e + 2.0 ** -8
+    tol = mag * e + HALF_STEP[got.dtype] * ref.abs() * 1.01 + 1e-30
+    err = (got.double().cpu() - ref).abs()
+    live = ~ref.isnan()
+    assert bool((err <= tol)[live].all()), float((err / tol)[live].max())
+
+
+def attend_case(be, seed, batch, nodes, hq, hk, dim, page, lens, dtype, width=2, counts=None, order="dense", scale=None, poison=True, chain=False):
+    """Random inputs with NaN in every cache slot behind a sequence's length, run and checked."""
+    most = max(max(lens), 0)
+    cache = make_cache(batch, -(-max(most, 1) // page) + 1, page, hk, dim, seed=seed, order=order)
+    if poison:
+        keep = torch.zeros(cache.k.shape[:2], dtype=torch.bool)
+        table = cache.page_table.cpu().long()
+        for b, n in enumerate(lens):
+            s = torch.arange(max(n, 0))
+            keep[table[b, s // page], s % page] = True
+        for x in (cache.k, cache.v):
+            x.masked_fill_(~keep[:, :, None, None].cuda(), math.nan)
+    q = (2 * normal(seed + 5, batch, nodes, hq, dim)).to(dtype)
+    k, v = (normal(seed + 6 + i, batch, nodes, hk, dim).to(BF16) for i in range(2))
+    parents = None if chain or nodes == 1 else random_tree(seed + 8, batch, nodes, width)
+    i32 = lambda x: None if x is None else torch.as_tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    out = torch.full(q.shape, 7.0, dtype=dtype).cuda()
+    got = be.tree_attention(q.cuda(), k.cuda(), v.cuda(), cache, i32(lens), parents=i32(parents), node_counts=i32(counts), scale=scale, out=out)
+    ref = attend_ref(q, k, v, cache.k.cpu(), cache.v.cpu(), cache.page_table.cpu(), lens, parents, counts, dim ** -0.5 if scale is None else scale)
+    assert_attention(got, *ref, most + nodes)
+    dead = ref[0].isnan()
+    assert bool((got.cpu()[dead] == 7.0).all())                                  # rows of nobody stay as they were
+    be.check_device_status()
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("length", [0, 1, 5, 63, 64, 65, 127, 1000])
+def test_attention_lengths_of_one_token(be, dtype, length):
+    attend_case(be, 100 + length, 2, 1, 10, 2, 128, 16, [length, max(length - 1, 0)], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim, hq, hk", [(8, 1, 1), (64, 4, 4), (72, 6, 2), (80, 16, 1), (128, 5, 1), (192, 8, 2), (256, 12, 2), (256, 3, 1)])
+@pytest.mark.parametrize("nodes", [1, 5, 16, 64])
+def test_attention_shapes(be, dtype, dim, hq, hk, nodes):
+    """All bands of rows (16, 32, 64, several tiles) and all padded head sizes."""
+    attend_case(be, 7 * dim + nodes, 2, nodes, hq, hk, dim, 24, [150, 33], dtype, width=4)
+
+
+@pytest.mark.parametrize("page", [1, 5, 7, 64, 100])
+@pytest.mark.parametrize("order", ["dense", "heads"])
+def test_attention_pages_that_end_inside_a_tile(be, page, order):
+    attend_case(be, page, 3, 3, 4, 2, 64, page, [131, 64, 0], BF16, order=order)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_ragged_batch_with_dead_rows(be, dtype):
+    lens = [17, -1, 400, 0, 64, 1, -5, 900]
+    counts = [6, 6, 1, 3, 0, 6, 2, 5]
+    attend_case(be, 40, 8, 6, 6, 3, 64, 16, lens, dtype, counts=counts, width=3)
+
+
+def test_attention_large_ragged_batch(be):
+    lens = [(37 * i) % 300 - 1 for i in range(300)]
+    attend_case(be, 41, 300, 2, 2, 1, 64, 32, lens, BF16, poison=False)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_long_sequences_are_split(be, dtype):
+    """One item over every CTA, with a border inside a page; chains and trees."""
+    attend_case(be, 42, 1, 4, 4, 1, 128, 48, [20011], dtype, width=2)
+    attend_case(be, 43, 2, 7, 5, 1, 256, 16, [3000, 9000], dtype, chain=True)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+def test_attention_scales(be, scale):
+    attend_case(be, 44, 2, 5, 4, 2, 64, 16, [100, 7], F32, scale=scale)
+
+
+def test_attention_strided_rows_and_same_bits_again(be):
+    """q, k and v as slices of one fused row, out as a slice; the same call gives the same bits."""
+    b, t, hq, hk, d = 3, 4, 6, 2, 64
+    fused = normal(50, b, t, hq + 2 * hk, d).to(BF16)
+    g = fused.cuda()
+    cache = make_cache(b, 8, 16, hk, d, seed=51)
+    lens = [100, 3, 65]
+    par = random_tree(52, b, t, 2)
+    wide = torch.zeros(b, t, 2 * hq, d, dtype=BF16).cuda()
+    q, k, v = g.split([hq, hk, hk], 2)
+    dev = lambda x: torch.as_tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    got = be.tree_attention(q, k, v, cache, dev(lens), parents=dev(par), out=wide[:, :, hq:])
+    cq, ck, cv = fused.split([hq, hk, hk], 2)
+    assert_attention(got, *attend_ref(cq, ck, cv, cache.k.cpu(), cache.v.cpu(), cache.page_table.cpu(), lens, par, None, d ** -0.5), 104)
+    assert not wide[:, :, :hq].any()
+    again = be.tree_attention(q, k, v, cache, dev(lens), parents=dev(par))
+    assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_masked_nodes_hold_anything(be, dtype):
+    """Node 1 and node 2 are siblings; what node 2 holds reaches node 2 only."""
+    b, t, d = 1, 4, 64
+    cache = make_cache(b, 4, 16, 1, d, seed=60)
+    q = normal(61, b, t, 2, d).to(dtype)
+    k, v = normal(62, b, t, 1, d).to(BF16), normal(63, b, t, 1, d).to(BF16)
+    par = torch.tensor([[-1, 0, 0, 1]], dtype=torch.int32)
+    lens = torch.tensor([50], dtype=torch.int32).cuda()
+    clean = be.tree_attention(q.cuda(), k.cuda(), v.cuda(), cache, lens, parents=par.cuda()).cpu()
+    v2 = v.clone()
+    v2[0, 2, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, math.inf])
+    dirty = be.tree_attention(q.cuda(), k.cuda(), v2.cuda(), cache, lens, parents=par.cuda()).cpu()
+    assert torch.equal(dirty[:, [0, 1, 3]], clean[:, [0, 1, 3]])
+    for h in range(2):
+        assert dirty[0, 2, h, 0] == math.inf and dirty[0, 2, h, 1] == -math.inf and dirty[0, 2, h, 2].isnan()
+    assert torch.equal(dirty[0, 2, :, 4:], clean[0, 2, :, 4:])
+    for bad in (math.nan, math.inf, torch.finfo(BF16).min):
+        k2, v3 = k.clone(), v2.clone()
+        k2[0, 2] = bad
+        v3[0, 2] = bad
+        dirty = be.tree_attention(q.cuda(), k2.cuda(), v3.cuda(), cache, lens, parents=par.cuda()).cpu()
+        assert torch.equal(dirty[:, [0, 1, 3]], clean[:, [0, 1, 3]])
+
+
+def test_attention_reports_bad_indexes(be):
+    from lattice_b200 import Lq4Error
+    d = 64
+    q, k = normal(70, 1, 3, 2, d).to(BF16).cuda(), normal(71, 1, 3, 1, d).to(BF16).cuda()
+    dev = lambda x: torch.as_tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    for what in ("page", "negative page", "length", "count", "parent", "parent of itself"):
+        cache = make_cache(1, 4, 16, 1, d, seed=72)
+        lens, par, counts = [40], [[-1, 0, 1]], None
+        if what == "page":
+            cache.page_table[0, 1] = cache.k.shape[0]
+        if what == "negative page":
+            cache.page_table[0, 1] = -7
+        if what == "length":
+            lens = [65]
+        if what == "count":
+            counts = dev([4])
+        if what == "parent":
+            par = [[-1, 2, 0]]
+        if what == "parent of itself":
+            par = [[0, 0, 1]]
+        got = be.tree_attention(q, k, k, cache, dev(lens), parents=dev(par), node_counts=counts)
+        with pytest.raises(Lq4Error):
+            be.check_device_status()
+        be.check_device_status()
+        if "page" in what:                                                       # the keys of that page are not seen
+            keep = [s for s in range(40) if s // 16 != 1]
+            kk = cache.k.cpu()[cache.page_table.cpu()[0, [0, 2]].long()].reshape(-1, 1, d)
+            kk = torch.cat([kk[:16], kk[16:24]])
+            assert len(keep) == kk.shape[0]
+            vv = cache.v.cpu()[cache.page_table.cpu()[0, [0, 2]].long()].reshape(-1, 1, d)
+            vv = torch.cat([vv[:16], vv[16:24]])
+            ref = attend_ref(q.cpu(), k.cpu(), k.cpu(), kk[None], vv[None], torch.zeros(1, 1, dtype=torch.int32), [24], torch.tensor(par), None, d ** -0.5)
+            assert_attention(got, *ref, 64)
+
+
+def test_attention_in_a_captured_graph(be):
+    """A graph replays with other lengths, pages and values; the launch does not depend on them."""
+    b, t, d = 2, 3, 64
+    cache = make_cache(b, 40, 16, 2, d, seed=80)
+    q, k, v = normal(81, b, t, 4, d).to(BF16).cuda(), normal(82, b, t, 2, d).to(BF16).cuda(), normal(83, b, t, 2, d).to(BF16).cuda()
+    lens, par = torch.tensor([5, 600], dtype=torch.int32).cuda(), random_tree(84, b, t, 2).cuda()
+    out = torch.empty(b, t, 4, d, dtype=BF16, device="cuda")
+    call = lambda: be.tree_attention(q, k, v, cache, lens, parents=par, out=out)  # noqa: E731
+    call()                                                                       # the workspace grows outside the capture
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for new in ([5, 600], [639, 0], [64, -1]):
+        lens.copy_(torch.tensor(new, dtype=torch.int32))
+        q.copy_(normal(85 + new[0], b, t, 4, d).to(BF16))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        ref = attend_ref(q.cpu(), k.cpu(), v.cpu(), cache.k.cpu(), cache.v.cpu(), cache.page_table.cpu(), new, par.cpu(), None, d ** -0.5)
+        assert_attention(out, *ref, 640)
+        assert bool((out.cpu()[ref[0].isnan()] == 7.0).all())
+    be.check_device_status()
+
+
+def test_attention_python_refusals(be):
+    cache = make_cache(2, 2, 16, 2, 64)
+    q, k = normal(90, 2, 3, 4, 64).to(BF16).cuda(), normal(91, 2, 3, 2, 64).to(BF16).cuda()
+    lens = torch.zeros(2, dtype=torch.int32).cuda()
+    for bad in (dict(q=q[:1]), dict(q=q[:, :2]), dict(q=q.half()), dict(q=q.cpu()), dict(k=k.float(), v=k.float()), dict(k=k[:, :, :1], v=k[:, :, :1]),
+                dict(parents=lens), dict(kv_lens=lens.long()), dict(out=q.float()), dict(node_counts=lens[:1])):
+        a = dict(q=q, k=k, v=k, kv_lens=lens)
+        a.update(bad)
+        with pytest.raises((ValueError, TypeError)):
+            be.tree_attention(a.pop("q"), a.pop("k"), a.pop("v"), cache, a.pop("kv_lens"), **a)
