@@ -571,6 +571,43 @@ typedef struct {
 } lq4_tree_attention_args;
 lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args, void* stream);
 
+/* Verification of drafted tokens against the target's distribution, from given uniforms.  Node 0 of a sequence
+ * is its last certain token; the other nodes are drafts, tokens[b, t] drafted behind node parents[b, t] < t
+ * (parents NULL: a chain; a node with another parent is never visited).  Row t of the logits is the
+ * distribution behind node t:  p = softmax(target / temperature), q = softmax(draft / temperature).  From node 0
+ * on, the children of the current node are tried in index order: the first is accepted with probability
+ * min(1, p / q), a refusal leaves norm(max(p - q, 0)) for the next (draft_logits NULL: the drafts are certain, one is
+ * accepted with probability p and a refusal takes its token out of p).  An accepted child becomes the current
+ * node; when none is, or there are none, the next token is drawn from what is left:
+ *   accepted          iff  u q(t) < p'(t), u = uniforms[b, child], p' the current residual (certain: u < p'(t))
+ *   next_token[b]     the smallest j with  sum(p'[0..j]) > uniforms[b, 0] * sum(p')
+ *   temperature 0     (below 1e-20) accepts the argmax (ties to the lower id) and returns it
+ * NaN and -inf logits carry no mass; +inf takes all of it; a row without mass accepts nothing and gives next_token -1.
+ * A drafted token outside the vocabulary is never accepted and changes nothing.  If nothing is left of p after
+ * the refusals (by rounding), the token comes from p.  Uniforms lie in [0, 1).
+ *   path[b, 0 .. path_len[b])   the accepted nodes from node 0 on (rising), -1 behind them: `index` and `counts`
+ *                               of lq4_kv_append
+ * Sequences with node_counts[b] <= 0 get path_len 0 and next_token -1.  Exponentials are f32 over the vocabulary and
+ * f64 for the drafted tokens; sums and comparisons are f64.  One launch, no workspace.  Stands behind the
+ * lm_head projection over all nodes' rows, where a plain step calls lq4_logits_topk. */
+typedef struct {
+    const void* target_logits;        /* [batch, nodes, vocab], F32 or BF16 */
+    const void* draft_logits;         /* the same type, or NULL */
+    int32_t dtype;
+    uint32_t batch, nodes, vocab;     /* nodes 1..64 */
+    uint64_t target_batch, target_node;          /* strides in elements; the innermost is 1 */
+    uint64_t draft_batch, draft_node;
+    const int32_t* tokens;            /* [batch, nodes]; tokens[b, 0] is not read */
+    const int32_t* parents;           /* [batch, nodes] or NULL; parents[b, 0] is not read */
+    const int32_t* node_counts;       /* [batch] or NULL */
+    const float* uniforms;            /* [batch, nodes] */
+    const float* temperature;         /* [batch] or NULL (1) */
+    int32_t* path;                    /* [batch, nodes] */
+    int32_t* path_len;                /* [batch] */
+    int32_t* next_token;              /* [batch] */
+} lq4_verify_args;
+lq4_status lq4_verify_draft(lq4_ctx* ctx, const lq4_verify_args* args, void* stream);
+
 /* ---- resident objects ---------------------------------------------------- */
 
 /* Validates every block (scale finite and > 0, bias finite) on the host and only

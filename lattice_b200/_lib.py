@@ -122,6 +122,14 @@ class TreeAttentionArgs(C.Structure):
                [("kv_lens", C.c_void_p), ("node_counts", C.c_void_p), ("parents", C.c_void_p), ("scale", C.c_float)]
 
 
+class VerifyArgs(C.Structure):
+    _fields_ = [("target_logits", C.c_void_p), ("draft_logits", C.c_void_p), ("dtype", C.c_int32), ("batch", C.c_uint32),
+                ("nodes", C.c_uint32), ("vocab", C.c_uint32), ("target_batch", C.c_uint64), ("target_node", C.c_uint64),
+                ("draft_batch", C.c_uint64), ("draft_node", C.c_uint64)] + \
+               [(n, C.c_void_p) for n in ("tokens", "parents", "node_counts", "uniforms", "temperature", "path", "path_len",
+                                          "next_token")]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "lq4_ctx_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
@@ -170,6 +178,7 @@ SIGNATURES = {
     "lq4_rope_frequencies": (C.c_int32, [C.POINTER(RopeScaling), C.c_void_p, C.c_void_p]),
     "lq4_kv_append": (C.c_int32, [C.c_void_p, C.POINTER(KvAppendArgs), C.c_void_p]),
     "lq4_tree_attention": (C.c_int32, [C.c_void_p, C.POINTER(TreeAttentionArgs), C.c_void_p]),
+    "lq4_verify_draft": (C.c_int32, [C.c_void_p, C.POINTER(VerifyArgs), C.c_void_p]),
     "lq4_weights_upload": (C.c_int32, [C.c_void_p, C.c_uint64, C.c_uint64, C.POINTER(C.c_void_p)]),
     "lq4_weights_load_q4_file": (C.c_int32, [C.c_char_p, C.POINTER(C.c_uint64), C.c_uint32, C.POINTER(C.c_void_p)]),
     "lq4_weights_payload": (C.c_void_p, [C.c_void_p]),

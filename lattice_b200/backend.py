@@ -26,7 +26,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, TreeAttentionArgs, check
+from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, TreeAttentionArgs, VerifyArgs, check
 from .attention import KvCache, RopeTable
 
 
@@ -639,6 +639,41 @@ class CudaQ4Backend:
                           C.pointer(rot) if rot is not None else None, _lib.PATH_AUTO, None, None)
         check(_lib.lib().lq4_lm_head_topk(self._ctx, C.byref(args), top_k, cand.data_ptr(), _stream()))
         return self._split_candidates(cand)
+
+    # ---- verification of drafted tokens -----------------------------------------------------
+    def verify_draft(self, target_logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, *,
+                     draft_logits: Optional[torch.Tensor] = None, parents: Optional[torch.Tensor] = None,
+                     node_counts: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None
+                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Which drafted tokens the target accepts, and the token behind them.  ``target_logits`` (and
+        ``draft_logits``; None: certain drafts) are ``[batch, nodes, vocab]``, f32 or bf16: row ``t`` is the
+        distribution behind node ``t``, node 0 being the last certain token; ``tokens`` and ``parents`` (None: a
+        chain) are ``[batch, nodes]`` int32, ``uniforms`` ``[batch, nodes]`` f32 in [0, 1) (entry 0 draws the last
+        token), ``temperature`` ``[batch]`` f32 (0: greedy).  Returns ``(path, path_len, next_token)``: the
+        accepted nodes from node 0 on with -1 behind them, their number, the next token; ``path`` and
+        ``path_len`` are ``index`` and ``counts`` of ``kv_append``."""
+        b, t, vocab = target_logits.shape
+        if draft_logits is not None and (draft_logits.shape != target_logits.shape or draft_logits.dtype != target_logits.dtype):
+            raise ValueError("verify_draft: draft_logits must have target_logits' shape and type")
+        rows = []
+        for x in (target_logits, draft_logits):
+            if x is not None and x.get_device() != self.device:
+                raise ValueError(f"verify_draft: logits must lie on cuda:{self.device}")
+            rows.append(x if x is None or x.stride(2) == 1 else x.contiguous())
+        for name, x, shape in (("uniforms", uniforms, (b, t)), ("temperature", temperature, (b,))):
+            if x is not None and (x.dtype != torch.float32 or x.shape != shape or not x.is_contiguous() or x.get_device() != self.device):
+                raise ValueError(f"verify_draft: {name} must be a contiguous float32 tensor of shape {list(shape)} on cuda:{self.device}")
+        out = torch.empty(b * (t + 2), dtype=torch.int32, device=target_logits.device)
+        path, path_len, token = out[:b * t].view(b, t), out[b * t:b * (t + 1)], out[b * (t + 1):]
+        target, draft = rows
+        args = VerifyArgs(target.data_ptr(), draft.data_ptr() if draft is not None else None, self._dtype_of(target), b, t, vocab,
+                          target.stride(0), target.stride(1), draft.stride(0) if draft is not None else 0,
+                          draft.stride(1) if draft is not None else 0, self._int32("tokens", tokens, b, t),
+                          self._int32("parents", parents, b, t), self._int32("node_counts", node_counts, b), uniforms.data_ptr(),
+                          temperature.data_ptr() if temperature is not None else None, path.data_ptr(), path_len.data_ptr(),
+                          token.data_ptr())
+        check(_lib.lib().lq4_verify_draft(self._ctx, C.byref(args), self._own_stream()))
+        return path, path_len, token
 
     def prepare_group(self, problems, outs: Optional[List[torch.Tensor]] = None,
                       gather: Optional[GatherDesc] = None, wait_gather: Optional[GatherDesc] = None) -> "PreparedGroup":

@@ -1722,6 +1722,32 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* a, vo
     return LQ4_OK;
 }
 
+lq4_status lq4_verify_draft(lq4_ctx* ctx, const lq4_verify_args* a, void* stream) {
+    if (!a) return fail(LQ4_ERR_NULL, "args is NULL");
+    if (!act_dtype(a->dtype)) return fail(LQ4_ERR_DTYPE, "logits must be F32 or BF16");
+    if (a->nodes == 0 || a->nodes > LQ4_MAX_TREE_NODES) return fail(LQ4_ERR_SHAPE, "nodes must be in 1..64");
+    if (a->vocab == 0) return fail(LQ4_ERR_SHAPE, "vocab must be non-zero");
+    if (a->vocab > 0x3fffffffu || a->batch > 0x3ffffffu) return fail(LQ4_ERR_OVERFLOW, "vocab or batch does not fit");
+    if (a->batch) {
+        if (!a->target_logits || !a->tokens || !a->uniforms || !a->path || !a->path_len || !a->next_token)
+            return fail(LQ4_ERR_NULL, "target_logits, tokens, uniforms and the outputs must be non-NULL");
+        const size_t e = act_size(a->dtype);
+        if (!aligned(a->target_logits, e) || !aligned(a->draft_logits, e)) return fail(LQ4_ERR_ALIGN, "logits are not aligned to their element type");
+        for (const void* q : {(const void*)a->tokens, (const void*)a->parents, (const void*)a->node_counts, (const void*)a->uniforms,
+                              (const void*)a->temperature, (const void*)a->path, (const void*)a->path_len, (const void*)a->next_token})
+            if (!aligned(q, 4)) return fail(LQ4_ERR_ALIGN, "an array is misaligned");
+        if (mul_overflows(a->target_batch, a->batch, 1ull << 59) || mul_overflows(a->draft_batch, a->batch, 1ull << 59) ||
+            a->target_node > (1ull << 52) || a->draft_node > (1ull << 52))
+            return fail(LQ4_ERR_OVERFLOW, "strides do not fit");
+    }
+    if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
+    if (a->batch == 0) return LQ4_OK;
+    LQ4_ON_DEVICE(ctx);
+    LQ4_CUDA(launch_verify_draft(*a, ctx->status, ctx->sm_count, ctx->pdl, (cudaStream_t)stream));
+    ctx->launches += 1;
+    return LQ4_OK;
+}
+
 static float f16_bits_to_f32_host(uint16_t h) {
     const uint32_t sign = (uint32_t)(h >> 15) << 31, e = (h >> 10) & 0x1f, f = h & 0x3ff;
     uint32_t bits;

@@ -46,4 +46,7 @@ struct AttendWorkspace {
 cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorkspace& ws, int32_t* status, int sm_count,
                                   int use_pdl, cudaStream_t s);
 
+// ---- lq4_verify.cu --------------------------------------------------------------
+cudaError_t launch_verify_draft(const lq4_verify_args& a, int32_t* status, int sm_count, int use_pdl, cudaStream_t s);
+
 }  // namespace lq4

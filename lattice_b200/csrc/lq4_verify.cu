@@ -1,0 +1,491 @@
+// Verification of drafted tokens (a chain or a tree) against the target's distribution, from given uniforms.
+//
+// At a node with target distribution p and draft distribution q the children are tried in index order, and a
+// refused child leaves the residual norm(max(p' - q, 0)) of what was there before it.  Unrolled, the residual
+// after r refusals is max(p - a_r q, 0) / Z_r with a_0 = 0, Z_0 = 1 and
+//
+//     a_{r+1} = a_r + Z_r,     Z_{r+1} = sum_j max(p_j - a_{r+1} q_j, 0):
+//
+// two numbers carry the whole state, and a refusal costs one sum over the vocabulary.  A child with token t is
+// accepted iff u q(t) Z < max(p(t) - a q(t), 0).  Certain drafts (no draft distribution) take the refused tokens
+// out of p instead: accepted iff u Z < p(t), Z -= p(t) on refusal.  The last token is the smallest j whose
+// cumulated residual exceeds u_0 times its sum; temperature 0 compares with the argmax throughout.
+//
+// One thread-block cluster per sequence walks down from the root and reads only the rows of the nodes it
+// visits (a tree of 64 nodes has few on its path); the vocabulary is cut over the cluster, 256 logits per warp
+// step.  Per node: one pass for (max, sum) of p and q, exchanged through distributed shared memory with one
+// cluster barrier; one pass per refusal; and the rescan of one warp's share for the last token.  Every CTA
+// takes every decision itself from the same numbers, in the same order.
+//
+// Decisions lie next to borders, so everything that is summed or compared is f64; only the exponentials over the
+// vocabulary are f32 (expf), the drafted tokens' own are f64.
+#include "lq4_attend.cuh"
+
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+namespace lq4 {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr uint32_t kVThreads = 512, kVWarps = kVThreads / 32, kMaxCluster = 16;
+constexpr uint32_t kNoToken = 0xffffffffu;
+
+struct VerifyParams {
+    const void* target;
+    const void* draft;                  // NULL: certain drafts
+    uint64_t target_batch, target_node, draft_batch, draft_node;
+    uint32_t nodes, vocab;
+    const int32_t* tokens;
+    const int32_t* parents;
+    const int32_t* node_counts;
+    const float* uniforms;
+    const float* temperature;
+    int32_t* path;
+    int32_t* path_len;
+    int32_t* next_token;
+    int32_t* status;
+};
+
+// (max, sum of exp((x - max) / tau)) of a share of a row
+struct MaxSum {
+    float m;
+    double s;
+};
+
+// exp((x - m) * it); a row whose maximum is +inf has all its mass on the entries that are.
+__device__ __forceinline__ float mass(float x, float m, float it) {
+    if (m == INFINITY) return x == m ? 1.0f : 0.0f;
+    return expf((x - m) * it);
+}
+__device__ __forceinline__ double mass64(float x, float m, double tau) {
+    if (m == INFINITY) return x == m ? 1.0 : 0.0;
+    return exp(((double)x - (double)m) / tau);
+}
+__device__ __forceinline__ MaxSum join(const MaxSum& a, const MaxSum& b, float it) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return {m, 0.0};
+    return {m, a.s * (a.m == m ? 1.0f : mass(a.m, m, it)) + b.s * (b.m == m ? 1.0f : mass(b.m, m, it))};
+}
+__device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }      // NaN carries no mass
+
+// Order of candidates: higher logit first, ties to the lower id (0: nothing that ranks).
+__device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) {
+    if (v == -INFINITY) return 0;
+    if (v == 0.0f) v = 0.0f;
+    uint32_t u = __float_as_uint(v);
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return ((uint64_t)u << 32) | (uint32_t)~id;
+}
+
+// Elements [j, j + 8) of a row as f32, -inf outside it and for NaN.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int64_t j, uint32_t vocab, float (&x)[8]) {
+    constexpr bool f32 = std::is_same<T, float>::value;
+    if (j >= 0 && j + 8 <= (int64_t)vocab && (reinterpret_cast<uintptr_t>(row + j) & 15) == 0) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + j));
+        if constexpr (f32) {
+            const uint4 b = __ldg(reinterpret_cast<const uint4*>(row + j) + 1);
+            x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
+            x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
+        } else {
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = -INFINITY;
+            if (j + i >= 0 && j + i < (int64_t)vocab) {
+                if constexpr (f32)
+                    x[i] = __ldg(row + j + i);
+                else
+                    x[i] = bf16_to_f32(__ldg(row + j + i));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = clean(x[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ float one_logit(const T* row, uint32_t j) {
+    if constexpr (std::is_same<T, float>::value)
+        return clean(row[j]);
+    else
+        return clean(bf16_to_f32(row[j]));
+}
+
+struct Exchange {                       // what a CTA tells the others
+    MaxSum p, q;
+    uint64_t best;
+    double total;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t b = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    __shared__ Exchange slots[2][kMaxCluster];
+    __shared__ MaxSum wp[kVWarps], wq[kVWarps];
+    __shared__ uint64_t wbest[kVWarps];
+    __shared__ double wtot[kVWarps];
+    __shared__ int32_t parent[LQ4_MAX_TREE_NODES], token[LQ4_MAX_TREE_NODES];
+    __shared__ float uni[LQ4_MAX_TREE_NODES];
+    __shared__ double child_p[LQ4_MAX_TREE_NODES], child_q[LQ4_MAX_TREE_NODES];
+    __shared__ uint32_t gone[LQ4_MAX_TREE_NODES];
+    __shared__ uint32_t s_action, s_child, s_gone;
+    __shared__ double s_a, s_z;
+
+    pdl_wait_prior_grids();
+    pdl_launch_dependents();
+    int32_t n = p.node_counts ? p.node_counts[b] : (int32_t)p.nodes;
+    if (n > (int32_t)p.nodes) {
+        n = (int32_t)p.nodes;
+        if (tid == 0 && rank == 0) atomicOr(p.status, kDevErrBadIndex);
+    }
+    const uint64_t first = (uint64_t)b * p.nodes;
+    if (n <= 0) {                                                        // uniform over the cluster
+        if (rank == 0) {
+            if (tid < p.nodes) p.path[first + tid] = -1;
+            if (tid == 0) p.path_len[b] = 0, p.next_token[b] = -1;
+        }
+        return;
+    }
+    if (tid < (uint32_t)n) {
+        parent[tid] = p.parents ? p.parents[first + tid] : (int32_t)tid - 1;
+        token[tid] = tid ? p.tokens[first + tid] : -1;
+        uni[tid] = p.uniforms[first + tid];
+    }
+    const float tau = p.temperature ? p.temperature[b] : 1.0f;
+    const bool greedy = !(tau >= 1e-20f);
+    const float it = greedy ? 1.0f : 1.0f / tau;
+    const bool sampled = p.draft != nullptr && !greedy;
+    const T* target_rows = static_cast<const T*>(p.target) + b * p.target_batch;
+    const T* draft_rows = static_cast<const T*>(p.draft) + b * p.draft_batch;
+    uint32_t turn = 0;                                                   // which half of `slots` comes next
+    if (rank == 0 && tid < p.nodes) p.path[first + tid] = tid == 0 ? 0 : -1;
+    uint32_t cur = 0, count = 1;
+    __syncthreads();
+
+    // this warp's part of a row: steps of 256 logits, from the row's own 16-byte border on
+    const uint32_t all_warps = ranks * kVWarps, me = rank * kVWarps + warp;
+
+    for (;;) {
+        const T* prow = target_rows + cur * p.target_node;
+        const T* qrow = sampled ? draft_rows + cur * p.draft_node : nullptr;
+        const int64_t shift = (int64_t)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
+        const uint32_t steps = (uint32_t)((p.vocab + shift + 255) / 256), per = (steps + all_warps - 1) / all_warps;
+        const uint32_t c0 = min(me * per, steps), c1 = min(c0 + per, steps);
+        const int64_t j_lane = (int64_t)lane * 8 - shift;
+        bool inner = false;                                              // does this node have children?
+        for (uint32_t c = cur + 1; c < (uint32_t)n; ++c) inner |= parent[c] == (int32_t)cur;
+
+        // ---- (max, sum) of p, of q where children need it; the argmax for greedy sequences
+        MaxSum sp{-INFINITY, 0.0}, sq{-INFINITY, 0.0};
+        uint64_t best = 0;
+        for (uint32_t c = c0; c < c1; ++c) {
+            const int64_t j = (int64_t)c * 256 + j_lane;
+            float x[8], y[8];
+            load8(prow, j, p.vocab, x);
+            if (sampled && inner) load8(qrow, j, p.vocab, y);
+            if (greedy) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint64_t k = rank_key(x[i], (uint32_t)(j + i));
+                    best = k > best ? k : best;
+                }
+                continue;
+            }
+            auto add = [&](MaxSum& s, const float (&v)[8]) {
+                float m = v[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+                if (m == -INFINITY) return;
+                if (m > s.m) {
+                    if (s.m != -INFINITY) s.s *= mass(s.m, m, it);
+                    s.m = m;
+                }
+                float t = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t += mass(v[i], s.m, it);
+                s.s += t;
+            };
+            add(sp, x);
+            if (sampled && inner) add(sq, y);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            if (greedy) {
+                const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+                best = k > best ? k : best;
+            } else {
+                sp = join(sp, {__shfl_xor_sync(0xffffffffu, sp.m, o), __shfl_xor_sync(0xffffffffu, sp.s, o)}, it);
+                if (sampled && inner) sq = join(sq, {__shfl_xor_sync(0xffffffffu, sq.m, o), __shfl_xor_sync(0xffffffffu, sq.s, o)}, it);
+            }
+        }
+        if (lane == 0) wp[warp] = sp, wq[warp] = sq, wbest[warp] = best;
+        __syncthreads();
+        if (tid < ranks) {                                               // one thread per CTA to tell
+            Exchange e{{-INFINITY, 0.0}, {-INFINITY, 0.0}, 0, 0.0};
+            for (uint32_t w = 0; w < kVWarps; ++w) {
+                e.p = join(e.p, wp[w], it);
+                e.q = join(e.q, wq[w], it);
+                e.best = wbest[w] > e.best ? wbest[w] : e.best;
+            }
+            *cluster.map_shared_rank(&slots[turn][rank], tid) = e;
+        }
+        cluster.sync();
+        MaxSum P{-INFINITY, 0.0}, Q{-INFINITY, 0.0};
+        best = 0;
+        for (uint32_t r = 0; r < ranks; ++r) {
+            const Exchange& e = slots[turn][r];
+            P = join(P, e.p, it);
+            Q = join(Q, e.q, it);
+            best = e.best > best ? e.best : best;
+        }
+        turn ^= 1;
+        const double ip = P.s > 0.0 ? 1.0 / P.s : 0.0, iq = Q.s > 0.0 ? 1.0 / Q.s : 0.0;
+
+        // ---- the children's probabilities
+        if (!greedy && tid < (uint32_t)n && tid > cur && parent[tid] == (int32_t)cur && (uint32_t)token[tid] < p.vocab) {
+            child_p[tid] = P.m == -INFINITY ? 0.0 : mass64(one_logit(prow, token[tid]), P.m, tau) * ip;
+            child_q[tid] = !sampled || Q.m == -INFINITY ? 0.0 : mass64(one_logit(qrow, token[tid]), Q.m, tau) * iq;
+        }
+        if (tid == 0) s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
+        __syncthreads();
+
+        // The residual times P.s: without a refusal its terms are the f32 masses themselves, whose f64 sums are exact
+        // as a rule, so that equal masses meet a border where they should.
+        auto residual = [&](float (&x)[8], float (&y)[8], int64_t j, double a, uint32_t ngone, double (&w)[8]) {
+            const double k = a * iq * P.s;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = P.m == -INFINITY ? 0.0 : (double)mass(x[i], P.m, it);
+                if (a != 0.0 && Q.m != -INFINITY) w[i] = fmax(w[i] - k * (double)mass(y[i], Q.m, it), 0.0);
+            }
+            for (uint32_t g = 0; g < ngone; ++g) {
+                const int64_t d = (int64_t)gone[g] - j;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d == i) w[i] = 0.0;
+            }
+        };
+        // Its sum over the vocabulary; every warp's share stays in wtot, every CTA's in the slots.
+        uint32_t last_turn = 0;
+        auto residual_pass = [&](double a, uint32_t ngone) -> double {
+            double sum = 0.0;
+            for (uint32_t c = c0; c < c1; ++c) {
+                const int64_t j = (int64_t)c * 256 + j_lane;
+                float x[8], y[8];
+                double w[8];
+                load8(prow, j, p.vocab, x);
+                if (a != 0.0) load8(qrow, j, p.vocab, y);
+                residual(x, y, j, a, ngone, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += w[i];
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            __syncthreads();                                             // wtot of the pass before is read
+            if (lane == 0) wtot[warp] = sum;
+            __syncthreads();
+            if (tid < ranks) {
+                double t = 0.0;
+                for (uint32_t w = 0; w < kVWarps; ++w) t += wtot[w];
+                cluster.map_shared_rank(&slots[turn][rank], tid)->total = t;
+            }
+            cluster.sync();
+            double t = 0.0;
+            for (uint32_t r = 0; r < ranks; ++r) t += slots[turn][r].total;
+            last_turn = turn;
+            turn ^= 1;
+            return t;
+        };
+
+        // ---- the children, one after the other
+        constexpr uint32_t kFinish = 0, kAccept = 1, kRefused = 2;
+        bool passed = false;                                             // wtot holds the residual of (s_a, 0 gone)
+        double last_sum = 0.0;
+        uint32_t action;
+        for (;;) {
+            if (tid == 0) {
+                uint32_t c = s_child, act = kFinish;
+                for (; c < (uint32_t)n; ++c) {
+                    if (parent[c] != (int32_t)cur || (uint32_t)token[c] >= p.vocab) continue;
+                    const double u = uni[c];
+                    if (greedy) {
+                        if (best && (uint32_t)token[c] == ~(uint32_t)best) { act = kAccept; break; }
+                    } else if (sampled) {
+                        if (u * child_q[c] * s_z < fmax(child_p[c] - s_a * child_q[c], 0.0)) { act = kAccept; break; }
+                        s_a += s_z;
+                        act = kRefused;
+                        break;
+                    } else {
+                        bool before = false;
+                        for (uint32_t g = 0; g < s_gone; ++g) before |= gone[g] == (uint32_t)token[c];
+                        if (before) continue;
+                        if (u * s_z < child_p[c]) { act = kAccept; break; }
+                        s_z -= child_p[c];
+                        gone[s_gone++] = token[c];
+                    }
+                }
+                s_action = act;
+                s_child = c;
+            }
+            __syncthreads();
+            action = s_action;
+            if (action != kRefused) break;
+            last_sum = residual_pass(s_a, 0);
+            passed = true;
+            __syncthreads();
+            if (tid == 0) s_z = last_sum * ip, s_child += 1;
+            __syncthreads();
+        }
+        if (action == kAccept) {
+            cur = s_child;
+            if (rank == 0 && tid == 0) p.path[first + count] = (int32_t)cur;
+            ++count;
+            __syncthreads();
+            continue;
+        }
+
+        // ---- the last token
+        if (rank == 0 && tid == 0) p.path_len[b] = (int32_t)count;
+        if (greedy) {
+            if (rank == 0 && tid == 0) p.next_token[b] = best ? (int32_t)~(uint32_t)best : -1;
+            break;
+        }
+        double a = s_a;
+        uint32_t ngone = s_gone;
+        if (!passed) last_sum = residual_pass(a, ngone);
+        double z = last_sum;
+        if (!(z > 0.0) && (a != 0.0 || ngone)) a = 0.0, ngone = 0, z = residual_pass(0.0, 0);   // nothing is left of p: p itself
+        if (!(z > 0.0)) {
+            if (rank == 0 && tid == 0) p.next_token[b] = -1;             // the row is empty
+            break;
+        }
+        const double border = (double)uni[0] * z;
+        double base = 0.0;
+        uint32_t owner = ranks;
+        for (uint32_t r = 0; r < ranks; ++r) {
+            const double t = slots[last_turn][r].total;
+            if (base + t > border) { owner = r; break; }
+            base += t;
+        }
+        if (owner == ranks) {                                            // a uniform of 1 or more: the last entry with mass
+            base = 0.0;
+            for (uint32_t r = 0; r < ranks; ++r)
+                if (slots[last_turn][r].total > 0.0) owner = r;
+        }
+        if (owner == rank) {
+            uint32_t who = kVWarps;
+            for (uint32_t w = 0; w < kVWarps; ++w) {
+                if (base + wtot[w] > border) { who = w; break; }
+                base += wtot[w];
+            }
+            if (who == kVWarps)
+                for (uint32_t w = 0; w < kVWarps; ++w)
+                    if (wtot[w] > 0.0) who = w;
+            if (who == warp) {
+                uint32_t found = kNoToken, last = kNoToken;
+                for (uint32_t c = c0; c < c1 && found == kNoToken; ++c) {
+                    const int64_t j = (int64_t)c * 256 + j_lane;
+                    float x[8], y[8];
+                    double w[8], sum = 0.0;
+                    load8(prow, j, p.vocab, x);
+                    if (a != 0.0) load8(qrow, j, p.vocab, y);
+                    residual(x, y, j, a, ngone, w);
+                    uint32_t mine = kNoToken, top = kNoToken;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        sum += w[i];
+                        if (w[i] > 0.0) top = (uint32_t)(j + i);
+                    }
+                    double incl = sum;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= (uint32_t)o) incl += t;
+                    }
+                    double run = base + incl - sum;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        run += w[i];
+                        if (mine == kNoToken && run > border && w[i] > 0.0) mine = (uint32_t)(j + i);
+                    }
+                    const uint32_t hits = __ballot_sync(0xffffffffu, mine != kNoToken);
+                    if (hits) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
+                    const uint32_t some = __ballot_sync(0xffffffffu, top != kNoToken);
+                    if (some) last = __shfl_sync(0xffffffffu, top, 31 - __clz(some));
+                    base += __shfl_sync(0xffffffffu, incl, 31);
+                }
+                if (lane == 0) p.next_token[b] = (int32_t)(found != kNoToken ? found : last);
+            }
+        }
+        break;
+    }
+    cluster.sync();                                                      // nobody leaves while others may still write its slots
+}
+
+template <typename T>
+cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl, cudaStream_t s) {
+    auto fn = verify_kernel<T>;
+    static DeviceOnce once;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (once.needs(dev)) {
+        if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        once.mark(dev);
+    }
+    // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
+    uint32_t ranks = kMaxCluster;
+    while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(batch * ranks);
+    cfg.blockDim = dim3(kVThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = use_pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+}  // namespace
+
+cudaError_t launch_verify_draft(const lq4_verify_args& a, int32_t* status, int sm_count, int use_pdl, cudaStream_t s) {
+    VerifyParams p{};
+    p.target = a.target_logits;
+    p.draft = a.draft_logits;
+    p.target_batch = a.target_batch, p.target_node = a.target_node;
+    p.draft_batch = a.draft_batch, p.draft_node = a.draft_node;
+    p.nodes = a.nodes;
+    p.vocab = a.vocab;
+    p.tokens = a.tokens;
+    p.parents = a.parents;
+    p.node_counts = a.node_counts;
+    p.uniforms = a.uniforms;
+    p.temperature = a.temperature;
+    p.path = a.path;
+    p.path_len = a.path_len;
+    p.next_token = a.next_token;
+    p.status = status;
+    return a.dtype == LQ4_DTYPE_F32 ? run<float>(p, a.batch, sm_count, use_pdl, s) : run<uint16_t>(p, a.batch, sm_count, use_pdl, s);
+}
+
+}  // namespace lq4

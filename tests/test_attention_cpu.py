@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from lattice_b200 import KvCache, Lq4Error, RopeTable, _lib, build as lq4_build, rope_frequencies
-from lattice_b200._lib import KvAppendArgs, KvCacheDesc, RopeArgs, RopeDesc, RopePart, RopeScaling, TreeAttentionArgs
+from lattice_b200._lib import KvAppendArgs, KvCacheDesc, RopeArgs, RopeDesc, RopePart, RopeScaling, TreeAttentionArgs, VerifyArgs
 
 
 @pytest.fixture(scope="module")
@@ -198,3 +198,24 @@ def test_attention_refusals(L, change, status):
     a = attend_args(**change)
     assert L.lq4_tree_attention(None, C.byref(a), None) == status
     assert L.lq4_tree_attention(None, None, None) == _lib.ERR_NULL
+
+
+def verify_args(**change):
+    fields = dict(target_logits=P, draft_logits=P, dtype=0, batch=2, nodes=4, vocab=100, target_batch=400, target_node=100, draft_batch=400,
+                  draft_node=100, tokens=P, parents=P, node_counts=P, uniforms=P, temperature=P, path=P, path_len=P, next_token=P)
+    fields.update(change)
+    return VerifyArgs(**fields)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(), _lib.ERR_NULL), (dict(dtype=2), _lib.ERR_DTYPE), (dict(nodes=0), _lib.ERR_SHAPE), (dict(nodes=65), _lib.ERR_SHAPE),
+    (dict(vocab=0), _lib.ERR_SHAPE), (dict(vocab=1 << 30), _lib.ERR_OVERFLOW), (dict(batch=1 << 26), _lib.ERR_OVERFLOW),
+    (dict(target_batch=1 << 60), _lib.ERR_OVERFLOW), (dict(draft_node=1 << 53), _lib.ERR_OVERFLOW),
+    (dict(target_logits=None), _lib.ERR_NULL), (dict(tokens=None), _lib.ERR_NULL), (dict(uniforms=None), _lib.ERR_NULL), (dict(path=None), _lib.ERR_NULL),
+    (dict(path_len=None), _lib.ERR_NULL), (dict(next_token=None), _lib.ERR_NULL), (dict(target_logits=P + 2), _lib.ERR_ALIGN),
+    (dict(draft_logits=P + 1, dtype=1), _lib.ERR_ALIGN), (dict(uniforms=P + 2), _lib.ERR_ALIGN), (dict(path=P + 1), _lib.ERR_ALIGN),
+])
+def test_verify_refusals(L, change, status):
+    a = verify_args(**change)
+    assert L.lq4_verify_draft(None, C.byref(a), None) == status
+    assert L.lq4_verify_draft(None, None, None) == _lib.ERR_NULL

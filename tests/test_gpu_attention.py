@@ -1,5 +1,7 @@
 """Rotary positions, cache append, tree attention and draft verification on the GPU, against plain 64-bit implementations."""
+import itertools
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -475,3 +477,199 @@ def test_attention_python_refusals(be):
         a.update(bad)
         with pytest.raises((ValueError, TypeError)):
             be.tree_attention(a.pop("q"), a.pop("k"), a.pop("v"), cache, a.pop("kv_lens"), **a)
+
+
+# ---- verification of drafted tokens --------------------------------------------------------------------------------
+
+def distribution(logits, tau):
+    """softmax(logits / tau) in 64 bits; NaN and -inf carry nothing, +inf takes all; None for a row without mass."""
+    x = np.where(np.isnan(logits), -np.inf, logits.astype(np.float64))
+    m = x.max()
+    if m == -np.inf:
+        return None
+    w = (x == m).astype(np.float64) if m == np.inf else np.exp((x - m) / tau)
+    return w / w.sum()
+
+
+def verify_ref(target, draft, tokens, parents, n, uniforms, tau):
+    """One sequence by the definition: residual distributions as vectors, renormalised after every refusal."""
+    nodes, vocab = target.shape
+    if n <= 0:
+        return [-1] * nodes, 0, -1
+    path, cur = [0], 0
+    while True:
+        children = [c for c in range(cur + 1, n) if (parents[c] if parents is not None else c - 1) == cur]
+        if tau < 1e-20:
+            x = np.where(np.isnan(target[cur]), -np.inf, target[cur])
+            best = int(np.argmax(x)) if x.max() > -np.inf else -1
+            step = next((c for c in children if tokens[c] == best and best >= 0), None)
+        else:
+            p = distribution(target[cur], tau)
+            q = distribution(draft[cur], tau) if draft is not None else None
+            left, step = (p if p is not None else np.zeros(vocab)), None
+            gone = set()
+            for c in children:
+                t = int(tokens[c])
+                if not 0 <= t < vocab:
+                    continue
+                u = float(uniforms[c])
+                if draft is not None:
+                    qt = q[t] if q is not None else 0.0
+                    if u * qt < left[t]:
+                        step = c
+                        break
+                    left = np.maximum(left - q, 0) if q is not None else left
+                    left = left / left.sum() if left.sum() > 0 else left
+                else:
+                    if t in gone:
+                        continue
+                    if u < left[t]:
+                        step = c
+                        break
+                    gone.add(t)
+                    left = left.copy()
+                    left[t] = 0
+                    left = left / left.sum() if left.sum() > 0 else left
+        if step is None:
+            break
+        path.append(step)
+        cur = step
+    if tau < 1e-20:
+        token = best
+    elif p is None:
+        token = -1
+    else:
+        left = left if left.sum() > 0 else p
+        if vocab <= 1000:                                                        # sums without rounding: equal masses can meet a border exactly
+            total = np.array(list(itertools.accumulate(Fraction(x) for x in left.tolist())))
+            border = Fraction(float(uniforms[0])) * total[-1]
+        else:
+            total = np.cumsum(left)
+            border = float(uniforms[0]) * total[-1]
+        over = np.nonzero(total > border)[0]
+        token = int(over[0]) if len(over) else int(np.nonzero(left)[0][-1])
+    return path + [-1] * (nodes - len(path)), len(path), token
+
+
+def check_verify(be, target, draft, tokens, parents, counts, uniforms, tau):
+    gpu = lambda x: None if x is None else x.cuda()  # noqa: E731
+    got = be.verify_draft(gpu(target), gpu(tokens), gpu(uniforms), draft_logits=gpu(draft), parents=gpu(parents), node_counts=gpu(counts), temperature=gpu(tau))
+    path, count, token = (x.cpu().numpy() for x in got)
+    for b in range(target.shape[0]):
+        ref = verify_ref(target[b].float().numpy(), None if draft is None else draft[b].float().numpy(), tokens[b].numpy(),
+                         None if parents is None else parents[b].numpy(), target.shape[1] if counts is None else int(counts[b]),
+                         uniforms[b].numpy(), 1.0 if tau is None else float(tau[b]))
+        assert path[b].tolist() == ref[0] and count[b] == ref[1] and token[b] == ref[2], (b, path[b].tolist(), int(count[b]), int(token[b]), ref)
+    be.check_device_status()
+    return path, count, token
+
+
+def verify_inputs(seed, batch, nodes, vocab, dtype, sampled, width=3, spread=2.0):
+    g = rng(seed)
+    target = (spread * torch.randn(batch, nodes, vocab, generator=g)).to(dtype)
+    draft = (target.float() + 0.7 * torch.randn(batch, nodes, vocab, generator=g)).to(dtype)
+    at = torch.arange(nodes)
+    parents = (at - 1 - (torch.rand(batch, nodes, generator=g) * at.clamp(max=width)).long()).clamp(min=-1).to(torch.int32)
+    of_parent = torch.take_along_dim(draft.float(), parents.clamp(min=0).long()[..., None], 1)
+    noise = -torch.log(-torch.log(torch.rand(batch, nodes, vocab, generator=g).clamp(1e-30, 1 - 1e-7)))
+    tokens = (of_parent + noise).argmax(-1).to(torch.int32)
+    return target, draft if sampled else None, tokens, parents, torch.rand(batch, nodes, generator=g)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 255, 256, 257, 4099, 50001])
+def test_verify_vocabularies(be, vocab, dtype, sampled):
+    target, draft, tokens, parents, u = verify_inputs(vocab, 9, 7, vocab, dtype, sampled)
+    tau = torch.tensor([0.0, 1.0, 0.5, 2.0, 1e-3, 1e-30, 1.0, 0.7, 0.7])
+    check_verify(be, target, draft, tokens, parents, None, u, tau)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("nodes, width", [(1, 1), (2, 1), (5, 1), (17, 4), (64, 8), (64, 63)])
+def test_verify_trees(be, nodes, width, sampled):
+    """Chains, trees and a star; few distinct tokens, so that siblings repeat one another; dead nodes."""
+    target, draft, tokens, parents, u = verify_inputs(200 + nodes + width, 60, nodes, 23, F32, sampled, width)
+    counts = torch.randint(0, nodes + 1, (60,), generator=rng(3), dtype=torch.int32)
+    counts[:30] = nodes
+    path, count, _ = check_verify(be, target, draft, tokens, parents if width > 1 else None, counts, u, None)
+    if nodes > 4:
+        assert count.max() >= 3                                                  # the walk goes deep in some of them
+
+
+def test_verify_large_batch_and_full_vocabulary(be):
+    target, draft, tokens, parents, u = verify_inputs(4, 300, 4, 1000, BF16, True)
+    check_verify(be, target, draft, tokens, parents, None, u, None)
+    target, draft, tokens, parents, u = verify_inputs(5, 2, 6, 248320, F32, True)
+    check_verify(be, target, draft, tokens, parents, None, u, torch.tensor([0.9, 0.0]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_verify_strange_rows(be, dtype):
+    """Masked, infinite, NaN and empty rows; uniforms at the borders; tokens and parents out of range."""
+    inf, nan = math.inf, math.nan
+    target = torch.zeros(12, 3, 300).to(dtype)
+    draft = torch.zeros(12, 3, 300).to(dtype)
+    tokens = torch.full((12, 3), 5, dtype=torch.int32)
+    u = torch.full((12, 3), 0.25)
+    parents = torch.tensor([[-1, 0, 1]] * 12, dtype=torch.int32)
+    target[0] = -inf                                                             # no mass: nothing accepted, token -1
+    target[1, :, :299] = -inf                                                    # one entry has it all
+    target[2, :, 7] = inf
+    target[3, :, 100:] = nan
+    draft[4] = -inf                                                              # a draft without mass: 0 < p accepts
+    target[5, :, 5] = -inf                                                       # the drafted token is masked out
+    draft[6, :, 5] = inf
+    tokens[7] = -3
+    tokens[8] = 300
+    parents[9] = torch.tensor([5, 1, 7])                                         # no children of node 0
+    u[10] = 0.0                                                                  # accepts; the first entry with mass
+    target[10, :, :9] = -inf
+    target[10, :, 5] = 0.0
+    u[11] = 1.0 - 2.0 ** -24                                                     # the last one
+    draft[11, :, 5] = 3.0
+    for d in (draft, None):
+        check_verify(be, target, d, tokens, parents, None, u, None)
+        check_verify(be, target, d, tokens, parents, None, u, torch.zeros(12))
+
+
+def test_verify_strides_and_same_again(be):
+    wide = (2 * torch.randn(3, 5, 2, 77, generator=rng(8))).cuda()
+    target, draft = wide[:, :, 0, 3:70], wide[:, :, 1, 3:70]
+    tokens = torch.randint(0, 67, (3, 5), generator=rng(9), dtype=torch.int32)
+    u = torch.rand(3, 5, generator=rng(10))
+    a = be.verify_draft(target, tokens.cuda(), u.cuda(), draft_logits=draft)
+    b = be.verify_draft(target.contiguous(), tokens.cuda(), u.cuda(), draft_logits=draft.contiguous())
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    check_verify(be, target.cpu().contiguous(), draft.cpu().contiguous(), tokens, None, None, u, None)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+def test_verify_keeps_the_targets_distribution(be, sampled):
+    """The first token that a verification emits is distributed as the target says, whatever was drafted."""
+    n, vocab = 60000, 6
+    g = rng(11)
+    target, draft = torch.randn(3, vocab, generator=g), torch.randn(3, vocab, generator=g)
+    q = torch.softmax(draft[0], -1)
+    tokens = torch.multinomial(q, 3 * n, True, generator=g).view(n, 3).to(torch.int32)   # nodes 1 and 2: siblings
+    parents = torch.tensor([[-1, 0, 0]] * n, dtype=torch.int32)
+    u = torch.rand(n, 3, generator=g)
+    path, count, token = be.verify_draft(target.expand(n, 3, vocab).cuda(), tokens.cuda(), u.cuda(), parents=parents.cuda(),
+                                         draft_logits=draft.expand(n, 3, vocab).cuda() if sampled else None)
+    path, count, token = path.cpu().long(), count.cpu(), token.cpu()
+    first = torch.where(count > 1, torch.gather(tokens, 1, path[:, 1:2].clamp(min=0))[:, 0], token)
+    seen = torch.bincount(first, minlength=vocab).double() / n
+    p = torch.softmax(target[0].double(), -1)
+    assert bool(((seen - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all())        # five standard deviations of a frequency
+    assert 0 < int((count > 1).sum()) < n
+
+
+def test_verify_refusals(be):
+    target, draft, tokens, parents, u = (x.cuda() for x in verify_inputs(12, 2, 3, 50, F32, True))
+    for bad in (dict(draft_logits=draft.bfloat16()), dict(draft_logits=draft[:1]), dict(tokens=tokens.long()), dict(uniforms=u.double()), dict(uniforms=u[:1]),
+                dict(parents=parents[:, :2]), dict(temperature=u), dict(target_logits=target.half()), dict(target_logits=target.cpu())):
+        a = dict(target_logits=target, tokens=tokens, uniforms=u)
+        a.update(bad)
+        with pytest.raises((ValueError, TypeError)):
+            be.verify_draft(a.pop("target_logits"), a.pop("tokens"), a.pop("uniforms"), **a)
