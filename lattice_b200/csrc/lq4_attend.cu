@@ -25,86 +25,13 @@
 // A key that a row may not see contributes nothing whatever it holds: its score is replaced by -inf, and a
 // non-finite V entry of a node (0 * inf would reach the rows that do not see it) is cleared in shared memory
 // and added back at the end for the rows that do see it.
-#include "lq4_attend.cuh"
-
-#include <cuda_bf16.h>
+#include "lq4_attend_dev.cuh"
 
 #include <atomic>
 
 namespace lq4 {
 
 namespace {
-
-constexpr uint32_t kKeys = 64;                 // keys per tile
-constexpr uint32_t kMaxNodes = LQ4_MAX_TREE_NODES;
-constexpr uint32_t kMinShare = 1;              // tiles a CTA takes at least
-
-struct AttendParams {
-    CacheView c;
-    const void* q;
-    void* out;
-    const uint16_t* k;                         // the nodes' own rows
-    const uint16_t* v;
-    uint64_t q_batch, q_node, q_head, out_batch, out_node, out_head, kv_batch, kv_node, kv_head;
-    const int32_t* kv_lens;
-    const int32_t* node_counts;
-    const int32_t* parents;
-    uint32_t batch, nodes, group, kv_heads, head_dim, row_tiles;
-    float scale_log2;                          // scale * log2(e)
-    float* part_o;                             // [2 * grid][BM][D]
-    float2* part_ml;                           // [2 * grid][BM] (max, sum)
-    uint32_t grid;
-    int32_t* status;
-};
-
-// What the lengths of sequence b come to: committed keys, live nodes, tiles.
-struct Seq {
-    int32_t len, nodes;
-    uint32_t tiles;                            // key tiles of an item, the nodes' own tile last; 0: nothing to do
-    bool bad;
-};
-__device__ __forceinline__ Seq sequence(const AttendParams& p, uint32_t b) {
-    Seq s;
-    s.len = p.kv_lens[b];
-    s.nodes = p.node_counts ? p.node_counts[b] : (int32_t)p.nodes;
-    s.bad = false;
-    const int64_t cap = (int64_t)p.c.max_pages * p.c.page_size;
-    if (s.len > cap) s.len = (int32_t)cap, s.bad = true;
-    if (s.nodes > (int32_t)p.nodes) s.nodes = (int32_t)p.nodes, s.bad = true;
-    s.tiles = (s.len < 0 || s.nodes <= 0) ? 0 : ((uint32_t)s.len + kKeys - 1) / kKeys + 1;
-    return s;
-}
-
-// Units (tiles of all items) before sequence b and in all, by one warp.
-__device__ __forceinline__ void warp_prefix(const AttendParams& p, uint32_t b, uint64_t& before, uint64_t& total) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint64_t x = 0, y = 0;
-    for (uint32_t i = lane; i < p.batch; i += 32) {
-        const uint64_t t = sequence(p, i).tiles;
-        y += t;
-        if (i < b) x += t;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-    }
-    const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
-    before = x * items;
-    total = y * items;
-}
-
-__device__ __forceinline__ uint64_t cta_share(uint64_t total, uint32_t grid) {
-    const uint64_t per = (total + grid - 1) / grid;
-    return per < kMinShare ? kMinShare : per;
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -116,11 +43,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // (a, b) -> one word of bf16 and what the rounding left of each.
 __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
@@ -134,6 +56,9 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
 // with the row's, so that eight rows of one chunk (an ldmatrix) lie in eight different bank groups.
 template <int D>
 __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t c) { return r * (D * 2) + ((c ^ (r & 7)) << 4); }
+
+// From this many rows per kv head on bf16 activations take the tcgen05 kernel.
+constexpr uint32_t kTcMinRows = 48;
 
 template <int D, int WM, int NQ>
 struct Shape {
@@ -165,119 +90,53 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
 
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    // this CTA's units, and the sequence the first of them lies in
     const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
-    uint64_t u, u_end, seq_first;
-    uint32_t b;
-    {
-        uint64_t* wsum = ctl + 2;                                        // (WM * WN <= 8 warps: 8 words would do; 4 used per half)
-        const uint32_t per = (p.batch + NT - 1) / NT, i0 = tid * per, i1 = min(i0 + per, p.batch);
-        uint64_t mine = 0;
-        for (uint32_t i = i0; i < i1; ++i) mine += sequence(p, i).tiles;
-        uint64_t incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= (uint32_t)o) incl += t;
-        }
-        uint64_t* wtot = reinterpret_cast<uint64_t*>(ml);                // one word per warp (ml is free here)
-        if (lane == 31) wtot[warp] = incl;
-        __syncthreads();
-        uint64_t before = incl - mine, total = 0;
-        for (uint32_t w = 0; w < (uint32_t)(WM * WN); ++w) {
-            if (w < warp) before += wtot[w];
-            total += wtot[w];
-        }
-        total *= items;
-        const uint64_t share = cta_share(total, p.grid);
-        u = (uint64_t)blockIdx.x * share;
-        u_end = min(u + share, total);
-        if (u >= u_end) return;                                          // (uniform over the CTA)
-        if (u >= before * items && u < (before + mine) * items) {
-            uint32_t i = i0;
-            for (; i < i1; ++i) {
-                const uint64_t t = sequence(p, i).tiles;
-                if (u < (before + t) * items) break;
-                before += t;
-            }
-            wsum[0] = i;
-            wsum[1] = before * items;
-        }
-        __syncthreads();
-        b = (uint32_t)wsum[0];
-        seq_first = wsum[1];
-    }
+    const Range range = cta_range<NT>(p, ctl, reinterpret_cast<uint64_t*>(ml));
+    uint64_t u = range.begin, seq_first = range.seq_first;
+    const uint64_t u_end = range.end;
+    uint32_t b = range.seq;
 
     while (u < u_end) {
-        Seq sq = sequence(p, b);
-        if (sq.tiles == 0 || u >= seq_first + sq.tiles * items) {        // on to the next sequence
-            seq_first += sq.tiles * items;
-            ++b;
-            continue;
-        }
-        const uint32_t in_seq_item = (uint32_t)((u - seq_first) / sq.tiles);
-        const uint32_t t0 = (uint32_t)((u - seq_first) - (uint64_t)in_seq_item * sq.tiles);
-        const uint32_t h = in_seq_item / p.row_tiles, rt = in_seq_item - h * p.row_tiles;
-        const uint32_t n_tiles = (uint32_t)min((uint64_t)(sq.tiles - t0), u_end - u);
-        const bool has_nodes = t0 + n_tiles == sq.tiles;                 // this piece ends with the nodes' own tile
+        const Piece x = next_piece(p, u, u_end, b, seq_first);
+        const Seq& sq = x.sq;
+        const uint32_t h = x.h, rt = x.rt, t0 = x.t0, n_tiles = x.n_tiles;
         const uint32_t rows = p.nodes * p.group;
         if (sq.bad && tid == 0) atomicOr(p.status, kDevErrBadIndex);
 
         // q -> NQ bf16 terms in shared memory (rows behind the last one are zero)
         for (uint32_t i = tid; i < BM * (D / 2); i += NT) {
             const uint32_t r = i / (D / 2), d = (i - r * (D / 2)) * 2, row = rt * BM + r;
-            float x = 0.0f, y = 0.0f;
+            float q0 = 0.0f, q1 = 0.0f;
             if (row < rows && d < p.head_dim) {
                 const uint32_t t = row / p.group, g = row - t * p.group;
                 if ((int32_t)t < sq.nodes) {
                     const uint64_t at = b * p.q_batch + t * p.q_node + (uint64_t)(h * p.group + g) * p.q_head + d;
                     if constexpr (NQ == 1) {
-                        x = bf16_to_f32(static_cast<const uint16_t*>(p.q)[at]);
-                        y = bf16_to_f32(static_cast<const uint16_t*>(p.q)[at + 1]);
+                        q0 = bf16_to_f32(static_cast<const uint16_t*>(p.q)[at]);
+                        q1 = bf16_to_f32(static_cast<const uint16_t*>(p.q)[at + 1]);
                     } else {
-                        x = static_cast<const float*>(p.q)[at];
-                        y = static_cast<const float*>(p.q)[at + 1];
+                        q0 = static_cast<const float*>(p.q)[at];
+                        q1 = static_cast<const float*>(p.q)[at + 1];
                     }
                 }
             }
+            q0 *= p.q_sign;
+            q1 *= p.q_sign;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                const uint32_t w = split_pair(x, y);
+                const uint32_t w = split_pair(q0, q1);
                 *reinterpret_cast<uint32_t*>(smem + ST * S::kStage + n * (BM * D * 2) + tile_at<D>(r, d >> 3) + (d & 7) * 2) = w;
             }
         }
-        if (has_nodes && tid < p.nodes) {
-            uint64_t path = 0;
-            int32_t at = (int32_t)tid;
+        if (x.has_nodes && tid < p.nodes) {
             bool bad = false;
-            while (at >= 0) {
-                path |= 1ull << at;
-                int32_t up = p.parents ? p.parents[(uint64_t)b * p.nodes + at] : at - 1;
-                if (up < -1 || up >= at) up = -1, bad = (int32_t)tid < sq.nodes;   // a parent comes before its children
-                at = up;
-            }
-            anc[tid] = path;
-            if (bad) atomicOr(p.status, kDevErrBadIndex);
+            anc[tid] = node_path(p, b, tid, bad);
+            if (bad && (int32_t)tid < sq.nodes) atomicOr(p.status, kDevErrBadIndex);
         }
 
         // where the keys of tile `i` of this piece lie; page ids come from memory, so this runs a stage ahead
-        auto key_page = [&](uint32_t i) -> int32_t {                     // (threads 0..63)
-            const uint32_t key = (t0 + i) * kKeys + tid;
-            if (i >= n_tiles || t0 + i + 1 == sq.tiles || key >= (uint32_t)sq.len) return -1;
-            return p.c.table[(uint64_t)b * p.c.max_pages + key / p.c.page_size];
-        };
-        auto put_keys = [&](uint32_t i, int32_t page) {
-            const uint32_t key = (t0 + i) * kKeys + tid;
-            uint64_t at = ~0ull;
-            if (i >= n_tiles) {                                          // (belongs to the next CTA)
-            } else if (t0 + i + 1 == sq.tiles) {
-                if ((int32_t)tid < sq.nodes) at = b * p.kv_batch + tid * p.kv_node + h * p.kv_head;
-            } else if (key < (uint32_t)sq.len) {
-                if (page < 0 || (uint32_t)page >= p.c.pages)
-                    atomicOr(p.status, kDevErrBadIndex);
-                else
-                    at = (uint64_t)page * p.c.page_stride + (uint64_t)(key % p.c.page_size) * p.c.slot_stride + h * p.c.head_stride;
-            }
+        auto put_keys = [&](uint32_t i, int32_t page) {                  // (threads 0..63)
+            const uint64_t at = key_offset(p, x, i, tid, page);
             offs[(i % ST) * kKeys + tid] = at;
             const uint32_t bits = __ballot_sync(0xffffffffu, at != ~0ull);
             if (lane == 0) reinterpret_cast<uint32_t*>(valid + (i & 7))[warp] = bits;
@@ -303,7 +162,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
         if (tid < kKeys) {
             int32_t page[ST];
 #pragma unroll
-            for (int i = 0; i < ST; ++i) page[i] = key_page(i);
+            for (int i = 0; i < ST; ++i) page[i] = key_page(p, x, i, tid);
 #pragma unroll
             for (int i = 0; i < ST; ++i) put_keys(i, page[i]);
         }
@@ -322,24 +181,14 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
             __syncthreads();                                             // tile i is here; everybody is done with tile i - 1
             load_tile(i + ST - 1);
             int32_t page = -1;
-            if (tid < kKeys) page = key_page(i + ST);
+            if (tid < kKeys) page = key_page(p, x, i + ST, tid);
             const uint32_t kst = sbase + (i % ST) * S::kStage, vst = kst + S::kTile;
             const bool own = t0 + i + 1 == sq.tiles;
             uint64_t see[2];
             see[0] = see[1] = valid[i & 7];
             if (own) {
                 bool odd = false;                                        // clear non-finite V entries of the nodes
-                for (uint32_t idx = tid; idx < kKeys * CPR; idx += NT) {
-                    uint4* w = reinterpret_cast<uint4*>(smem + (vst - sbase) + idx * 16);
-                    uint32_t x[4] = {w->x, w->y, w->z, w->w};
-                    bool hit = false;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, hit = true;
-                        if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, hit = true;
-                    }
-                    if (hit) *w = make_uint4(x[0], x[1], x[2], x[3]), odd = true;
-                }
+                for (uint32_t idx = tid; idx < kKeys * CPR; idx += NT) odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + (vst - sbase) + idx * 16));
                 fix = __syncthreads_or(odd);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -347,8 +196,11 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                     if (t < p.nodes) see[j] &= anc[t];
                 }
             }
-            // scores of this warp's keys
+            // scores of this warp's keys.  The tensor cores cut off what falls below their accumulator's last bit; with
+            // f32 activations the leading term's sum is therefore taken every 32 channels and added in f32.
             float s[NK / 8][4];
+#pragma unroll
+            for (int j = 0; j < NK / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
             {
                 float part[NQ][NK / 8][4];
 #pragma unroll
@@ -367,20 +219,23 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                         ldsm4(a, qbase + n * (BM * D * 2) + tile_at<D>(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
 #pragma unroll
                         for (int j = 0; j < NK / 16; ++j) {
-                            mma_bf16(part[n][2 * j], a, kf[j][0], kf[j][1]);
-                            mma_bf16(part[n][2 * j + 1], a, kf[j][2], kf[j][3]);
+                            mma_bf16(NQ == 1 ? s[2 * j] : part[n][2 * j], a, kf[j][0], kf[j][1]);
+                            mma_bf16(NQ == 1 ? s[2 * j + 1] : part[n][2 * j + 1], a, kf[j][2], kf[j][3]);
                         }
                     }
-                }
+                    if (NQ > 1 && (ks & 1)) {
 #pragma unroll
-                for (int j = 0; j < NK / 8; ++j)
+                        for (int j = 0; j < NK / 8; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = part[NQ - 1][j][e];
-#pragma unroll
-                        for (int n = NQ - 2; n >= 0; --n) x += part[n][j][e];
-                        s[j][e] = x * p.scale_log2;
+                            for (int e = 0; e < 4; ++e) s[j][e] += part[0][j][e], part[0][j][e] = 0.0f;
                     }
+                }
+                if constexpr (NQ > 1) {
+#pragma unroll
+                    for (int j = 0; j < NK / 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[j][e] += part[1][j][e] + part[2][j][e];
+                }
             }
             if ((see[0] & see[1]) != ~0ull) {
 #pragma unroll
@@ -389,21 +244,23 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                     for (int e = 0; e < 4; ++e)
                         if (!((see[e >> 1] >> (wn * NK + j * 8 + qc + (e & 1))) & 1)) s[j][e] = -INFINITY;
             }
-            // running maximum and sum
+            // Running maximum and sum, in units of log2.  The maximum is rounded once, to m; an exponent is one fused
+            // operation from the unscaled score, so its error goes with its distance from the maximum.
             float base[2], corr[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float x = m[r];
+                float top = s[0][2 * r];
 #pragma unroll
-                for (int j = 0; j < NK / 8; ++j) x = fmaxf(x, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                base[r] = x == -INFINITY ? 0.0f : x;
+                for (int j = 0; j < NK / 8; ++j) top = fmaxf(top, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                top = fmaxf(m[r], top * p.scale_log2);
+                base[r] = top == -INFINITY ? 0.0f : top;
                 corr[r] = exp2_fast(m[r] - base[r]);
-                m[r] = x;
+                m[r] = top;
                 l[r] *= corr[r];
             }
-            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+            if (NQ == 1 && __any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
 #pragma unroll
                 for (int d = 0; d < D / 8; ++d) {
                     o[d][0] *= corr[0];
@@ -416,25 +273,35 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
             for (int j = 0; j < NK / 8; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[j][e] = exp2_fast(s[j][e] - base[e >> 1]);
+                    s[j][e] = exp2_fast(fmaf(s[j][e], p.scale_log2, -base[e >> 1]));
                     l[e >> 1] += s[j][e];
                 }
-            // O += P V
+            // O = corr O + P V, the tile's product in accumulators of its own for f32 activations (as above)
+            uint32_t a[NK / 16][NQ][4];
 #pragma unroll
-            for (int j = 0; j < NK / 16; ++j) {
-                uint32_t a[NQ][4];
+            for (int j = 0; j < NK / 16; ++j)
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) a[n][w] = split_pair(s[2 * j + (w >> 1)][2 * (w & 1)], s[2 * j + (w >> 1)][2 * (w & 1) + 1]);
+                    for (int w = 0; w < 4; ++w) a[j][n][w] = split_pair(s[2 * j + (w >> 1)][2 * (w & 1)], s[2 * j + (w >> 1)][2 * (w & 1) + 1]);
 #pragma unroll
-                for (int dt = 0; dt < D / 16; ++dt) {
+            for (int dt = 0; dt < D / 16; ++dt) {
+                float t[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int j = 0; j < NK / 16; ++j) {
                     uint32_t vf[4];
                     ldsm4_t(vf, vst + tile_at<D>(wn * NK + j * 16 + (lane & 15), 2 * dt + (lane >> 4)));
 #pragma unroll
                     for (int n = NQ - 1; n >= 0; --n) {
-                        mma_bf16(o[2 * dt], a[n], vf[0], vf[1]);
-                        mma_bf16(o[2 * dt + 1], a[n], vf[2], vf[3]);
+                        mma_bf16(NQ == 1 ? o[2 * dt] : t[0], a[j][n], vf[0], vf[1]);
+                        mma_bf16(NQ == 1 ? o[2 * dt + 1] : t[1], a[j][n], vf[2], vf[3]);
+                    }
+                }
+                if constexpr (NQ > 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[2 * dt][e] = fmaf(o[2 * dt][e], corr[e >> 1], t[0][e]);
+                        o[2 * dt + 1][e] = fmaf(o[2 * dt + 1][e], corr[e >> 1], t[1][e]);
                     }
                 }
             }
@@ -463,7 +330,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                 *reinterpret_cast<float2*>(os + (wn * BM + row) * (D + 8) + d * 8 + qc) = make_float2(o[d][2 * r] * f, o[d][2 * r + 1] * f);
         }
         __syncthreads();
-        const bool whole = t0 == 0 && has_nodes;
+        const bool whole = t0 == 0 && x.has_nodes;
         const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
         for (uint32_t i = tid; i < BM * (D / 4); i += NT) {
             const uint32_t r = i / (D / 4), d = (i - r * (D / 4)) * 4, row = rt * BM + r;
@@ -473,33 +340,27 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
 #pragma unroll
             for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + r].x);
             const float safe = top == -INFINITY ? 0.0f : top;
-            float x[4] = {0, 0, 0, 0};
+            float y[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < WN; ++w) {
                 const float2 e = ml[w * BM + r];
                 sum += e.y * exp2_fast(e.x - safe);
-                const float4 y = *reinterpret_cast<const float4*>(os + (w * BM + r) * (D + 8) + d);
-                x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+                const float4 v = *reinterpret_cast<const float4*>(os + (w * BM + r) * (D + 8) + d);
+                y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
             }
-            if (fix) {
-                for (uint32_t j = 0; j < (uint32_t)sq.nodes; ++j)
-                    if ((anc[t] >> j) & 1)
-                        for (int e = 0; e < 4; ++e) {
-                            const float y = bf16_to_f32(p.v[b * p.kv_batch + j * p.kv_node + h * p.kv_head + d + e]);
-                            if (!isfinite(y)) x[e] += y;
-                        }
-            }
+            if (fix)
+                for (int e = 0; e < 4; ++e) y[e] += nonfinite_sum(p, x, anc[t], d + e);
             if (whole) {
                 const float inv = 1.0f / sum;
                 const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + d;
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (NQ == 1)
-                        static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(x[e] * inv);
+                        static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(y[e] * inv);
                     else
-                        static_cast<float*>(p.out)[at + e] = x[e] * inv;
+                        static_cast<float*>(p.out)[at + e] = y[e] * inv;
                 }
             } else {
-                *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(y[0], y[1], y[2], y[3]);
                 if (d == 0) p.part_ml[(uint64_t)slot * BM + r] = make_float2(top, sum);
             }
         }
@@ -509,8 +370,8 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
 }
 
 // Joins the partials of the items that a CTA border cut: one warp per row, the CTAs in order.
-template <int D, int BM>
-__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p, int bf16_out) {
+template <int D>
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p, uint32_t BM, int bf16_out) {
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t rows = p.nodes * p.group;
     const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -562,7 +423,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 }
 
 template <int D, int WM, int NQ>
-cudaError_t run(AttendParams p, const lq4_tree_attention_args& a, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
+cudaError_t run(AttendParams p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
     using S = Shape<D, WM, NQ>;
     static DeviceOnce once;
     auto fn = attend_kernel<D, WM, NQ>;
@@ -577,52 +438,35 @@ cudaError_t run(AttendParams p, const lq4_tree_attention_args& a, AttendWorkspac
     }
     p.grid = (uint32_t)(sm_count * per_sm);
     p.row_tiles = (p.nodes * p.group + S::BM - 1) / S::BM;
-    const size_t slots = (size_t)2 * p.grid * S::BM;
-    const size_t need = slots * (D * 4 + 8);
-    if (ws.bytes < need) {
-        ws.need = need;
-        return cudaSuccess;
-    }
-    p.part_ml = static_cast<float2*>(ws.p);
-    p.part_o = reinterpret_cast<float*>(p.part_ml + slots);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.grid);
-    cfg.blockDim = dim3(S::NT);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = use_pdl ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, fn, p);
-    if (e != cudaSuccess) return e;
-    const uint64_t warps = (uint64_t)p.batch * p.kv_heads * p.nodes * p.group;
-    cfg.gridDim = dim3((unsigned)((warps + 7) / 8));
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, attend_join_kernel<D, S::BM>, p, (int)(NQ == 1));
-    ws.launches = 2;
-    return e;
+    if (!attend_workspace(p, ws, S::BM, D)) return cudaSuccess;
+    if ((e = attend_launch(fn, dim3(p.grid), S::NT, S::kSmem, use_pdl, s, p)) != cudaSuccess) return e;
+    return launch_attend_join(p, S::BM, D, NQ == 1, ws, use_pdl, s);
 }
 
 template <int D, int NQ>
-cudaError_t run_rows(const AttendParams& p, const lq4_tree_attention_args& a, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
+cudaError_t run_rows(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
     // bands of 16 rows: as few as hold the rows of an item, at most four (more rows: several row tiles)
     const uint32_t rows = p.nodes * p.group;
-    if (rows <= 16) return run<D, 1, NQ>(p, a, ws, sm_count, use_pdl, s);
-    if (rows <= 32) return run<D, 2, NQ>(p, a, ws, sm_count, use_pdl, s);
-    return run<D, 4, NQ>(p, a, ws, sm_count, use_pdl, s);
+    if (rows <= 16) return run<D, 1, NQ>(p, ws, sm_count, use_pdl, s);
+    if (rows <= 32) return run<D, 2, NQ>(p, ws, sm_count, use_pdl, s);
+    return run<D, 4, NQ>(p, ws, sm_count, use_pdl, s);
 }
 
 template <int NQ>
-cudaError_t run_dim(const AttendParams& p, const lq4_tree_attention_args& a, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    if (p.head_dim <= 64) return run_rows<64, NQ>(p, a, ws, sm_count, use_pdl, s);
-    if (p.head_dim <= 128) return run_rows<128, NQ>(p, a, ws, sm_count, use_pdl, s);
-    return run_rows<256, NQ>(p, a, ws, sm_count, use_pdl, s);
+cudaError_t run_dim(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
+    if (p.head_dim <= 64) return run_rows<64, NQ>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 128) return run_rows<128, NQ>(p, ws, sm_count, use_pdl, s);
+    return run_rows<256, NQ>(p, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace
+
+cudaError_t launch_attend_join(const AttendParams& p, uint32_t rows, uint32_t D, bool bf16_out, AttendWorkspace& ws, int use_pdl, cudaStream_t s) {
+    const uint64_t warps = (uint64_t)p.batch * p.kv_heads * p.nodes * p.group;
+    auto fn = D == 64 ? attend_join_kernel<64> : D == 128 ? attend_join_kernel<128> : attend_join_kernel<256>;
+    ws.launches = 2;
+    return attend_launch(fn, dim3((unsigned)((warps + 7) / 8)), 256, 0, use_pdl, s, p, rows, (int)bf16_out);
+}
 
 cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorkspace& ws, int32_t* status, int sm_count, int use_pdl, cudaStream_t s) {
     AttendParams p{};
@@ -642,11 +486,17 @@ cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorksp
     p.kv_heads = a.cache->kv_heads;
     p.group = a.q_heads / a.cache->kv_heads;
     p.head_dim = a.cache->head_dim;
-    p.scale_log2 = a.scale * 1.44269504088896340736f;
+    // the scale's sign goes into q (a zero scale too), so that a larger product is a larger score
+    p.q_sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
+    p.scale_log2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
     p.status = status;
+    const uintptr_t q_at = reinterpret_cast<uintptr_t>(a.q), out_at = reinterpret_cast<uintptr_t>(a.out);
+    p.q_vec = !(q_at % 16 || a.q_batch % 8 || a.q_node % 8 || a.q_head % 8);
+    p.out_vec = !(out_at % 16 || a.out_batch % 8 || a.out_node % 8 || a.out_head % 8);
     ws.need = 0;
     ws.launches = 0;
-    return a.dtype == LQ4_DTYPE_BF16 ? run_dim<1>(p, a, ws, sm_count, use_pdl, s) : run_dim<3>(p, a, ws, sm_count, use_pdl, s);
+    if (a.dtype == LQ4_DTYPE_BF16 && p.nodes * p.group > kTcMinRows) return launch_attend_tc(p, ws, sm_count, use_pdl, s);
+    return a.dtype == LQ4_DTYPE_BF16 ? run_dim<1>(p, ws, sm_count, use_pdl, s) : run_dim<3>(p, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace lq4

@@ -1,0 +1,251 @@
+// What the kernels of lq4_tree_attention share: the lengths of the sequences, the cut of the work over the CTAs, small
+// wrappers.  Included by lq4_attend.cu and lq4_attend_tc.cu only.
+#pragma once
+
+#include "lq4_attend.cuh"
+
+#include <cuda_bf16.h>
+
+namespace lq4 {
+
+constexpr uint32_t kKeys = 64;                 // keys per tile
+constexpr uint32_t kMaxNodes = LQ4_MAX_TREE_NODES;
+constexpr uint32_t kMinShare = 1;              // tiles a CTA takes at least
+
+struct AttendParams {
+    CacheView c;
+    const void* q;
+    void* out;
+    const uint16_t* k;                         // the nodes' own rows
+    const uint16_t* v;
+    uint64_t q_batch, q_node, q_head, out_batch, out_node, out_head, kv_batch, kv_node, kv_head;
+    const int32_t* kv_lens;
+    const int32_t* node_counts;
+    const int32_t* parents;
+    uint32_t batch, nodes, group, kv_heads, head_dim, row_tiles;
+    float q_sign, scale_log2;                  // scale = q_sign * scale_log2 / log2(e), scale_log2 > 0
+    float* part_o;                             // [2 * grid][BM][D]
+    float2* part_ml;                           // [2 * grid][BM] (max, sum)
+    uint32_t grid;
+    int32_t* status;
+    bool q_vec, out_vec;                       // 16-byte accesses fit q / out
+};
+
+// What the lengths of sequence b come to: committed keys, live nodes, tiles.
+struct Seq {
+    int32_t len, nodes;
+    uint32_t tiles;                            // key tiles of an item, the nodes' own tile last; 0: nothing to do
+    bool bad;
+};
+__device__ __forceinline__ Seq sequence(const AttendParams& p, uint32_t b) {
+    Seq s;
+    s.len = p.kv_lens[b];
+    s.nodes = p.node_counts ? p.node_counts[b] : (int32_t)p.nodes;
+    s.bad = false;
+    const int64_t cap = (int64_t)p.c.max_pages * p.c.page_size;
+    if (s.len > cap) s.len = (int32_t)cap, s.bad = true;
+    if (s.nodes > (int32_t)p.nodes) s.nodes = (int32_t)p.nodes, s.bad = true;
+    s.tiles = (s.len < 0 || s.nodes <= 0) ? 0 : ((uint32_t)s.len + kKeys - 1) / kKeys + 1;
+    return s;
+}
+
+// Units (tiles of all items) before sequence b and in all, by one warp.
+__device__ __forceinline__ void warp_prefix(const AttendParams& p, uint32_t b, uint64_t& before, uint64_t& total) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint64_t x = 0, y = 0;
+    for (uint32_t i = lane; i < p.batch; i += 32) {
+        const uint64_t t = sequence(p, i).tiles;
+        y += t;
+        if (i < b) x += t;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
+    before = x * items;
+    total = y * items;
+}
+
+__device__ __forceinline__ uint64_t cta_share(uint64_t total, uint32_t grid) {
+    const uint64_t per = (total + grid - 1) / grid;
+    return per < kMinShare ? kMinShare : per;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// A CTA's share of the range of all tiles, and the sequence its first tile lies in.
+struct Range {
+    uint64_t begin, end;                       // units; empty: nothing to do
+    uint64_t seq_first;                        // unit that sequence `seq` starts at
+    uint32_t seq;
+};
+// Called by all NT threads; `word2` holds two words, `warp_words` one per warp of shared memory, free to overwrite
+// until the next barrier.
+template <int NT>
+__device__ __forceinline__ Range cta_range(const AttendParams& p, uint64_t* word2, uint64_t* warp_words) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
+    const uint32_t per = (p.batch + NT - 1) / NT, i0 = tid * per, i1 = min(i0 + per, p.batch);
+    uint64_t mine = 0;
+    for (uint32_t i = i0; i < i1; ++i) mine += sequence(p, i).tiles;
+    uint64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += t;
+    }
+    if (lane == 31) warp_words[warp] = incl;
+    __syncthreads();
+    uint64_t before = incl - mine, total = 0;
+    for (uint32_t w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += warp_words[w];
+        total += warp_words[w];
+    }
+    total *= items;
+    const uint64_t share = cta_share(total, p.grid);
+    Range r;
+    r.begin = min((uint64_t)blockIdx.x * share, total);
+    r.end = min(r.begin + share, total);
+    r.seq = 0;
+    r.seq_first = 0;
+    if (r.begin >= r.end) return r;                                      // (uniform over the CTA)
+    if (r.begin >= before * items && r.begin < (before + mine) * items) {
+        uint32_t i = i0;
+        for (; i < i1; ++i) {
+            const uint64_t t = sequence(p, i).tiles;
+            if (r.begin < (before + t) * items) break;
+            before += t;
+        }
+        word2[0] = i;
+        word2[1] = before * items;
+    }
+    __syncthreads();
+    r.seq = (uint32_t)word2[0];
+    r.seq_first = word2[1];
+    __syncthreads();
+    return r;
+}
+
+// One piece of a CTA's range: consecutive tiles of one item.
+struct Piece {
+    Seq sq;
+    uint32_t b, h, rt, t0, n_tiles;
+    bool has_nodes;                            // it ends with the nodes' own tile
+};
+// The piece that unit `u` starts; moves the sequence cursor (b, seq_first) on to it.
+__device__ __forceinline__ Piece next_piece(const AttendParams& p, uint64_t u, uint64_t u_end, uint32_t& b, uint64_t& seq_first) {
+    const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
+    Piece x;
+    x.sq = sequence(p, b);
+    while (u >= seq_first + x.sq.tiles * items) {                        // (u lies before the end of all units)
+        seq_first += x.sq.tiles * items;
+        x.sq = sequence(p, ++b);
+    }
+    const uint32_t item = (uint32_t)((u - seq_first) / x.sq.tiles);
+    x.t0 = (uint32_t)((u - seq_first) - (uint64_t)item * x.sq.tiles);
+    x.b = b;
+    x.h = item / p.row_tiles;
+    x.rt = item - x.h * p.row_tiles;
+    x.n_tiles = (uint32_t)min((uint64_t)(x.sq.tiles - x.t0), u_end - u);
+    x.has_nodes = x.t0 + x.n_tiles == x.sq.tiles;
+    return x;
+}
+
+// A node's path from the root, itself included, as a bit mask; a parent that does not come before its node counts as none.
+__device__ __forceinline__ uint64_t node_path(const AttendParams& p, uint32_t b, uint32_t node, bool& bad) {
+    uint64_t path = 0;
+    int32_t at = (int32_t)node;
+    while (at >= 0) {
+        path |= 1ull << at;
+        int32_t up = p.parents ? p.parents[(uint64_t)b * p.nodes + at] : at - 1;
+        if (up < -1 || up >= at) up = -1, bad = true;
+        at = up;
+    }
+    return path;
+}
+
+// Where key `tid` of a piece's tile `i` lies, in two steps, because the page id comes from memory.
+__device__ __forceinline__ int32_t key_page(const AttendParams& p, const Piece& x, uint32_t i, uint32_t tid) {
+    const uint32_t key = (x.t0 + i) * kKeys + tid;
+    if (i >= x.n_tiles || x.t0 + i + 1 == x.sq.tiles || key >= (uint32_t)x.sq.len) return -1;
+    return p.c.table[(uint64_t)x.b * p.c.max_pages + key / p.c.page_size];
+}
+// Element offset of the key's row in the cache (in k and v of the nodes for their own tile), ~0: there is none.
+__device__ __forceinline__ uint64_t key_offset(const AttendParams& p, const Piece& x, uint32_t i, uint32_t tid, int32_t page) {
+    const uint32_t key = (x.t0 + i) * kKeys + tid;
+    if (i >= x.n_tiles) return ~0ull;
+    if (x.t0 + i + 1 == x.sq.tiles) return (int32_t)tid < x.sq.nodes ? x.b * p.kv_batch + tid * p.kv_node + x.h * p.kv_head : ~0ull;
+    if (key >= (uint32_t)x.sq.len) return ~0ull;
+    if (page < 0 || (uint32_t)page >= p.c.pages) {
+        atomicOr(p.status, kDevErrBadIndex);
+        return ~0ull;
+    }
+    return (uint64_t)page * p.c.page_stride + (uint64_t)(key % p.c.page_size) * p.c.slot_stride + x.h * p.c.head_stride;
+}
+// Clears non-finite entries of eight bf16 values; true if there were any.
+__device__ __forceinline__ bool clear_nonfinite(uint4* at) {
+    uint32_t x[4] = {at->x, at->y, at->z, at->w};
+    bool hit = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u, hit = true;
+        if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0x0000ffffu, hit = true;
+    }
+    if (hit) *at = make_uint4(x[0], x[1], x[2], x[3]);
+    return hit;
+}
+// What the cleared entries of column d come to for a node with this path.
+static __device__ __noinline__ float nonfinite_sum(const AttendParams& p, const Piece& x, uint64_t path, uint32_t d) {
+    float sum = 0.0f;
+    for (uint32_t j = 0; j < (uint32_t)x.sq.nodes; ++j)
+        if ((path >> j) & 1) {
+            const float y = bf16_to_f32(p.v[x.b * p.kv_batch + j * p.kv_node + x.h * p.kv_head + d]);
+            if (!isfinite(y)) sum += y;
+        }
+    return sum;
+}
+
+// ---- host side --------------------------------------------------------------------
+// Points p at the workspace for `grid` CTAs of `rows` rows of D channels; false (and ws.need set) if it is too small.
+inline bool attend_workspace(AttendParams& p, AttendWorkspace& ws, uint32_t rows, uint32_t D) {
+    const size_t slots = (size_t)2 * p.grid * rows, need = slots * (D * sizeof(float) + sizeof(float2));
+    if (ws.bytes < need) {
+        ws.need = need;
+        return false;
+    }
+    p.part_ml = static_cast<float2*>(ws.p);
+    p.part_o = reinterpret_cast<float*>(p.part_ml + slots);
+    return true;
+}
+template <typename... Args>
+cudaError_t attend_launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size_t smem, int use_pdl, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = use_pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+// lq4_attend.cu: joins the partials of a launch with items of `rows` rows and D channels; completes ws.launches.
+cudaError_t launch_attend_join(const AttendParams& p, uint32_t rows, uint32_t D, bool bf16_out, AttendWorkspace& ws, int use_pdl, cudaStream_t s);
+// lq4_attend_tc.cu: bf16 activations, items of 128 rows.
+cudaError_t launch_attend_tc(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s);
+
+}  // namespace lq4
