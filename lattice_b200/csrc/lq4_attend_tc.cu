@@ -10,15 +10,19 @@
 //   P = exp2(S - max)      one thread per row: no shuffles; bf16 pairs back to tensor memory
 //   O[128, D] += P V       A = P from tensor memory, B = V as it lies in the cache (keys outer: MN-major)
 //
-//   warps 0..3   softmax: a thread reads its row of S, hands the buffer back at once (the next S is computed
-//                while this one is exponentiated), writes P, and at the end of a piece drains O
-//   warp 4       tensor memory allocation; one lane issues all MMAs
-//   warps 5..7   loaders: cp.async of K and V rows, each looked up through the page table, two stages; they run
-//                ahead over the borders of pieces
+// The exponentials cost as much as the MMAs, so up to D = 128 a CTA runs two streams, each with its own S, P and O: while
+// one is exponentiated the tensor cores work on the other.  With up to 128 rows per item the streams take the
+// key tiles in turn and their O meet at the end of a piece; with more the item has 256 rows and each stream has 128 of
+// them, so that a tile of keys in shared memory serves both.  (At D = 256 tensor memory holds one O.)
+//
+//   warps 0..4N-1   softmax, four warps per stream: a thread reads its row of S, hands the buffer back at once (the
+//                   stream's next S is computed while this one is exponentiated), writes P, and drains O at the end
+//   next warp       tensor memory allocation; one lane issues all MMAs
+//   last 4 warps    loaders: cp.async of K and V rows, each looked up through the page table, into one ring of slots
+//                   (K, V, K, V, ...); they run ahead over the borders of pieces
 //
 // The running maximum only moves when it has grown by more than 2^8 (the final division takes the same base out
-// again), so O is rescaled in tensor memory a few times per sequence instead of per tile.  Up to D = 128 a CTA
-// takes half an SM (256 columns, 100 KB): one CTA's softmax runs beside the other's MMAs.
+// again), so O is rescaled in tensor memory a few times per sequence instead of per tile.
 #include "lq4_attend_dev.cuh"
 
 #include <atomic>
@@ -27,7 +31,7 @@ namespace lq4 {
 
 namespace {
 
-constexpr int kTcThreads = 256, kTcRows = 128, kSoftmax = 128, kLoaders = 96, kTcStages = 2;
+constexpr int kTcRows = 128, kLoaders = 128;
 constexpr float kLazy = 8.0f;                  // how far (log2) a row's maximum may outgrow its base
 
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
@@ -56,6 +60,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -105,52 +115,58 @@ __device__ __forceinline__ uint32_t swz(uint32_t rows, uint32_t r, uint32_t c) {
     return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-template <int D>
+// NS streams; WIDE: items of 256 rows.
+template <int D, int NS, bool WIDE>
 struct TcShape {
-    static constexpr uint32_t kTile = kKeys * D * 2, kStage = 2 * kTile, kQ = kTcRows * D * 2;
-    static constexpr uint32_t kOffs = kTcStages * kStage + kQ, kValid = kOffs + 2 * kKeys * 8, kAnc = kValid + 8 * 8;
-    static constexpr uint32_t kBars = kAnc + 2 * kMaxNodes * 8, kCtl = kBars + 16 * 8, kSmem = kCtl + 192 + 1024;      // + alignment slack
-    static constexpr uint32_t kColS = D, kColP = D + 64, kCols = D + 96 <= 256 ? 256 : 512;
-    static constexpr int kPerSm = D <= 128 ? 2 : 1;
-    static_assert(kSmem <= (uint32_t)kMaxSmem, "shared memory");
+    static constexpr int kSoftmax = 128 * NS, kThreads = kSoftmax + 32 + kLoaders, kItemRows = WIDE ? 256 : 128;
+    static constexpr uint32_t kSlot = kKeys * D * 2, kQ = kTcRows * D * 2 * (WIDE ? 2 : 1);
+    static constexpr uint32_t kFit = ((uint32_t)kMaxSmem - kQ - 5120) / kSlot, kSlots = kFit > 12 ? 12 : kFit;
+    static constexpr uint32_t kOffs = kSlots * kSlot + kQ, kValid = kOffs + 2 * kKeys * 8, kAnc = kValid + 16 * 8, kMeet = kAnc + kMaxNodes * 8;
+    static constexpr uint32_t kBars = kMeet + kTcRows * 8, kCtl = kBars + 48 * 8, kSmem = kCtl + 256 + 1024;      // + alignment slack
+    static constexpr uint32_t kColO = 0, kColS = NS * D, kColP = kColS + NS * 64, kCols = kColP + NS * 32 <= 256 ? 256 : 512;
+    static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kColP + NS * 32 <= 512, "shared or tensor memory");
+    static_assert(NS == 2 || !WIDE, "256 rows take two streams");
+    static_assert(kTcRows * 32 * 4 <= kQ, "the streams meet in Q's place");
 };
 
-template <int D>
-__global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kernel(const __grid_constant__ AttendParams p) {
-    using S = TcShape<D>;
-    constexpr int CPR = D / 8;
+template <int D, int NS, bool WIDE>
+__global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc_kernel(const __grid_constant__ AttendParams p) {
+    using S = TcShape<D, NS, WIDE>;
+    constexpr int CPR = D / 8, kSoftmax = S::kSoftmax, kMmaWarp = kSoftmax / 32;
+    constexpr uint32_t SL = S::kSlots;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);      // swizzle atoms are 1024 bytes
     uint64_t* offs = reinterpret_cast<uint64_t*>(smem + S::kOffs);      // [2][64] element offset of a key's row
-    volatile uint64_t* valid = reinterpret_cast<uint64_t*>(smem + S::kValid);    // [8] which of a tile's keys there are
-    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);        // [nodes] (the piece's)
+    volatile uint64_t* valid = reinterpret_cast<uint64_t*>(smem + S::kValid);    // [16] which of a tile's keys there are
+    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);        // [nodes] of the piece's sequence
+    float2* meet = reinterpret_cast<float2*>(smem + S::kMeet);          // [128] (max, sum) of stream 1's rows
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..10: warp sums; 12: tensor memory; 16..19: fixes
-    uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // two stages each
-    uint64_t *s_full = bars + 8, *s_free = bars + 9, *p_full = bars + 10, *o_done = bars + 11, *q_full = bars + 12, *drained = bars + 13;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 12);
-    volatile uint32_t* fixes = reinterpret_cast<uint32_t*>(ctl + 16);    // [8] a tile's V held inf or NaN
-    const uint32_t sbase = smem_u32(smem), qbase = sbase + kTcStages * S::kStage;
+    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..14: warp sums; 16: tensor memory; 18..25: fixes
+    uint64_t *full = bars, *empty = bars + SL, *s_full = bars + 2 * SL, *s_free = s_full + 2, *p_full = s_full + 4, *o_done = s_full + 6;
+    uint64_t *q_full = s_full + 8, *drained = s_full + 9;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16);
+    volatile uint32_t* fixes = reinterpret_cast<uint32_t*>(ctl + 18);    // [16] a tile's V held inf or NaN
+    const uint32_t sbase = smem_u32(smem), qbase = sbase + SL * S::kSlot;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     pdl_wait_prior_grids();
-    const Range range = cta_range<kTcThreads>(p, ctl, ctl + 2);
+    const Range range = cta_range<S::kThreads>(p, ctl, ctl + 2);
     if (range.begin >= range.end) return;
-    if (warp == 4) {
+    if (warp == kMmaWarp) {
         tmem_alloc(tmem_slot, S::kCols);
         tmem_relinquish();
         if (lane == 0) {
-            for (int i = 0; i < kTcStages; ++i) {
-                mbar_init(k_full + i, kLoaders);
-                mbar_init(k_empty + i, 1);
-                mbar_init(v_full + i, kLoaders);
-                mbar_init(v_empty + i, 1);
+            for (uint32_t i = 0; i < SL; ++i) {
+                mbar_init(full + i, kLoaders / 32);                      // one arrival per warp
+                mbar_init(empty + i, 1);
             }
-            mbar_init(s_full, 1);
-            mbar_init(s_free, kSoftmax);
-            mbar_init(p_full, kSoftmax);
-            mbar_init(o_done, 1);
-            mbar_init(q_full, kSoftmax);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(s_full + i, 1);
+                mbar_init(s_free + i, 4);
+                mbar_init(p_full + i, 4);
+                mbar_init(o_done + i, 1);
+            }
+            mbar_init(q_full, kSoftmax / 32);
             mbar_init(drained, 1);
             mbar_fence_init();
         }
@@ -165,26 +181,31 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
     uint64_t u = range.begin, seq_first = range.seq_first;
     const uint64_t u_end = range.end;
     uint32_t b = range.seq;
-    uint32_t tile = 0;                                                   // tiles of this CTA so far
+    uint32_t tile = 0;                                                   // tiles of this CTA before the current piece
     // Once a wait has run out the CTA goes on without waiting, so that its barriers still match; the results are
     // rubbish then, and reported.
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok) ok = mbar_wait(bar, parity);
     };
+    auto wait_group = [&](uint32_t g) { wait(full + g % SL, (g / SL) & 1); };      // group 2n: K of tile n, 2n + 1: V
 
-    if (warp < 4) {
+    if (tid < (uint32_t)kSoftmax) {
         // ---- softmax: thread = row ---------------------------------------------------------------------
-        const uint32_t lanes = tmem + (warp << 21);                      // this warp's lanes: 32 * warp << 16
+        const uint32_t str = tid >> 7, r = tid & 127;
+        const uint32_t lanes = tmem + ((warp & 3) << 21);                // this warp's 32 lanes, at bit 16
+        const uint32_t col_o = lanes + S::kColO + str * D, col_s = lanes + S::kColS + str * 64, col_p = lanes + S::kColP + str * 32;
         const uint32_t rows = p.nodes * p.group;
+        uint32_t used = 0;                                               // steps of this stream so far
         while (u < u_end) {
             const Piece x = next_piece(p, u, u_end, b, seq_first);
             if (x.sq.bad && tid == 0) atomicOr(p.status, kDevErrBadIndex);
-            const uint32_t row = x.rt * kTcRows + tid, t = row / p.group, g = row - t * p.group;
+            const uint32_t row = x.rt * S::kItemRows + (WIDE ? tid : r), t = row / p.group, g = row - t * p.group;
             const bool live = row < rows && (int32_t)t < x.sq.nodes;
-            // Q: all MMAs that read the last one are done (o_done of its last tile)
-            for (uint32_t i = tid; i < kTcRows * CPR; i += kSoftmax) {
-                const uint32_t r = i / CPR, c = i % CPR, qrow = x.rt * kTcRows + r, qt = qrow / p.group, qg = qrow - qt * p.group;
+            // Q: all MMAs that read the last one are done (o_done of its last step)
+#pragma unroll 4
+            for (uint32_t i = tid; i < S::kItemRows * CPR; i += kSoftmax) {
+                const uint32_t qr = i / CPR, c = i % CPR, qrow = x.rt * S::kItemRows + qr, qt = qrow / p.group, qg = qrow - qt * p.group;
                 uint32_t w[4] = {0, 0, 0, 0};
                 if (qrow < rows && (int32_t)qt < x.sq.nodes && c * 8 < p.head_dim) {
                     const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_batch + qt * p.q_node + (uint64_t)(x.h * p.group + qg) * p.q_head + c * 8;
@@ -203,7 +224,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
                         }
                     }
                 }
-                *reinterpret_cast<uint4*>(smem + kTcStages * S::kStage + swz(kTcRows, r, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(smem + SL * S::kSlot + (qr >> 7) * (kTcRows * D * 2) + swz(kTcRows, qr & 127, c)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             if (x.has_nodes && tid < p.nodes) {
                 bool bad = false;
@@ -212,54 +233,59 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
             }
             fence_async_smem();
             named_bar_sync(2, kSoftmax);                                 // (anc is read by other threads)
-            mbar_arrive(q_full);
+            if (lane == 0) mbar_arrive(q_full);
 
             float m = -INFINITY, l = 0.0f;                               // base (log2) and sum of this row
-            for (uint32_t i = 0; i < x.n_tiles; ++i, ++tile) {
-                // (V's barrier cannot move on before this thread has handed over P; it also covers `valid` and `fixes`)
-                wait(v_full + tile % kTcStages, (tile / kTcStages) & 1);
-                wait(s_full, tile & 1);
+            bool first = true;
+            for (uint32_t i = WIDE || NS == 1 ? 0 : str; i < x.n_tiles; i += WIDE || NS == 1 ? 1 : 2) {
+                const uint32_t n = tile + i;
+                // (V's slot cannot be filled again before this thread has handed over P; V's barrier covers `valid` and `fixes`)
+                wait_group(2 * n + 1);
+                wait(s_full + str, used & 1);
                 __syncwarp();
                 tc_fence_after();
                 float s[64];
-                tmem_ld32<0>(lanes + S::kColS, s);
-                tmem_ld32<32>(lanes + S::kColS + 32, s);
-                uint64_t see = valid[tile & 7];
+                tmem_ld32<0>(col_s, s);
+                tmem_ld32<32>(col_s + 32, s);
+                uint64_t see = valid[n & 15];
                 tmem_ld_wait();
                 tc_fence_before();
-                mbar_arrive(s_free);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free + str);
                 if (x.t0 + i + 1 == x.sq.tiles && t < p.nodes) see &= anc[t];
                 if (see != ~0ull) {
 #pragma unroll
                     for (int j = 0; j < 64; ++j)
                         if (!((see >> j) & 1)) s[j] = -INFINITY;
                 }
-                float top = s[0];
+                float top;
+                {
+                    float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int j = 1; j < 64; ++j) top = fmaxf(top, s[j]);
-                top *= p.scale_log2;
-                // P's buffer and O are free once the MMA before has read and written them
-                if (i > 0) wait(o_done, (tile - 1) & 1);
+                    for (int j = 4; j < 64; ++j) t4[j & 3] = fmaxf(t4[j & 3], s[j]);
+                    top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
+                }
+                // P's buffer and O are free once the stream's MMA before has read and written them
+                if (!first) wait(o_done + str, (used - 1) & 1);
                 __syncwarp();
                 tc_fence_after();
-                if (i == 0) {
+                if (first) {
                     m = top;
                 } else {
                     const bool grow = top > m + kLazy;                   // (m -inf: at the first finite score)
                     if (__any_sync(0xffffffffu, grow)) {
-                        const float base = grow ? top : m;
                         const float f = grow ? exp2_fast(m - top) : 1.0f;
                         l *= f;
-                        m = base;
+                        m = grow ? top : m;
 #pragma unroll 1
                         for (int d = 0; d < D; d += 32) {
                             float o[32];
-                            tmem_ld32<0>(lanes + d, o);
+                            tmem_ld32<0>(col_o + d, o);
                             tmem_ld_wait();
                             uint32_t w[32];
 #pragma unroll
                             for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                            tmem_st32(lanes + d, w);
+                            tmem_st32(col_o + d, w);
                         }
                         tmem_st_wait();
                     }
@@ -276,27 +302,67 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
                     w[j] = *reinterpret_cast<const uint32_t*>(&y);
                 }
                 l += sum0 + sum1;
-                tmem_st32(lanes + S::kColP, w);
+                tmem_st32(col_p, w);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(p_full);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + str);
+                first = false;
+                ++used;
             }
-            wait(o_done, (tile - 1) & 1);
+            if (!first) wait(o_done + str, (used - 1) & 1);
             __syncwarp();
             tc_fence_after();
-            // ---- O of this piece: the result, or a partial
+            // ---- O of this piece: the result, or a partial.  Two streams over the keys: stream 1 hands its O to stream 0
+            // through Q's place, 32 columns at a time (both have waited for all MMAs of their own that read Q; the
+            // barrier below covers the other's).
+            constexpr bool kMeets = NS == 2 && !WIDE;
+            float f = 1.0f, f_other = 0.0f;
+            if constexpr (kMeets) {
+                if (str == 1) meet[r] = make_float2(m, l);
+                named_bar_sync(2, kSoftmax);
+                if (str == 0) {
+                    const float2 e = meet[r];
+                    const float top = fmaxf(m, e.x), safe = top == -INFINITY ? 0.0f : top;
+                    f = exp2_fast(m - safe);
+                    f_other = exp2_fast(e.x - safe);
+                    l = l * f + e.y * f_other;
+                    m = top;
+                }
+            }
             const bool whole = x.t0 == 0 && x.has_nodes;
-            const uint64_t slot = ((uint64_t)2 * blockIdx.x + (x.t0 == 0 ? 1 : 0)) * kTcRows + tid;
-            const bool fix = x.has_nodes && fixes[(tile - 1) & 7];       // (the nodes' tile is a piece's last one)
+            const uint64_t slot = ((uint64_t)2 * blockIdx.x + (x.t0 == 0 ? 1 : 0)) * S::kItemRows + (WIDE ? tid : r);
+            const bool fix = x.has_nodes && fixes[(tile + x.n_tiles - 1) & 15];      // (the nodes' tile is a piece's last one)
             const float inv = 1.0f / l;
-            if (!whole && live) p.part_ml[slot] = make_float2(m, l);
+            if (!whole && live && (!kMeets || str == 0)) p.part_ml[slot] = make_float2(m, l);
             const uint64_t to = b * p.out_batch + t * p.out_node + (uint64_t)(x.h * p.group + g) * p.out_head;
+            float* pass = reinterpret_cast<float*>(smem + SL * S::kSlot) + r;      // [columns][128]: lanes side by side
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
                 float o[32];
                 __syncwarp();
-                tmem_ld32<0>(lanes + d, o);
+                if (kMeets && str == 1) {
+                    if (first) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                    } else {
+                        tmem_ld32<0>(col_o + d, o);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) pass[e * 128] = o[e];
+                    named_bar_sync(3, 256);
+                    named_bar_sync(4, 256);                              // stream 0 has it
+                    continue;
+                }
+                tmem_ld32<0>(col_o + d, o);
                 tmem_ld_wait();
+                if constexpr (kMeets) {
+                    named_bar_sync(3, 256);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = o[e] * f + (f_other == 0.0f ? 0.0f : pass[e * 128] * f_other);
+                    named_bar_sync(4, 256);
+                }
                 if (!live) continue;
                 if (fix) {
 #pragma unroll
@@ -329,112 +395,132 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
             }
             __syncwarp();
             tc_fence_before();
-            named_bar_sync(2, kSoftmax);                                 // everybody has read anc and O
+            named_bar_sync(2, kSoftmax);                                 // everybody has read anc, meet and O
+            tile += x.n_tiles;
             u += x.n_tiles;
         }
-    } else if (warp == 4) {
-        // ---- MMA issue: one lane ----------------------------------------------------------------------------
-        if (lane == 0) {
-            uint32_t piece = 0;
-            auto scores = [&](uint32_t n) {                              // S of tile n
-                wait(k_full + n % kTcStages, (n / kTcStages) & 1);
-                if (n > 0) wait(s_free, (n - 1) & 1);
-                tc_fence_after();
-                const uint32_t k = sbase + (n % kTcStages) * S::kStage;
+    } else if (warp == kMmaWarp) {
+        // ---- MMA issue --------------------------------------------------------------------------------------
+        // Steps v of a piece: NS streams in turn over the tiles; with 256 rows both streams take every tile.  The whole warp
+        // walks through the steps with warp-uniform values (descriptors then live in uniform registers); one lane issues.
+        const bool leader = elect_lane();
+        auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+        const uint32_t tm = uniform(tmem), ring = uniform(sbase) >> 4, q0 = uniform(qbase) >> 4;
+        const uint64_t kmajor = smem_desc(0, 16), mnmajor = smem_desc(0, kKeys * 128);
+        uint32_t piece = 0, n_s[2] = {0, 0}, n_p[2] = {0, 0}, at = 0;    // S and PV steps per stream, tiles so far
+        auto scores = [&](uint32_t v) {
+            const uint32_t str = v % NS, n = at + (WIDE ? v >> 1 : v);
+            wait_group(2 * n);
+            if (n_s[str] > 0) wait(s_free + str, (n_s[str] - 1) & 1);
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t k = kmajor + (ring + (2 * n % SL) * (S::kSlot >> 4)), q = kmajor + (q0 + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0));
+            const uint32_t d = tm + S::kColS + str * 64;
+            if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint32_t chunk = ks >> 2, in = (ks & 3) * 32;
-                    mma_ss(tmem + S::kColS, smem_desc(qbase + chunk * (kTcRows * 128) + in, 16), smem_desc(k + chunk * (kKeys * 128) + in, 16),
-                           instr_desc(kKeys, 0), ks > 0);
-                }
-                mma_commit(k_empty + n % kTcStages);
-                mma_commit(s_full);
-            };
-            while (u < u_end) {
-                const Piece x = next_piece(p, u, u_end, b, seq_first);
-                wait(q_full, piece & 1);
-                scores(tile);
-                for (uint32_t i = 0; i < x.n_tiles; ++i, ++tile) {
-                    if (i + 1 < x.n_tiles) scores(tile + 1);
-                    wait(v_full + tile % kTcStages, (tile / kTcStages) & 1);
-                    wait(p_full, tile & 1);
-                    tc_fence_after();
-                    const uint32_t v = sbase + (tile % kTcStages) * S::kStage + S::kTile;
-#pragma unroll
-                    for (int ks = 0; ks < (int)kKeys / 16; ++ks)
-                        mma_ts(tmem, tmem + S::kColP + ks * 8, smem_desc(v + ks * 2048, kKeys * 128), instr_desc(D, 1), i > 0 || ks > 0);
-                    mma_commit(v_empty + tile % kTcStages);
-                    mma_commit(o_done);
-                }
-                ++piece;
-                u += x.n_tiles;
+                for (int ks = 0; ks < D / 16; ++ks)
+                    mma_ss(d, q + ((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32 >> 4), k + ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32 >> 4), instr_desc(kKeys, 0), ks > 0);
+                if (!WIDE || str == 1) mma_commit(empty + 2 * n % SL);
+                mma_commit(s_full + str);
             }
-            mma_commit(drained);                                         // tensor memory is freed behind the last MMA
-            if (!mbar_wait(drained, 0)) ok = false;
+            ++n_s[str];
+        };
+        while (u < u_end) {
+            const Piece x = next_piece(p, u, u_end, b, seq_first);
+            const uint32_t tiles = uniform(x.n_tiles), steps = WIDE ? 2 * tiles : tiles;
+            wait(q_full, piece & 1);
+            for (uint32_t v = 0; v < NS && v < steps; ++v) scores(v);
+            for (uint32_t v = 0; v < steps; ++v) {
+                const uint32_t str = v % NS, n = at + (WIDE ? v >> 1 : v);
+                if (v + NS < steps) scores(v + NS);
+                wait_group(2 * n + 1);
+                wait(p_full + str, n_p[str] & 1);
+                __syncwarp();
+                tc_fence_after();
+                const uint64_t vt = mnmajor + (ring + ((2 * n + 1) % SL) * (S::kSlot >> 4));
+                const uint32_t o = tm + S::kColO + str * D, pr = tm + S::kColP + str * 32;
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(o, pr + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), v >= NS || ks > 0);
+                    if (!WIDE || str == 1) mma_commit(empty + (2 * n + 1) % SL);
+                    mma_commit(o_done + str);
+                }
+                ++n_p[str];
+            }
+            ++piece;
+            at += tiles;
+            u += tiles;
         }
+        if (leader) mma_commit(drained);                                 // tensor memory is freed behind the last MMA
+        if (!mbar_wait(drained, 0)) ok = false;
         __syncwarp();
     } else {
         // ---- loaders ---------------------------------------------------------------------------------------
-        // Groups of copies in order: K and V of a tile, then the next tile's.  A group is handed on when it has landed,
-        // kLag groups behind the newest one; before a thread blocks on a stage that is still in use it hands on all
-        // it has, since that stage may only become free after them.
-        constexpr uint32_t kLag = 2;
-        const uint32_t lt = tid - (kTcThreads - kLoaders);
+        // A group is handed on when it has landed, kLag groups behind the newest one; before a thread blocks on a slot
+        // that is still in use it hands on all it has, oldest first, since the slot may only become free after them.
+        constexpr uint32_t kLag = SL > 6 ? 4 : 2;
+        const uint32_t lt = tid - (S::kThreads - kLoaders);
         uint32_t issued = 0, handed = 0;
         auto hand = [&](uint32_t upto) {
+            if (handed >= upto) return;
             fence_async_smem();
-            for (; handed < upto; ++handed) mbar_arrive((handed & 1 ? v_full : k_full) + (handed >> 1) % kTcStages);
+            __syncwarp();
+            for (; handed < upto; ++handed)
+                if (lane == 0) mbar_arrive(full + handed % SL);
         };
-        auto acquire = [&](uint64_t* empty) {
-            if (tile < (uint32_t)kTcStages) return;
-            uint64_t* bar = empty + tile % kTcStages;
-            const uint32_t parity = (tile / kTcStages - 1) & 1;
-            if (!ok || mbar_try_wait(bar, parity)) return;
+        auto acquire = [&]() {
+            if (issued < SL) return;
+            uint64_t* bar = empty + issued % SL;
+            const uint32_t parity = (issued / SL - 1) & 1;
+            if (__any_sync(0xffffffffu, !ok || mbar_try_wait(bar, parity))) return;      // (what one lane has seen, all have)
+            if (issued - handed > 3) cp_wait<3>(), hand(issued - 3);
+            if (issued - handed > 2) cp_wait<2>(), hand(issued - 2);
+            if (issued - handed > 1) cp_wait<1>(), hand(issued - 1);
             cp_wait<0>();
             hand(issued);
             wait(bar, parity);
+            __syncwarp();
         };
-        // (threads of a warp may part company here; they meet again at the barrier of the next tile)
         while (u < u_end) {
             const Piece x = next_piece(p, u, u_end, b, seq_first);
             int32_t page = lt < kKeys ? key_page(p, x, 0, lt) : -1;
             for (uint32_t i = 0; i < x.n_tiles; ++i, ++tile) {
-                const uint32_t st = tile % kTcStages;
                 __syncwarp();
                 if (lt < kKeys) {
                     const uint64_t at = key_offset(p, x, i, lt, page);
                     offs[(tile & 1) * kKeys + lt] = at;
                     __syncwarp();
                     const uint32_t bits = __ballot_sync(0xffffffffu, at != ~0ull);
-                    if (lane == 0) reinterpret_cast<volatile uint32_t*>(valid + (tile & 7))[lt >> 5] = bits;
-                    if (lt == 0) fixes[tile & 7] = 0;
+                    if (lane == 0) reinterpret_cast<volatile uint32_t*>(valid + (tile & 15))[lt >> 5] = bits;
+                    if (lt == 0) fixes[tile & 15] = 0;
                     page = key_page(p, x, i + 1, lt);
                 }
                 __syncwarp();
                 named_bar_sync(1, kLoaders);
                 const bool own = x.t0 + i + 1 == x.sq.tiles;
-                auto load = [&](const uint16_t* base, uint32_t stage) {
-#pragma unroll 4
-                    for (uint32_t idx = lt; idx < kKeys * CPR; idx += kLoaders) {
-                        const uint32_t r = idx / CPR, c = idx % CPR;
+                auto load = [&](const uint16_t* base) {
+                    acquire();
+                    const uint32_t slot = sbase + (issued % SL) * S::kSlot;
+#pragma unroll 8
+                    for (uint32_t n = 0; n < kKeys * CPR / kLoaders; ++n) {
+                        const uint32_t idx = n * kLoaders + lt, r = idx / CPR, c = idx % CPR;
                         const uint64_t at = offs[(tile & 1) * kKeys + r];
                         const bool here = at != ~0ull && c * 8 < p.head_dim;
-                        cp_async16(stage + swz(kKeys, r, c), here ? base + at + c * 8 : p.k, here);
+                        cp_async16(slot + swz(kKeys, r, c), here ? base + at + c * 8 : p.k, here);
                     }
                     cp_commit();
                     ++issued;
                 };
-                const uint32_t kst = sbase + st * S::kStage;
-                acquire(k_empty);
-                load(own ? p.k : p.c.k, kst);
-                acquire(v_empty);
-                load(own ? p.v : p.c.v, kst + S::kTile);
+                load(own ? p.k : p.c.k);
+                load(own ? p.v : p.c.v);
                 if (own) {                                               // clear non-finite V of the nodes before it is used
                     cp_wait<0>();
                     bool odd = false;
-                    for (uint32_t idx = lt; idx < kKeys * CPR; idx += kLoaders)
-                        odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + st * S::kStage + S::kTile + swz(kKeys, idx / CPR, idx % CPR)));
-                    if (odd) fixes[tile & 7] = 1;
+                    for (uint32_t n = 0; n < kKeys * CPR / kLoaders; ++n) {
+                        const uint32_t idx = n * kLoaders + lt;
+                        odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + ((issued - 1) % SL) * S::kSlot + swz(kKeys, idx / CPR, idx % CPR)));
+                    }
+                    if (odd) fixes[tile & 15] = 1;
                     hand(issued);
                 } else if (issued - handed > kLag) {
                     cp_wait<kLag>();
@@ -450,29 +536,30 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<D>::kPerSm) attend_tc_kern
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 4) tmem_dealloc(tmem, S::kCols);
+    if (warp == kMmaWarp) tmem_dealloc(tmem, S::kCols);
 }
 
-template <int D>
+template <int D, int NS, bool WIDE>
 cudaError_t run(AttendParams p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    using S = TcShape<D>;
+    using S = TcShape<D, NS, WIDE>;
     static DeviceOnce once;
-    auto fn = attend_tc_kernel<D>;
+    auto fn = attend_tc_kernel<D, NS, WIDE>;
     cudaError_t e = opt_in_smem(reinterpret_cast<const void*>(fn), S::kSmem, once);
     if (e != cudaSuccess) return e;
-    p.grid = (uint32_t)(sm_count * S::kPerSm);
-    p.row_tiles = (p.nodes * p.group + kTcRows - 1) / kTcRows;
-    if (!attend_workspace(p, ws, kTcRows, D)) return cudaSuccess;
-    if ((e = attend_launch(fn, dim3(p.grid), kTcThreads, S::kSmem, use_pdl, s, p)) != cudaSuccess) return e;
-    return launch_attend_join(p, kTcRows, D, true, ws, use_pdl, s);
+    p.grid = (uint32_t)sm_count;
+    p.row_tiles = (p.nodes * p.group + S::kItemRows - 1) / S::kItemRows;
+    if (!attend_workspace(p, ws, S::kItemRows, D)) return cudaSuccess;
+    if ((e = attend_launch(fn, dim3(p.grid), S::kThreads, S::kSmem, use_pdl, s, p)) != cudaSuccess) return e;
+    return launch_attend_join(p, S::kItemRows, D, true, ws, use_pdl, s);
 }
 
 }  // namespace
 
 cudaError_t launch_attend_tc(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    if (p.head_dim <= 64) return run<64>(p, ws, sm_count, use_pdl, s);
-    if (p.head_dim <= 128) return run<128>(p, ws, sm_count, use_pdl, s);
-    return run<256>(p, ws, sm_count, use_pdl, s);
+    const bool wide = p.nodes * p.group > (uint32_t)kTcRows;
+    if (p.head_dim <= 64) return wide ? run<64, 2, true>(p, ws, sm_count, use_pdl, s) : run<64, 2, false>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 128) return wide ? run<128, 2, true>(p, ws, sm_count, use_pdl, s) : run<128, 2, false>(p, ws, sm_count, use_pdl, s);
+    return run<256, 1, false>(p, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace lq4
