@@ -26,6 +26,7 @@
 #include "lq4_attend_dev.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace lq4 {
 
@@ -407,48 +408,75 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
         auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
         const uint32_t tm = uniform(tmem), ring = uniform(sbase) >> 4, q0 = uniform(qbase) >> 4;
         const uint64_t kmajor = smem_desc(0, 16), mnmajor = smem_desc(0, kKeys * 128);
-        uint32_t piece = 0, n_s[2] = {0, 0}, n_p[2] = {0, 0}, at = 0;    // S and PV steps per stream, tiles so far
-        auto scores = [&](uint32_t v) {
-            const uint32_t str = v % NS, n = at + (WIDE ? v >> 1 : v);
-            wait_group(2 * n);
-            if (n_s[str] > 0) wait(s_free + str, (n_s[str] - 1) & 1);
+        // Everything an iteration looks up is kept running: the ring position of the next K and V group with its phase, and
+        // the phases of the streams' barriers.
+        struct Ring {
+            uint32_t slot, phase;
+            __device__ __forceinline__ void step() {                     // K to K or V to V: two groups on
+                slot += 2;
+                if (slot >= SL) slot -= SL, phase ^= 1;
+            }
+        } kr{0, 0}, vr{1, 0};
+        uint32_t piece = 0, ph_s[NS], ph_p[NS], s_any = 0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) ph_s[i] = 1, ph_p[i] = 0;           // s_free: phase 1 of the step before the first
+        auto scores = [&](auto stream) {                                 // next S of a stream, from K's ring position
+            constexpr uint32_t str = decltype(stream)::value;
+            constexpr bool new_k = !WIDE || str == 0, last_use = !WIDE || str == NS - 1;
+            if (new_k) wait(full + kr.slot, kr.phase);
+            if (s_any >> str & 1) wait(s_free + str, ph_s[str]);
+            s_any |= 1u << str;
+            ph_s[str] ^= 1;
             __syncwarp();
             tc_fence_after();
-            const uint64_t k = kmajor + (ring + (2 * n % SL) * (S::kSlot >> 4)), q = kmajor + (q0 + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0));
+            const uint64_t k = kmajor + (ring + kr.slot * (S::kSlot >> 4)), q = kmajor + (q0 + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0));
             const uint32_t d = tm + S::kColS + str * 64;
             if (leader) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                     mma_ss(d, q + ((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32 >> 4), k + ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32 >> 4), instr_desc(kKeys, 0), ks > 0);
-                if (!WIDE || str == 1) mma_commit(empty + 2 * n % SL);
+                if (last_use) mma_commit(empty + kr.slot);
                 mma_commit(s_full + str);
             }
-            ++n_s[str];
+            if (last_use) kr.step();
         };
+        auto values = [&](auto stream, uint32_t accumulate) {            // O of a stream += its P times V at the ring position
+            constexpr uint32_t str = decltype(stream)::value;
+            constexpr bool new_v = !WIDE || str == 0, last_use = !WIDE || str == NS - 1;
+            if (new_v) wait(full + vr.slot, vr.phase);
+            wait(p_full + str, ph_p[str]);
+            ph_p[str] ^= 1;
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t vt = mnmajor + (ring + vr.slot * (S::kSlot >> 4));
+            const uint32_t o = tm + S::kColO + str * D, pr = tm + S::kColP + str * 32;
+            if (leader) {
+#pragma unroll
+                for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(o, pr + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), ks > 0 ? 1u : accumulate);
+                if (last_use) mma_commit(empty + vr.slot);
+                mma_commit(o_done + str);
+            }
+            if (last_use) vr.step();
+        };
+        constexpr std::integral_constant<uint32_t, 0> stream0{};
+        constexpr std::integral_constant<uint32_t, NS - 1> stream1{};    // (stream 0 again where there is one)
         while (u < u_end) {
             const Piece x = next_piece(p, u, u_end, b, seq_first);
-            const uint32_t tiles = uniform(x.n_tiles), steps = WIDE ? 2 * tiles : tiles;
+            const uint32_t tiles = uniform(x.n_tiles);
             wait(q_full, piece & 1);
-            for (uint32_t v = 0; v < NS && v < steps; ++v) scores(v);
-            for (uint32_t v = 0; v < steps; ++v) {
-                const uint32_t str = v % NS, n = at + (WIDE ? v >> 1 : v);
-                if (v + NS < steps) scores(v + NS);
-                wait_group(2 * n + 1);
-                wait(p_full + str, n_p[str] & 1);
-                __syncwarp();
-                tc_fence_after();
-                const uint64_t vt = mnmajor + (ring + ((2 * n + 1) % SL) * (S::kSlot >> 4));
-                const uint32_t o = tm + S::kColO + str * D, pr = tm + S::kColP + str * 32;
-                if (leader) {
-#pragma unroll
-                    for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(o, pr + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), v >= NS || ks > 0);
-                    if (!WIDE || str == 1) mma_commit(empty + (2 * n + 1) % SL);
-                    mma_commit(o_done + str);
+            // rounds of NS steps; with 128 rows and two streams the last round may have one
+            const uint32_t steps = WIDE ? 2 * tiles : tiles;
+            scores(stream0);
+            if (NS == 2 && steps > 1) scores(stream1);
+            for (uint32_t v = 0; v < steps; v += NS) {
+                if (v + NS < steps) scores(stream0);
+                values(stream0, v > 0);
+                if (NS == 2) {
+                    if (v + NS + 1 < steps) scores(stream1);
+                    if (v + 1 < steps) values(stream1, v > 0);
                 }
-                ++n_p[str];
             }
             ++piece;
-            at += tiles;
             u += tiles;
         }
         if (leader) mma_commit(drained);                                 // tensor memory is freed behind the last MMA
