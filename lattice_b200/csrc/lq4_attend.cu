@@ -57,8 +57,9 @@ __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
 template <int D>
 __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t c) { return r * (D * 2) + ((c ^ (r & 7)) << 4); }
 
-// From this many rows per kv head on bf16 activations take the tcgen05 kernel.
-constexpr uint32_t kTcMinRows = 48;
+// More rows than this per kv head and bf16 activations take the tcgen05 kernel: 16 sequences of 8192 tokens, 8 kv heads of
+// 128, 5 rows: 101 us here and 129 us there; 25 rows: 164 us and 128 us; 64 rows: 217 us and 132 us (B200).
+constexpr uint32_t kTcMinRows = 16;
 
 template <int D, int WM, int NQ>
 struct Shape {
@@ -90,7 +91,6 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
 
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
     const Range range = cta_range<NT>(p, ctl, reinterpret_cast<uint64_t*>(ml));
     uint64_t u = range.begin, seq_first = range.seq_first;
     const uint64_t u_end = range.end;

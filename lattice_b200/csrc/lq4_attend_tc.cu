@@ -17,16 +17,15 @@
 //
 //   warps 0..4N-1   softmax, four warps per stream: a thread reads its row of S, hands the buffer back at once (the
 //                   stream's next S is computed while this one is exponentiated), writes P, and drains O at the end
-//   next warp       tensor memory allocation; one lane issues all MMAs
+//   next N warps    MMA issue, a warp per stream (the first one allocates tensor memory)
 //   last 4 warps    loaders: cp.async of K and V rows, each looked up through the page table, into one ring of slots
-//                   (K, V, K, V, ...); they run ahead over the borders of pieces
+//                   (K, V, K, V, ...), a warp per tile; they run ahead over the borders of pieces
 //
 // The running maximum only moves when it has grown by more than 2^8 (the final division takes the same base out
 // again), so O is rescaled in tensor memory a few times per sequence instead of per tile.
 #include "lq4_attend_dev.cuh"
 
 #include <atomic>
-#include <type_traits>
 
 namespace lq4 {
 
@@ -119,12 +118,17 @@ __device__ __forceinline__ uint32_t swz(uint32_t rows, uint32_t r, uint32_t c) {
 // NS streams; WIDE: items of 256 rows.
 template <int D, int NS, bool WIDE>
 struct TcShape {
-    static constexpr int kSoftmax = 128 * NS, kThreads = kSoftmax + 32 + kLoaders, kItemRows = WIDE ? 256 : 128;
+    static constexpr int kSoftmax = 128 * NS, kThreads = kSoftmax + 32 * NS + kLoaders, kItemRows = WIDE ? 256 : 128;
     static constexpr uint32_t kSlot = kKeys * D * 2, kQ = kTcRows * D * 2 * (WIDE ? 2 : 1);
-    static constexpr uint32_t kFit = ((uint32_t)kMaxSmem - kQ - 5120) / kSlot, kSlots = kFit > 12 ? 12 : kFit;
-    static constexpr uint32_t kOffs = kSlots * kSlot + kQ, kValid = kOffs + 2 * kKeys * 8, kAnc = kValid + 16 * 8, kMeet = kAnc + kMaxNodes * 8;
-    static constexpr uint32_t kBars = kMeet + kTcRows * 8, kCtl = kBars + 48 * 8, kSmem = kCtl + 256 + 1024;      // + alignment slack
+    // Rings of slots: one that all streams read in order, or one per stream where they take the tiles in turn (a wait on a slot's
+    // barrier is only good as long as the reader goes through the slot's uses one by one).
+    static constexpr uint32_t kRings = NS == 2 && !WIDE ? 2 : 1;
+    static constexpr uint32_t kFit = ((uint32_t)kMaxSmem - kQ - 5120) / kSlot / kRings, kRing = kFit > 12 / kRings ? 12 / kRings : kFit, kSlots = kRing * kRings;
+    static constexpr uint32_t kValid = kSlots * kSlot + kQ, kFixes = kValid + 16 * 8, kAnc = kFixes + 16 * 8, kMeet = kAnc + kMaxNodes * 8;
+    static constexpr uint32_t kBars = kMeet + kTcRows * 8, kCtl = kBars + 56 * 8, kSmem = kCtl + 160 + 1024;      // + alignment slack
     static constexpr uint32_t kColO = 0, kColS = NS * D, kColP = kColS + NS * 64, kCols = kColP + NS * 32 <= 256 ? 256 : 512;
+    static constexpr uint32_t kTeams = kSlots >= 8 ? 4 : 2, kTeam = 4 / kTeams;      // loaders: teams, warps of a team
+    static_assert(2 * kTeams / kRings <= kRing && kLoaders == 128, "a team's next tile is at most a ring ahead of its last one");
     static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kColP + NS * 32 <= 512, "shared or tensor memory");
     static_assert(NS == 2 || !WIDE, "256 rows take two streams");
     static_assert(kTcRows * 32 * 4 <= kQ, "the streams meet in Q's place");
@@ -134,19 +138,18 @@ template <int D, int NS, bool WIDE>
 __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc_kernel(const __grid_constant__ AttendParams p) {
     using S = TcShape<D, NS, WIDE>;
     constexpr int CPR = D / 8, kSoftmax = S::kSoftmax, kMmaWarp = kSoftmax / 32;
-    constexpr uint32_t SL = S::kSlots;
+    constexpr uint32_t SL = S::kSlots, RING = S::kRing, RINGS = S::kRings;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);      // swizzle atoms are 1024 bytes
-    uint64_t* offs = reinterpret_cast<uint64_t*>(smem + S::kOffs);      // [2][64] element offset of a key's row
-    volatile uint64_t* valid = reinterpret_cast<uint64_t*>(smem + S::kValid);    // [16] which of a tile's keys there are
+    volatile uint32_t* valid = reinterpret_cast<uint32_t*>(smem + S::kValid);    // [16][2] which of a tile's 64 keys there are
+    volatile uint32_t* fixes = reinterpret_cast<uint32_t*>(smem + S::kFixes);    // [16][2] V of the tile held inf or NaN (by warp of a team)
     uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);        // [nodes] of the piece's sequence
     float2* meet = reinterpret_cast<float2*>(smem + S::kMeet);          // [128] (max, sum) of stream 1's rows
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..14: warp sums; 16: tensor memory; 18..25: fixes
+    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..15: warp sums; 16: tensor memory
     uint64_t *full = bars, *empty = bars + SL, *s_full = bars + 2 * SL, *s_free = s_full + 2, *p_full = s_full + 4, *o_done = s_full + 6;
-    uint64_t *q_full = s_full + 8, *drained = s_full + 9;
+    uint64_t *q_full = s_full + 8, *drained = s_full + 9, *info = s_full + 10;      // info: [16], the loaders are at most 7 tiles ahead
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16);
-    volatile uint32_t* fixes = reinterpret_cast<uint32_t*>(ctl + 18);    // [16] a tile's V held inf or NaN
     const uint32_t sbase = smem_u32(smem), qbase = sbase + SL * S::kSlot;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -158,8 +161,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
         tmem_relinquish();
         if (lane == 0) {
             for (uint32_t i = 0; i < SL; ++i) {
-                mbar_init(full + i, kLoaders / 32);                      // one arrival per warp
-                mbar_init(empty + i, 1);
+                mbar_init(full + i, S::kTeam);
+                mbar_init(empty + i, WIDE ? 2 : 1);                      // by the streams that read the tile
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(s_full + i, 1);
@@ -168,7 +171,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 mbar_init(o_done + i, 1);
             }
             mbar_init(q_full, kSoftmax / 32);
-            mbar_init(drained, 1);
+            mbar_init(drained, NS);
+            for (int i = 0; i < 16; ++i) mbar_init(info + i, S::kTeam);
             mbar_fence_init();
         }
     }
@@ -189,7 +193,6 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok) ok = mbar_wait(bar, parity);
     };
-    auto wait_group = [&](uint32_t g) { wait(full + g % SL, (g / SL) & 1); };      // group 2n: K of tile n, 2n + 1: V
 
     if (tid < (uint32_t)kSoftmax) {
         // ---- softmax: thread = row ---------------------------------------------------------------------
@@ -238,17 +241,16 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
 
             float m = -INFINITY, l = 0.0f;                               // base (log2) and sum of this row
             bool first = true;
-            for (uint32_t i = WIDE || NS == 1 ? 0 : str; i < x.n_tiles; i += WIDE || NS == 1 ? 1 : 2) {
+            for (uint32_t i = RINGS == 2 ? (str - tile) & 1 : 0; i < x.n_tiles; i += RINGS) {      // (tile n belongs to stream n & 1)
                 const uint32_t n = tile + i;
-                // (V's slot cannot be filled again before this thread has handed over P; V's barrier covers `valid` and `fixes`)
-                wait_group(2 * n + 1);
+                wait(info + (n & 15), (n >> 4) & 1);                     // `valid` of this tile is there
                 wait(s_full + str, used & 1);
                 __syncwarp();
                 tc_fence_after();
                 float s[64];
                 tmem_ld32<0>(col_s, s);
                 tmem_ld32<32>(col_s + 32, s);
-                uint64_t see = valid[n & 15];
+                uint64_t see = (uint64_t)valid[(n & 15) * 2 + 1] << 32 | valid[(n & 15) * 2];
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -263,7 +265,11 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 {
                     float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int j = 4; j < 64; ++j) t4[j & 3] = fmaxf(t4[j & 3], s[j]);
+                    for (int j = 4; j < 60; j += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) t4[e] = fmaxf(fmaxf(t4[e], s[j + e]), s[j + 4 + e]);      // (one instruction)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t4[e] = fmaxf(t4[e], s[60 + e]);
                     top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
                 }
                 // P's buffer and O are free once the stream's MMA before has read and written them
@@ -305,6 +311,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 l += sum0 + sum1;
                 tmem_st32(col_p, w);
                 tmem_st_wait();
+                // the nodes' tile: `fixes` comes with V, whose slot is not filled again before this P is handed over
+                if (x.t0 + i + 1 == x.sq.tiles) wait(full + (n & (RINGS - 1)) * RING + (2 * (n / RINGS) + 1) % RING, (2 * (n / RINGS) + 1) / RING & 1);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + str);
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             }
             const bool whole = x.t0 == 0 && x.has_nodes;
             const uint64_t slot = ((uint64_t)2 * blockIdx.x + (x.t0 == 0 ? 1 : 0)) * S::kItemRows + (WIDE ? tid : r);
-            const bool fix = x.has_nodes && fixes[(tile + x.n_tiles - 1) & 15];      // (the nodes' tile is a piece's last one)
+            const bool fix = x.has_nodes && (fixes[((tile + x.n_tiles - 1) & 15) * 2] | (S::kTeam == 2 ? fixes[((tile + x.n_tiles - 1) & 15) * 2 + 1] : 0));      // (the nodes' tile is a piece's last one)
             const float inv = 1.0f / l;
             if (!whole && live && (!kMeets || str == 0)) p.part_ml[slot] = make_float2(m, l);
             const uint64_t to = b * p.out_batch + t * p.out_node + (uint64_t)(x.h * p.group + g) * p.out_head;
@@ -342,22 +350,20 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             for (int d = 0; d < D; d += 32) {
                 float o[32];
                 __syncwarp();
-                if (kMeets && str == 1) {
-                    if (first) {
+                if (kMeets && first) {                                   // this stream had no tile of the piece
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-                    } else {
-                        tmem_ld32<0>(col_o + d, o);
-                        tmem_ld_wait();
-                    }
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                } else {
+                    tmem_ld32<0>(col_o + d, o);
+                    tmem_ld_wait();
+                }
+                if (kMeets && str == 1) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) pass[e * 128] = o[e];
                     named_bar_sync(3, 256);
                     named_bar_sync(4, 256);                              // stream 0 has it
                     continue;
                 }
-                tmem_ld32<0>(col_o + d, o);
-                tmem_ld_wait();
                 if constexpr (kMeets) {
                     named_bar_sync(3, 256);
 #pragma unroll
@@ -400,82 +406,68 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             tile += x.n_tiles;
             u += x.n_tiles;
         }
-    } else if (warp == kMmaWarp) {
-        // ---- MMA issue --------------------------------------------------------------------------------------
-        // Steps v of a piece: NS streams in turn over the tiles; with 256 rows both streams take every tile.  The whole warp
-        // walks through the steps with warp-uniform values (descriptors then live in uniform registers); one lane issues.
+    } else if (warp < kMmaWarp + NS) {
+        // ---- MMA issue: a warp per stream ------------------------------------------------------------------
+        // The whole warp walks through the stream's tiles with warp-uniform values (descriptors then live in uniform
+        // registers); one lane issues.  Everything a step looks up is kept running: ring position and phase of the next K
+        // and V group, phases of the stream's barriers.
         const bool leader = elect_lane();
         auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
-        const uint32_t tm = uniform(tmem), ring = uniform(sbase) >> 4, q0 = uniform(qbase) >> 4;
+        const uint32_t str = uniform(warp - kMmaWarp);
+        const uint32_t tm = uniform(tmem), ring = uniform(sbase) >> 4;
+        const uint32_t col_s = tm + S::kColS + str * 64, col_p = tm + S::kColP + str * 32, col_o = tm + S::kColO + str * D;
         const uint64_t kmajor = smem_desc(0, 16), mnmajor = smem_desc(0, kKeys * 128);
-        // Everything an iteration looks up is kept running: the ring position of the next K and V group with its phase, and
-        // the phases of the streams' barriers.
+        const uint64_t q = kmajor + (uniform(qbase) >> 4) + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0);
         struct Ring {
             uint32_t slot, phase;
-            __device__ __forceinline__ void step() {                     // K to K or V to V: two groups on
-                slot += 2;
-                if (slot >= SL) slot -= SL, phase ^= 1;
+            __device__ __forceinline__ void move(uint32_t groups) {
+                slot += groups;
+                if (slot >= RING) slot -= RING, phase ^= 1;
             }
         } kr{0, 0}, vr{1, 0};
-        uint32_t piece = 0, ph_s[NS], ph_p[NS], s_any = 0;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) ph_s[i] = 1, ph_p[i] = 0;           // s_free: phase 1 of the step before the first
-        auto scores = [&](auto stream) {                                 // next S of a stream, from K's ring position
-            constexpr uint32_t str = decltype(stream)::value;
-            constexpr bool new_k = !WIDE || str == 0, last_use = !WIDE || str == NS - 1;
-            if (new_k) wait(full + kr.slot, kr.phase);
-            if (s_any >> str & 1) wait(s_free + str, ph_s[str]);
-            s_any |= 1u << str;
-            ph_s[str] ^= 1;
+        const uint32_t ring0 = RINGS == 2 ? str * RING : 0;              // first slot of the stream's ring
+        uint32_t piece = 0, ph_s = 1, ph_p = 0, at = 0;                  // s_free: phase 1 of the step before the first; tiles so far
+        bool s_any = false;
+        auto scores = [&]() {
+            wait(full + ring0 + kr.slot, kr.phase);
+            if (s_any) wait(s_free + str, ph_s);
+            s_any = true;
+            ph_s ^= 1;
             __syncwarp();
             tc_fence_after();
-            const uint64_t k = kmajor + (ring + kr.slot * (S::kSlot >> 4)), q = kmajor + (q0 + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0));
-            const uint32_t d = tm + S::kColS + str * 64;
+            const uint64_t k = kmajor + (ring + (ring0 + kr.slot) * (S::kSlot >> 4));
             if (leader) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
-                    mma_ss(d, q + ((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32 >> 4), k + ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32 >> 4), instr_desc(kKeys, 0), ks > 0);
-                if (last_use) mma_commit(empty + kr.slot);
+                    mma_ss(col_s, q + ((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32 >> 4), k + ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32 >> 4), instr_desc(kKeys, 0), ks > 0);
+                mma_commit(empty + ring0 + kr.slot);
                 mma_commit(s_full + str);
             }
-            if (last_use) kr.step();
+            kr.move(2);
         };
-        auto values = [&](auto stream, uint32_t accumulate) {            // O of a stream += its P times V at the ring position
-            constexpr uint32_t str = decltype(stream)::value;
-            constexpr bool new_v = !WIDE || str == 0, last_use = !WIDE || str == NS - 1;
-            if (new_v) wait(full + vr.slot, vr.phase);
-            wait(p_full + str, ph_p[str]);
-            ph_p[str] ^= 1;
-            __syncwarp();
-            tc_fence_after();
-            const uint64_t vt = mnmajor + (ring + vr.slot * (S::kSlot >> 4));
-            const uint32_t o = tm + S::kColO + str * D, pr = tm + S::kColP + str * 32;
-            if (leader) {
-#pragma unroll
-                for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(o, pr + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), ks > 0 ? 1u : accumulate);
-                if (last_use) mma_commit(empty + vr.slot);
-                mma_commit(o_done + str);
-            }
-            if (last_use) vr.step();
-        };
-        constexpr std::integral_constant<uint32_t, 0> stream0{};
-        constexpr std::integral_constant<uint32_t, NS - 1> stream1{};    // (stream 0 again where there is one)
         while (u < u_end) {
             const Piece x = next_piece(p, u, u_end, b, seq_first);
             const uint32_t tiles = uniform(x.n_tiles);
+            const uint32_t steps = RINGS == 2 ? (tiles + 1 - ((str - at) & 1)) / 2 : tiles;      // of this stream
             wait(q_full, piece & 1);
-            // rounds of NS steps; with 128 rows and two streams the last round may have one
-            const uint32_t steps = WIDE ? 2 * tiles : tiles;
-            scores(stream0);
-            if (NS == 2 && steps > 1) scores(stream1);
-            for (uint32_t v = 0; v < steps; v += NS) {
-                if (v + NS < steps) scores(stream0);
-                values(stream0, v > 0);
-                if (NS == 2) {
-                    if (v + NS + 1 < steps) scores(stream1);
-                    if (v + 1 < steps) values(stream1, v > 0);
+            if (steps > 0) scores();
+            for (uint32_t v = 0; v < steps; ++v) {
+                if (v + 1 < steps) scores();
+                wait(full + ring0 + vr.slot, vr.phase);
+                wait(p_full + str, ph_p);
+                ph_p ^= 1;
+                __syncwarp();
+                tc_fence_after();
+                const uint64_t vt = mnmajor + (ring + (ring0 + vr.slot) * (S::kSlot >> 4));
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(col_o, col_p + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), v > 0 || ks > 0);
+                    mma_commit(empty + ring0 + vr.slot);
+                    mma_commit(o_done + str);
                 }
+                vr.move(2);
             }
+            at += tiles;
             ++piece;
             u += tiles;
         }
@@ -483,82 +475,114 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
         if (!mbar_wait(drained, 0)) ok = false;
         __syncwarp();
     } else {
-        // ---- loaders ---------------------------------------------------------------------------------------
-        // A group is handed on when it has landed, kLag groups behind the newest one; before a thread blocks on a slot
-        // that is still in use it hands on all it has, oldest first, since the slot may only become free after them.
-        constexpr uint32_t kLag = SL > 6 ? 4 : 2;
-        const uint32_t lt = tid - (S::kThreads - kLoaders);
-        uint32_t issued = 0, handed = 0;
-        auto hand = [&](uint32_t upto) {
-            if (handed >= upto) return;
-            fence_async_smem();
-            __syncwarp();
-            for (; handed < upto; ++handed)
-                if (lane == 0) mbar_arrive(full + handed % SL);
-        };
-        auto acquire = [&]() {
-            if (issued < SL) return;
-            uint64_t* bar = empty + issued % SL;
-            const uint32_t parity = (issued / SL - 1) & 1;
-            if (__any_sync(0xffffffffu, !ok || mbar_try_wait(bar, parity))) return;      // (what one lane has seen, all have)
-            if (issued - handed > 3) cp_wait<3>(), hand(issued - 3);
-            if (issued - handed > 2) cp_wait<2>(), hand(issued - 2);
-            if (issued - handed > 1) cp_wait<1>(), hand(issued - 1);
-            cp_wait<0>();
-            hand(issued);
-            wait(bar, parity);
-            __syncwarp();
-        };
+        // ---- loaders: teams take the tiles in turn -----------------------------------------------------------
+        // A lone warp pays some five cycles per dependent instruction and waits for its own copies; teams (a warp each where
+        // the ring is long enough, else two) that each look up, copy and hand on whole tiles overlap all of it.  A lane
+        // holds where its keys lie; table index and slot advance without a division, and the page ids are fetched one turn ahead.
+        // A team's next tile is at most half a ring ahead of its last one, so that a slot's barrier is never two phases off.
+        constexpr uint32_t kWarps = S::kTeams, kOn = kWarps * kKeys, kHold = 2 / S::kTeam, kCopies = kHold * CPR;
+        const uint32_t lw = (warp - (S::kThreads - kLoaders) / 32) / S::kTeam;      // team
+        const uint32_t key0 = ((warp - (S::kThreads - kLoaders) / 32) % S::kTeam) * 32;      // this warp's first key of a tile
+        struct Ring {
+            uint32_t slot, phase;                                        // phase: of `empty` before the slot is filled again
+            __device__ __forceinline__ void move(uint32_t groups) {
+                slot += groups;
+                while (slot >= RING) slot -= RING, phase ^= 1;
+            }
+        } kr{0, 1}, vr{1, 1};
+        kr.move(2 * (lw / RINGS));
+        vr.move(2 * (lw / RINGS));
+        const uint32_t ring0 = RINGS == 2 ? (lw & 1) * RING : 0;         // (a team's tiles are all even or all odd)
+        const uint32_t page_size = p.c.page_size, pages_on = kOn / page_size, slots_on = kOn - pages_on * page_size;
         while (u < u_end) {
             const Piece x = next_piece(p, u, u_end, b, seq_first);
-            int32_t page = lt < kKeys ? key_page(p, x, 0, lt) : -1;
-            for (uint32_t i = 0; i < x.n_tiles; ++i, ++tile) {
-                __syncwarp();
-                if (lt < kKeys) {
-                    const uint64_t at = key_offset(p, x, i, lt, page);
-                    offs[(tile & 1) * kKeys + lt] = at;
-                    __syncwarp();
-                    const uint32_t bits = __ballot_sync(0xffffffffu, at != ~0ull);
-                    if (lane == 0) reinterpret_cast<volatile uint32_t*>(valid + (tile & 15))[lt >> 5] = bits;
-                    if (lt == 0) fixes[tile & 15] = 0;
-                    page = key_page(p, x, i + 1, lt);
+            const int32_t* const table = p.c.table + (uint64_t)x.b * p.c.max_pages;
+            const uint32_t plain = x.n_tiles - x.has_nodes;              // tiles of cached keys in this piece
+            uint32_t i = (lw - tile) & (kWarps - 1);
+            struct Key {
+                uint32_t key, entry, in_page;
+                int32_t page;
+            } k2[kHold];
+            auto fetch = [&](Key& k) { k.page = i < plain && k.key < (uint32_t)x.sq.len ? table[k.entry] : -1; };
+#pragma unroll
+            for (uint32_t h = 0; h < kHold; ++h) {
+                k2[h].key = (x.t0 + i) * kKeys + key0 + h * 32 + lane;
+                k2[h].entry = k2[h].key / page_size;
+                k2[h].in_page = k2[h].key - k2[h].entry * page_size;
+                fetch(k2[h]);
+            }
+            while (i < x.n_tiles) {
+                const uint32_t n = tile + i;
+                const bool own = i == plain;
+                uint64_t at[kHold];
+                i += kWarps;
+#pragma unroll
+                for (uint32_t h = 0; h < kHold; ++h) {
+                    Key& k = k2[h];
+                    at[h] = ~0ull;
+                    if (own) {
+                        const uint32_t node = key0 + h * 32 + lane;
+                        if (node < (uint32_t)x.sq.nodes) at[h] = x.b * p.kv_batch + node * p.kv_node + x.h * p.kv_head;
+                    } else if (k.key < (uint32_t)x.sq.len) {
+                        if ((uint32_t)k.page < p.c.pages)
+                            at[h] = (uint32_t)k.page * p.c.page_stride + k.in_page * p.c.slot_stride + x.h * p.c.head_stride;
+                        else
+                            atomicOr(p.status, kDevErrBadIndex);
+                    }
+                    k.key += kOn;
+                    k.entry += pages_on;
+                    k.in_page += slots_on;
+                    if (k.in_page >= page_size) k.in_page -= page_size, ++k.entry;
+                    fetch(k);
                 }
                 __syncwarp();
-                named_bar_sync(1, kLoaders);
-                const bool own = x.t0 + i + 1 == x.sq.tiles;
-                auto load = [&](const uint16_t* base) {
-                    acquire();
-                    const uint32_t slot = sbase + (issued % SL) * S::kSlot;
+#pragma unroll
+                for (uint32_t h = 0; h < kHold; ++h) {
+                    const uint32_t bits = __ballot_sync(0xffffffffu, at[h] != ~0ull);
+                    if (lane == 0) valid[(n & 15) * 2 + key0 / 32 + h] = bits;
+                }
+                if (lane == 0) {
+                    fixes[(n & 15) * 2 + key0 / 32] = 0;
+                    mbar_arrive(info + (n & 15));
+                }
+                auto copy = [&](const uint16_t* base, const Ring& r, uint32_t group) {
+                    if (group >= RING) wait(empty + ring0 + r.slot, r.phase);
+                    __syncwarp();
+                    const uint32_t slot = sbase + (ring0 + r.slot) * S::kSlot;
 #pragma unroll 8
-                    for (uint32_t n = 0; n < kKeys * CPR / kLoaders; ++n) {
-                        const uint32_t idx = n * kLoaders + lt, r = idx / CPR, c = idx % CPR;
-                        const uint64_t at = offs[(tile & 1) * kKeys + r];
-                        const bool here = at != ~0ull && c * 8 < p.head_dim;
-                        cp_async16(slot + swz(kKeys, r, c), here ? base + at + c * 8 : p.k, here);
+                    for (uint32_t c = 0; c < kCopies; ++c) {
+                        const uint32_t idx = c * 32 + lane, row = idx / CPR, chunk = idx % CPR;      // (row < 32 or not: the same for all lanes)
+                        const uint64_t from = __shfl_sync(0xffffffffu, c < CPR ? at[0] : at[kHold - 1], row & 31);
+                        const bool here = from != ~0ull && chunk * 8 < p.head_dim;
+                        cp_async16(slot + swz(kKeys, key0 + row, chunk), here ? base + from + chunk * 8 : p.k, here);
                     }
                     cp_commit();
-                    ++issued;
                 };
-                load(own ? p.k : p.c.k);
-                load(own ? p.v : p.c.v);
+                copy(own ? p.k : p.c.k, kr, 2 * (n / RINGS));
+                copy(own ? p.v : p.c.v, vr, 2 * (n / RINGS) + 1);
+                cp_wait<1>();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + ring0 + kr.slot);
+                cp_wait<0>();
                 if (own) {                                               // clear non-finite V of the nodes before it is used
-                    cp_wait<0>();
                     bool odd = false;
-                    for (uint32_t n = 0; n < kKeys * CPR / kLoaders; ++n) {
-                        const uint32_t idx = n * kLoaders + lt;
-                        odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + ((issued - 1) % SL) * S::kSlot + swz(kKeys, idx / CPR, idx % CPR)));
+                    __syncwarp();
+                    for (uint32_t c = 0; c < kCopies; ++c) {
+                        const uint32_t idx = c * 32 + lane;
+                        odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + (ring0 + vr.slot) * S::kSlot + swz(kKeys, key0 + idx / CPR, idx % CPR)));
                     }
-                    if (odd) fixes[tile & 15] = 1;
-                    hand(issued);
-                } else if (issued - handed > kLag) {
-                    cp_wait<kLag>();
-                    hand(issued - kLag);
+                    if (__any_sync(0xffffffffu, odd) && lane == 0) fixes[(n & 15) * 2 + key0 / 32] = 1;
                 }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + ring0 + vr.slot);
+                kr.move(2 * kWarps / RINGS);
+                vr.move(2 * kWarps / RINGS);
             }
+            tile += x.n_tiles;
             u += x.n_tiles;
         }
-        cp_wait<0>();
-        hand(issued);
     }
     if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);
     tc_fence_before();
