@@ -174,11 +174,11 @@ SIGNATURES = {
     "lq4_block_hadamard_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.POINTER(RotDesc), C.c_void_p]),
     "lq4_cross_head_hadamard_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
     "lq4_block_rot_signs_from_seed": (C.c_int32, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
-    "lq4_rope_rows": (C.c_int32, [C.c_void_p, C.POINTER(RopeArgs), C.c_void_p]),
+    "lq4_rope_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "lq4_rope_frequencies": (C.c_int32, [C.POINTER(RopeScaling), C.c_void_p, C.c_void_p]),
-    "lq4_kv_append": (C.c_int32, [C.c_void_p, C.POINTER(KvAppendArgs), C.c_void_p]),
-    "lq4_tree_attention": (C.c_int32, [C.c_void_p, C.POINTER(TreeAttentionArgs), C.c_void_p]),
-    "lq4_verify_draft": (C.c_int32, [C.c_void_p, C.POINTER(VerifyArgs), C.c_void_p]),
+    "lq4_kv_append": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lq4_tree_attention": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lq4_verify_draft": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "lq4_weights_upload": (C.c_int32, [C.c_void_p, C.c_uint64, C.c_uint64, C.POINTER(C.c_void_p)]),
     "lq4_weights_load_q4_file": (C.c_int32, [C.c_char_p, C.POINTER(C.c_uint64), C.c_uint32, C.POINTER(C.c_void_p)]),
     "lq4_weights_payload": (C.c_void_p, [C.c_void_p]),

@@ -35,7 +35,7 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: str = "plain
 class RopeTable:
     """Frequencies on the device (f64, one per pair), how a pair lies in a head, and the scale of rotated entries."""
 
-    __slots__ = ("freq", "desc")
+    __slots__ = ("freq", "desc", "address", "device")
 
     def __init__(self, freq: torch.Tensor, layout: str = "half", scale: float = 1.0):
         if layout not in _LAYOUTS:
@@ -44,6 +44,7 @@ class RopeTable:
             raise TypeError("freq must be a contiguous 1-D float64 device tensor, one entry per pair")
         self.freq = freq
         self.desc = RopeDesc(freq.data_ptr(), 2 * freq.numel(), _LAYOUTS[layout], scale)
+        self.address, self.device = C.addressof(self.desc), freq.get_device()
 
     @classmethod
     def from_config(cls, rot_dim: int, device, layout: str = "half", **scaling) -> "RopeTable":
@@ -57,7 +58,7 @@ class KvCache:
     (any strides but the innermost, the same for both: a ``[pages, kv_heads, page_size, head_dim]`` allocation comes
     as its transposed view), ``page_table`` is ``[batch, max_pages]`` int32.  The tensors are referenced, not copied."""
 
-    __slots__ = ("k", "v", "page_table", "desc", "device")
+    __slots__ = ("k", "v", "page_table", "desc", "address", "device", "rows_shape")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor):
         if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
@@ -72,8 +73,10 @@ class KvCache:
         self.k, self.v, self.page_table = k, v, page_table
         pages, size, heads, dim = k.shape
         s0, s1, s2, _ = k.stride()
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, s0, s1, s2, page_table.data_ptr(),
-                                page_table.shape[0], page_table.shape[1])
+        batch, max_pages = page_table.shape
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, s0, s1, s2, page_table.data_ptr(), batch, max_pages)
+        self.address = C.addressof(self.desc)
+        self.rows_shape = (batch, heads, dim)                            # of rows to append or attend with, but for their number
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, page_table: torch.Tensor) -> "KvCache":

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Tuple
 
@@ -26,12 +27,20 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import GatherDesc, KvAppendArgs, LinearArgs, LoraDesc, Lq4Error, RopeArgs, RopePart, RotDesc, TreeAttentionArgs, VerifyArgs, check
+from ._lib import GatherDesc, LinearArgs, LoraDesc, Lq4Error, RotDesc, check
 from .attention import KvCache, RopeTable
 
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def _raw_stream(device: int) -> int:
+    """The current stream of `device`, whichever device is current (the short way where torch has it)."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 class Q4WeightBuf:
@@ -151,6 +160,9 @@ class CudaQ4Backend:
         h = C.c_void_p()
         check(_lib.lib().lq4_ctx_create(device, C.byref(h)))
         self._ctx = h.value
+        self._lib = _lib.lib()
+        self._args = C.create_string_buffer(64 * (1 + _lib.MAX_ROPE_PARTS))      # arguments of the attention calls
+        self._args_at = C.addressof(self._args)
         self.num_hidden_layers = num_hidden_layers
         # module name -> (d_in, d_out); None disables the model-shape check of load_lora_adapter
         self.projection_shapes = projection_shapes
@@ -498,16 +510,19 @@ class CudaQ4Backend:
         return y
 
     # ---- rotary positions and the key/value cache --------------------------------------------
-    def _own_stream(self) -> int:
-        """The current stream of this backend's device, whichever device is current."""
-        return torch.cuda.current_stream(self.device).cuda_stream
+    # One decode step makes these calls once per layer on tiny inputs, so the host side counts: arguments are packed
+    # into a buffer of this backend (the library reads it before a call returns), checks are single comparisons.
+    _ROPE_PART = struct.Struct("@PPiiIiQQQQ")
+    _ROPE_ARGS = struct.Struct("@PIIIPP")
+    _APPEND_ARGS = struct.Struct("@PPPiIQQQPPPP")
+    _TREE_ARGS = struct.Struct("@PPiPPPII9QPPPf")
+    _VERIFY_ARGS = struct.Struct("@PPiIII4Q8P")
+    _ACT_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
-    def _int32(self, name: str, t: Optional[torch.Tensor], *shape: int) -> Optional[int]:
-        if t is None:
-            return None
-        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != self.device:
-            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on cuda:{self.device}")
-        return t.data_ptr()
+    def _int32(self, name: str, t: torch.Tensor, shape: tuple) -> int:
+        if t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() and t.get_device() == self.device:
+            return t.data_ptr()
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on cuda:{self.device}")
 
     def rope_rows(self, parts, positions: torch.Tensor, rope: Optional[RopeTable] = None, *,
                   out_dtype: Optional[torch.dtype] = None, outs: Optional[List[torch.Tensor]] = None) -> List[torch.Tensor]:
@@ -521,38 +536,53 @@ class CudaQ4Backend:
             return []
         if n > _lib.MAX_ROPE_PARTS:
             raise ValueError(f"rope_rows takes at most {_lib.MAX_ROPE_PARTS} tensors, got {n}")
+        dev, buf, at, types = self.device, self._args, self._args_at, self._ACT_DTYPES
         rows, _, dim = parts[0][0].shape
-        arr, ys = (RopePart * n)(), []
+        ys = []
         for i, (x, turn) in enumerate(parts):
-            if x.dim() != 3 or x.shape[0] != rows or x.shape[2] != dim or x.get_device() != self.device:
-                raise ValueError(f"rope_rows: tensors must be [rows, heads, head_dim] on cuda:{self.device}, of equal rows and head_dim")
-            if x.stride(2) != 1:
+            if x.dim() != 3 or x.get_device() != dev:
+                raise ValueError(f"rope_rows: tensors must be [rows, heads, head_dim] on cuda:{dev}")
+            (r, heads, d), (x_row, x_head, x_in) = x.shape, x.stride()
+            if r != rows or d != dim:
+                raise ValueError("rope_rows: tensors must have equal rows and head_dim")
+            if x_in != 1:
                 x = x.contiguous()
+                x_row, x_head, _ = x.stride()
             if outs is None:
-                y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+                y = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
+                y_row, y_head = heads * dim, dim
             else:
                 y = outs[i]
-                if y.shape != x.shape or y.get_device() != self.device or y.stride(2) != 1:
+                if y.shape != x.shape or y.get_device() != dev or y.stride(2) != 1:
                     raise ValueError("rope_rows: an output must have its input's shape and device and unit stride along head_dim")
+                y_row, y_head, _ = y.stride()
             ys.append(y)
-            xs, yst = x.stride(), y.stride()
-            arr[i] = RopePart(x.data_ptr(), y.data_ptr(), self._dtype_of(x), self._dtype_of(y), x.shape[1], turn, xs[0], xs[1], yst[0], yst[1])
-        if rope is not None and rope.freq.get_device() != self.device:
-            raise ValueError(f"rope_rows: the frequencies must lie on cuda:{self.device}")
-        args = RopeArgs(arr, n, rows, dim, self._int32("positions", positions, rows), C.pointer(rope.desc) if rope is not None else None)
-        check(_lib.lib().lq4_rope_rows(self._ctx, C.byref(args), self._own_stream()))
+            if x.dtype not in types or y.dtype not in types:
+                raise TypeError(f"rope_rows: types are float32 and bfloat16, got {x.dtype} and {y.dtype}")
+            self._ROPE_PART.pack_into(buf, 64 + 64 * i, x.data_ptr(), y.data_ptr(), types[x.dtype], types[y.dtype], heads, turn,
+                                      x_row, x_head, y_row, y_head)
+        if rope is not None and rope.device != dev:
+            raise ValueError(f"rope_rows: the frequencies must lie on cuda:{dev}")
+        self._ROPE_ARGS.pack_into(buf, 0, at + 64, n, rows, dim, self._int32("positions", positions, (rows,)),
+                                  rope.address if rope is not None else 0)
+        status = self._lib.lq4_rope_rows(self._ctx, at, _raw_stream(dev))
+        if status:
+            check(status)
         return ys
 
     def _cache_rows(self, what: str, cache: KvCache, k: torch.Tensor, v: torch.Tensor):
         """Checks ``[batch, rows, kv_heads, head_dim]`` rows against a cache; returns (k, v) the kernels can read."""
-        d = cache.desc
-        if cache.device != self.device:
-            raise ValueError(f"{what}: the cache lies on cuda:{cache.device}, this backend on cuda:{self.device}")
-        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != d.batch or k.shape[2] != d.kv_heads or k.shape[3] != d.head_dim:
-            raise ValueError(f"{what}: k and v must be [{d.batch}, rows, {d.kv_heads}, {d.head_dim}], got {list(k.shape)} and {list(v.shape)}")
-        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device:
-            raise ValueError(f"{what}: k and v must have one type and lie on cuda:{self.device}")
-        if k.stride() != v.stride() or k.stride(3) != 1:
+        dev = self.device
+        if cache.device != dev or k.get_device() != dev or v.get_device() != dev:
+            raise ValueError(f"{what}: the cache, k and v must lie on cuda:{dev}")
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or (shape[0], shape[2], shape[3]) != cache.rows_shape:
+            b, h, d = cache.rows_shape
+            raise ValueError(f"{what}: k and v must be [{b}, rows, {h}, {d}], got {list(shape)} and {list(v.shape)}")
+        if v.dtype is not k.dtype:
+            raise TypeError(f"{what}: k and v must have one type, got {k.dtype} and {v.dtype}")
+        stride = k.stride()
+        if v.stride() != stride or stride[3] != 1:
             k, v = k.contiguous(), v.contiguous()
         return k, v
 
@@ -563,15 +593,20 @@ class CudaQ4Backend:
         ``kv_lens[b]`` cached ones: all of them, the first ``counts[b]``, or the rows ``index[b, :counts[b]]``
         (what ``verify_draft`` accepted).  Returns the new lengths (a new int32 tensor, or ``new_lens``)."""
         k, v = self._cache_rows("kv_append", cache, k, v)
-        b, rows = k.shape[:2]
+        b, rows, _, _ = k.shape
+        if k.dtype not in self._ACT_DTYPES:
+            raise TypeError(f"kv_append: k and v must be float32 or bfloat16, got {k.dtype}")
+        lens_at = self._int32("kv_lens", kv_lens, (b,))
         if new_lens is None:
             new_lens = torch.empty_like(kv_lens)
-        ks = k.stride()
-        args = KvAppendArgs(C.pointer(cache.desc), k.data_ptr(), v.data_ptr(), self._dtype_of(k), rows, ks[0], ks[1], ks[2],
-                            self._int32("kv_lens", kv_lens, b), self._int32("counts", counts, b),
-                            self._int32("index", index, b, rows), self._int32("new_lens", new_lens, b))
-        check(_lib.lib().lq4_kv_append(self._ctx, C.byref(args), self._own_stream()))
-        if rows == 0 and b:
+        s0, s1, s2, _ = k.stride()
+        self._APPEND_ARGS.pack_into(self._args, 0, cache.address, k.data_ptr(), v.data_ptr(), self._ACT_DTYPES[k.dtype], rows, s0, s1, s2, lens_at,
+                                    0 if counts is None else self._int32("counts", counts, (b,)),
+                                    0 if index is None else self._int32("index", index, (b, rows)), self._int32("new_lens", new_lens, (b,)))
+        status = self._lib.lq4_kv_append(self._ctx, self._args_at, _raw_stream(self.device))
+        if status:
+            check(status)
+        if rows == 0:
             new_lens.copy_(kv_lens)
         return new_lens
 
@@ -585,23 +620,31 @@ class CudaQ4Backend:
         how many nodes of a sequence are live (the others' rows of ``out`` are left as they were), ``scale``
         defaults to ``head_dim ** -0.5``."""
         k, v = self._cache_rows("tree_attention", cache, k, v)
-        if k.dtype != torch.bfloat16:
-            raise TypeError(f"tree_attention: the nodes' k and v must be bfloat16, got {k.dtype}")
+        if k.dtype is not torch.bfloat16 or q.dtype not in self._ACT_DTYPES:
+            raise TypeError(f"tree_attention: q must be float32 or bfloat16 and the nodes' k and v bfloat16, got {q.dtype} and {k.dtype}")
         b, t, heads, dim = q.shape
-        if b != k.shape[0] or t != k.shape[1] or dim != k.shape[3] or q.get_device() != self.device:
-            raise ValueError(f"tree_attention: q must be [{k.shape[0]}, {k.shape[1]}, q_heads, {k.shape[3]}] on cuda:{self.device}, got {list(q.shape)}")
-        if q.stride(3) != 1:
+        kb, kt, _, kd = k.shape
+        if b != kb or t != kt or dim != kd or q.get_device() != self.device:
+            raise ValueError(f"tree_attention: q must be [{kb}, {kt}, q_heads, {kd}] on cuda:{self.device}, got {list(q.shape)}")
+        q0, q1, q2, q3 = q.stride()
+        if q3 != 1:
             q = q.contiguous()
+            q0, q1, q2, _ = q.stride()
         if out is None:
-            out = torch.empty((b, t, heads, dim), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or out.get_device() != self.device:
-            raise ValueError("tree_attention: out must have q's shape, type and device and unit stride along head_dim")
-        qs, os_, ks = q.stride(), out.stride(), k.stride()
-        args = TreeAttentionArgs(q.data_ptr(), out.data_ptr(), self._dtype_of(q), k.data_ptr(), v.data_ptr(), C.pointer(cache.desc),
-                                 t, heads, qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], ks[0], ks[1], ks[2],
-                                 self._int32("kv_lens", kv_lens, b), self._int32("node_counts", node_counts, b),
-                                 self._int32("parents", parents, b, t), dim ** -0.5 if scale is None else scale)
-        check(_lib.lib().lq4_tree_attention(self._ctx, C.byref(args), self._own_stream()))
+            out = torch.empty_like(q)
+        elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != self.device:
+            raise ValueError("tree_attention: out must have q's shape, type and device")
+        o0, o1, o2, o3 = out.stride()
+        if o3 != 1:
+            raise ValueError("tree_attention: out must have unit stride along head_dim")
+        k0, k1, k2, _ = k.stride()
+        self._TREE_ARGS.pack_into(self._args, 0, q.data_ptr(), out.data_ptr(), self._ACT_DTYPES[q.dtype], k.data_ptr(), v.data_ptr(), cache.address,
+                                  t, heads, q0, q1, q2, o0, o1, o2, k0, k1, k2, self._int32("kv_lens", kv_lens, (b,)),
+                                  0 if node_counts is None else self._int32("node_counts", node_counts, (b,)),
+                                  0 if parents is None else self._int32("parents", parents, (b, t)), dim ** -0.5 if scale is None else scale)
+        status = self._lib.lq4_tree_attention(self._ctx, self._args_at, _raw_stream(self.device))
+        if status:
+            check(status)
         return out
 
     # ---- lm_head: vocabulary projection + exact top-k --------------------------------------
@@ -652,27 +695,42 @@ class CudaQ4Backend:
         token), ``temperature`` ``[batch]`` f32 (0: greedy).  Returns ``(path, path_len, next_token)``: the
         accepted nodes from node 0 on with -1 behind them, their number, the next token; ``path`` and
         ``path_len`` are ``index`` and ``counts`` of ``kv_append``."""
+        dev = self.device
         b, t, vocab = target_logits.shape
-        if draft_logits is not None and (draft_logits.shape != target_logits.shape or draft_logits.dtype != target_logits.dtype):
-            raise ValueError("verify_draft: draft_logits must have target_logits' shape and type")
-        rows = []
-        for x in (target_logits, draft_logits):
-            if x is not None and x.get_device() != self.device:
-                raise ValueError(f"verify_draft: logits must lie on cuda:{self.device}")
-            rows.append(x if x is None or x.stride(2) == 1 else x.contiguous())
+        if target_logits.dtype not in self._ACT_DTYPES:
+            raise TypeError(f"verify_draft: logits must be float32 or bfloat16, got {target_logits.dtype}")
+        s0, s1, s2 = target_logits.stride()
+        if s2 != 1:
+            target_logits = target_logits.contiguous()
+            s0, s1, _ = target_logits.stride()
+        draft_at, d0, d1, d2 = 0, 0, 0, 1
+        if draft_logits is not None:
+            if draft_logits.shape != target_logits.shape or draft_logits.dtype is not target_logits.dtype:
+                raise ValueError("verify_draft: draft_logits must have target_logits' shape and type")
+            d0, d1, d2 = draft_logits.stride()
+            if d2 != 1:
+                draft_logits = draft_logits.contiguous()
+                d0, d1, _ = draft_logits.stride()
+            draft_at = draft_logits.data_ptr()
+        if target_logits.get_device() != dev or (draft_at and draft_logits.get_device() != dev):
+            raise ValueError(f"verify_draft: logits must lie on cuda:{dev}")
+        f32 = []
         for name, x, shape in (("uniforms", uniforms, (b, t)), ("temperature", temperature, (b,))):
-            if x is not None and (x.dtype != torch.float32 or x.shape != shape or not x.is_contiguous() or x.get_device() != self.device):
-                raise ValueError(f"verify_draft: {name} must be a contiguous float32 tensor of shape {list(shape)} on cuda:{self.device}")
-        out = torch.empty(b * (t + 2), dtype=torch.int32, device=target_logits.device)
-        path, path_len, token = out[:b * t].view(b, t), out[b * t:b * (t + 1)], out[b * (t + 1):]
-        target, draft = rows
-        args = VerifyArgs(target.data_ptr(), draft.data_ptr() if draft is not None else None, self._dtype_of(target), b, t, vocab,
-                          target.stride(0), target.stride(1), draft.stride(0) if draft is not None else 0,
-                          draft.stride(1) if draft is not None else 0, self._int32("tokens", tokens, b, t),
-                          self._int32("parents", parents, b, t), self._int32("node_counts", node_counts, b), uniforms.data_ptr(),
-                          temperature.data_ptr() if temperature is not None else None, path.data_ptr(), path_len.data_ptr(),
-                          token.data_ptr())
-        check(_lib.lib().lq4_verify_draft(self._ctx, C.byref(args), self._own_stream()))
+            if x is None:
+                f32.append(0)
+            elif x.dtype is torch.float32 and x.shape == shape and x.is_contiguous() and x.get_device() == dev:
+                f32.append(x.data_ptr())
+            else:
+                raise ValueError(f"verify_draft: {name} must be a contiguous float32 tensor of shape {list(shape)} on cuda:{dev}")
+        path = torch.empty_like(tokens)
+        path_len, token = tokens.new_empty((2, b)).unbind()
+        self._VERIFY_ARGS.pack_into(self._args, 0, target_logits.data_ptr(), draft_at, self._ACT_DTYPES[target_logits.dtype], b, t, vocab, s0, s1, d0, d1,
+                                    self._int32("tokens", tokens, (b, t)), 0 if parents is None else self._int32("parents", parents, (b, t)),
+                                    0 if node_counts is None else self._int32("node_counts", node_counts, (b,)), f32[0], f32[1], path.data_ptr(),
+                                    path_len.data_ptr(), token.data_ptr())
+        status = self._lib.lq4_verify_draft(self._ctx, self._args_at, _raw_stream(dev))
+        if status:
+            check(status)
         return path, path_len, token
 
     def prepare_group(self, problems, outs: Optional[List[torch.Tensor]] = None,

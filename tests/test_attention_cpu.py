@@ -219,3 +219,15 @@ def test_verify_refusals(L, change, status):
     a = verify_args(**change)
     assert L.lq4_verify_draft(None, C.byref(a), None) == status
     assert L.lq4_verify_draft(None, None, None) == _lib.ERR_NULL
+
+
+def test_packed_arguments_match_the_structures():
+    from lattice_b200.backend import CudaQ4Backend as B
+    for packer, desc in ((B._ROPE_PART, RopePart), (B._ROPE_ARGS, RopeArgs), (B._APPEND_ARGS, KvAppendArgs), (B._TREE_ARGS, TreeAttentionArgs),
+                         (B._VERIFY_ARGS, VerifyArgs)):
+        buf = C.create_string_buffer(C.sizeof(desc))
+        values = list(range(1, len(packer.unpack(bytes(packer.size))) + 1))
+        packer.pack_into(buf, 0, *values)
+        got = desc.from_buffer(buf)
+        flat = [C.cast(v, C.c_void_p).value if hasattr(v, "contents") else v for v in (getattr(got, n) for n, _ in desc._fields_)]
+        assert flat == values and -(-packer.size // 8) * 8 == C.sizeof(desc)
