@@ -13,9 +13,12 @@
 //
 // One thread-block cluster per sequence walks down from the root and reads only the rows of the nodes it
 // visits (a tree of 64 nodes has few on its path); the vocabulary is cut over the cluster, 256 logits per warp
-// step.  Per node: one pass for (max, sum) of p and q, exchanged through distributed shared memory with one
-// cluster barrier; one pass per refusal; and the rescan of one warp's share for the last token.  Every CTA
-// takes every decision itself from the same numbers, in the same order.
+// step.  The rows of a node are read once: a warp's share (four steps at most, as a rule) stays in registers as
+// masses relative to the warp's own maximum, (max, sum) of p and q go through distributed shared memory with one
+// cluster barrier, a refusal is a pass over the registers with another barrier, and the last token comes from the one
+// warp that the border falls into.  Longer shares are read again instead.  Every CTA takes every decision itself from the
+// same numbers, in the same order.  What bounds it is the chain of latencies per node (rows, two reductions, a
+// barrier); the first child's rows are fetched into L2 meanwhile.
 //
 // Decisions lie next to borders, so everything that is summed or compared is f64; only the exponentials over the
 // vocabulary are f32 (expf), the drafted tokens' own are f64.
@@ -68,7 +71,12 @@ __device__ __forceinline__ double mass64(float x, float m, double tau) {
 __device__ __forceinline__ MaxSum join(const MaxSum& a, const MaxSum& b, float it) {
     const float m = fmaxf(a.m, b.m);
     if (m == -INFINITY) return {m, 0.0};
-    return {m, a.s * (a.m == m ? 1.0f : mass(a.m, m, it)) + b.s * (b.m == m ? 1.0f : mass(b.m, m, it))};
+    // (the same bits whichever comes first: all lanes and CTAs go on with one result)
+    return {m, __dadd_rn(__dmul_rn(a.s, a.m == m ? 1.0 : (double)mass(a.m, m, it)), __dmul_rn(b.s, b.m == m ? 1.0 : (double)mass(b.m, m, it)))};
+}
+__device__ __forceinline__ MaxSum join_lanes(MaxSum a, int first, float it) {      // over lanes that differ in bits first, first / 2, ... 1
+    for (int o = first; o; o >>= 1) a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)}, it);
+    return a;
 }
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }      // NaN carries no mass
 
@@ -129,8 +137,11 @@ struct Exchange {                       // what a CTA tells the others
     double total;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
+constexpr uint32_t kHeld = 4;            // steps of a warp's share that stay in registers
+
+// HELD: every warp's share is at most kHeld steps.
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_constant__ VerifyParams p) {
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t b = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -177,84 +188,153 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
     uint32_t cur = 0, count = 1;
     __syncthreads();
 
-    // this warp's part of a row: steps of 256 logits, from the row's own 16-byte border on
     const uint32_t all_warps = ranks * kVWarps, me = rank * kVWarps + warp;
-
     for (;;) {
+        // this warp's part of the row: steps of 256 logits, from the row's own 16-byte border on
         const T* prow = target_rows + cur * p.target_node;
         const T* qrow = sampled ? draft_rows + cur * p.draft_node : nullptr;
         const int64_t shift = (int64_t)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
         const uint32_t steps = (uint32_t)((p.vocab + shift + 255) / 256), per = (steps + all_warps - 1) / all_warps;
         const uint32_t c0 = min(me * per, steps), c1 = min(c0 + per, steps);
         const int64_t j_lane = (int64_t)lane * 8 - shift;
-        bool inner = false;                                              // does this node have children?
-        for (uint32_t c = cur + 1; c < (uint32_t)n; ++c) inner |= parent[c] == (int32_t)cur;
+        uint32_t child = (uint32_t)n;                                    // the first one
+        for (uint32_t c = (uint32_t)n - 1; c > cur; --c)
+            if (parent[c] == (int32_t)cur) child = c;
+        const bool with_q = sampled && child < (uint32_t)n;
 
         // ---- (max, sum) of p, of q where children need it; the argmax for greedy sequences
-        MaxSum sp{-INFINITY, 0.0}, sq{-INFINITY, 0.0};
+        MaxSum sp{-INFINITY, 0.0}, sq{-INFINITY, 0.0};                   // of this warp
         uint64_t best = 0;
-        for (uint32_t c = c0; c < c1; ++c) {
-            const int64_t j = (int64_t)c * 256 + j_lane;
-            float x[8], y[8];
-            load8(prow, j, p.vocab, x);
-            if (sampled && inner) load8(qrow, j, p.vocab, y);
-            if (greedy) {
+        float ep[HELD ? kHeld : 1][8], eq[HELD ? kHeld : 1][8];          // masses relative to sp.m and sq.m
+        if constexpr (HELD) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint64_t k = rank_key(x[i], (uint32_t)(j + i));
-                    best = k > best ? k : best;
-                }
-                continue;
+            for (uint32_t h = 0; h < kHeld; ++h) {                       // all loads are under way before the first use
+                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
+                const uint32_t live = c0 + h < c1 ? p.vocab : 0;
+                load8(prow, j, live, ep[h]);
+                if (with_q)
+                    load8(qrow, j, live, eq[h]);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) eq[h][i] = -INFINITY;
             }
-            auto add = [&](MaxSum& s, const float (&v)[8]) {
-                float m = v[0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
-                if (m == -INFINITY) return;
-                if (m > s.m) {
-                    if (s.m != -INFINITY) s.s *= mass(s.m, m, it);
-                    s.m = m;
+            if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
+                const T* next_p = target_rows + child * p.target_node;
+                const T* next_q = sampled ? draft_rows + child * p.draft_node : next_p;
+                for (uint32_t h = 0; h < kHeld; ++h) {
+                    const int64_t j = (int64_t)(c0 + h) * 256 + lane * 8;
+                    if (c0 + h < c1 && j < (int64_t)p.vocab && (lane & (sizeof(T) == 4 ? 3 : 7)) == 0) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(next_p + j));
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(next_q + j));
+                    }
                 }
-                float t = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t += mass(v[i], s.m, it);
-                s.s += t;
-            };
-            add(sp, x);
-            if (sampled && inner) add(sq, y);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
+            }
             if (greedy) {
+#pragma unroll
+                for (uint32_t h = 0; h < kHeld; ++h)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint64_t k = rank_key(ep[h][i], (uint32_t)((int64_t)(c0 + h) * 256 + j_lane + i));
+                        best = k > best ? k : best;
+                    }
+            } else {
+                auto masses = [&](float (&v)[HELD ? kHeld : 1][8], MaxSum& s) {
+                    float m = -INFINITY;
+#pragma unroll
+                    for (uint32_t h = 0; h < kHeld; ++h)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) m = fmaxf(m, v[h][i]);
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    double t = 0.0;
+#pragma unroll
+                    for (uint32_t h = 0; h < kHeld; ++h)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[h][i] = m == -INFINITY ? 0.0f : mass(v[h][i], m, it);
+                            t += v[h][i];
+                        }
+                    s = {m, t};
+                };
+                masses(ep, sp);
+                if (with_q) masses(eq, sq);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    sp.s += __shfl_xor_sync(0xffffffffu, sp.s, o);
+                    sq.s += __shfl_xor_sync(0xffffffffu, sq.s, o);
+                }
+            }
+        } else {
+            for (uint32_t c = c0; c < c1; ++c) {
+                const int64_t j = (int64_t)c * 256 + j_lane;
+                float x[8], y[8];
+                load8(prow, j, p.vocab, x);
+                if (with_q) load8(qrow, j, p.vocab, y);
+                if (greedy) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint64_t k = rank_key(x[i], (uint32_t)(j + i));
+                        best = k > best ? k : best;
+                    }
+                    continue;
+                }
+                auto add = [&](MaxSum& s, const float (&v)[8]) {
+                    float m = v[0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+                    if (m == -INFINITY) return;
+                    if (m > s.m) {
+                        if (s.m != -INFINITY) s.s *= mass(s.m, m, it);
+                        s.m = m;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s.s += mass(v[i], s.m, it);
+                };
+                add(sp, x);
+                if (with_q) add(sq, y);
+            }
+            if (!greedy) {
+                sp = join_lanes(sp, 16, it);
+                if (with_q) sq = join_lanes(sq, 16, it);
+            }
+        }
+        if (greedy) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
                 const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
                 best = k > best ? k : best;
-            } else {
-                sp = join(sp, {__shfl_xor_sync(0xffffffffu, sp.m, o), __shfl_xor_sync(0xffffffffu, sp.s, o)}, it);
-                if (sampled && inner) sq = join(sq, {__shfl_xor_sync(0xffffffffu, sq.m, o), __shfl_xor_sync(0xffffffffu, sq.s, o)}, it);
             }
         }
         if (lane == 0) wp[warp] = sp, wq[warp] = sq, wbest[warp] = best;
         __syncthreads();
-        if (tid < ranks) {                                               // one thread per CTA to tell
-            Exchange e{{-INFINITY, 0.0}, {-INFINITY, 0.0}, 0, 0.0};
-            for (uint32_t w = 0; w < kVWarps; ++w) {
-                e.p = join(e.p, wp[w], it);
-                e.q = join(e.q, wq[w], it);
-                e.best = wbest[w] > e.best ? wbest[w] : e.best;
+        if (warp == 0) {                                                 // the CTA's, told to all CTAs
+            Exchange e;
+            e.p = join_lanes(wp[lane & (kVWarps - 1)], kVWarps / 2, it);
+            e.q = join_lanes(wq[lane & (kVWarps - 1)], kVWarps / 2, it);
+            e.best = wbest[lane & (kVWarps - 1)];
+#pragma unroll
+            for (int o = kVWarps / 2; o; o >>= 1) {
+                const uint64_t k = __shfl_xor_sync(0xffffffffu, e.best, o);
+                e.best = k > e.best ? k : e.best;
             }
-            *cluster.map_shared_rank(&slots[turn][rank], tid) = e;
+            e.total = 0.0;
+            if (lane < ranks) *cluster.map_shared_rank(&slots[turn][rank], lane) = e;
         }
         cluster.sync();
         MaxSum P{-INFINITY, 0.0}, Q{-INFINITY, 0.0};
         best = 0;
-        for (uint32_t r = 0; r < ranks; ++r) {
-            const Exchange& e = slots[turn][r];
-            P = join(P, e.p, it);
-            Q = join(Q, e.q, it);
-            best = e.best > best ? e.best : best;
+        if (lane < ranks) P = slots[turn][lane].p, Q = slots[turn][lane].q, best = slots[turn][lane].best;
+        P = join_lanes(P, 16, it);
+        Q = join_lanes(Q, 16, it);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+            best = k > best ? k : best;
         }
         turn ^= 1;
         const double ip = P.s > 0.0 ? 1.0 / P.s : 0.0, iq = Q.s > 0.0 ? 1.0 / Q.s : 0.0;
+        const double fp = P.m == -INFINITY || sp.m == -INFINITY ? 0.0 : mass64(sp.m, P.m, tau);      // warp's masses -> the row's
+        const double fq = Q.m == -INFINITY || sq.m == -INFINITY ? 0.0 : mass64(sq.m, Q.m, tau);
 
         // ---- the children's probabilities
         if (!greedy && tid < (uint32_t)n && tid > cur && parent[tid] == (int32_t)cur && (uint32_t)token[tid] < p.vocab) {
@@ -265,13 +345,27 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
         __syncthreads();
 
         // The residual times P.s: without a refusal its terms are the f32 masses themselves, whose f64 sums are exact
-        // as a rule, so that equal masses meet a border where they should.
-        auto residual = [&](float (&x)[8], float (&y)[8], int64_t j, double a, uint32_t ngone, double (&w)[8]) {
+        // as a rule, so that equal masses meet a border where they should.  Step h of the share, at logit j.
+        auto residual = [&](uint32_t h, int64_t j, double a, uint32_t ngone, double (&w)[8]) {
             const double k = a * iq * P.s;
+            if constexpr (HELD) {
+                const double kq = k * fq;
+                if (a != 0.0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = P.m == -INFINITY ? 0.0 : (double)mass(x[i], P.m, it);
-                if (a != 0.0 && Q.m != -INFINITY) w[i] = fmax(w[i] - k * (double)mass(y[i], Q.m, it), 0.0);
+                    for (int i = 0; i < 8; ++i) w[i] = fmax((double)ep[h][i] * fp - kq * (double)eq[h][i], 0.0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = (double)ep[h][i] * fp;
+                }
+            } else {
+                float x[8], y[8];
+                load8(prow, j, p.vocab, x);
+                if (a != 0.0) load8(qrow, j, p.vocab, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = P.m == -INFINITY ? 0.0 : (double)mass(x[i], P.m, it);
+                    if (a != 0.0 && Q.m != -INFINITY) w[i] = fmax(w[i] - k * (double)mass(y[i], Q.m, it), 0.0);
+                }
             }
             for (uint32_t g = 0; g < ngone; ++g) {
                 const int64_t d = (int64_t)gone[g] - j;
@@ -284,25 +378,27 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
         uint32_t last_turn = 0;
         auto residual_pass = [&](double a, uint32_t ngone) -> double {
             double sum = 0.0;
-            for (uint32_t c = c0; c < c1; ++c) {
-                const int64_t j = (int64_t)c * 256 + j_lane;
-                float x[8], y[8];
+            auto step = [&](uint32_t h) {
                 double w[8];
-                load8(prow, j, p.vocab, x);
-                if (a != 0.0) load8(qrow, j, p.vocab, y);
-                residual(x, y, j, a, ngone, w);
+                residual(h, (int64_t)(c0 + h) * 256 + j_lane, a, ngone, w);
+                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            };
+            if constexpr (HELD) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += w[i];
+                for (uint32_t h = 0; h < kHeld; ++h) step(h);
+            } else {
+                for (uint32_t h = 0; h < c1 - c0; ++h) step(h);
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             __syncthreads();                                             // wtot of the pass before is read
             if (lane == 0) wtot[warp] = sum;
             __syncthreads();
-            if (tid < ranks) {
-                double t = 0.0;
-                for (uint32_t w = 0; w < kVWarps; ++w) t += wtot[w];
-                cluster.map_shared_rank(&slots[turn][rank], tid)->total = t;
+            if (warp == 0) {
+                double t = wtot[lane & (kVWarps - 1)];
+#pragma unroll
+                for (int o = kVWarps / 2; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                if (lane < ranks) cluster.map_shared_rank(&slots[turn][rank], lane)->total = t;
             }
             cluster.sync();
             double t = 0.0;
@@ -398,13 +494,10 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
                     if (wtot[w] > 0.0) who = w;
             if (who == warp) {
                 uint32_t found = kNoToken, last = kNoToken;
-                for (uint32_t c = c0; c < c1 && found == kNoToken; ++c) {
-                    const int64_t j = (int64_t)c * 256 + j_lane;
-                    float x[8], y[8];
+                auto scan = [&](uint32_t h) {
+                    const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
                     double w[8], sum = 0.0;
-                    load8(prow, j, p.vocab, x);
-                    if (a != 0.0) load8(qrow, j, p.vocab, y);
-                    residual(x, y, j, a, ngone, w);
+                    residual(h, j, a, ngone, w);
                     uint32_t mine = kNoToken, top = kNoToken;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -424,10 +517,16 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
                         if (mine == kNoToken && run > border && w[i] > 0.0) mine = (uint32_t)(j + i);
                     }
                     const uint32_t hits = __ballot_sync(0xffffffffu, mine != kNoToken);
-                    if (hits) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
+                    if (hits && found == kNoToken) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
                     const uint32_t some = __ballot_sync(0xffffffffu, top != kNoToken);
                     if (some) last = __shfl_sync(0xffffffffu, top, 31 - __clz(some));
                     base += __shfl_sync(0xffffffffu, incl, 31);
+                };
+                if constexpr (HELD) {
+#pragma unroll
+                    for (uint32_t h = 0; h < kHeld; ++h) scan(h);
+                } else {
+                    for (uint32_t h = 0; h < c1 - c0 && found == kNoToken; ++h) scan(h);
                 }
                 if (lane == 0) p.next_token[b] = (int32_t)(found != kNoToken ? found : last);
             }
@@ -439,8 +538,14 @@ __global__ void __launch_bounds__(kVThreads) verify_kernel(const __grid_constant
 
 template <typename T>
 cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl, cudaStream_t s) {
-    auto fn = verify_kernel<T>;
-    static DeviceOnce once;
+    // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
+    uint32_t ranks = kMaxCluster;
+    while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
+    const uint64_t steps = ((uint64_t)p.vocab + 7 + 255) / 256;         // (a row may start up to 7 logits behind a border)
+    const bool held = (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeld;
+    auto fn = held ? verify_kernel<T, true> : verify_kernel<T, false>;
+    static DeviceOnce once_of[2];
+    DeviceOnce& once = once_of[held];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -448,9 +553,6 @@ cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl
         if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         once.mark(dev);
     }
-    // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
-    uint32_t ranks = kMaxCluster;
-    while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(batch * ranks);
     cfg.blockDim = dim3(kVThreads);
