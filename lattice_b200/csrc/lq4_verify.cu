@@ -20,8 +20,10 @@
 // same numbers, in the same order.  What bounds it is the chain of latencies per node (rows, two reductions, a
 // barrier); the first child's rows are fetched into L2 meanwhile.
 //
-// Decisions lie next to borders, so everything that is summed or compared is f64; only the exponentials over the
-// vocabulary are f32 (expf), the drafted tokens' own are f64.
+// Decisions lie next to borders.  Masses over the vocabulary are f32 (expf; eight at a time are added in f32) and the
+// drafted tokens' own f64; all further sums are pairs of f32 (some 48 bits, any size of residual; sums of equal masses are
+// exact, so that they meet a border where they should).  f64 is left to one warp per CTA: this part does about two f64
+// operations a cycle and SM, and sums in f64 took most of the time of a node.
 #include "lq4_attend.cuh"
 
 #include <cooperative_groups.h>
@@ -53,7 +55,40 @@ struct VerifyParams {
     int32_t* status;
 };
 
-// (max, sum of exp((x - max) / tau)) of a share of a row
+// An unevaluated sum h + l of two f32, |l| at most half a step of h.
+struct Pair {
+    float h, l;
+};
+__device__ __forceinline__ Pair plus(const Pair& a, const Pair& b) {
+    const float s = __fadd_rn(a.h, b.h), t = __fsub_rn(s, a.h);
+    const float e = __fadd_rn(__fadd_rn(__fsub_rn(a.h, __fsub_rn(s, t)), __fsub_rn(b.h, t)), __fadd_rn(a.l, b.l));
+    const float h = __fadd_rn(s, e);
+    return {h, __fsub_rn(e, __fsub_rn(h, s))};
+}
+__device__ __forceinline__ bool above(const Pair& a, const Pair& b) { return a.h > b.h || (a.h == b.h && a.l > b.l); }
+__device__ __forceinline__ double value(const Pair& a) { return (double)a.h + (double)a.l; }
+__device__ __forceinline__ Pair pair_of(double x) {
+    const float h = (float)x;
+    return {h, (float)(x - (double)h)};
+}
+__device__ __forceinline__ Pair lanes_sum(Pair x, int first = 16) {
+    for (int o = first; o; o >>= 1) x = plus(x, {__shfl_xor_sync(0xffffffffu, x.h, o), __shfl_xor_sync(0xffffffffu, x.l, o)});
+    return x;
+}
+__device__ __forceinline__ Pair lanes_prefix(Pair x, uint32_t lane) {      // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const Pair up = {__shfl_up_sync(0xffffffffu, x.h, o), __shfl_up_sync(0xffffffffu, x.l, o)};
+        if (lane >= (uint32_t)o) x = plus(up, x);
+    }
+    return x;
+}
+
+// (max, sum of exp((x - max) / tau)) of a share of a row: as a warp has it, and for the join of warps and CTAs
+struct WarpSum {
+    float m;
+    Pair s;
+};
 struct MaxSum {
     float m;
     double s;
@@ -89,14 +124,27 @@ __device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) {
     return ((uint64_t)u << 32) | (uint32_t)~id;
 }
 
-// Elements [j, j + 8) of a row as f32, -inf outside it and for NaN.
+// Elements [j, j + 8) of a row: fetched as they lie where 16-byte loads fit, and then read as f32, -inf outside the row
+// and for NaN.  In two steps, so that many fetches can be under way before the first value is used.
+struct Raw {
+    uint4 a, b;
+    bool fits;
+};
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t j, uint32_t vocab, float (&x)[8]) {
+__device__ __forceinline__ void fetch8(const T* row, int64_t j, uint32_t vocab, Raw& r) {
+    r.fits = j >= 0 && j + 8 <= (int64_t)vocab && (reinterpret_cast<uintptr_t>(row + j) & 15) == 0;
+    if (r.fits) {
+        r.a = __ldg(reinterpret_cast<const uint4*>(row + j));
+        if (std::is_same<T, float>::value) r.b = __ldg(reinterpret_cast<const uint4*>(row + j) + 1);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void read8(const T* row, int64_t j, uint32_t vocab, const Raw& r, float (&x)[8]) {
     constexpr bool f32 = std::is_same<T, float>::value;
-    if (j >= 0 && j + 8 <= (int64_t)vocab && (reinterpret_cast<uintptr_t>(row + j) & 15) == 0) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + j));
+    if (r.fits) {
+        const uint4 a = r.a;
         if constexpr (f32) {
-            const uint4 b = __ldg(reinterpret_cast<const uint4*>(row + j) + 1);
+            const uint4 b = r.b;
             x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
             x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
         } else {
@@ -124,6 +172,13 @@ __device__ __forceinline__ void load8(const T* row, int64_t j, uint32_t vocab, f
 }
 
 template <typename T>
+__device__ __forceinline__ void load8(const T* row, int64_t j, uint32_t vocab, float (&x)[8]) {
+    Raw r;
+    fetch8(row, j, vocab, r);
+    read8(row, j, vocab, r, x);
+}
+
+template <typename T>
 __device__ __forceinline__ float one_logit(const T* row, uint32_t j) {
     if constexpr (std::is_same<T, float>::value)
         return clean(row[j]);
@@ -134,7 +189,11 @@ __device__ __forceinline__ float one_logit(const T* row, uint32_t j) {
 struct Exchange {                       // what a CTA tells the others
     MaxSum p, q;
     uint64_t best;
-    double total;
+    Pair total;
+};
+struct Row {                            // the current node's distributions, for all warps of a CTA
+    float pm, qm, q_over_p;             // maxima; (mass of q) * q_over_p = q(t) in units of p's masses
+    uint64_t best;
 };
 
 constexpr uint32_t kHeld = 4;            // steps of a warp's share that stay in registers
@@ -147,9 +206,12 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     const uint32_t b = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     __shared__ Exchange slots[2][kMaxCluster];
-    __shared__ MaxSum wp[kVWarps], wq[kVWarps];
+    __shared__ WarpSum wp[kVWarps], wq[kVWarps];
     __shared__ uint64_t wbest[kVWarps];
-    __shared__ double wtot[kVWarps];
+    __shared__ Pair wtot[kVWarps], s_base, s_border;
+    __shared__ uint32_t s_who;
+    __shared__ Row row;
+    __shared__ double s_ip;                                              // 1 / (sum of p's masses)
     __shared__ int32_t parent[LQ4_MAX_TREE_NODES], token[LQ4_MAX_TREE_NODES];
     __shared__ float uni[LQ4_MAX_TREE_NODES];
     __shared__ double child_p[LQ4_MAX_TREE_NODES], child_q[LQ4_MAX_TREE_NODES];
@@ -203,20 +265,17 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         const bool with_q = sampled && child < (uint32_t)n;
 
         // ---- (max, sum) of p, of q where children need it; the argmax for greedy sequences
-        MaxSum sp{-INFINITY, 0.0}, sq{-INFINITY, 0.0};                   // of this warp
+        WarpSum sp{-INFINITY, {0.0f, 0.0f}}, sq = sp;                    // of this warp
         uint64_t best = 0;
         float ep[HELD ? kHeld : 1][8], eq[HELD ? kHeld : 1][8];          // masses relative to sp.m and sq.m
         if constexpr (HELD) {
+            Raw rp[kHeld], rq[kHeld];                                    // all loads are under way before the first use
 #pragma unroll
-            for (uint32_t h = 0; h < kHeld; ++h) {                       // all loads are under way before the first use
+            for (uint32_t h = 0; h < kHeld; ++h) {
                 const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
                 const uint32_t live = c0 + h < c1 ? p.vocab : 0;
-                load8(prow, j, live, ep[h]);
-                if (with_q)
-                    load8(qrow, j, live, eq[h]);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) eq[h][i] = -INFINITY;
+                fetch8(prow, j, live, rp[h]);
+                if (with_q) fetch8(qrow, j, live, rq[h]);
             }
             if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
                 const T* next_p = target_rows + child * p.target_node;
@@ -229,6 +288,13 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                     }
                 }
             }
+#pragma unroll
+            for (uint32_t h = 0; h < kHeld; ++h) {
+                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
+                const uint32_t live = c0 + h < c1 ? p.vocab : 0;
+                read8(prow, j, live, rp[h], ep[h]);
+                if (with_q) read8(qrow, j, live, rq[h], eq[h]);
+            }
             if (greedy) {
 #pragma unroll
                 for (uint32_t h = 0; h < kHeld; ++h)
@@ -238,7 +304,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                         best = k > best ? k : best;
                     }
             } else {
-                auto masses = [&](float (&v)[HELD ? kHeld : 1][8], MaxSum& s) {
+                auto masses = [&](float (&v)[HELD ? kHeld : 1][8], WarpSum& s) {
                     float m = -INFINITY;
 #pragma unroll
                     for (uint32_t h = 0; h < kHeld; ++h)
@@ -246,23 +312,21 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                         for (int i = 0; i < 8; ++i) m = fmaxf(m, v[h][i]);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    double t = 0.0;
+                    Pair sum{0.0f, 0.0f};
 #pragma unroll
-                    for (uint32_t h = 0; h < kHeld; ++h)
+                    for (uint32_t h = 0; h < kHeld; ++h) {
+                        float t = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             v[h][i] = m == -INFINITY ? 0.0f : mass(v[h][i], m, it);
                             t += v[h][i];
                         }
-                    s = {m, t};
+                        sum = plus(sum, {t, 0.0f});
+                    }
+                    s = {m, lanes_sum(sum)};
                 };
                 masses(ep, sp);
                 if (with_q) masses(eq, sq);
-#pragma unroll
-                for (int o = 16; o; o >>= 1) {
-                    sp.s += __shfl_xor_sync(0xffffffffu, sp.s, o);
-                    sq.s += __shfl_xor_sync(0xffffffffu, sq.s, o);
-                }
             }
         } else {
             for (uint32_t c = c0; c < c1; ++c) {
@@ -278,25 +342,27 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                     }
                     continue;
                 }
-                auto add = [&](MaxSum& s, const float (&v)[8]) {
+                auto add = [&](WarpSum& s, const float (&v)[8]) {
                     float m = v[0];
 #pragma unroll
                     for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
-                    if (m == -INFINITY) return;
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    if (m == -INFINITY) return;                          // (one maximum for the warp)
                     if (m > s.m) {
-                        if (s.m != -INFINITY) s.s *= mass(s.m, m, it);
+                        const float f = s.m == -INFINITY ? 0.0f : mass(s.m, m, it);
+                        s.s = {s.s.h * f, s.s.l * f};
                         s.m = m;
                     }
+                    float t = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) s.s += mass(v[i], s.m, it);
+                    for (int i = 0; i < 8; ++i) t += mass(v[i], s.m, it);
+                    s.s = plus(s.s, {t, 0.0f});
                 };
                 add(sp, x);
                 if (with_q) add(sq, y);
             }
-            if (!greedy) {
-                sp = join_lanes(sp, 16, it);
-                if (with_q) sq = join_lanes(sq, 16, it);
-            }
+            if (!greedy) sp.s = lanes_sum(sp.s), sq.s = lanes_sum(sq.s);
         }
         if (greedy) {
 #pragma unroll
@@ -309,79 +375,95 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         __syncthreads();
         if (warp == 0) {                                                 // the CTA's, told to all CTAs
             Exchange e;
-            e.p = join_lanes(wp[lane & (kVWarps - 1)], kVWarps / 2, it);
-            e.q = join_lanes(wq[lane & (kVWarps - 1)], kVWarps / 2, it);
+            const WarpSum x = wp[lane & (kVWarps - 1)], y = wq[lane & (kVWarps - 1)];
+            e.p = join_lanes({x.m, value(x.s)}, kVWarps / 2, it);
+            e.q = join_lanes({y.m, value(y.s)}, kVWarps / 2, it);
             e.best = wbest[lane & (kVWarps - 1)];
 #pragma unroll
             for (int o = kVWarps / 2; o; o >>= 1) {
                 const uint64_t k = __shfl_xor_sync(0xffffffffu, e.best, o);
                 e.best = k > e.best ? k : e.best;
             }
-            e.total = 0.0;
+            e.total = {0.0f, 0.0f};
             if (lane < ranks) *cluster.map_shared_rank(&slots[turn][rank], lane) = e;
         }
         cluster.sync();
-        MaxSum P{-INFINITY, 0.0}, Q{-INFINITY, 0.0};
-        best = 0;
-        if (lane < ranks) P = slots[turn][lane].p, Q = slots[turn][lane].q, best = slots[turn][lane].best;
-        P = join_lanes(P, 16, it);
-        Q = join_lanes(Q, 16, it);
+        if (warp == 0) {
+            MaxSum P{-INFINITY, 0.0}, Q{-INFINITY, 0.0};
+            best = 0;
+            if (lane < ranks) P = slots[turn][lane].p, Q = slots[turn][lane].q, best = slots[turn][lane].best;
+            P = join_lanes(P, kMaxCluster / 2, it);                      // (lanes 16.. have nothing; lane 0's is what counts)
+            if (with_q) Q = join_lanes(Q, kMaxCluster / 2, it);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
-            best = k > best ? k : best;
+            for (int o = kMaxCluster / 2; o; o >>= 1) {
+                const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+                best = k > best ? k : best;
+            }
+            const float top_p = __shfl_sync(0xffffffffu, P.m, 0), top_q = __shfl_sync(0xffffffffu, Q.m, 0);
+            const double sum_p = __shfl_sync(0xffffffffu, P.s, 0), sum_q = __shfl_sync(0xffffffffu, Q.s, 0);
+            const bool has_p = top_p != -INFINITY, has_q = with_q && top_q != -INFINITY;      // (a row without mass has neither)
+            const double ip = has_p ? 1.0 / sum_p : 0.0, iq = has_q ? 1.0 / sum_q : 0.0;
+            if (lane == 0) {
+                row = {top_p, top_q, (float)(iq * sum_p), best};
+                s_ip = ip;
+                s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
+            }
+            // the children's probabilities
+            for (uint32_t c = lane; c < (uint32_t)n; c += 32) {
+                if (greedy || c <= cur || parent[c] != (int32_t)cur || (uint32_t)token[c] >= p.vocab) continue;
+                double pt = 0.0, qt = 0.0;
+                if (has_p) pt = mass64(one_logit(prow, token[c]), top_p, tau) * ip;
+                if (has_q) qt = mass64(one_logit(qrow, token[c]), top_q, tau) * iq;
+                child_p[c] = pt;
+                child_q[c] = qt;
+            }
         }
         turn ^= 1;
-        const double ip = P.s > 0.0 ? 1.0 / P.s : 0.0, iq = Q.s > 0.0 ? 1.0 / Q.s : 0.0;
-        const double fp = P.m == -INFINITY || sp.m == -INFINITY ? 0.0 : mass64(sp.m, P.m, tau);      // warp's masses -> the row's
-        const double fq = Q.m == -INFINITY || sq.m == -INFINITY ? 0.0 : mass64(sq.m, Q.m, tau);
-
-        // ---- the children's probabilities
-        if (!greedy && tid < (uint32_t)n && tid > cur && parent[tid] == (int32_t)cur && (uint32_t)token[tid] < p.vocab) {
-            child_p[tid] = P.m == -INFINITY ? 0.0 : mass64(one_logit(prow, token[tid]), P.m, tau) * ip;
-            child_q[tid] = !sampled || Q.m == -INFINITY ? 0.0 : mass64(one_logit(qrow, token[tid]), Q.m, tau) * iq;
-        }
-        if (tid == 0) s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
         __syncthreads();
+        const float pm = row.pm, qm = row.qm;
+        best = row.best;
+        const float fp = pm == -INFINITY || sp.m == -INFINITY ? 0.0f : mass(sp.m, pm, it);      // the warp's masses -> the row's
+        const float fq = qm == -INFINITY || sq.m == -INFINITY ? 0.0f : mass(sq.m, qm, it);
 
-        // The residual times P.s: without a refusal its terms are the f32 masses themselves, whose f64 sums are exact
-        // as a rule, so that equal masses meet a border where they should.  Step h of the share, at logit j.
-        auto residual = [&](uint32_t h, int64_t j, double a, uint32_t ngone, double (&w)[8]) {
-            const double k = a * iq * P.s;
+        // The residual, in units of p's masses: without a refusal its terms are those masses.  Step h of the share, at logit j.
+        auto residual = [&](uint32_t h, int64_t j, float a, uint32_t ngone, float (&w)[8]) {
+            const float k = a * row.q_over_p;
             if constexpr (HELD) {
-                const double kq = k * fq;
-                if (a != 0.0) {
+                const float kq = k * fq;
+                if (a != 0.0f) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = fmax((double)ep[h][i] * fp - kq * (double)eq[h][i], 0.0);
+                    for (int i = 0; i < 8; ++i) w[i] = fmaxf(fmaf(-eq[h][i], kq, ep[h][i] * fp), 0.0f);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = (double)ep[h][i] * fp;
+                    for (int i = 0; i < 8; ++i) w[i] = ep[h][i] * fp;
                 }
             } else {
                 float x[8], y[8];
                 load8(prow, j, p.vocab, x);
-                if (a != 0.0) load8(qrow, j, p.vocab, y);
+                if (a != 0.0f) load8(qrow, j, p.vocab, y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    w[i] = P.m == -INFINITY ? 0.0 : (double)mass(x[i], P.m, it);
-                    if (a != 0.0 && Q.m != -INFINITY) w[i] = fmax(w[i] - k * (double)mass(y[i], Q.m, it), 0.0);
+                    w[i] = pm == -INFINITY ? 0.0f : mass(x[i], pm, it);
+                    if (a != 0.0f && qm != -INFINITY) w[i] = fmaxf(fmaf(-mass(y[i], qm, it), k, w[i]), 0.0f);
                 }
             }
             for (uint32_t g = 0; g < ngone; ++g) {
                 const int64_t d = (int64_t)gone[g] - j;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (d == i) w[i] = 0.0;
+                    if (d == i) w[i] = 0.0f;
             }
         };
         // Its sum over the vocabulary; every warp's share stays in wtot, every CTA's in the slots.
         uint32_t last_turn = 0;
-        auto residual_pass = [&](double a, uint32_t ngone) -> double {
-            double sum = 0.0;
+        auto residual_pass = [&](float a, uint32_t ngone) -> Pair {
+            Pair sum{0.0f, 0.0f};
             auto step = [&](uint32_t h) {
-                double w[8];
+                float w[8], t = 0.0f;
                 residual(h, (int64_t)(c0 + h) * 256 + j_lane, a, ngone, w);
-                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t += w[i];
+                sum = plus(sum, {t, 0.0f});
             };
             if constexpr (HELD) {
 #pragma unroll
@@ -389,29 +471,25 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             } else {
                 for (uint32_t h = 0; h < c1 - c0; ++h) step(h);
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            sum = lanes_sum(sum);
             __syncthreads();                                             // wtot of the pass before is read
             if (lane == 0) wtot[warp] = sum;
             __syncthreads();
             if (warp == 0) {
-                double t = wtot[lane & (kVWarps - 1)];
-#pragma unroll
-                for (int o = kVWarps / 2; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                const Pair t = lanes_sum(wtot[lane & (kVWarps - 1)], kVWarps / 2);
                 if (lane < ranks) cluster.map_shared_rank(&slots[turn][rank], lane)->total = t;
             }
             cluster.sync();
-            double t = 0.0;
-            for (uint32_t r = 0; r < ranks; ++r) t += slots[turn][r].total;
+            const Pair t = lanes_sum(lane < ranks ? slots[turn][lane].total : Pair{0.0f, 0.0f}, kMaxCluster / 2);      // (lanes 0..15)
             last_turn = turn;
             turn ^= 1;
-            return t;
+            return {__shfl_sync(0xffffffffu, t.h, 0), __shfl_sync(0xffffffffu, t.l, 0)};
         };
 
         // ---- the children, one after the other
         constexpr uint32_t kFinish = 0, kAccept = 1, kRefused = 2;
         bool passed = false;                                             // wtot holds the residual of (s_a, 0 gone)
-        double last_sum = 0.0;
+        Pair last_sum{0.0f, 0.0f};
         uint32_t action;
         for (;;) {
             if (tid == 0) {
@@ -441,10 +519,10 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             __syncthreads();
             action = s_action;
             if (action != kRefused) break;
-            last_sum = residual_pass(s_a, 0);
+            last_sum = residual_pass((float)s_a, 0);
             passed = true;
             __syncthreads();
-            if (tid == 0) s_z = last_sum * ip, s_child += 1;
+            if (tid == 0) s_z = value(last_sum) * s_ip, s_child += 1;
             __syncthreads();
         }
         if (action == kAccept) {
@@ -461,75 +539,67 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             if (rank == 0 && tid == 0) p.next_token[b] = best ? (int32_t)~(uint32_t)best : -1;
             break;
         }
-        double a = s_a;
+        float a = (float)s_a;
         uint32_t ngone = s_gone;
         if (!passed) last_sum = residual_pass(a, ngone);
-        double z = last_sum;
-        if (!(z > 0.0) && (a != 0.0 || ngone)) a = 0.0, ngone = 0, z = residual_pass(0.0, 0);   // nothing is left of p: p itself
-        if (!(z > 0.0)) {
+        Pair z = last_sum;
+        if (!(z.h > 0.0f) && (a != 0.0f || ngone)) a = 0.0f, ngone = 0, z = residual_pass(0.0f, 0);   // nothing is left of p: p itself
+        if (!(z.h > 0.0f)) {
             if (rank == 0 && tid == 0) p.next_token[b] = -1;             // the row is empty
             break;
         }
-        const double border = (double)uni[0] * z;
-        double base = 0.0;
-        uint32_t owner = ranks;
-        for (uint32_t r = 0; r < ranks; ++r) {
-            const double t = slots[last_turn][r].total;
-            if (base + t > border) { owner = r; break; }
-            base += t;
+        // The smallest j whose prefix exceeds u z: the CTA, the warp, the lane, the entry.  (By rounding, or for a uniform of 1
+        // or more, there may be none: then the last entry with mass.)
+        if (warp == 0) {
+            auto find = [&](const Pair share, const Pair before, const Pair border, Pair& base) -> uint32_t {
+                const Pair incl = plus(before, lanes_prefix(share, lane));
+                const uint32_t hits = __ballot_sync(0xffffffffu, above(incl, border)), some = __ballot_sync(0xffffffffu, share.h > 0.0f);
+                const uint32_t who = hits & some ? __ffs(hits & some) - 1 : some ? 31 - __clz(some) : 0;
+                base = {__shfl_sync(0xffffffffu, incl.h, who ? who - 1 : 0), __shfl_sync(0xffffffffu, incl.l, who ? who - 1 : 0)};
+                if (who == 0) base = before;
+                return who;
+            };
+            const Pair none{0.0f, 0.0f}, border = pair_of((double)uni[0] * value(z));
+            Pair base;
+            const uint32_t owner = find(lane < ranks ? slots[last_turn][lane].total : none, none, border, base);
+            uint32_t who = kNoToken;
+            if (owner == rank) who = find(lane < kVWarps ? wtot[lane] : none, base, border, base);
+            if (lane == 0) s_who = who, s_base = base, s_border = border;
         }
-        if (owner == ranks) {                                            // a uniform of 1 or more: the last entry with mass
-            base = 0.0;
-            for (uint32_t r = 0; r < ranks; ++r)
-                if (slots[last_turn][r].total > 0.0) owner = r;
-        }
-        if (owner == rank) {
-            uint32_t who = kVWarps;
-            for (uint32_t w = 0; w < kVWarps; ++w) {
-                if (base + wtot[w] > border) { who = w; break; }
-                base += wtot[w];
-            }
-            if (who == kVWarps)
-                for (uint32_t w = 0; w < kVWarps; ++w)
-                    if (wtot[w] > 0.0) who = w;
-            if (who == warp) {
-                uint32_t found = kNoToken, last = kNoToken;
-                auto scan = [&](uint32_t h) {
-                    const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
-                    double w[8], sum = 0.0;
-                    residual(h, j, a, ngone, w);
-                    uint32_t mine = kNoToken, top = kNoToken;
+        __syncthreads();
+        if (s_who == warp) {
+            Pair base = s_base;
+            const Pair border = s_border;
+            uint32_t found = kNoToken, last = kNoToken;
+            auto scan = [&](uint32_t h) {
+                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
+                float w[8], part[8], t = 0.0f;
+                residual(h, j, a, ngone, w);
+                uint32_t mine = kNoToken, end = kNoToken;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        sum += w[i];
-                        if (w[i] > 0.0) top = (uint32_t)(j + i);
-                    }
-                    double incl = sum;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double t = __shfl_up_sync(0xffffffffu, incl, o);
-                        if (lane >= (uint32_t)o) incl += t;
-                    }
-                    double run = base + incl - sum;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        run += w[i];
-                        if (mine == kNoToken && run > border && w[i] > 0.0) mine = (uint32_t)(j + i);
-                    }
-                    const uint32_t hits = __ballot_sync(0xffffffffu, mine != kNoToken);
-                    if (hits && found == kNoToken) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
-                    const uint32_t some = __ballot_sync(0xffffffffu, top != kNoToken);
-                    if (some) last = __shfl_sync(0xffffffffu, top, 31 - __clz(some));
-                    base += __shfl_sync(0xffffffffu, incl, 31);
-                };
-                if constexpr (HELD) {
-#pragma unroll
-                    for (uint32_t h = 0; h < kHeld; ++h) scan(h);
-                } else {
-                    for (uint32_t h = 0; h < c1 - c0 && found == kNoToken; ++h) scan(h);
+                for (int i = 0; i < 8; ++i) {
+                    t += w[i];
+                    part[i] = t;
+                    if (w[i] > 0.0f) end = (uint32_t)(j + i);
                 }
-                if (lane == 0) p.next_token[b] = (int32_t)(found != kNoToken ? found : last);
+                const Pair incl = plus(base, lanes_prefix({t, 0.0f}, lane));
+                Pair before = {__shfl_up_sync(0xffffffffu, incl.h, 1), __shfl_up_sync(0xffffffffu, incl.l, 1)};
+                if (lane == 0) before = base;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (mine == kNoToken && w[i] > 0.0f && above(plus(before, {part[i], 0.0f}), border)) mine = (uint32_t)(j + i);
+                const uint32_t hits = __ballot_sync(0xffffffffu, mine != kNoToken), some = __ballot_sync(0xffffffffu, end != kNoToken);
+                if (hits && found == kNoToken) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
+                if (some) last = __shfl_sync(0xffffffffu, end, 31 - __clz(some));
+                base = {__shfl_sync(0xffffffffu, incl.h, 31), __shfl_sync(0xffffffffu, incl.l, 31)};
+            };
+            if constexpr (HELD) {
+#pragma unroll
+                for (uint32_t h = 0; h < kHeld; ++h) scan(h);
+            } else {
+                for (uint32_t h = 0; h < c1 - c0 && found == kNoToken; ++h) scan(h);
             }
+            if (lane == 0) p.next_token[b] = (int32_t)(found != kNoToken ? found : last);
         }
         break;
     }
