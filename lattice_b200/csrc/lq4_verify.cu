@@ -20,10 +20,11 @@
 // same numbers, in the same order.  What bounds it is the chain of latencies per node (rows, two reductions, a
 // barrier); the first child's rows are fetched into L2 meanwhile.
 //
-// Decisions lie next to borders.  Masses over the vocabulary are f32 (expf; eight at a time are added in f32) and the
-// drafted tokens' own f64; all further sums are pairs of f32 (some 48 bits, any size of residual; sums of equal masses are
-// exact, so that they meet a border where they should).  f64 is left to one warp per CTA: this part does about two f64
-// operations a cycle and SM, and sums in f64 took most of the time of a node.
+// Decisions lie next to borders.  Masses are f32 (ex2.approx of the rounded distance from the maximum: a few 2^-23, and
+// exactly 1 at the maximum; eight at a time are added in f32); all further sums are pairs of f32 (some 48 bits, any size of
+// residual; sums of equal masses are exact, so that they meet a border where they should).  f64 is left to one lane: this
+// part does about two f64 operations a cycle and SM.  Code is kept short for the same reason as the loads are early: a
+// node's pass runs through it once, and instruction fetches count.
 #include "lq4_attend.cuh"
 
 #include <cooperative_groups.h>
@@ -84,34 +85,39 @@ __device__ __forceinline__ Pair lanes_prefix(Pair x, uint32_t lane) {      // in
     return x;
 }
 
-// (max, sum of exp((x - max) / tau)) of a share of a row: as a warp has it, and for the join of warps and CTAs
+// (max, sum of exp((x - max) / tau)) of a share of a row
 struct WarpSum {
     float m;
     Pair s;
 };
-struct MaxSum {
-    float m;
-    double s;
-};
 
-// exp((x - m) * it); a row whose maximum is +inf has all its mass on the entries that are.
-__device__ __forceinline__ float mass(float x, float m, float it) {
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// exp((x - m) / tau), c = log2(e) / tau; a row whose maximum is +inf has all its mass on the entries that are.
+__device__ __forceinline__ float mass(float x, float m, float c) {
     if (m == INFINITY) return x == m ? 1.0f : 0.0f;
-    return expf((x - m) * it);
+    return exp2_fast((x - (m == -INFINITY ? 0.0f : m)) * c);
 }
-__device__ __forceinline__ double mass64(float x, float m, double tau) {
-    if (m == INFINITY) return x == m ? 1.0 : 0.0;
-    return exp(((double)x - (double)m) / tau);
+// The same beyond f32's range and free of the distance's rounding, for the drafted tokens: their p and q are compared however
+// small they are.
+__device__ __forceinline__ double mass_wide(float x, float m, float c) {
+    if (x == -INFINITY || m == INFINITY) return x == m ? 1.0 : 0.0;
+    const float d = __fsub_rn(x, m), t = __fsub_rn(d, x);
+    const float e = __fsub_rn(__fsub_rn(x, __fsub_rn(d, t)), __fadd_rn(m, t));      // d + e = x - m
+    const float y = d * c, n = rintf(y);
+    if (!(y > -1000.0f)) return 0.0;
+    const double f = exp2_fast((y - n) + fmaf(d, c, -y) + e * c);
+    return __hiloint2double(__double2hiint(f) + ((int)n << 20), __double2loint(f));
 }
-__device__ __forceinline__ MaxSum join(const MaxSum& a, const MaxSum& b, float it) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, 0.0};
-    // (the same bits whichever comes first: all lanes and CTAs go on with one result)
-    return {m, __dadd_rn(__dmul_rn(a.s, a.m == m ? 1.0 : (double)mass(a.m, m, it)), __dmul_rn(b.s, b.m == m ? 1.0 : (double)mass(b.m, m, it)))};
-}
-__device__ __forceinline__ MaxSum join_lanes(MaxSum a, int first, float it) {      // over lanes that differ in bits first, first / 2, ... 1
-    for (int o = first; o; o >>= 1) a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)}, it);
-    return a;
+// The sums of several shares, over lanes that differ in bits first, first / 2, .. 1: one maximum, scaled sums.
+__device__ __forceinline__ WarpSum join_lanes(WarpSum a, int first, float c) {
+    float m = a.m;
+    for (int o = first; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float f = mass(a.m, m, c);                                     // (nothing has mass: 0)
+    return {m, lanes_sum({a.s.h * f, a.s.l * f}, first)};
 }
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }      // NaN carries no mass
 
@@ -124,26 +130,42 @@ __device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) {
     return ((uint64_t)u << 32) | (uint32_t)~id;
 }
 
-// Elements [j, j + 8) of a row: fetched as they lie where 16-byte loads fit, and then read as f32, -inf outside the row
-// and for NaN.  In two steps, so that many fetches can be under way before the first value is used.
+// Elements [j, j + 8) of a row: fetched as they lie where a 16-byte load fits, and then read as f32, -inf outside the row and
+// for NaN.  In two steps, so that many fetches can be under way before the first value is used.  The few at a row's ends,
+// and rows of the draft that lie otherwise than the target's, come one by one.
 struct Raw {
     uint4 a, b;
-    bool fits;
+};
+struct Eight {
+    float x[8];
 };
 template <typename T>
-__device__ __forceinline__ void fetch8(const T* row, int64_t j, uint32_t vocab, Raw& r) {
-    r.fits = j >= 0 && j + 8 <= (int64_t)vocab && (reinterpret_cast<uintptr_t>(row + j) & 15) == 0;
-    if (r.fits) {
+__device__ __noinline__ Eight edge8(const T* row, int32_t j, int32_t end) {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r.x[i] = -INFINITY;
+        if (j + i >= 0 && j + i < end) {
+            if constexpr (std::is_same<T, float>::value)
+                r.x[i] = __ldg(row + j + i);
+            else
+                r.x[i] = bf16_to_f32(__ldg(row + j + i));
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void fetch8(const T* row, int32_t j, bool fits, Raw& r) {
+    if (fits) {
         r.a = __ldg(reinterpret_cast<const uint4*>(row + j));
         if (std::is_same<T, float>::value) r.b = __ldg(reinterpret_cast<const uint4*>(row + j) + 1);
     }
 }
 template <typename T>
-__device__ __forceinline__ void read8(const T* row, int64_t j, uint32_t vocab, const Raw& r, float (&x)[8]) {
-    constexpr bool f32 = std::is_same<T, float>::value;
-    if (r.fits) {
+__device__ __forceinline__ void read8(const T* row, int32_t j, int32_t end, bool fits, const Raw& r, float (&x)[8]) {
+    if (fits) {
         const uint4 a = r.a;
-        if constexpr (f32) {
+        if constexpr (std::is_same<T, float>::value) {
             const uint4 b = r.b;
             x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
             x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
@@ -156,26 +178,18 @@ __device__ __forceinline__ void read8(const T* row, int64_t j, uint32_t vocab, c
             }
         }
     } else {
+        const Eight e = edge8(row, j, end);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = -INFINITY;
-            if (j + i >= 0 && j + i < (int64_t)vocab) {
-                if constexpr (f32)
-                    x[i] = __ldg(row + j + i);
-                else
-                    x[i] = bf16_to_f32(__ldg(row + j + i));
-            }
-        }
+        for (int i = 0; i < 8; ++i) x[i] = e.x[i];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = clean(x[i]);
 }
-
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t j, uint32_t vocab, float (&x)[8]) {
+__device__ __forceinline__ void load8(const T* row, int32_t j, int32_t end, bool fits, float (&x)[8]) {
     Raw r;
-    fetch8(row, j, vocab, r);
-    read8(row, j, vocab, r, x);
+    fetch8(row, j, fits, r);
+    read8(row, j, end, fits, r, x);
 }
 
 template <typename T>
@@ -187,12 +201,12 @@ __device__ __forceinline__ float one_logit(const T* row, uint32_t j) {
 }
 
 struct Exchange {                       // what a CTA tells the others
-    MaxSum p, q;
+    WarpSum p, q;
     uint64_t best;
     Pair total;
 };
 struct Row {                            // the current node's distributions, for all warps of a CTA
-    float pm, qm, q_over_p;             // maxima; (mass of q) * q_over_p = q(t) in units of p's masses
+    float pm, qm, q_over_p;             // maxima; q(t) in units of p's masses is (mass of q) * q_over_p
     uint64_t best;
 };
 
@@ -241,7 +255,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     }
     const float tau = p.temperature ? p.temperature[b] : 1.0f;
     const bool greedy = !(tau >= 1e-20f);
-    const float it = greedy ? 1.0f : 1.0f / tau;
+    const float it = greedy ? 1.0f : 1.44269504088896340736f / tau;      // log2(e) / tau
     const bool sampled = p.draft != nullptr && !greedy;
     const T* target_rows = static_cast<const T*>(p.target) + b * p.target_batch;
     const T* draft_rows = static_cast<const T*>(p.draft) + b * p.draft_batch;
@@ -255,10 +269,12 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         // this warp's part of the row: steps of 256 logits, from the row's own 16-byte border on
         const T* prow = target_rows + cur * p.target_node;
         const T* qrow = sampled ? draft_rows + cur * p.draft_node : nullptr;
-        const int64_t shift = (int64_t)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
-        const uint32_t steps = (uint32_t)((p.vocab + shift + 255) / 256), per = (steps + all_warps - 1) / all_warps;
+        const int32_t shift = (int32_t)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
+        const uint32_t steps = (p.vocab + shift + 255) / 256, per = (steps + all_warps - 1) / all_warps;
         const uint32_t c0 = min(me * per, steps), c1 = min(c0 + per, steps);
-        const int64_t j_lane = (int64_t)lane * 8 - shift;
+        const bool q_alike = ((reinterpret_cast<uintptr_t>(prow) ^ reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
+        auto at = [&](uint32_t c) { return (int32_t)(c * 256 + lane * 8) - shift; };      // this lane's first logit of step c
+        auto fits = [&](int32_t j, int32_t end) { return j >= 0 && j + 8 <= end; };
         uint32_t child = (uint32_t)n;                                    // the first one
         for (uint32_t c = (uint32_t)n - 1; c > cur; --c)
             if (parent[c] == (int32_t)cur) child = c;
@@ -266,23 +282,24 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 
         // ---- (max, sum) of p, of q where children need it; the argmax for greedy sequences
         WarpSum sp{-INFINITY, {0.0f, 0.0f}}, sq = sp;                    // of this warp
+        const int32_t vocab = (int32_t)p.vocab;
         uint64_t best = 0;
         float ep[HELD ? kHeld : 1][8], eq[HELD ? kHeld : 1][8];          // masses relative to sp.m and sq.m
         if constexpr (HELD) {
             Raw rp[kHeld], rq[kHeld];                                    // all loads are under way before the first use
 #pragma unroll
             for (uint32_t h = 0; h < kHeld; ++h) {
-                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
-                const uint32_t live = c0 + h < c1 ? p.vocab : 0;
-                fetch8(prow, j, live, rp[h]);
-                if (with_q) fetch8(qrow, j, live, rq[h]);
+                const int32_t j = at(c0 + h);
+                const bool f = fits(j, c0 + h < c1 ? vocab : 0);
+                fetch8(prow, j, f, rp[h]);
+                fetch8(qrow, j, f && q_alike && with_q, rq[h]);
             }
             if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
                 const T* next_p = target_rows + child * p.target_node;
                 const T* next_q = sampled ? draft_rows + child * p.draft_node : next_p;
                 for (uint32_t h = 0; h < kHeld; ++h) {
-                    const int64_t j = (int64_t)(c0 + h) * 256 + lane * 8;
-                    if (c0 + h < c1 && j < (int64_t)p.vocab && (lane & (sizeof(T) == 4 ? 3 : 7)) == 0) {
+                    const uint32_t j = (c0 + h) * 256 + lane * 8;
+                    if (c0 + h < c1 && j < p.vocab && (lane & (sizeof(T) == 4 ? 3 : 7)) == 0) {
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(next_p + j));
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(next_q + j));
                     }
@@ -290,19 +307,19 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             }
 #pragma unroll
             for (uint32_t h = 0; h < kHeld; ++h) {
-                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
-                const uint32_t live = c0 + h < c1 ? p.vocab : 0;
-                read8(prow, j, live, rp[h], ep[h]);
-                if (with_q) read8(qrow, j, live, rq[h], eq[h]);
+                const int32_t j = at(c0 + h), end = c0 + h < c1 ? vocab : 0;
+                read8(prow, j, end, fits(j, end), rp[h], ep[h]);
+                if (with_q) read8(qrow, j, end, fits(j, end) && q_alike, rq[h], eq[h]);
             }
             if (greedy) {
+                float top = -INFINITY;
+                int32_t id = -1;
 #pragma unroll
                 for (uint32_t h = 0; h < kHeld; ++h)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint64_t k = rank_key(ep[h][i], (uint32_t)((int64_t)(c0 + h) * 256 + j_lane + i));
-                        best = k > best ? k : best;
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        if (ep[h][i] > top) top = ep[h][i], id = at(c0 + h) + i;      // (rising ids: ties stay with the lower)
+                best = rank_key(top, (uint32_t)id);
             } else {
                 auto masses = [&](float (&v)[HELD ? kHeld : 1][8], WarpSum& s) {
                     float m = -INFINITY;
@@ -312,15 +329,20 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                         for (int i = 0; i < 8; ++i) m = fmaxf(m, v[h][i]);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const float base = m == -INFINITY ? 0.0f : m;
                     Pair sum{0.0f, 0.0f};
 #pragma unroll
                     for (uint32_t h = 0; h < kHeld; ++h) {
                         float t = 0.0f;
+                        if (m == INFINITY) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            v[h][i] = m == -INFINITY ? 0.0f : mass(v[h][i], m, it);
-                            t += v[h][i];
+                            for (int i = 0; i < 8; ++i) v[h][i] = v[h][i] == m ? 1.0f : 0.0f;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[h][i] = exp2_fast((v[h][i] - base) * it);
                         }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) t += v[h][i];
                         sum = plus(sum, {t, 0.0f});
                     }
                     s = {m, lanes_sum(sum)};
@@ -330,10 +352,11 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             }
         } else {
             for (uint32_t c = c0; c < c1; ++c) {
-                const int64_t j = (int64_t)c * 256 + j_lane;
+                const int32_t j = at(c);
+                const bool f = fits(j, vocab);
                 float x[8], y[8];
-                load8(prow, j, p.vocab, x);
-                if (with_q) load8(qrow, j, p.vocab, y);
+                load8(prow, j, vocab, f, x);
+                if (with_q) load8(qrow, j, vocab, f && q_alike, y);
                 if (greedy) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -375,9 +398,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         __syncthreads();
         if (warp == 0) {                                                 // the CTA's, told to all CTAs
             Exchange e;
-            const WarpSum x = wp[lane & (kVWarps - 1)], y = wq[lane & (kVWarps - 1)];
-            e.p = join_lanes({x.m, value(x.s)}, kVWarps / 2, it);
-            e.q = join_lanes({y.m, value(y.s)}, kVWarps / 2, it);
+            e.p = join_lanes(wp[lane & (kVWarps - 1)], kVWarps / 2, it);
+            e.q = join_lanes(wq[lane & (kVWarps - 1)], kVWarps / 2, it);
             e.best = wbest[lane & (kVWarps - 1)];
 #pragma unroll
             for (int o = kVWarps / 2; o; o >>= 1) {
@@ -389,44 +411,38 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         }
         cluster.sync();
         if (warp == 0) {
-            MaxSum P{-INFINITY, 0.0}, Q{-INFINITY, 0.0};
+            const uint32_t r = lane & (kMaxCluster - 1);                 // (both halves of the warp come to the same)
+            WarpSum P{-INFINITY, {0.0f, 0.0f}}, Q = P;
             best = 0;
-            if (lane < ranks) P = slots[turn][lane].p, Q = slots[turn][lane].q, best = slots[turn][lane].best;
-            P = join_lanes(P, kMaxCluster / 2, it);                      // (lanes 16.. have nothing; lane 0's is what counts)
-            if (with_q) Q = join_lanes(Q, kMaxCluster / 2, it);
+            if (r < ranks) P = slots[turn][r].p, Q = slots[turn][r].q, best = slots[turn][r].best;
+            P = join_lanes(P, kMaxCluster / 2, it);
+            Q = join_lanes(Q, kMaxCluster / 2, it);
 #pragma unroll
             for (int o = kMaxCluster / 2; o; o >>= 1) {
                 const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
                 best = k > best ? k : best;
             }
-            const float top_p = __shfl_sync(0xffffffffu, P.m, 0), top_q = __shfl_sync(0xffffffffu, Q.m, 0);
-            const double sum_p = __shfl_sync(0xffffffffu, P.s, 0), sum_q = __shfl_sync(0xffffffffu, Q.s, 0);
-            const bool has_p = top_p != -INFINITY, has_q = with_q && top_q != -INFINITY;      // (a row without mass has neither)
-            const double ip = has_p ? 1.0 / sum_p : 0.0, iq = has_q ? 1.0 / sum_q : 0.0;
+            const bool has_p = P.m != -INFINITY, has_q = with_q && Q.m != -INFINITY;      // (a row without mass has neither)
             if (lane == 0) {
-                row = {top_p, top_q, (float)(iq * sum_p), best};
-                s_ip = ip;
+                s_ip = has_p ? 1.0 / value(P.s) : 0.0;
+                row = {P.m, Q.m, has_q ? (float)(value(P.s) / value(Q.s)) : 0.0f, best};
                 s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
             }
-            // the children's probabilities
+            // the children's masses
             for (uint32_t c = lane; c < (uint32_t)n; c += 32) {
                 if (greedy || c <= cur || parent[c] != (int32_t)cur || (uint32_t)token[c] >= p.vocab) continue;
-                double pt = 0.0, qt = 0.0;
-                if (has_p) pt = mass64(one_logit(prow, token[c]), top_p, tau) * ip;
-                if (has_q) qt = mass64(one_logit(qrow, token[c]), top_q, tau) * iq;
-                child_p[c] = pt;
-                child_q[c] = qt;
+                child_p[c] = has_p ? mass_wide(one_logit(prow, token[c]), P.m, it) : 0.0;
+                child_q[c] = has_q ? mass_wide(one_logit(qrow, token[c]), Q.m, it) : 0.0;
             }
         }
         turn ^= 1;
         __syncthreads();
         const float pm = row.pm, qm = row.qm;
         best = row.best;
-        const float fp = pm == -INFINITY || sp.m == -INFINITY ? 0.0f : mass(sp.m, pm, it);      // the warp's masses -> the row's
-        const float fq = qm == -INFINITY || sq.m == -INFINITY ? 0.0f : mass(sq.m, qm, it);
+        const float fp = mass(sp.m, pm, it), fq = mass(sq.m, qm, it);    // the warp's masses -> the row's
 
         // The residual, in units of p's masses: without a refusal its terms are those masses.  Step h of the share, at logit j.
-        auto residual = [&](uint32_t h, int64_t j, float a, uint32_t ngone, float (&w)[8]) {
+        auto residual = [&](uint32_t h, int32_t j, float a, uint32_t ngone, float (&w)[8]) {
             const float k = a * row.q_over_p;
             if constexpr (HELD) {
                 const float kq = k * fq;
@@ -439,16 +455,17 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                 }
             } else {
                 float x[8], y[8];
-                load8(prow, j, p.vocab, x);
-                if (a != 0.0f) load8(qrow, j, p.vocab, y);
+                const bool f = fits(j, vocab);
+                load8(prow, j, vocab, f, x);
+                if (a != 0.0f) load8(qrow, j, vocab, f && q_alike, y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    w[i] = pm == -INFINITY ? 0.0f : mass(x[i], pm, it);
+                    w[i] = mass(x[i], pm, it);
                     if (a != 0.0f && qm != -INFINITY) w[i] = fmaxf(fmaf(-mass(y[i], qm, it), k, w[i]), 0.0f);
                 }
             }
             for (uint32_t g = 0; g < ngone; ++g) {
-                const int64_t d = (int64_t)gone[g] - j;
+                const int32_t d = (int32_t)gone[g] - j;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (d == i) w[i] = 0.0f;
@@ -460,7 +477,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             Pair sum{0.0f, 0.0f};
             auto step = [&](uint32_t h) {
                 float w[8], t = 0.0f;
-                residual(h, (int64_t)(c0 + h) * 256 + j_lane, a, ngone, w);
+                residual(h, at(c0 + h), a, ngone, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t += w[i];
                 sum = plus(sum, {t, 0.0f});
@@ -500,7 +517,9 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                     if (greedy) {
                         if (best && (uint32_t)token[c] == ~(uint32_t)best) { act = kAccept; break; }
                     } else if (sampled) {
-                        if (u * child_q[c] * s_z < fmax(child_p[c] - s_a * child_q[c], 0.0)) { act = kAccept; break; }
+                        // u q Z < max(p - a q, 0), times the sum of p's masses
+                        const double q = child_q[c] * row.q_over_p;
+                        if (u * q * s_z < fmax(child_p[c] - s_a * q, 0.0)) { act = kAccept; break; }
                         s_a += s_z;
                         act = kRefused;
                         break;
@@ -508,8 +527,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                         bool before = false;
                         for (uint32_t g = 0; g < s_gone; ++g) before |= gone[g] == (uint32_t)token[c];
                         if (before) continue;
-                        if (u * s_z < child_p[c]) { act = kAccept; break; }
-                        s_z -= child_p[c];
+                        if (u * s_z < child_p[c] * s_ip) { act = kAccept; break; }
+                        s_z -= child_p[c] * s_ip;
                         gone[s_gone++] = token[c];
                     }
                 }
@@ -572,7 +591,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             const Pair border = s_border;
             uint32_t found = kNoToken, last = kNoToken;
             auto scan = [&](uint32_t h) {
-                const int64_t j = (int64_t)(c0 + h) * 256 + j_lane;
+                const int32_t j = at(c0 + h);
                 float w[8], part[8], t = 0.0f;
                 residual(h, j, a, ngone, w);
                 uint32_t mine = kNoToken, end = kNoToken;
