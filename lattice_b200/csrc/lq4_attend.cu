@@ -44,22 +44,15 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// (a, b) -> one word of bf16 and what the rounding left of each.
-__device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    a -= __low2float(t);
-    b -= __high2float(t);
-    return *reinterpret_cast<const uint32_t*>(&t);
-}
-
 // Byte offset of 16-byte chunk `c` of row `r` in a tile of D-element bf16 rows: the chunk's low bits are mixed
 // with the row's, so that eight rows of one chunk (an ldmatrix) lie in eight different bank groups.
 template <int D>
 __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t c) { return r * (D * 2) + ((c ^ (r & 7)) << 4); }
 
-// More rows than this per kv head and bf16 activations take the tcgen05 kernel: 16 sequences of 8192 tokens, 8 kv heads of
-// 128, 5 rows: 101 us here and 129 us there; 25 rows: 164 us and 128 us; 64 rows: 217 us and 132 us (B200).
-constexpr uint32_t kTcMinRows = 16;
+// More rows than this per kv head take the tcgen05 kernel.  16 sequences of 8192 tokens, 8 kv heads of 128 (B200), bf16: 16
+// rows 108 us here and 126 us there, 25 rows 164 and 128 us, 64 rows 217 and 132 us; f32: 25 rows 238 and 304 us, 64
+// rows 357 and 315 us, 128 rows 691 and 335 us.  (f32 and head_dim above 128: three terms of Q leave no room there.)
+constexpr uint32_t kTcMinRows = 16, kTcMinRowsF32 = 32;
 
 template <int D, int WM, int NQ>
 struct Shape {
@@ -493,10 +486,11 @@ cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorksp
     const uintptr_t q_at = reinterpret_cast<uintptr_t>(a.q), out_at = reinterpret_cast<uintptr_t>(a.out);
     p.q_vec = !(q_at % 16 || a.q_batch % 8 || a.q_node % 8 || a.q_head % 8);
     p.out_vec = !(out_at % 16 || a.out_batch % 8 || a.out_node % 8 || a.out_head % 8);
+    const bool f32 = a.dtype == LQ4_DTYPE_F32;
     ws.need = 0;
     ws.launches = 0;
-    if (a.dtype == LQ4_DTYPE_BF16 && p.nodes * p.group > kTcMinRows) return launch_attend_tc(p, ws, sm_count, use_pdl, s);
-    return a.dtype == LQ4_DTYPE_BF16 ? run_dim<1>(p, ws, sm_count, use_pdl, s) : run_dim<3>(p, ws, sm_count, use_pdl, s);
+    if (p.nodes * p.group > (f32 ? kTcMinRowsF32 : kTcMinRows) && (!f32 || p.head_dim <= 128)) return launch_attend_tc(p, f32, ws, sm_count, use_pdl, s);
+    return !f32 ? run_dim<1>(p, ws, sm_count, use_pdl, s) : run_dim<3>(p, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace lq4

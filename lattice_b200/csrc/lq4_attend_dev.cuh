@@ -85,6 +85,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// (a, b) -> one word of bf16 and what the rounding left of each.
+__device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    a -= __low2float(t);
+    b -= __high2float(t);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
 // A CTA's share of the range of all tiles, and the sequence its first tile lies in.
 struct Range {
     uint64_t begin, end;                       // units; empty: nothing to do
@@ -245,7 +253,7 @@ cudaError_t attend_launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size
 }
 // lq4_attend.cu: joins the partials of a launch with items of `rows` rows and D channels; completes ws.launches.
 cudaError_t launch_attend_join(const AttendParams& p, uint32_t rows, uint32_t D, bool bf16_out, AttendWorkspace& ws, int use_pdl, cudaStream_t s);
-// lq4_attend_tc.cu: bf16 activations, items of 128 rows.
-cudaError_t launch_attend_tc(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s);
+// lq4_attend_tc.cu: items of 128 or 256 rows; f32 activations up to head_dim 128.
+cudaError_t launch_attend_tc(const AttendParams& p, bool f32, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s);
 
 }  // namespace lq4

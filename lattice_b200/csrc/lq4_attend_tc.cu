@@ -1,4 +1,4 @@
-// lq4_tree_attention for bf16 activations and many rows per kv head (a large tree), on the 5th-generation tensor cores.
+// lq4_tree_attention for many rows per kv head (a large tree), on the 5th-generation tensor cores.
 //
 // With R query rows on a key/value head there are R flops per byte of cache, so beyond some 50 rows the HBM
 // stream is no longer the bound and mma.sync (552 TFLOP/s measured here) is; tcgen05.mma has three times that.  The work
@@ -18,11 +18,15 @@
 //   warps 0..4N-1   softmax, four warps per stream: a thread reads its row of S, hands the buffer back at once (the
 //                   stream's next S is computed while this one is exponentiated), writes P, and drains O at the end
 //   next N warps    MMA issue, a warp per stream (the first one allocates tensor memory)
-//   last 4 warps    loaders: cp.async of K and V rows, each looked up through the page table, into one ring of slots
+//   last warps      loaders: cp.async of K and V rows, each looked up through the page table, into one ring of slots
 //                   (K, V, K, V, ...), a warp per tile; they run ahead over the borders of pieces
 //
 // The running maximum only moves when it has grown by more than 2^8 (the final division takes the same base out
 // again), so O is rescaled in tensor memory a few times per sequence instead of per tile.
+//
+// f32 activations (up to D = 128): q and P are three bf16 terms each, 24 bits, smallest products first.  The accumulators
+// in tensor memory cut off below their last bit at every MMA, some 10^-5 over a few hundred of them, so P V of a tile
+// starts from zero and the softmax threads add it to O in their registers; one stream.
 #include "lq4_attend_dev.cuh"
 
 #include <atomic>
@@ -31,7 +35,7 @@ namespace lq4 {
 
 namespace {
 
-constexpr int kTcRows = 128, kLoaders = 128;
+constexpr int kTcRows = 128;
 constexpr float kLazy = 8.0f;                  // how far (log2) a row's maximum may outgrow its base
 
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
@@ -94,6 +98,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32
         "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&u)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+                 "r"(u[6]), "r"(u[7]), "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -115,28 +124,31 @@ __device__ __forceinline__ uint32_t swz(uint32_t rows, uint32_t r, uint32_t c) {
     return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// NS streams; WIDE: items of 256 rows.
-template <int D, int NS, bool WIDE>
+// NS streams; WIDE: items of 256 rows; NQ bf16 terms of q and P: 1 for bf16 activations, 3 for f32.
+template <int D, int NS, bool WIDE, int NQ>
 struct TcShape {
-    static constexpr int kSoftmax = 128 * NS, kThreads = kSoftmax + 32 * NS + kLoaders, kItemRows = WIDE ? 256 : 128;
-    static constexpr uint32_t kSlot = kKeys * D * 2, kQ = kTcRows * D * 2 * (WIDE ? 2 : 1);
+    static constexpr int kSoftmax = 128 * NS, kItemRows = WIDE ? 256 : 128;
+    static constexpr uint32_t kSlot = kKeys * D * 2, kQTerm = kTcRows * D * 2, kQ = kQTerm * (WIDE ? 2 : 1) * NQ;
     // Rings of slots: one that all streams read in order, or one per stream where they take the tiles in turn (a wait on a slot's
     // barrier is only good as long as the reader goes through the slot's uses one by one).
     static constexpr uint32_t kRings = NS == 2 && !WIDE ? 2 : 1;
     static constexpr uint32_t kFit = ((uint32_t)kMaxSmem - kQ - 5120) / kSlot / kRings, kRing = kFit > 12 / kRings ? 12 / kRings : kFit, kSlots = kRing * kRings;
     static constexpr uint32_t kValid = kSlots * kSlot + kQ, kFixes = kValid + 16 * 8, kAnc = kFixes + 16 * 8, kMeet = kAnc + kMaxNodes * 8;
     static constexpr uint32_t kBars = kMeet + kTcRows * 8, kCtl = kBars + 56 * 8, kSmem = kCtl + 160 + 1024;      // + alignment slack
-    static constexpr uint32_t kColO = 0, kColS = NS * D, kColP = kColS + NS * 64, kCols = kColP + NS * 32 <= 256 ? 256 : 512;
-    static constexpr uint32_t kTeams = kSlots >= 8 ? 4 : 2, kTeam = 4 / kTeams;      // loaders: teams, warps of a team
-    static_assert(2 * kTeams / kRings <= kRing && kLoaders == 128, "a team's next tile is at most a ring ahead of its last one");
-    static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kColP + NS * 32 <= 512, "shared or tensor memory");
+    static constexpr uint32_t kColO = 0, kColS = NS * D, kColP = kColS + NS * 64, kCols = kColP + NS * 32 * NQ <= 256 ? 256 : 512;
+    // Loaders: teams, warps of a team.  (Seven warps for three terms: with nine a thread has 168 registers, and O spills.)
+    static constexpr uint32_t kTeams = NQ == 1 && kSlots >= 8 ? 4 : 2, kTeam = NQ == 1 ? 4 / kTeams : 1;
+    static constexpr int kLoaders = 32 * kTeams * kTeam, kThreads = kSoftmax + 32 * NS + kLoaders;
+    static_assert(2 * kTeams / kRings <= kRing, "a team's next tile is at most a ring ahead of its last one");
+    static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kColP + NS * 32 * NQ <= 512, "shared or tensor memory");
+    static_assert(NQ == 1 || NS == 1, "three terms take one stream");
     static_assert(NS == 2 || !WIDE, "256 rows take two streams");
     static_assert(kTcRows * 32 * 4 <= kQ, "the streams meet in Q's place");
 };
 
-template <int D, int NS, bool WIDE>
-__global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc_kernel(const __grid_constant__ AttendParams p) {
-    using S = TcShape<D, NS, WIDE>;
+template <int D, int NS, bool WIDE, int NQ>
+__global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) attend_tc_kernel(const __grid_constant__ AttendParams p) {
+    using S = TcShape<D, NS, WIDE, NQ>;
     constexpr int CPR = D / 8, kSoftmax = S::kSoftmax, kMmaWarp = kSoftmax / 32;
     constexpr uint32_t SL = S::kSlots, RING = S::kRing, RINGS = S::kRings;
     extern __shared__ unsigned char smem_raw[];
@@ -210,25 +222,51 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
 #pragma unroll 4
             for (uint32_t i = tid; i < S::kItemRows * CPR; i += kSoftmax) {
                 const uint32_t qr = i / CPR, c = i % CPR, qrow = x.rt * S::kItemRows + qr, qt = qrow / p.group, qg = qrow - qt * p.group;
-                uint32_t w[4] = {0, 0, 0, 0};
-                if (qrow < rows && (int32_t)qt < x.sq.nodes && c * 8 < p.head_dim) {
-                    const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.q_batch + qt * p.q_node + (uint64_t)(x.h * p.group + qg) * p.q_head + c * 8;
-                    if (p.q_vec) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(src);
-                        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                    } else {
+                const bool here = qrow < rows && (int32_t)qt < x.sq.nodes && c * 8 < p.head_dim;
+                const uint64_t from = b * p.q_batch + qt * p.q_node + (uint64_t)(x.h * p.group + qg) * p.q_head + c * 8;
+                const uint32_t to = SL * S::kSlot + (qr >> 7) * S::kQTerm + swz(kTcRows, qr & 127, c);
+                if constexpr (NQ == 1) {
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    if (here) {
+                        const uint16_t* src = static_cast<const uint16_t*>(p.q) + from;
+                        if (p.q_vec) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(src);
+                            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-                    }
-                    if (p.q_sign != 1.0f) {
+                            for (int e = 0; e < 4; ++e) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
+                        }
+                        if (p.q_sign != 1.0f) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(w[e] << 16) * p.q_sign, __uint_as_float(w[e] & 0xffff0000u) * p.q_sign);
-                            w[e] = *reinterpret_cast<const uint32_t*>(&y);
+                            for (int e = 0; e < 4; ++e) {
+                                const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(w[e] << 16) * p.q_sign, __uint_as_float(w[e] & 0xffff0000u) * p.q_sign);
+                                w[e] = *reinterpret_cast<const uint32_t*>(&y);
+                            }
                         }
                     }
+                    *reinterpret_cast<uint4*>(smem + to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                    if (here) {
+                        const float* src = static_cast<const float*>(p.q) + from;
+                        if (p.q_vec) {
+                            const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
+                            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = src[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] *= p.q_sign;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = split_pair(v[2 * e], v[2 * e + 1]);
+                        *reinterpret_cast<uint4*>(smem + to + n * S::kQTerm) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
-                *reinterpret_cast<uint4*>(smem + SL * S::kSlot + (qr >> 7) * (kTcRows * D * 2) + swz(kTcRows, qr & 127, c)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             if (x.has_nodes && tid < p.nodes) {
                 bool bad = false;
@@ -241,6 +279,21 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
 
             float m = -INFINITY, l = 0.0f;                               // base (log2) and sum of this row
             bool first = true;
+            float acc[NQ == 1 ? 1 : D];                                  // f32 activations: O
+            auto fold = [&]() {                                          // O += the tile's P V
+                if constexpr (NQ > 1) {
+#pragma unroll
+                    for (int d = 0; d < D; d += 32) {
+                        float o[32];
+                        tmem_ld32<0>(col_o + d, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) acc[d + e] += o[e];
+                    }
+                }
+            };
+#pragma unroll
+            for (int d = 0; d < (NQ == 1 ? 1 : D); ++d) acc[d] = 0.0f;
             for (uint32_t i = RINGS == 2 ? (str - tile) & 1 : 0; i < x.n_tiles; i += RINGS) {      // (tile n belongs to stream n & 1)
                 const uint32_t n = tile + i;
                 wait(info + (n & 15), (n >> 4) & 1);                     // `valid` of this tile is there
@@ -276,7 +329,16 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 if (!first) wait(o_done + str, (used - 1) & 1);
                 __syncwarp();
                 tc_fence_after();
-                if (first) {
+                if constexpr (NQ > 1) {
+                    if (!first) fold();
+                    if (__any_sync(0xffffffffu, top > m)) {
+                        const float up = fmaxf(m, top), f = m == up ? 1.0f : exp2_fast(m - up);      // (m -inf: 0)
+                        l *= f;
+                        m = up;
+#pragma unroll
+                        for (int d = 0; d < D; ++d) acc[d] *= f;
+                    }
+                } else if (first) {
                     m = top;
                 } else {
                     const bool grow = top > m + kLazy;                   // (m -inf: at the first finite score)
@@ -299,17 +361,36 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
                 float sum0 = 0.0f, sum1 = 0.0f;
-                uint32_t w[32];
+                if constexpr (NQ == 1) {
+                    uint32_t w[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float a = exp2_fast(fmaf(s[2 * j], p.scale_log2, -base)), c = exp2_fast(fmaf(s[2 * j + 1], p.scale_log2, -base));
-                    sum0 += a;
-                    sum1 += c;
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(a, c);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&y);
+                    for (int j = 0; j < 32; ++j) {
+                        const float a = exp2_fast(fmaf(s[2 * j], p.scale_log2, -base)), c = exp2_fast(fmaf(s[2 * j + 1], p.scale_log2, -base));
+                        sum0 += a;
+                        sum1 += c;
+                        const __nv_bfloat162 y = __floats2bfloat162_rn(a, c);
+                        w[j] = *reinterpret_cast<const uint32_t*>(&y);
+                    }
+                    tmem_st32(col_p, w);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {                        // 16 keys at a time
+                        float e[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            e[j] = exp2_fast(fmaf(s[16 * k + j], p.scale_log2, -base));
+                            (j & 1 ? sum1 : sum0) += e[j];
+                        }
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) w[j] = split_pair(e[2 * j], e[2 * j + 1]);
+                            tmem_st8(col_p + 32 * n + 8 * k, w);
+                        }
+                    }
                 }
                 l += sum0 + sum1;
-                tmem_st32(col_p, w);
                 tmem_st_wait();
                 // the nodes' tile: `fixes` comes with V, whose slot is not filled again before this P is handed over
                 if (x.t0 + i + 1 == x.sq.tiles) wait(full + (n & (RINGS - 1)) * RING + (2 * (n / RINGS) + 1) % RING, (2 * (n / RINGS) + 1) / RING & 1);
@@ -322,6 +403,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             if (!first) wait(o_done + str, (used - 1) & 1);
             __syncwarp();
             tc_fence_after();
+            if (NQ > 1 && !first) fold();
             // ---- O of this piece: the result, or a partial.  Two streams over the keys: stream 1 hands its O to stream 0
             // through Q's place, 32 columns at a time (both have waited for all MMAs of their own that read Q; the
             // barrier below covers the other's).
@@ -346,6 +428,56 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             if (!whole && live && (!kMeets || str == 0)) p.part_ml[slot] = make_float2(m, l);
             const uint64_t to = b * p.out_batch + t * p.out_node + (uint64_t)(x.h * p.group + g) * p.out_head;
             float* pass = reinterpret_cast<float*>(smem + SL * S::kSlot) + r;      // [columns][128]: lanes side by side
+            auto put = [&](int d, float (&o)[32]) {                      // 32 columns of this row
+                if (fix) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (d + e < (int)p.head_dim) o[e] += nonfinite_sum(p, x, anc[t], d + e);
+                }
+                if (!whole) {
+                    float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        if (d + e >= (int)p.head_dim) break;             // (a multiple of 8)
+                        if constexpr (NQ > 1) {
+                            float* out = static_cast<float*>(p.out) + to + d + e;
+                            if (p.out_vec) {
+                                reinterpret_cast<float4*>(out)[0] = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                                reinterpret_cast<float4*>(out)[1] = make_float4(o[e + 4] * inv, o[e + 5] * inv, o[e + 6] * inv, o[e + 7] * inv);
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) out[k] = o[e + k] * inv;
+                            }
+                            continue;
+                        }
+                        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + to + d;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
+                            w[k] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                        if (p.out_vec) {
+                            *reinterpret_cast<uint4*>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) out[e + k] = __ushort_as_bfloat16((unsigned short)(w[k >> 1] >> (16 * (k & 1))));
+                        }
+                    }
+                }
+            };
+            if constexpr (NQ > 1) {
+#pragma unroll
+                for (int d = 0; d < D; d += 32) {
+                    float o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = acc[d + e];
+                    if (live) put(d, o);
+                }
+            } else {
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
                 float o[32];
@@ -370,35 +502,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                     for (int e = 0; e < 32; ++e) o[e] = o[e] * f + (f_other == 0.0f ? 0.0f : pass[e * 128] * f_other);
                     named_bar_sync(4, 256);
                 }
-                if (!live) continue;
-                if (fix) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (d + e < (int)p.head_dim) o[e] += nonfinite_sum(p, x, anc[t], d + e);
-                }
-                if (!whole) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + d);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                } else {
-                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + to + d;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        if (d + e >= (int)p.head_dim) break;             // (a multiple of 8)
-                        uint32_t w[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const __nv_bfloat162 y = __floats2bfloat162_rn(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
-                            w[k] = *reinterpret_cast<const uint32_t*>(&y);
-                        }
-                        if (p.out_vec) {
-                            *reinterpret_cast<uint4*>(out + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) out[e + k] = __ushort_as_bfloat16((unsigned short)(w[k >> 1] >> (16 * (k & 1))));
-                        }
-                    }
-                }
+                if (live) put(d, o);
+            }
             }
             __syncwarp();
             tc_fence_before();
@@ -417,7 +522,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
         const uint32_t tm = uniform(tmem), ring = uniform(sbase) >> 4;
         const uint32_t col_s = tm + S::kColS + str * 64, col_p = tm + S::kColP + str * 32, col_o = tm + S::kColO + str * D;
         const uint64_t kmajor = smem_desc(0, 16), mnmajor = smem_desc(0, kKeys * 128);
-        const uint64_t q = kmajor + (uniform(qbase) >> 4) + (WIDE ? str * (kTcRows * D * 2 >> 4) : 0);
+        const uint64_t q = kmajor + (uniform(qbase) >> 4) + (WIDE ? str * (S::kQTerm >> 4) : 0);
         struct Ring {
             uint32_t slot, phase;
             __device__ __forceinline__ void move(uint32_t groups) {
@@ -438,8 +543,10 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
             const uint64_t k = kmajor + (ring + (ring0 + kr.slot) * (S::kSlot >> 4));
             if (leader) {
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    mma_ss(col_s, q + ((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32 >> 4), k + ((ks >> 2) * (kKeys * 128) + (ks & 3) * 32 >> 4), instr_desc(kKeys, 0), ks > 0);
+                for (int ks = 0; ks < NQ * (D / 16); ++ks) {             // the smallest term first
+                    const int n = NQ - 1 - ks / (D / 16), c = ks % (D / 16) >> 2, in = (ks & 3) * 32;
+                    mma_ss(col_s, q + (n * S::kQTerm + c * (kTcRows * 128) + in >> 4), k + (c * (kKeys * 128) + in >> 4), instr_desc(kKeys, 0), ks > 0);
+                }
                 mma_commit(empty + ring0 + kr.slot);
                 mma_commit(s_full + str);
             }
@@ -461,7 +568,10 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
                 const uint64_t vt = mnmajor + (ring + (ring0 + vr.slot) * (S::kSlot >> 4));
                 if (leader) {
 #pragma unroll
-                    for (int ks = 0; ks < (int)kKeys / 16; ++ks) mma_ts(col_o, col_p + ks * 8, vt + (ks * 2048 >> 4), instr_desc(D, 1), v > 0 || ks > 0);
+                    for (int ks = 0; ks < NQ * ((int)kKeys / 16); ++ks) {
+                        const int n = NQ - 1 - ks / 4, c = ks & 3;
+                        mma_ts(col_o, col_p + n * 32 + c * 8, vt + (c * 2048 >> 4), instr_desc(D, 1), (NQ == 1 && v > 0) || ks > 0);
+                    }
                     mma_commit(empty + ring0 + vr.slot);
                     mma_commit(o_done + str);
                 }
@@ -481,8 +591,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
         // holds where its keys lie; table index and slot advance without a division, and the page ids are fetched one turn ahead.
         // A team's next tile is at most half a ring ahead of its last one, so that a slot's barrier is never two phases off.
         constexpr uint32_t kWarps = S::kTeams, kOn = kWarps * kKeys, kHold = 2 / S::kTeam, kCopies = kHold * CPR;
-        const uint32_t lw = (warp - (S::kThreads - kLoaders) / 32) / S::kTeam;      // team
-        const uint32_t key0 = ((warp - (S::kThreads - kLoaders) / 32) % S::kTeam) * 32;      // this warp's first key of a tile
+        const uint32_t lw = (warp - (S::kThreads - S::kLoaders) / 32) / S::kTeam;      // team
+        const uint32_t key0 = ((warp - (S::kThreads - S::kLoaders) / 32) % S::kTeam) * 32;      // this warp's first key of a tile
         struct Ring {
             uint32_t slot, phase;                                        // phase: of `empty` before the slot is filled again
             __device__ __forceinline__ void move(uint32_t groups) {
@@ -591,27 +701,28 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE>::kThreads), 1) attend_tc
     if (warp == kMmaWarp) tmem_dealloc(tmem, S::kCols);
 }
 
-template <int D, int NS, bool WIDE>
+template <int D, int NS, bool WIDE, int NQ>
 cudaError_t run(AttendParams p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    using S = TcShape<D, NS, WIDE>;
+    using S = TcShape<D, NS, WIDE, NQ>;
     static DeviceOnce once;
-    auto fn = attend_tc_kernel<D, NS, WIDE>;
+    auto fn = attend_tc_kernel<D, NS, WIDE, NQ>;
     cudaError_t e = opt_in_smem(reinterpret_cast<const void*>(fn), S::kSmem, once);
     if (e != cudaSuccess) return e;
     p.grid = (uint32_t)sm_count;
     p.row_tiles = (p.nodes * p.group + S::kItemRows - 1) / S::kItemRows;
     if (!attend_workspace(p, ws, S::kItemRows, D)) return cudaSuccess;
     if ((e = attend_launch(fn, dim3(p.grid), S::kThreads, S::kSmem, use_pdl, s, p)) != cudaSuccess) return e;
-    return launch_attend_join(p, S::kItemRows, D, true, ws, use_pdl, s);
+    return launch_attend_join(p, S::kItemRows, D, NQ == 1, ws, use_pdl, s);
 }
 
 }  // namespace
 
-cudaError_t launch_attend_tc(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
+cudaError_t launch_attend_tc(const AttendParams& p, bool f32, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
     const bool wide = p.nodes * p.group > (uint32_t)kTcRows;
-    if (p.head_dim <= 64) return wide ? run<64, 2, true>(p, ws, sm_count, use_pdl, s) : run<64, 2, false>(p, ws, sm_count, use_pdl, s);
-    if (p.head_dim <= 128) return wide ? run<128, 2, true>(p, ws, sm_count, use_pdl, s) : run<128, 2, false>(p, ws, sm_count, use_pdl, s);
-    return run<256, 1, false>(p, ws, sm_count, use_pdl, s);
+    if (f32) return p.head_dim <= 64 ? run<64, 1, false, 3>(p, ws, sm_count, use_pdl, s) : run<128, 1, false, 3>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 64) return wide ? run<64, 2, true, 1>(p, ws, sm_count, use_pdl, s) : run<64, 2, false, 1>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 128) return wide ? run<128, 2, true, 1>(p, ws, sm_count, use_pdl, s) : run<128, 2, false, 1>(p, ws, sm_count, use_pdl, s);
+    return run<256, 1, false, 1>(p, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace lq4

@@ -5,10 +5,10 @@
 // rope_kernel: pair i of a head is a complex number turned by the angle pos * freq[i].  The angle of a far
 // position does not fit f32 (10^6 radians leave 2^-4 of a turn), so it is formed in f64 as a number of
 // TURNS, its whole part is dropped there, and only the remainder in [-1/2, 1/2] goes to f32 and sincospi:
-// three f64 operations per (row, pair), shared by all heads of the row through shared memory.  A CTA takes a
-// few rows (256 angles, one per thread) and all heads, or a slice of the heads when the rows alone would not
-// fill the GPU; a thread moves 2V elements per step (V pairs: both halves are in its registers before it
-// stores, so the call may work in place).
+// three f64 operations per (row, pair), shared by the heads of a CTA through shared memory.  A CTA takes a
+// few rows (256 angles, one per thread) and the heads of one tensor, or a slice of them when the rows alone would not
+// fill the GPU; a thread keeps its place in the head and has 64 to 128 bytes of several heads under way at a time (V
+// pairs per step: both halves are in its registers before it stores, so the call may work in place).
 #include "lq4_attend.cuh"
 
 #include <cuda_bf16.h>
@@ -18,52 +18,65 @@ namespace lq4 {
 namespace {
 
 constexpr uint32_t kRopeThreads = 256;
-constexpr uint32_t kRopeMaxPairs = 512;        // head_dim <= 1024
 
 struct RopeParams {
     lq4_rope_part part[LQ4_MAX_ROPE_PARTS];
+    uint32_t first_cta[LQ4_MAX_ROPE_PARTS];    // of a part, along grid.y
     uint32_t n_parts, rows, head_dim, half;    // half = rot_dim / 2
-    uint32_t heads;                            // of all parts together
     uint32_t rows_per_cta, heads_per_cta;
+    uint32_t lanes;                            // threads of a head, a power of two
     const int32_t* positions;
     const double* freq;
     int32_t interleaved;
     float scale;
 };
 
-// V consecutive elements, f32 or bf16 in memory, f32 in registers.
+// V consecutive elements of type T (float or bf16 bits): fetched as they lie in memory, and read as f32.
+template <typename T, int V>
+struct Raw {
+    uint32_t w[V * sizeof(T) / 4 ? V * sizeof(T) / 4 : 1];
+};
+template <typename T, int V>
+__device__ __forceinline__ void fetch_vec(const T* p, Raw<T, V>& r) {
+    constexpr int kBytes = V * sizeof(T);
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) {
+            const uint4 t = reinterpret_cast<const uint4*>(p)[i];
+            r.w[4 * i] = t.x, r.w[4 * i + 1] = t.y, r.w[4 * i + 2] = t.z, r.w[4 * i + 3] = t.w;
+        }
+    } else if constexpr (kBytes == 8) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = t.x, r.w[1] = t.y;
+    } else if constexpr (kBytes == 4) {
+        r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+        r.w[0] = (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void read_vec(const Raw<T, V>& r, float (&v)[V]) {
+    if constexpr (sizeof(T) == 4 || V == 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __uint_as_float(r.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+        }
+    }
+}
 template <int V>
 __device__ __forceinline__ void load_vec(const void* base, int dtype, uint64_t at, float (&v)[V]) {
     if (dtype == LQ4_DTYPE_F32) {
-        const float* p = static_cast<const float*>(base) + at;
-        if constexpr (V >= 4) {
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i) {
-                const float4 t = reinterpret_cast<const float4*>(p)[i];
-                v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
-            }
-        } else {
-            v[0] = p[0];
-        }
+        Raw<float, V> r;
+        fetch_vec<float, V>(static_cast<const float*>(base) + at, r);
+        read_vec<float, V>(r, v);
     } else {
-        const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-        if constexpr (V >= 4) {
-            uint32_t w[V / 2];
-            if constexpr (V == 8) {
-                const uint4 t = *reinterpret_cast<const uint4*>(p);
-                w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
-            } else {
-                const uint2 t = *reinterpret_cast<const uint2*>(p);
-                w[0] = t.x, w[1] = t.y;
-            }
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        } else {
-            v[0] = bf16_to_f32(p[0]);
-        }
+        Raw<uint16_t, V> r;
+        fetch_vec<uint16_t, V>(static_cast<const uint16_t*>(base) + at, r);
+        read_vec<uint16_t, V>(r, v);
     }
 }
 
@@ -94,75 +107,100 @@ __device__ __forceinline__ void store_vec(void* base, int dtype, uint64_t at, co
     }
 }
 
+// The heads [head0, head0 + nheads) of one tensor, rows [row0, row0 + nrows): see above.
+template <typename T, int V>
+__device__ __forceinline__ void rope_heads(const RopeParams& p, const lq4_rope_part& t, const float2* cs, uint32_t row0, uint32_t nrows,
+                                           uint32_t head0, uint32_t nheads) {
+    constexpr int kItems = sizeof(T) == 4 ? 2 : 4;                        // (row, head) items of a thread at a time
+    const bool turns = t.turn != 0;
+    // units of a head: half / V pair units of 2V elements, then the copied tail (or all of the head) in units of V
+    const uint32_t pair_units = turns ? p.half / V : 0, units = pair_units + (p.head_dim - 2 * V * pair_units) / V;
+    const uint32_t step = kRopeThreads / p.lanes, off = p.interleaved ? V : p.half;
+    const float sign = t.turn < 0 ? -1.0f : 1.0f;
+    const T* const x = static_cast<const T*>(t.x) + row0 * t.x_row + head0 * t.x_head;
+    const uint64_t out = row0 * t.out_row + head0 * t.out_head;
+    for (uint32_t u = threadIdx.x & (p.lanes - 1); u < units; u += p.lanes) {
+        const bool pair = u < pair_units;
+        const uint32_t e = pair ? (p.interleaved ? 2 * u * V : u * V) : (u + pair_units) * V;
+        uint32_t r = 0, h = threadIdx.x / p.lanes;
+        while (h >= nheads) h -= nheads, ++r;
+        while (r < nrows) {
+            Raw<T, V> first[kItems], second[kItems];
+            uint32_t row[kItems], head[kItems];
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                while (h >= nheads) h -= nheads, ++r;
+                row[k] = r, head[k] = h;
+                if (r < nrows) {
+                    const T* src = x + r * t.x_row + h * t.x_head + e;
+                    fetch_vec<T, V>(src, first[k]);
+                    if (pair) fetch_vec<T, V>(src + off, second[k]);
+                }
+                h += step;
+            }
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                if (row[k] >= nrows) break;
+                const uint64_t dst = out + row[k] * t.out_row + head[k] * t.out_head + e;
+                float a[V], b[V];
+                read_vec<T, V>(first[k], a);
+                if (pair) {
+                    read_vec<T, V>(second[k], b);
+                    const float2* c = cs + row[k] * p.half + u * V;
+                    if (p.interleaved) {
+                        // pairs (v[2i], v[2i + 1]) over the 2V consecutive elements a | b
+                        float v[2 * V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) v[j] = a[j], v[V + j] = b[j];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            const float cn = c[j].x, sn = c[j].y * sign, x1 = v[2 * j], x2 = v[2 * j + 1];
+                            v[2 * j] = x1 * cn - x2 * sn;
+                            v[2 * j + 1] = x1 * sn + x2 * cn;
+                        }
+#pragma unroll
+                        for (int j = 0; j < V; ++j) a[j] = v[j], b[j] = v[V + j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            const float cn = c[j].x, sn = c[j].y * sign, x1 = a[j], x2 = b[j];
+                            a[j] = x1 * cn - x2 * sn;
+                            b[j] = x1 * sn + x2 * cn;
+                        }
+                    }
+                    store_vec<V>(t.out, t.out_dtype, dst + off, b);
+                }
+                store_vec<V>(t.out, t.out_dtype, dst, a);
+            }
+            while (h >= nheads) h -= nheads, ++r;
+        }
+    }
+}
+
 template <int V>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeParams p) {
     extern __shared__ float2 cs[];                                        // [rows_per_cta][half] (cos, sin), times scale
-    const uint32_t tid = threadIdx.x;
-    const uint32_t row0 = blockIdx.x * p.rows_per_cta;
-    const uint32_t nrows = min(p.rows_per_cta, p.rows - row0);
-    const uint32_t head0 = blockIdx.y * p.heads_per_cta;
-    const uint32_t nheads = min(p.heads_per_cta, p.heads - head0);
+    uint32_t part = p.n_parts - 1;
+    while (blockIdx.y < p.first_cta[part]) --part;
+    const lq4_rope_part t = p.part[part];
+    const uint32_t row0 = blockIdx.x * p.rows_per_cta, nrows = min(p.rows_per_cta, p.rows - row0);
+    const uint32_t head0 = (blockIdx.y - p.first_cta[part]) * p.heads_per_cta, nheads = min(p.heads_per_cta, t.heads - head0);
     pdl_wait_prior_grids();
-    for (uint32_t i = tid; i < nrows * p.half; i += kRopeThreads) {
-        const uint32_t r = i / p.half, pair = i - r * p.half;
-        double turns = (double)p.positions[row0 + r] * p.freq[pair] * 0.15915494309189533577;      // over 2 pi
-        turns -= rint(turns);
-        float sn, cn;
-        sincospif(2.0f * (float)turns, &sn, &cn);
-        cs[i] = make_float2(cn * p.scale, sn * p.scale);
-    }
-    __syncthreads();
-    // units of a head: half / V pair units of 2V elements, then the copied tail in units of V
-    const uint32_t pair_units = p.half / V, units = pair_units + (p.head_dim - 2 * p.half) / V;
-    const uint32_t copy_units = p.head_dim / V;                           // of a part that does not turn (>= units)
-    const uint32_t per_row = nheads * copy_units, total = nrows * per_row;
-    for (uint32_t i = tid; i < total; i += kRopeThreads) {
-        const uint32_t r = i / per_row, rest = i - r * per_row;
-        uint32_t h = rest / copy_units;
-        const uint32_t u = rest - h * copy_units;
-        h += head0;
-        uint32_t part = 0;
-        while (h >= p.part[part].heads) h -= p.part[part++].heads;
-        const lq4_rope_part& t = p.part[part];
-        const uint64_t src = (uint64_t)(row0 + r) * t.x_row + (uint64_t)h * t.x_head;
-        const uint64_t dst = (uint64_t)(row0 + r) * t.out_row + (uint64_t)h * t.out_head;
-        if (t.turn == 0 || (u >= pair_units && u < units)) {
-            const uint32_t e = t.turn == 0 ? u * V : 2 * p.half + (u - pair_units) * V;
-            float v[V];
-            load_vec<V>(t.x, t.x_dtype, src + e, v);
-            store_vec<V>(t.out, t.out_dtype, dst + e, v);
-        } else if (u < pair_units) {
-            const uint32_t e0 = p.interleaved ? 2 * u * V : u * V, e1 = p.interleaved ? e0 + V : e0 + p.half;
-            float a[V], b[V];
-            load_vec<V>(t.x, t.x_dtype, src + e0, a);
-            load_vec<V>(t.x, t.x_dtype, src + e1, b);
-            const float2* c = cs + r * p.half + u * V;
-            const float sign = t.turn < 0 ? -1.0f : 1.0f;
-            if (p.interleaved) {
-                // pairs (v[2i], v[2i + 1]) over the 2V consecutive elements a | b
-                float v[2 * V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = a[j], v[V + j] = b[j];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float cn = c[j].x, sn = c[j].y * sign, x1 = v[2 * j], x2 = v[2 * j + 1];
-                    v[2 * j] = x1 * cn - x2 * sn;
-                    v[2 * j + 1] = x1 * sn + x2 * cn;
-                }
-#pragma unroll
-                for (int j = 0; j < V; ++j) a[j] = v[j], b[j] = v[V + j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float cn = c[j].x, sn = c[j].y * sign, x1 = a[j], x2 = b[j];
-                    a[j] = x1 * cn - x2 * sn;
-                    b[j] = x1 * sn + x2 * cn;
-                }
-            }
-            store_vec<V>(t.out, t.out_dtype, dst + e0, a);
-            store_vec<V>(t.out, t.out_dtype, dst + e1, b);
+    if (t.turn != 0) {
+        for (uint32_t i = threadIdx.x; i < nrows * p.half; i += kRopeThreads) {
+            const uint32_t r = i / p.half, pair = i - r * p.half;
+            double turns = (double)p.positions[row0 + r] * p.freq[pair] * 0.15915494309189533577;      // over 2 pi
+            turns -= rint(turns);
+            float sn, cn;
+            sincospif(2.0f * (float)turns, &sn, &cn);
+            cs[i] = make_float2(cn * p.scale, sn * p.scale);
         }
+        __syncthreads();
     }
+    if (t.x_dtype == LQ4_DTYPE_F32)
+        rope_heads<float, V>(p, t, cs, row0, nrows, head0, nheads);
+    else
+        rope_heads<uint16_t, V>(p, t, cs, row0, nrows, head0, nheads);
     pdl_launch_dependents();
 }
 
@@ -255,10 +293,11 @@ bool vec_fits(const lq4_rope_args& a, uint32_t half, uint32_t vec) {
 
 cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, cudaStream_t s) {
     RopeParams p{};
+    uint32_t heads = 0;
     for (uint32_t i = 0; i < a.n_parts; ++i) {
         if (!a.parts[i].heads) continue;
         p.part[p.n_parts++] = a.parts[i];
-        p.heads += a.parts[i].heads;
+        heads += a.parts[i].heads;
     }
     p.rows = a.rows;
     p.head_dim = a.head_dim;
@@ -270,18 +309,25 @@ cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, 
         p.scale = a.rope->scale;
     }
     const uint32_t vec = vec_fits(a, p.half, 8) ? 8 : vec_fits(a, p.half, 4) ? 4 : 1;
-    // one angle per thread, at most as many rows as there are; heads are split while the CTAs do not fill
-    // the GPU twice and a CTA still has a unit for every thread
+    // one angle per thread, at most as many rows as there are; heads are split while the CTAs do not fill the GPU
+    // four times over and a CTA still has a unit for every thread
     p.rows_per_cta = p.half ? kRopeThreads / p.half : 4;
     if (p.rows_per_cta == 0) p.rows_per_cta = 1;
     if (p.rows_per_cta > p.rows) p.rows_per_cta = p.rows;
     const uint32_t row_ctas = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
-    uint32_t splits = (2u * sm_count + row_ctas - 1) / row_ctas;
-    const uint32_t units = p.rows_per_cta * p.heads * (p.head_dim / vec), most = (units + kRopeThreads - 1) / kRopeThreads;
+    uint32_t splits = (4u * sm_count + row_ctas - 1) / row_ctas;
+    const uint32_t units = p.rows_per_cta * heads * (p.head_dim / vec), most = (units + kRopeThreads - 1) / kRopeThreads;
     if (splits > most) splits = most;
-    if (splits > p.heads) splits = p.heads;
-    p.heads_per_cta = (p.heads + splits - 1) / splits;
-    const dim3 grid(row_ctas, (p.heads + p.heads_per_cta - 1) / p.heads_per_cta);
+    if (splits > heads) splits = heads;
+    p.heads_per_cta = (heads + splits - 1) / splits;
+    uint32_t ctas = 0;
+    for (uint32_t i = 0; i < p.n_parts; ++i) {
+        p.first_cta[i] = ctas;
+        ctas += (p.part[i].heads + p.heads_per_cta - 1) / p.heads_per_cta;
+    }
+    p.lanes = 1;
+    while (p.lanes < kRopeThreads && p.lanes < a.head_dim / vec) p.lanes <<= 1;
+    const dim3 grid(row_ctas, ctas);
     const size_t smem = (size_t)p.rows_per_cta * p.half * sizeof(float2);
     auto fn = vec == 8 ? rope_kernel<8> : vec == 4 ? rope_kernel<4> : rope_kernel<1>;
     return launch(fn, grid, kRopeThreads, smem, use_pdl, s, p);

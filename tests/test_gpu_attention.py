@@ -61,7 +61,7 @@ def assert_rope(got, ref, mag):
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("rows, heads, dim, rot, src, dst", [
     (1, 1, 8, 2, F32, F32), (1, 40, 128, 128, F32, BF16), (3, 5, 80, 20, BF16, F32), (7, 2, 130, 6, F32, F32), (257, 3, 64, 64, BF16, BF16),
-    (33, 24, 256, 64, BF16, BF16), (2, 1, 1024, 1024, F32, F32), (1000, 1, 6, 4, F32, BF16), (5, 3, 72, 16, BF16, BF16),
+    (33, 24, 256, 64, BF16, BF16), (2, 1, 1024, 1024, F32, F32), (1000, 1, 6, 4, F32, BF16), (5, 3, 72, 16, BF16, BF16), (9, 3, 602, 300, F32, BF16), (40, 7, 1022, 10, BF16, F32),
 ])
 def test_rope_against_64_bits(be, layout, rows, heads, dim, rot, src, dst):
     from lattice_b200 import RopeTable, rope_frequencies
@@ -346,9 +346,11 @@ def test_attention_ragged_batch_with_dead_rows(be, dtype):
     attend_case(be, 40, 8, 6, 6, 3, 64, 16, lens, dtype, counts=counts, width=3)
 
 
-def test_attention_large_ragged_batch(be):
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nodes, hq", [(2, 2), (5, 8)])
+def test_attention_large_ragged_batch(be, nodes, hq, dtype):
     lens = [(37 * i) % 300 - 1 for i in range(300)]
-    attend_case(be, 41, 300, 2, 2, 1, 64, 32, lens, BF16, poison=False)
+    attend_case(be, 41, 300, nodes, hq, 1, 64, 32, lens, dtype, poison=False)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -356,6 +358,36 @@ def test_attention_long_sequences_are_split(be, dtype):
     """One item over every CTA, with a border inside a page; chains and trees."""
     attend_case(be, 42, 1, 4, 4, 1, 128, 48, [20011], dtype, width=2)
     attend_case(be, 43, 2, 7, 5, 1, 256, 16, [3000, 9000], dtype, chain=True)
+    attend_case(be, 45, 1, 16, 8, 1, 128, 48, [20011], dtype, width=3)
+    attend_case(be, 46, 2, 64, 8, 2, 64, 5, [5000, 777], dtype, width=5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 128, 129, 256, 257])
+def test_attention_rows_at_the_kernels_borders(be, dtype, rows):
+    """Rows per kv head where another kernel or another number of row tiles takes over: one node of `rows` query heads."""
+    attend_case(be, rows, 2, 1, rows, 1, 72, 16, [70, 129], dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nodes, hq, d", [(3, 4, 64), (5, 24, 64), (64, 6, 128), (9, 8, 256)])
+def test_attention_unaligned_rows(be, nodes, hq, d, dtype):
+    """q and out with odd strides and offsets, which no vector access fits."""
+    b, hk = 2, 2
+    cache = make_cache(b, 8, 16, hk, d, seed=55)
+    q = (2 * normal(56, b, nodes, hq, d)).to(dtype)
+    k, v = normal(57, b, nodes, hk, d).to(BF16), normal(58, b, nodes, hk, d).to(BF16)
+    shape, stride = (b, nodes, hq, d), (nodes * (hq * (d + 1) + 3) + 1, hq * (d + 1) + 3, d + 1, 1)
+    room = torch.zeros(2, b * stride[0] + 8, dtype=dtype).cuda()
+    qs, out = torch.as_strided(room[0], shape, stride, 1), torch.as_strided(room[1], shape, stride, room.shape[1] + 3)
+    qs.copy_(q)
+    lens, par = [100, 65], random_tree(59, b, nodes, 2)
+    dev = lambda x: torch.as_tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    got = be.tree_attention(qs, k.cuda(), v.cuda(), cache, dev(lens), parents=dev(par), out=out)
+    ref = attend_ref(q, k, v, cache.k.cpu(), cache.v.cpu(), cache.page_table.cpu(), lens, par, None, d ** -0.5)
+    assert_attention(got, *ref, 164)
+    room[1].as_strided(shape, stride, room.shape[1] + 3).zero_()
+    assert not room[1].any()                                                     # nothing between the rows was written
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
@@ -383,11 +415,12 @@ def test_attention_strided_rows_and_same_bits_again(be):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_attention_masked_nodes_hold_anything(be, dtype):
+@pytest.mark.parametrize("hq, d", [(2, 64), (32, 64), (12, 128), (80, 128), (8, 256)])
+def test_attention_masked_nodes_hold_anything(be, hq, d, dtype):
     """Node 1 and node 2 are siblings; what node 2 holds reaches node 2 only."""
-    b, t, d = 1, 4, 64
+    b, t = 1, 4
     cache = make_cache(b, 4, 16, 1, d, seed=60)
-    q = normal(61, b, t, 2, d).to(dtype)
+    q = normal(61, b, t, hq, d).to(dtype)
     k, v = normal(62, b, t, 1, d).to(BF16), normal(63, b, t, 1, d).to(BF16)
     par = torch.tensor([[-1, 0, 0, 1]], dtype=torch.int32)
     lens = torch.tensor([50], dtype=torch.int32).cuda()
@@ -396,7 +429,7 @@ def test_attention_masked_nodes_hold_anything(be, dtype):
     v2[0, 2, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, math.inf])
     dirty = be.tree_attention(q.cuda(), k.cuda(), v2.cuda(), cache, lens, parents=par.cuda()).cpu()
     assert torch.equal(dirty[:, [0, 1, 3]], clean[:, [0, 1, 3]])
-    for h in range(2):
+    for h in range(hq):
         assert dirty[0, 2, h, 0] == math.inf and dirty[0, 2, h, 1] == -math.inf and dirty[0, 2, h, 2].isnan()
     assert torch.equal(dirty[0, 2, :, 4:], clean[0, 2, :, 4:])
     for bad in (math.nan, math.inf, torch.finfo(BF16).min):
@@ -407,10 +440,11 @@ def test_attention_masked_nodes_hold_anything(be, dtype):
         assert torch.equal(dirty[:, [0, 1, 3]], clean[:, [0, 1, 3]])
 
 
-def test_attention_reports_bad_indexes(be):
+@pytest.mark.parametrize("hq", [2, 16])
+def test_attention_reports_bad_indexes(be, hq):
     from lattice_b200 import Lq4Error
     d = 64
-    q, k = normal(70, 1, 3, 2, d).to(BF16).cuda(), normal(71, 1, 3, 1, d).to(BF16).cuda()
+    q, k = normal(70, 1, 3, hq, d).to(BF16).cuda(), normal(71, 1, 3, 1, d).to(BF16).cuda()
     dev = lambda x: torch.as_tensor(x, dtype=torch.int32).cuda()  # noqa: E731
     for what in ("page", "negative page", "length", "count", "parent", "parent of itself"):
         cache = make_cache(1, 4, 16, 1, d, seed=72)
@@ -442,13 +476,14 @@ def test_attention_reports_bad_indexes(be):
             assert_attention(got, *ref, 64)
 
 
-def test_attention_in_a_captured_graph(be):
+@pytest.mark.parametrize("hq", [4, 24])
+def test_attention_in_a_captured_graph(be, hq):
     """A graph replays with other lengths, pages and values; the launch does not depend on them."""
     b, t, d = 2, 3, 64
     cache = make_cache(b, 40, 16, 2, d, seed=80)
-    q, k, v = normal(81, b, t, 4, d).to(BF16).cuda(), normal(82, b, t, 2, d).to(BF16).cuda(), normal(83, b, t, 2, d).to(BF16).cuda()
+    q, k, v = normal(81, b, t, hq, d).to(BF16).cuda(), normal(82, b, t, 2, d).to(BF16).cuda(), normal(83, b, t, 2, d).to(BF16).cuda()
     lens, par = torch.tensor([5, 600], dtype=torch.int32).cuda(), random_tree(84, b, t, 2).cuda()
-    out = torch.empty(b, t, 4, d, dtype=BF16, device="cuda")
+    out = torch.empty(b, t, hq, d, dtype=BF16, device="cuda")
     call = lambda: be.tree_attention(q, k, v, cache, lens, parents=par, out=out)  # noqa: E731
     call()                                                                       # the workspace grows outside the capture
     torch.cuda.synchronize()
@@ -457,7 +492,7 @@ def test_attention_in_a_captured_graph(be):
         call()
     for new in ([5, 600], [639, 0], [64, -1]):
         lens.copy_(torch.tensor(new, dtype=torch.int32))
-        q.copy_(normal(85 + new[0], b, t, 4, d).to(BF16))
+        q.copy_(normal(85 + new[0], b, t, hq, d).to(BF16))
         out.fill_(7.0)
         g.replay()
         torch.cuda.synchronize()
@@ -673,3 +708,87 @@ def test_verify_refusals(be):
         a.update(bad)
         with pytest.raises((ValueError, TypeError)):
             be.verify_draft(a.pop("target_logits"), a.pop("tokens"), a.pop("uniforms"), **a)
+
+
+# ---- a speculative decode step, all of it --------------------------------------------------------------------------
+
+def test_two_backends_on_two_streams(be):
+    """Each backend has its own workspace: two attentions that run side by side do not disturb one another."""
+    from lattice_b200 import CudaQ4Backend
+    other = CudaQ4Backend(0)
+    calls, want = [], []
+    for i, (b_, nodes, hq, dtype) in enumerate([(be, 1, 8, BF16), (other, 16, 8, BF16)]):
+        cache = make_cache(2, 100, 32, 2, 128, seed=95 + i)
+        q = normal(96 + i, 2, nodes, hq, 128).to(dtype).cuda()
+        k = normal(97 + i, 2, nodes, 2, 128).to(BF16).cuda()
+        lens = torch.tensor([3000, 1234], dtype=torch.int32).cuda()
+        calls.append((b_, q, k, cache, lens))
+        want.append(b_.tree_attention(q, k, k, cache, lens).clone())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(20):
+        for i, (b_, q, k, cache, lens) in enumerate(calls):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(b_.tree_attention(q, k, k, cache, lens))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+    be.check_device_status()
+    other.check_device_status()
+    other.close()
+
+
+@pytest.mark.parametrize("types", [BF16, F32])
+def test_speculative_step(be, types):
+    """Projections, rotary positions, attention of the tree, o_proj, lm_head over all nodes, verification, append, and the
+    next step over what was accepted: every stage against 64 bits on the inputs that the GPU had."""
+    from lattice_b200 import Q4WeightBuf, RopeTable, synth
+    import oracle
+    b, t, hidden, hq, hk, d, vocab = 2, 6, 256, 4, 2, 64, 1000
+    weights = []
+    for i, (n, k) in enumerate([((hq + 2 * hk) * d, hidden), (hidden, hq * d), (vocab, hidden)]):
+        w = synth.weights(2, n, k, i)
+        weights.append(Q4WeightBuf.from_host_payload(oracle.quantize_f32_to_q4(w), n, k))
+    w_qkv, w_o, w_head = weights
+    table = RopeTable.from_config(d, "cuda", theta=1e6)
+    cache = make_cache(b, 12, 16, hk, d, seed=300)
+    lens = torch.tensor([33, 90], dtype=torch.int32).cuda()
+    draft_of = (2 * torch.randn(b, t, vocab, generator=rng(301))).cuda()
+    for step in range(3):
+        par = random_tree(302 + step, b, t, 2)
+        par[:, 1:] = par[:, 1:].clamp(min=0)                                     # node 0 is the last certain token
+        depth = torch.tensor([[len(p) - 1 for p in paths_of(par[i], t)] for i in range(b)])
+        x = (normal(310 + step, b * t, hidden) * 0.5).float().cuda()
+        fused = be.linear(x, w_qkv).view(b * t, hq + 2 * hk, d)
+        pos = (lens[:, None].cpu() + depth).to(torch.int32).view(-1)
+        q, k, v = fused.split([hq, hk, hk], 1)
+        q, = be.rope_rows([(q, 1)], pos.cuda(), table, out_dtype=types)
+        k, v = be.rope_rows([(k, 1), (v, 0)], pos.cuda(), table, out_dtype=BF16)
+        for y, part in ((q, fused[:, :hq]), (k, fused[:, hq:hq + hk])):
+            assert_rope(y, *rope_ref(part.cpu(), pos, table.freq.cpu().numpy(), "half", 1.0, 1))
+        q, k, v = q.view(b, t, hq, d), k.view(b, t, hk, d), v.view(b, t, hk, d)
+        att = be.tree_attention(q, k, v, cache, lens, parents=par.cuda())
+        ref = attend_ref(q.cpu(), k.cpu(), v.cpu(), cache.k.cpu(), cache.v.cpu(), cache.page_table.cpu(), lens.tolist(), par, None, d ** -0.5)
+        assert_attention(att, *ref, 200)
+        logits = be.linear(be.linear(att.view(b * t, hq * d), w_o), w_head).view(b, t, vocab)
+        assert bool(logits.isfinite().all())
+        draft = logits + 0.3 * draft_of
+        of_parent = torch.take_along_dim(draft, par.clamp(min=0).long()[..., None].cuda(), 1)
+        tokens = (of_parent + -torch.log(-torch.log(torch.rand(of_parent.shape, generator=rng(320 + step)).clamp(1e-30, 1 - 1e-7))).cuda()).argmax(-1).to(torch.int32)
+        u = torch.rand(b, t, generator=rng(330 + step))
+        path, count, token = check_verify(be, logits.cpu(), draft.cpu(), tokens.cpu(), par, None, u, None)
+        path, count = torch.from_numpy(path).cuda(), torch.from_numpy(count).cuda()
+        # the last accepted node, attended alone once its ancestors are in the cache
+        before = lens.clone()
+        lens = be.kv_append(cache, k, v, before, counts=count - 1, index=path)
+        last = torch.stack([path[i, count[i] - 1] for i in range(b)]).long()
+        pick = lambda y: y[torch.arange(b).cuda(), last][:, None].contiguous()  # noqa: E731
+        alone = be.tree_attention(pick(q), pick(k), pick(v), cache, lens)
+        ref = [r[torch.arange(b), last.cpu()][:, None] for r in ref]
+        assert_attention(alone, *ref, 200)
+        lens = be.kv_append(cache, pick(k), pick(v), lens)
+        assert (lens - before).tolist() == count.tolist()
+    be.check_device_status()
+    for w in weights:
+        w.free()
