@@ -14,13 +14,13 @@
 //              (a captured graph replays with others).  An item cut by a CTA border leaves (max, sum, O) partials,
 //              at most two per CTA, which attend_join_kernel merges in the order of the CTAs: the same lengths
 //              give the same bits.
-//   loads      cp.async, 16 bytes a lane, ST stages of K and V.  Every key's address is looked up on its own
-//              (slot -> page), so pages of any size may end anywhere inside a tile; the lookups run a stage ahead.
+//   loads      four warps of their own (load_stream): cp.async, 16 bytes a lane, into a ring of K and V tiles.  Every
+//              key's address is looked up on its own (slot -> page), so pages of any size may end anywhere inside a tile.
 //   math       mma.sync m16n8k16 on bf16.  K and V are bf16 in memory and exact.  q and the probabilities are one
 //              bf16 term each for bf16 activations (both roundings are of the size of the output's own), and three
 //              terms each (24 bits) for f32 ones, so that an f32 result keeps 32-bit accuracy.
-//   warps      WM x WN: WM bands of 16 rows, WN shares of the 64 keys.  Each warp keeps its own running maximum,
-//              sum and O over its keys; they meet in shared memory once per piece.
+//   warps      four for the math, WM x WN: WM bands of 16 rows, WN shares of the 64 keys.  Each warp keeps its own running
+//              maximum, sum and O over its keys; they meet in shared memory once per piece.
 //
 // A key that a row may not see contributes nothing whatever it holds: its score is replaced by -inf, and a
 // non-finite V entry of a node (0 * inf would reach the rows that do not see it) is cleared in shared memory
@@ -54,41 +54,70 @@ __device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t c) { return r *
 // rows 357 and 315 us, 128 rows 691 and 335 us.  (f32 and head_dim above 128: three terms of Q leave no room there.)
 constexpr uint32_t kTcMinRows = 16, kTcMinRowsF32 = 32;
 
+// WM bands of 16 rows, four warps on them (WN shares of the keys); NQ bf16 terms of q and P.
 template <int D, int WM, int NQ>
 struct Shape {
-    static constexpr int WN = WM == 4 ? 2 : 4, NT = 32 * WM * WN, BM = 16 * WM;
-    static constexpr int NK = kKeys / WN;                                         // keys of a warp
-    static constexpr int ST = D == 64 ? 4 : D == 128 ? 3 : NQ * WM < 4 ? 3 : 2;  // stages that fit beside Q
-    static constexpr uint32_t kTile = kKeys * D * 2, kStage = 2 * kTile;
-    static constexpr uint32_t kQ = NQ * BM * D * 2;
-    static constexpr uint32_t kOut = WN * BM * (D + 8) * 4;                       // merge area: stages, then Q
-    static constexpr uint32_t kMain = ST * kStage + kQ > kOut ? ST * kStage + kQ : kOut;
-    static constexpr uint32_t kOffs = kMain, kValid = kOffs + ST * kKeys * 8, kAnc = kValid + 8 * 8, kMl = kAnc + kMaxNodes * 8;
-    static constexpr uint32_t kCtl = kMl + WN * BM * 8, kSmem = kCtl + 64;
-    static_assert(kSmem <= (uint32_t)kMaxSmem, "shared memory");
+    static constexpr int WN = 4 / WM, BM = 16 * WM, NK = kKeys / WN;                  // NK keys of a warp
+    static constexpr int kMath = 128, kLoaders = 128, NT = kMath + kLoaders;
+    // two CTAs an SM where 128 registers a thread are enough
+    static constexpr int kPerSm = D <= 128 && NQ == 1 ? 2 : 1;
+    static constexpr uint32_t kSlot = kKeys * D * 2, kQ = NQ * BM * D * 2, kMeet = WN * BM * 36 * 4;
+    static constexpr uint32_t kRest = 16 * 8 + 16 * 8 + kMaxNodes * 8 + WN * BM * 8 + 256 + 64 * 8;
+    static constexpr uint32_t kFit = ((uint32_t)kMaxSmem / kPerSm - 1024 * (kPerSm - 1) - kQ - kMeet - kRest) / kSlot, kRing = kFit > 12 ? 12 : kFit;
+    static constexpr uint32_t kTeams = kRing >= 8 ? 4 : 2, kTeam = 4 / kTeams;
+    static constexpr uint32_t kOffQ = kRing * kSlot, kOffMeet = kOffQ + kQ, kValid = kOffMeet + kMeet, kFixes = kValid + 16 * 8, kAnc = kFixes + 16 * 8;
+    static constexpr uint32_t kMl = kAnc + kMaxNodes * 8, kCtl = kMl + WN * BM * 8, kBars = kCtl + 256, kSmem = kBars + 64 * 8;
+    static_assert(kRing >= 4 && kSmem <= (uint32_t)kMaxSmem / kPerSm, "shared memory");
 };
 
 template <int D, int WM, int NQ>
-__global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPerSm)) attend_kernel(const __grid_constant__ AttendParams p) {
     using S = Shape<D, WM, NQ>;
-    constexpr int WN = S::WN, NT = S::NT, BM = S::BM, NK = S::NK, ST = S::ST, CPR = D / 8;
+    constexpr int WN = S::WN, BM = S::BM, NK = S::NK;
+    constexpr uint32_t RING = S::kRing;
     extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* offs = reinterpret_cast<uint64_t*>(smem + S::kOffs);      // [ST][64] element offset of a key's row, ~0: none
-    uint64_t* valid = reinterpret_cast<uint64_t*>(smem + S::kValid);    // [8] which of the tile's keys there are
-    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);        // [nodes] a node's path from the root
-    float2* ml = reinterpret_cast<float2*>(smem + S::kMl);              // [WN][BM]
+    volatile uint32_t* valid = reinterpret_cast<uint32_t*>(smem + S::kValid);    // [16][2] which of a tile's 64 keys there are
+    volatile uint32_t* fixes = reinterpret_cast<uint32_t*>(smem + S::kFixes);    // [16][2] V of the tile held inf or NaN
+    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);                 // [nodes] a node's path from the root
+    float2* ml = reinterpret_cast<float2*>(smem + S::kMl);                       // [WN][BM] (max, sum)
+    float* os = reinterpret_cast<float*>(smem + S::kOffMeet);                    // [WN][BM][36] 32 columns of O
     uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);
-    const uint32_t sbase = smem_u32(smem), qbase = sbase + ST * S::kStage;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp / WN, wn = warp % WN;
-    const uint32_t quad = lane >> 2, qc = (lane & 3) * 2;
+    uint64_t *full = reinterpret_cast<uint64_t*>(smem + S::kBars), *empty = full + RING, *info = empty + RING;
+    const uint32_t sbase = smem_u32(smem), qbase = sbase + S::kOffQ;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    const Range range = cta_range<NT>(p, ctl, reinterpret_cast<uint64_t*>(ml));
+    const Range range = cta_range<S::NT>(p, ctl, ctl + 2);
+    if (range.begin >= range.end) return;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < RING; ++i) {
+            mbar_init(full + i, S::kTeam);
+            mbar_init(empty + i, S::kMath / 32);
+        }
+        for (int i = 0; i < 16; ++i) mbar_init(info + i, S::kTeam);
+        mbar_fence_init();
+    }
+    __syncthreads();
     uint64_t u = range.begin, seq_first = range.seq_first;
     const uint64_t u_end = range.end;
     uint32_t b = range.seq;
+    // Once a wait has run out the CTA goes on without waiting, so that its barriers still match; the results are
+    // rubbish then, and reported.
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait(bar, parity);
+    };
 
+    if (tid >= S::kMath) {
+        load_stream<D, RING, 1, S::kTeams, S::kTeam>(p, u, u_end, b, seq_first, warp - S::kMath / 32, smem, full, empty, info, valid, fixes, ok,
+                                                     [](uint32_t r, uint32_t c) { return tile_at<D>(r, c); });
+        if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);
+        return;
+    }
+
+    const uint32_t wm = warp / WN, wn = warp % WN, quad = lane >> 2, qc = (lane & 3) * 2;
+    uint32_t tile = 0, kslot = 0, phase = 0;                             // tiles so far, their K's slot (V: the next) and its phase
     while (u < u_end) {
         const Piece x = next_piece(p, u, u_end, b, seq_first);
         const Seq& sq = x.sq;
@@ -97,7 +126,8 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
         if (sq.bad && tid == 0) atomicOr(p.status, kDevErrBadIndex);
 
         // q -> NQ bf16 terms in shared memory (rows behind the last one are zero)
-        for (uint32_t i = tid; i < BM * (D / 2); i += NT) {
+#pragma unroll 4
+        for (uint32_t i = tid; i < BM * (D / 2); i += S::kMath) {
             const uint32_t r = i / (D / 2), d = (i - r * (D / 2)) * 2, row = rt * BM + r;
             float q0 = 0.0f, q1 = 0.0f;
             if (row < rows && d < p.head_dim) {
@@ -118,7 +148,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 const uint32_t w = split_pair(q0, q1);
-                *reinterpret_cast<uint32_t*>(smem + ST * S::kStage + n * (BM * D * 2) + tile_at<D>(r, d >> 3) + (d & 7) * 2) = w;
+                *reinterpret_cast<uint32_t*>(smem + S::kOffQ + n * (BM * D * 2) + tile_at<D>(r, d >> 3) + (d & 7) * 2) = w;
             }
         }
         if (x.has_nodes && tid < p.nodes) {
@@ -126,42 +156,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
             anc[tid] = node_path(p, b, tid, bad);
             if (bad && (int32_t)tid < sq.nodes) atomicOr(p.status, kDevErrBadIndex);
         }
-
-        // where the keys of tile `i` of this piece lie; page ids come from memory, so this runs a stage ahead
-        auto put_keys = [&](uint32_t i, int32_t page) {                  // (threads 0..63)
-            const uint64_t at = key_offset(p, x, i, tid, page);
-            offs[(i % ST) * kKeys + tid] = at;
-            const uint32_t bits = __ballot_sync(0xffffffffu, at != ~0ull);
-            if (lane == 0) reinterpret_cast<uint32_t*>(valid + (i & 7))[warp] = bits;
-        };
-        auto load_tile = [&](uint32_t i) {
-            if (i < n_tiles) {
-                const bool own = t0 + i + 1 == sq.tiles;
-                const uint16_t* kb = own ? p.k : p.c.k;
-                const uint16_t* vb = own ? p.v : p.c.v;
-                const uint32_t stage = sbase + (i % ST) * S::kStage;
-#pragma unroll
-                for (uint32_t n = 0; n < kKeys * CPR / NT; ++n) {
-                    const uint32_t idx = n * NT + tid, r = idx / CPR, c = idx % CPR;
-                    const uint64_t at = offs[(i % ST) * kKeys + r];
-                    const bool live = at != ~0ull && c * 8 < p.head_dim;
-                    const uint32_t dst = stage + tile_at<D>(r, c);
-                    cp_async16(dst, live ? kb + at + c * 8 : p.k, live);
-                    cp_async16(dst + S::kTile, live ? vb + at + c * 8 : p.k, live);
-                }
-            }
-            cp_commit();
-        };
-        if (tid < kKeys) {
-            int32_t page[ST];
-#pragma unroll
-            for (int i = 0; i < ST; ++i) page[i] = key_page(p, x, i, tid);
-#pragma unroll
-            for (int i = 0; i < ST; ++i) put_keys(i, page[i]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ST - 1; ++i) load_tile(i);
+        named_bar_sync(1, S::kMath);
 
         float o[D / 8][4];
 #pragma unroll
@@ -169,26 +164,22 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         bool fix = false;                                                // a node's V holds inf or NaN
 
-        for (uint32_t i = 0; i < n_tiles; ++i) {
-            cp_wait<ST - 2>();
-            __syncthreads();                                             // tile i is here; everybody is done with tile i - 1
-            load_tile(i + ST - 1);
-            int32_t page = -1;
-            if (tid < kKeys) page = key_page(p, x, i + ST, tid);
-            const uint32_t kst = sbase + (i % ST) * S::kStage, vst = kst + S::kTile;
+        for (uint32_t i = 0; i < n_tiles; ++i, ++tile) {
+            const uint32_t vslot = kslot + 1 == RING ? 0 : kslot + 1, vphase = kslot + 1 == RING ? phase ^ 1 : phase;
+            const uint32_t kst = sbase + kslot * S::kSlot, vst = sbase + vslot * S::kSlot;
             const bool own = t0 + i + 1 == sq.tiles;
+            wait(info + (tile & 15), (tile >> 4) & 1);
             uint64_t see[2];
-            see[0] = see[1] = valid[i & 7];
+            see[0] = see[1] = (uint64_t)valid[(tile & 15) * 2 + 1] << 32 | valid[(tile & 15) * 2];
             if (own) {
-                bool odd = false;                                        // clear non-finite V entries of the nodes
-                for (uint32_t idx = tid; idx < kKeys * CPR; idx += NT) odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + (vst - sbase) + idx * 16));
-                fix = __syncthreads_or(odd);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t t = (rt * BM + wm * 16 + quad + 8 * j) / p.group;
                     if (t < p.nodes) see[j] &= anc[t];
                 }
             }
+            wait(full + kslot, phase);
+            __syncwarp();
             // scores of this warp's keys.  The tensor cores cut off what falls below their accumulator's last bit; with
             // f32 activations the leading term's sum is therefore taken every 32 channels and added in f32.
             float s[NK / 8][4];
@@ -230,6 +221,8 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                         for (int e = 0; e < 4; ++e) s[j][e] += part[1][j][e] + part[2][j][e];
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + kslot);
             if ((see[0] & see[1]) != ~0ull) {
 #pragma unroll
                 for (int j = 0; j < NK / 8; ++j)
@@ -269,6 +262,9 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                     s[j][e] = exp2_fast(fmaf(s[j][e], p.scale_log2, -base[e >> 1]));
                     l[e >> 1] += s[j][e];
                 }
+            wait(full + vslot, vphase);
+            __syncwarp();
+            if (own) fix = (fixes[(tile & 15) * 2] | (S::kTeam == 2 ? fixes[(tile & 15) * 2 + 1] : 0)) != 0;
             // O = corr O + P V, the tile's product in accumulators of its own for f32 activations (as above)
             uint32_t a[NK / 16][NQ][4];
 #pragma unroll
@@ -298,76 +294,87 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), 1) attend_kernel(const
                     }
                 }
             }
-            if (tid < kKeys) put_keys(i + ST, page);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + vslot);
+            kslot += 2;
+            if (kslot >= RING) kslot -= RING, phase ^= 1;
         }
-        cp_wait<0>();
 
-        // the warps of a band meet: common maximum, scaled O to shared memory, one sum over the shares
+        // the warps of a band meet: common maximum, scaled O through shared memory 32 columns at a time, one sum over the shares
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
             if ((lane & 3) == 0) ml[wn * BM + wm * 16 + quad + 8 * r] = make_float2(m[r], l[r]);
         }
-        __syncthreads();                                                 // (everybody is done with the stages and Q, too)
-        float* os = reinterpret_cast<float*>(smem);
+        named_bar_sync(1, S::kMath);
+        float f[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const uint32_t row = wm * 16 + quad + 8 * r;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + row].x);
-            const float f = exp2_fast(m[r] - (top == -INFINITY ? 0.0f : top));
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d)
-                *reinterpret_cast<float2*>(os + (wn * BM + row) * (D + 8) + d * 8 + qc) = make_float2(o[d][2 * r] * f, o[d][2 * r + 1] * f);
+            for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + wm * 16 + quad + 8 * r].x);
+            f[r] = exp2_fast(m[r] - (top == -INFINITY ? 0.0f : top));
         }
-        __syncthreads();
         const bool whole = t0 == 0 && x.has_nodes;
         const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
-        for (uint32_t i = tid; i < BM * (D / 4); i += NT) {
-            const uint32_t r = i / (D / 4), d = (i - r * (D / 4)) * 4, row = rt * BM + r;
-            const uint32_t t = row / p.group, g = row - t * p.group;
-            if (row >= rows || (int32_t)t >= sq.nodes || d >= p.head_dim) continue;
-            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + r].x);
-            const float safe = top == -INFINITY ? 0.0f : top;
-            float y[4] = {0, 0, 0, 0};
+        for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
-            for (int w = 0; w < WN; ++w) {
-                const float2 e = ml[w * BM + r];
-                sum += e.y * exp2_fast(e.x - safe);
-                const float4 v = *reinterpret_cast<const float4*>(os + (w * BM + r) * (D + 8) + d);
-                y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
-            }
-            if (fix)
-                for (int e = 0; e < 4; ++e) y[e] += nonfinite_sum(p, x, anc[t], d + e);
-            if (whole) {
-                const float inv = 1.0f / sum;
-                const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + d;
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (NQ == 1)
-                        static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(y[e] * inv);
-                    else
-                        static_cast<float*>(p.out)[at + e] = y[e] * inv;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    *reinterpret_cast<float2*>(os + (wn * BM + wm * 16 + quad + 8 * r) * 36 + j * 8 + qc) = make_float2(o[4 * c + j][2 * r] * f[r], o[4 * c + j][2 * r + 1] * f[r]);
+            named_bar_sync(1, S::kMath);
+            for (uint32_t i = tid; i < BM * 8; i += S::kMath) {
+                const uint32_t r = i >> 3, d = c * 32 + (i & 7) * 4, row = rt * BM + r;
+                const uint32_t t = row / p.group, g = row - t * p.group;
+                if (row >= rows || (int32_t)t >= sq.nodes || d >= p.head_dim) continue;
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + r].x);
+                const float safe = top == -INFINITY ? 0.0f : top;
+                float y[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WN; ++w) {
+                    const float2 e = ml[w * BM + r];
+                    sum += e.y * exp2_fast(e.x - safe);
+                    const float4 v = *reinterpret_cast<const float4*>(os + (w * BM + r) * 36 + (i & 7) * 4);
+                    y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
                 }
-            } else {
-                *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-                if (d == 0) p.part_ml[(uint64_t)slot * BM + r] = make_float2(top, sum);
+                if (fix)
+                    for (int e = 0; e < 4; ++e) y[e] += nonfinite_sum(p, x, anc[t], d + e);
+                if (whole) {
+                    const float inv = 1.0f / sum;
+                    const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + d;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (NQ == 1)
+                            static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(y[e] * inv);
+                        else
+                            static_cast<float*>(p.out)[at + e] = y[e] * inv;
+                    }
+                } else {
+                    *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+                    if (d == 0) p.part_ml[(uint64_t)slot * BM + r] = make_float2(top, sum);
+                }
             }
+            named_bar_sync(1, S::kMath);                                 // the columns are read (at last: anc and ml, too)
         }
-        __syncthreads();                                                 // shared memory is free for the next piece
         u += n_tiles;
     }
+    if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);
 }
 
-// Joins the partials of the items that a CTA border cut: one warp per row, the CTAs in order.
-template <int D>
+// Joins the partials of the items that a CTA border cut, the CTAs in order: W warps per row, which take every W-th of them and
+// meet in shared memory (one row's partials may come from every CTA of the grid).
+template <int D, int W>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p, uint32_t BM, int bf16_out) {
-    const uint32_t lane = threadIdx.x & 31;
+    constexpr int V = D / 32;
+    __shared__ float part[W > 1 ? W : 1][D + 1];                         // O and, behind it, the sum
+    const uint32_t lane = threadIdx.x & 31, w = W > 1 ? threadIdx.x >> 5 : 0;
     const uint32_t rows = p.nodes * p.group;
-    const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint64_t id = W > 1 ? blockIdx.x : (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     pdl_wait_prior_grids();
     pdl_launch_dependents();
     if (id >= (uint64_t)p.batch * p.kv_heads * rows) return;
@@ -384,7 +391,6 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const uint32_t c0 = (uint32_t)(first / share), c1 = (uint32_t)((first + sq.tiles - 1) / share);
     if (c0 == c1) return;                                                // one CTA had it all and wrote it
     // the CTA that has the item's first tile keeps it in its slot 1, the others in slot 0
-    constexpr int V = D / 32;
     float top = -INFINITY;
     for (uint32_t c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(uint64_t)(2 * c + (c == c0)) * BM + r].x);
 #pragma unroll
@@ -394,7 +400,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.0f;
 #pragma unroll 4
-    for (uint32_t c = c0; c <= c1; ++c) {
+    for (uint32_t c = c0 + w; c <= c1; c += W) {
         const uint64_t slot = (uint64_t)(2 * c + (c == c0)) * BM + r;
         const float2 e = p.part_ml[slot];
         const float f = exp2_fast(e.x - safe);
@@ -402,6 +408,19 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
         const float* src = p.part_o + slot * D + lane * V;
 #pragma unroll
         for (int k = 0; k < V; ++k) acc[k] += src[k] * f;
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) part[w][lane * V + k] = acc[k];
+        if (lane == 0) part[w][D] = sum;
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int i = 1; i < W; ++i) {
+            sum += part[i][D];
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += part[i][lane * V + k];
+        }
     }
     const float inv = 1.0f / sum;
     const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + lane * V;
@@ -422,43 +441,34 @@ cudaError_t run(AttendParams p, AttendWorkspace& ws, int sm_count, int use_pdl, 
     auto fn = attend_kernel<D, WM, NQ>;
     cudaError_t e = opt_in_smem(reinterpret_cast<const void*>(fn), S::kSmem, once);
     if (e != cudaSuccess) return e;
-    static std::atomic<int> resident{0};       // CTAs an SM holds at once
-    int per_sm = resident.load(std::memory_order_relaxed);
-    if (!per_sm) {
-        if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, S::NT, S::kSmem)) != cudaSuccess) return e;
-        if (per_sm < 1) per_sm = 1;
-        resident.store(per_sm, std::memory_order_relaxed);
-    }
-    p.grid = (uint32_t)(sm_count * per_sm);
+    p.grid = (uint32_t)(sm_count * S::kPerSm);
     p.row_tiles = (p.nodes * p.group + S::BM - 1) / S::BM;
     if (!attend_workspace(p, ws, S::BM, D)) return cudaSuccess;
     if ((e = attend_launch(fn, dim3(p.grid), S::NT, S::kSmem, use_pdl, s, p)) != cudaSuccess) return e;
     return launch_attend_join(p, S::BM, D, NQ == 1, ws, use_pdl, s);
 }
 
-template <int D, int NQ>
-cudaError_t run_rows(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    // bands of 16 rows: as few as hold the rows of an item, at most four (more rows: several row tiles)
-    const uint32_t rows = p.nodes * p.group;
-    if (rows <= 16) return run<D, 1, NQ>(p, ws, sm_count, use_pdl, s);
-    if (rows <= 32) return run<D, 2, NQ>(p, ws, sm_count, use_pdl, s);
-    return run<D, 4, NQ>(p, ws, sm_count, use_pdl, s);
+// bf16 activations come here with up to 16 rows, f32 ones with up to 32 and, above a head_dim of 128, with any number (row tiles
+// of 32).
+template <int D>
+cudaError_t run_rows(const AttendParams& p, bool f32, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
+    if (!f32) return run<D, 1, 1>(p, ws, sm_count, use_pdl, s);
+    return p.nodes * p.group <= 16 ? run<D, 1, 3>(p, ws, sm_count, use_pdl, s) : run<D, 2, 3>(p, ws, sm_count, use_pdl, s);
 }
 
-template <int NQ>
-cudaError_t run_dim(const AttendParams& p, AttendWorkspace& ws, int sm_count, int use_pdl, cudaStream_t s) {
-    if (p.head_dim <= 64) return run_rows<64, NQ>(p, ws, sm_count, use_pdl, s);
-    if (p.head_dim <= 128) return run_rows<128, NQ>(p, ws, sm_count, use_pdl, s);
-    return run_rows<256, NQ>(p, ws, sm_count, use_pdl, s);
+template <int W>
+auto join_kernel(uint32_t D) {
+    return D == 64 ? attend_join_kernel<64, W> : D == 128 ? attend_join_kernel<128, W> : D == 192 ? attend_join_kernel<192, W> : attend_join_kernel<256, W>;
 }
 
 }  // namespace
 
 cudaError_t launch_attend_join(const AttendParams& p, uint32_t rows, uint32_t D, bool bf16_out, AttendWorkspace& ws, int use_pdl, cudaStream_t s) {
-    const uint64_t warps = (uint64_t)p.batch * p.kv_heads * p.nodes * p.group;
-    auto fn = D == 64 ? attend_join_kernel<64> : D == 128 ? attend_join_kernel<128> : attend_join_kernel<256>;
+    // a CTA per row where few rows share the grid's partials, else a warp per row
+    const uint64_t all = (uint64_t)p.batch * p.kv_heads * p.nodes * p.group;
+    const bool wide = all <= 8ull * p.grid;
     ws.launches = 2;
-    return attend_launch(fn, dim3((unsigned)((warps + 7) / 8)), 256, 0, use_pdl, s, p, rows, (int)bf16_out);
+    return attend_launch(wide ? join_kernel<8>(D) : join_kernel<1>(D), dim3((unsigned)(wide ? all : (all + 7) / 8)), 256, 0, use_pdl, s, p, rows, (int)bf16_out);
 }
 
 cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorkspace& ws, int32_t* status, int sm_count, int use_pdl, cudaStream_t s) {
@@ -490,7 +500,10 @@ cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorksp
     ws.need = 0;
     ws.launches = 0;
     if (p.nodes * p.group > (f32 ? kTcMinRowsF32 : kTcMinRows) && (!f32 || p.head_dim <= 128)) return launch_attend_tc(p, f32, ws, sm_count, use_pdl, s);
-    return !f32 ? run_dim<1>(p, ws, sm_count, use_pdl, s) : run_dim<3>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 64) return run_rows<64>(p, f32, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 128) return run_rows<128>(p, f32, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 192) return run_rows<192>(p, f32, ws, sm_count, use_pdl, s);
+    return run_rows<256>(p, f32, ws, sm_count, use_pdl, s);
 }
 
 }  // namespace lq4

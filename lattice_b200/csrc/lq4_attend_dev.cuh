@@ -76,6 +76,7 @@ __device__ __forceinline__ uint64_t cta_share(uint64_t total, uint32_t grid) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -184,24 +185,6 @@ __device__ __forceinline__ uint64_t node_path(const AttendParams& p, uint32_t b,
     return path;
 }
 
-// Where key `tid` of a piece's tile `i` lies, in two steps, because the page id comes from memory.
-__device__ __forceinline__ int32_t key_page(const AttendParams& p, const Piece& x, uint32_t i, uint32_t tid) {
-    const uint32_t key = (x.t0 + i) * kKeys + tid;
-    if (i >= x.n_tiles || x.t0 + i + 1 == x.sq.tiles || key >= (uint32_t)x.sq.len) return -1;
-    return p.c.table[(uint64_t)x.b * p.c.max_pages + key / p.c.page_size];
-}
-// Element offset of the key's row in the cache (in k and v of the nodes for their own tile), ~0: there is none.
-__device__ __forceinline__ uint64_t key_offset(const AttendParams& p, const Piece& x, uint32_t i, uint32_t tid, int32_t page) {
-    const uint32_t key = (x.t0 + i) * kKeys + tid;
-    if (i >= x.n_tiles) return ~0ull;
-    if (x.t0 + i + 1 == x.sq.tiles) return (int32_t)tid < x.sq.nodes ? x.b * p.kv_batch + tid * p.kv_node + x.h * p.kv_head : ~0ull;
-    if (key >= (uint32_t)x.sq.len) return ~0ull;
-    if (page < 0 || (uint32_t)page >= p.c.pages) {
-        atomicOr(p.status, kDevErrBadIndex);
-        return ~0ull;
-    }
-    return (uint64_t)page * p.c.page_stride + (uint64_t)(key % p.c.page_size) * p.c.slot_stride + x.h * p.c.head_stride;
-}
 // Clears non-finite entries of eight bf16 values; true if there were any.
 __device__ __forceinline__ bool clear_nonfinite(uint4* at) {
     uint32_t x[4] = {at->x, at->y, at->z, at->w};
@@ -223,6 +206,130 @@ static __device__ __noinline__ float nonfinite_sum(const AttendParams& p, const 
             if (!isfinite(y)) sum += y;
         }
     return sum;
+}
+
+// ---- loaders --------------------------------------------------------------------
+// The K and V rows of all tiles of a CTA's range, through cp.async into RINGS rings of RING slots (K and V of a tile in turn;
+// tile n goes to ring n % RINGS), by TEAMS teams of TEAM warps that take the tiles in turn; warp `w` of them.  A lone warp
+// pays some five cycles per dependent instruction and waits for its own copies; teams that each look up, copy and hand
+// on whole tiles overlap all of it.  A lane holds where its keys lie; table index and slot advance without a division, and
+// the page ids are fetched one turn ahead.  A team's next tile is at most a ring ahead of its last one, so that a slot's
+// barrier is never two phases off.
+//   full, empty   per slot: TEAM arrivals when it is filled; by the readers when it may be filled again
+//   info          [16] by tile: TEAM arrivals when `valid` is there (which of the 64 keys there are, [16][2])
+//   fixes         [16][2]: non-finite V entries of the nodes' tile were cleared; there when its V is
+//   place(r, c)   byte offset of 16-byte chunk c of row r in a slot
+template <int D, uint32_t RING, uint32_t RINGS, uint32_t TEAMS, uint32_t TEAM, typename Place>
+__device__ __forceinline__ void load_stream(const AttendParams& p, uint64_t u, uint64_t u_end, uint32_t b, uint64_t seq_first, uint32_t w, unsigned char* smem,
+                                            uint64_t* full, uint64_t* empty, uint64_t* info, volatile uint32_t* valid, volatile uint32_t* fixes, bool& ok, Place place) {
+    constexpr uint32_t CPR = D / 8, kWarps = TEAMS, kOn = kWarps * kKeys, kHold = 2 / TEAM, kCopies = kHold * CPR;
+    static_assert(2 * TEAMS / RINGS <= RING && (TEAMS & (TEAMS - 1)) == 0, "a team's next tile is at most a ring ahead of its last one");
+    const uint32_t lane = threadIdx.x & 31, sbase = smem_u32(smem);
+    const uint32_t lw = w / TEAM, key0 = (w % TEAM) * 32;                // team; this warp's first key of a tile
+    uint32_t tile = 0;                                                   // tiles before the current piece
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait(bar, parity);
+    };
+    struct Ring {
+        uint32_t slot, phase;                                        // phase: of `empty` before the slot is filled again
+        __device__ __forceinline__ void move(uint32_t groups) {
+            slot += groups;
+            while (slot >= RING) slot -= RING, phase ^= 1;
+        }
+    } kr{0, 1}, vr{1, 1};
+    kr.move(2 * (lw / RINGS));
+    vr.move(2 * (lw / RINGS));
+    const uint32_t ring0 = RINGS == 2 ? (lw & 1) * RING : 0;         // (a team's tiles are all even or all odd)
+    const uint32_t page_size = p.c.page_size, pages_on = kOn / page_size, slots_on = kOn - pages_on * page_size;
+    while (u < u_end) {
+        const Piece x = next_piece(p, u, u_end, b, seq_first);
+        const int32_t* const table = p.c.table + (uint64_t)x.b * p.c.max_pages;
+        const uint32_t plain = x.n_tiles - x.has_nodes;              // tiles of cached keys in this piece
+        uint32_t i = (lw - tile) & (kWarps - 1);
+        struct Key {
+            uint32_t key, entry, in_page;
+            int32_t page;
+        } k2[kHold];
+        auto fetch = [&](Key& k) { k.page = i < plain && k.key < (uint32_t)x.sq.len ? table[k.entry] : -1; };
+#pragma unroll
+        for (uint32_t h = 0; h < kHold; ++h) {
+            k2[h].key = (x.t0 + i) * kKeys + key0 + h * 32 + lane;
+            k2[h].entry = k2[h].key / page_size;
+            k2[h].in_page = k2[h].key - k2[h].entry * page_size;
+            fetch(k2[h]);
+        }
+        while (i < x.n_tiles) {
+            const uint32_t n = tile + i;
+            const bool own = i == plain;
+            uint64_t at[kHold];
+            i += kWarps;
+#pragma unroll
+            for (uint32_t h = 0; h < kHold; ++h) {
+                Key& k = k2[h];
+                at[h] = ~0ull;
+                if (own) {
+                    const uint32_t node = key0 + h * 32 + lane;
+                    if (node < (uint32_t)x.sq.nodes) at[h] = x.b * p.kv_batch + node * p.kv_node + x.h * p.kv_head;
+                } else if (k.key < (uint32_t)x.sq.len) {
+                    if ((uint32_t)k.page < p.c.pages)
+                        at[h] = (uint32_t)k.page * p.c.page_stride + k.in_page * p.c.slot_stride + x.h * p.c.head_stride;
+                    else
+                        atomicOr(p.status, kDevErrBadIndex);
+                }
+                k.key += kOn;
+                k.entry += pages_on;
+                k.in_page += slots_on;
+                if (k.in_page >= page_size) k.in_page -= page_size, ++k.entry;
+                fetch(k);
+            }
+            __syncwarp();
+#pragma unroll
+            for (uint32_t h = 0; h < kHold; ++h) {
+                const uint32_t bits = __ballot_sync(0xffffffffu, at[h] != ~0ull);
+                if (lane == 0) valid[(n & 15) * 2 + key0 / 32 + h] = bits;
+            }
+            if (lane == 0) {
+                fixes[(n & 15) * 2 + key0 / 32] = 0;
+                mbar_arrive(info + (n & 15));
+            }
+            auto copy = [&](const uint16_t* base, const Ring& r, uint32_t group) {
+                if (group >= RING) wait(empty + ring0 + r.slot, r.phase);
+                __syncwarp();
+                const uint32_t slot = sbase + (ring0 + r.slot) * (kKeys * D * 2);
+#pragma unroll 8
+                for (uint32_t c = 0; c < kCopies; ++c) {
+                    const uint32_t idx = c * 32 + lane, row = idx / CPR, chunk = idx % CPR;      // (row < 32 or not: the same for all lanes)
+                    const uint64_t from = __shfl_sync(0xffffffffu, c < CPR ? at[0] : at[kHold - 1], row & 31);
+                    const bool here = from != ~0ull && chunk * 8 < p.head_dim;
+                    cp_async16(slot + place(key0 + row, chunk), here ? base + from + chunk * 8 : p.k, here);
+                }
+                cp_commit();
+            };
+            copy(own ? p.k : p.c.k, kr, 2 * (n / RINGS));
+            copy(own ? p.v : p.c.v, vr, 2 * (n / RINGS) + 1);
+            cp_wait<1>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + ring0 + kr.slot);
+            cp_wait<0>();
+            if (own) {                                               // clear non-finite V of the nodes before it is used
+                bool odd = false;
+                __syncwarp();
+                for (uint32_t c = 0; c < kCopies; ++c) {
+                    const uint32_t idx = c * 32 + lane;
+                    odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + (ring0 + vr.slot) * (kKeys * D * 2) + place(key0 + idx / CPR, idx % CPR)));
+                }
+                if (__any_sync(0xffffffffu, odd) && lane == 0) fixes[(n & 15) * 2 + key0 / 32] = 1;
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + ring0 + vr.slot);
+            kr.move(2 * kWarps / RINGS);
+            vr.move(2 * kWarps / RINGS);
+        }
+        tile += x.n_tiles;
+        u += x.n_tiles;
+    }
 }
 
 // ---- host side --------------------------------------------------------------------

@@ -47,7 +47,6 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // D[tmem] (+)= A[smem] B[smem]; bf16, f32 accumulation; one thread issues.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -585,114 +584,9 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
         if (!mbar_wait(drained, 0)) ok = false;
         __syncwarp();
     } else {
-        // ---- loaders: teams take the tiles in turn -----------------------------------------------------------
-        // A lone warp pays some five cycles per dependent instruction and waits for its own copies; teams (a warp each where
-        // the ring is long enough, else two) that each look up, copy and hand on whole tiles overlap all of it.  A lane
-        // holds where its keys lie; table index and slot advance without a division, and the page ids are fetched one turn ahead.
-        // A team's next tile is at most half a ring ahead of its last one, so that a slot's barrier is never two phases off.
-        constexpr uint32_t kWarps = S::kTeams, kOn = kWarps * kKeys, kHold = 2 / S::kTeam, kCopies = kHold * CPR;
-        const uint32_t lw = (warp - (S::kThreads - S::kLoaders) / 32) / S::kTeam;      // team
-        const uint32_t key0 = ((warp - (S::kThreads - S::kLoaders) / 32) % S::kTeam) * 32;      // this warp's first key of a tile
-        struct Ring {
-            uint32_t slot, phase;                                        // phase: of `empty` before the slot is filled again
-            __device__ __forceinline__ void move(uint32_t groups) {
-                slot += groups;
-                while (slot >= RING) slot -= RING, phase ^= 1;
-            }
-        } kr{0, 1}, vr{1, 1};
-        kr.move(2 * (lw / RINGS));
-        vr.move(2 * (lw / RINGS));
-        const uint32_t ring0 = RINGS == 2 ? (lw & 1) * RING : 0;         // (a team's tiles are all even or all odd)
-        const uint32_t page_size = p.c.page_size, pages_on = kOn / page_size, slots_on = kOn - pages_on * page_size;
-        while (u < u_end) {
-            const Piece x = next_piece(p, u, u_end, b, seq_first);
-            const int32_t* const table = p.c.table + (uint64_t)x.b * p.c.max_pages;
-            const uint32_t plain = x.n_tiles - x.has_nodes;              // tiles of cached keys in this piece
-            uint32_t i = (lw - tile) & (kWarps - 1);
-            struct Key {
-                uint32_t key, entry, in_page;
-                int32_t page;
-            } k2[kHold];
-            auto fetch = [&](Key& k) { k.page = i < plain && k.key < (uint32_t)x.sq.len ? table[k.entry] : -1; };
-#pragma unroll
-            for (uint32_t h = 0; h < kHold; ++h) {
-                k2[h].key = (x.t0 + i) * kKeys + key0 + h * 32 + lane;
-                k2[h].entry = k2[h].key / page_size;
-                k2[h].in_page = k2[h].key - k2[h].entry * page_size;
-                fetch(k2[h]);
-            }
-            while (i < x.n_tiles) {
-                const uint32_t n = tile + i;
-                const bool own = i == plain;
-                uint64_t at[kHold];
-                i += kWarps;
-#pragma unroll
-                for (uint32_t h = 0; h < kHold; ++h) {
-                    Key& k = k2[h];
-                    at[h] = ~0ull;
-                    if (own) {
-                        const uint32_t node = key0 + h * 32 + lane;
-                        if (node < (uint32_t)x.sq.nodes) at[h] = x.b * p.kv_batch + node * p.kv_node + x.h * p.kv_head;
-                    } else if (k.key < (uint32_t)x.sq.len) {
-                        if ((uint32_t)k.page < p.c.pages)
-                            at[h] = (uint32_t)k.page * p.c.page_stride + k.in_page * p.c.slot_stride + x.h * p.c.head_stride;
-                        else
-                            atomicOr(p.status, kDevErrBadIndex);
-                    }
-                    k.key += kOn;
-                    k.entry += pages_on;
-                    k.in_page += slots_on;
-                    if (k.in_page >= page_size) k.in_page -= page_size, ++k.entry;
-                    fetch(k);
-                }
-                __syncwarp();
-#pragma unroll
-                for (uint32_t h = 0; h < kHold; ++h) {
-                    const uint32_t bits = __ballot_sync(0xffffffffu, at[h] != ~0ull);
-                    if (lane == 0) valid[(n & 15) * 2 + key0 / 32 + h] = bits;
-                }
-                if (lane == 0) {
-                    fixes[(n & 15) * 2 + key0 / 32] = 0;
-                    mbar_arrive(info + (n & 15));
-                }
-                auto copy = [&](const uint16_t* base, const Ring& r, uint32_t group) {
-                    if (group >= RING) wait(empty + ring0 + r.slot, r.phase);
-                    __syncwarp();
-                    const uint32_t slot = sbase + (ring0 + r.slot) * S::kSlot;
-#pragma unroll 8
-                    for (uint32_t c = 0; c < kCopies; ++c) {
-                        const uint32_t idx = c * 32 + lane, row = idx / CPR, chunk = idx % CPR;      // (row < 32 or not: the same for all lanes)
-                        const uint64_t from = __shfl_sync(0xffffffffu, c < CPR ? at[0] : at[kHold - 1], row & 31);
-                        const bool here = from != ~0ull && chunk * 8 < p.head_dim;
-                        cp_async16(slot + swz(kKeys, key0 + row, chunk), here ? base + from + chunk * 8 : p.k, here);
-                    }
-                    cp_commit();
-                };
-                copy(own ? p.k : p.c.k, kr, 2 * (n / RINGS));
-                copy(own ? p.v : p.c.v, vr, 2 * (n / RINGS) + 1);
-                cp_wait<1>();
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + ring0 + kr.slot);
-                cp_wait<0>();
-                if (own) {                                               // clear non-finite V of the nodes before it is used
-                    bool odd = false;
-                    __syncwarp();
-                    for (uint32_t c = 0; c < kCopies; ++c) {
-                        const uint32_t idx = c * 32 + lane;
-                        odd |= clear_nonfinite(reinterpret_cast<uint4*>(smem + (ring0 + vr.slot) * S::kSlot + swz(kKeys, key0 + idx / CPR, idx % CPR)));
-                    }
-                    if (__any_sync(0xffffffffu, odd) && lane == 0) fixes[(n & 15) * 2 + key0 / 32] = 1;
-                }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + ring0 + vr.slot);
-                kr.move(2 * kWarps / RINGS);
-                vr.move(2 * kWarps / RINGS);
-            }
-            tile += x.n_tiles;
-            u += x.n_tiles;
-        }
+        // ---- loaders -----------------------------------------------------------------------------------------
+        load_stream<D, RING, RINGS, S::kTeams, S::kTeam>(p, u, u_end, b, seq_first, warp - (S::kThreads - S::kLoaders) / 32, smem, full, empty, info, valid, fixes, ok,
+                                                         [](uint32_t r, uint32_t c) { return swz(kKeys, r, c); });
     }
     if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);
     tc_fence_before();
@@ -722,6 +616,7 @@ cudaError_t launch_attend_tc(const AttendParams& p, bool f32, AttendWorkspace& w
     if (f32) return p.head_dim <= 64 ? run<64, 1, false, 3>(p, ws, sm_count, use_pdl, s) : run<128, 1, false, 3>(p, ws, sm_count, use_pdl, s);
     if (p.head_dim <= 64) return wide ? run<64, 2, true, 1>(p, ws, sm_count, use_pdl, s) : run<64, 2, false, 1>(p, ws, sm_count, use_pdl, s);
     if (p.head_dim <= 128) return wide ? run<128, 2, true, 1>(p, ws, sm_count, use_pdl, s) : run<128, 2, false, 1>(p, ws, sm_count, use_pdl, s);
+    if (p.head_dim <= 192) return run<192, 1, false, 1>(p, ws, sm_count, use_pdl, s);
     return run<256, 1, false, 1>(p, ws, sm_count, use_pdl, s);
 }
 
