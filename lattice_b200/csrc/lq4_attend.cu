@@ -27,8 +27,6 @@
 // and added back at the end for the rows that do see it.
 #include "lq4_attend_dev.cuh"
 
-#include <atomic>
-
 namespace lq4 {
 
 namespace {

@@ -10,7 +10,6 @@ namespace lq4 {
 
 constexpr uint32_t kKeys = 64;                 // keys per tile
 constexpr uint32_t kMaxNodes = LQ4_MAX_TREE_NODES;
-constexpr uint32_t kMinShare = 1;              // tiles a CTA takes at least
 
 struct AttendParams {
     CacheView c;
@@ -70,7 +69,7 @@ __device__ __forceinline__ void warp_prefix(const AttendParams& p, uint32_t b, u
 
 __device__ __forceinline__ uint64_t cta_share(uint64_t total, uint32_t grid) {
     const uint64_t per = (total + grid - 1) / grid;
-    return per < kMinShare ? kMinShare : per;
+    return per ? per : 1;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {

@@ -1,6 +1,6 @@
 // lq4_tree_attention for many rows per kv head (a large tree), on the 5th-generation tensor cores.
 //
-// With R query rows on a key/value head there are R flops per byte of cache, so beyond some 50 rows the HBM
+// With R query rows on a key/value head there are R flops per byte of cache, so with some dozens of rows the HBM
 // stream is no longer the bound and mma.sync (552 TFLOP/s measured here) is; tcgen05.mma has three times that.  The work
 // is cut exactly as in lq4_attend.cu (tiles of 64 keys, an even share of all tiles per persistent CTA, partials
 // joined by attend_join_kernel); only what happens inside a piece differs.  An item has 128 rows (the lanes of
@@ -26,10 +26,9 @@
 //
 // f32 activations (up to D = 128): q and P are three bf16 terms each, 24 bits, smallest products first.  The accumulators
 // in tensor memory cut off below their last bit at every MMA, some 10^-5 over a few hundred of them, so P V of a tile
-// starts from zero and the softmax threads add it to O in their registers; one stream.
+// starts from zero and the softmax threads add it to O in their registers, a tile later; one stream, two buffers of P and
+// of P V.
 #include "lq4_attend_dev.cuh"
-
-#include <atomic>
 
 namespace lq4 {
 
@@ -134,12 +133,13 @@ struct TcShape {
     static constexpr uint32_t kFit = ((uint32_t)kMaxSmem - kQ - 5120) / kSlot / kRings, kRing = kFit > 12 / kRings ? 12 / kRings : kFit, kSlots = kRing * kRings;
     static constexpr uint32_t kValid = kSlots * kSlot + kQ, kFixes = kValid + 16 * 8, kAnc = kFixes + 16 * 8, kMeet = kAnc + kMaxNodes * 8;
     static constexpr uint32_t kBars = kMeet + kTcRows * 8, kCtl = kBars + 56 * 8, kSmem = kCtl + 160 + 1024;      // + alignment slack
-    static constexpr uint32_t kColO = 0, kColS = NS * D, kColP = kColS + NS * 64, kCols = kColP + NS * 32 * NQ <= 256 ? 256 : 512;
+    // Three terms: two buffers of O and P, so that a tile's P V runs beside the next tile's softmax.
+    static constexpr uint32_t kBufs = NQ == 1 ? NS : 2, kColO = 0, kColS = kBufs * D, kColP = kColS + NS * 64, kEnd = kColP + kBufs * 32 * NQ, kCols = kEnd <= 256 ? 256 : 512;
     // Loaders: teams, warps of a team.  (Seven warps for three terms: with nine a thread has 168 registers, and O spills.)
     static constexpr uint32_t kTeams = NQ == 1 && kSlots >= 8 ? 4 : 2, kTeam = NQ == 1 ? 4 / kTeams : 1;
     static constexpr int kLoaders = 32 * kTeams * kTeam, kThreads = kSoftmax + 32 * NS + kLoaders;
     static_assert(2 * kTeams / kRings <= kRing, "a team's next tile is at most a ring ahead of its last one");
-    static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kColP + NS * 32 * NQ <= 512, "shared or tensor memory");
+    static_assert(kSlots >= 4 && kSmem <= (uint32_t)kMaxSmem && kEnd <= 512, "shared or tensor memory");
     static_assert(NQ == 1 || NS == 1, "three terms take one stream");
     static_assert(NS == 2 || !WIDE, "256 rows take two streams");
     static_assert(kTcRows * 32 * 4 <= kQ, "the streams meet in Q's place");
@@ -279,15 +279,19 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             float m = -INFINITY, l = 0.0f;                               // base (log2) and sum of this row
             bool first = true;
             float acc[NQ == 1 ? 1 : D];                                  // f32 activations: O
-            auto fold = [&]() {                                          // O += the tile's P V
+            auto fold = [&](float f) {                                   // O = f (O + P V of the tile before)
                 if constexpr (NQ > 1) {
+                    const uint32_t last = used - 1;
+                    wait(o_done + (last & 1), last >> 1 & 1);
+                    __syncwarp();
+                    tc_fence_after();
 #pragma unroll
                     for (int d = 0; d < D; d += 32) {
                         float o[32];
-                        tmem_ld32<0>(col_o + d, o);
+                        tmem_ld32<0>(col_o + (last & 1) * D + d, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[d + e] += o[e];
+                        for (int e = 0; e < 32; ++e) acc[d + e] = (acc[d + e] + o[e]) * f;
                     }
                 }
             };
@@ -324,25 +328,23 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                     for (int e = 0; e < 4; ++e) t4[e] = fmaxf(t4[e], s[60 + e]);
                     top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
                 }
-                // P's buffer and O are free once the stream's MMA before has read and written them
-                if (!first) wait(o_done + str, (used - 1) & 1);
+                // P's buffer and O are free once the stream's MMA before has read and written them (three terms: two tiles
+                // before, which the last fold has waited for)
+                if (NQ == 1 && !first) wait(o_done + str, (used - 1) & 1);
                 __syncwarp();
                 tc_fence_after();
+                float f = 1.0f;
                 if constexpr (NQ > 1) {
-                    if (!first) fold();
-                    if (__any_sync(0xffffffffu, top > m)) {
-                        const float up = fmaxf(m, top), f = m == up ? 1.0f : exp2_fast(m - up);      // (m -inf: 0)
-                        l *= f;
-                        m = up;
-#pragma unroll
-                        for (int d = 0; d < D; ++d) acc[d] *= f;
-                    }
+                    const float up = fmaxf(m, top);
+                    if (m != up) f = exp2_fast(m - up);                  // (m -inf: 0)
+                    l *= f;
+                    m = up;
                 } else if (first) {
                     m = top;
                 } else {
                     const bool grow = top > m + kLazy;                   // (m -inf: at the first finite score)
                     if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? exp2_fast(m - top) : 1.0f;
+                        f = grow ? exp2_fast(m - top) : 1.0f;
                         l *= f;
                         m = grow ? top : m;
 #pragma unroll 1
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                             uint32_t w[8];
 #pragma unroll
                             for (int j = 0; j < 8; ++j) w[j] = split_pair(e[2 * j], e[2 * j + 1]);
-                            tmem_st8(col_p + 32 * n + 8 * k, w);
+                            tmem_st8(col_p + (used & 1) * (32 * NQ) + 32 * n + 8 * k, w);
                         }
                     }
                 }
@@ -396,13 +398,14 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + str);
+                if (NQ > 1 && !first) fold(f);                           // (its P V has had this tile's softmax to finish in)
                 first = false;
                 ++used;
             }
-            if (!first) wait(o_done + str, (used - 1) & 1);
+            if (NQ == 1 && !first) wait(o_done + str, (used - 1) & 1);
             __syncwarp();
             tc_fence_after();
-            if (NQ > 1 && !first) fold();
+            if (NQ > 1 && !first) fold(1.0f);
             // ---- O of this piece: the result, or a partial.  Two streams over the keys: stream 1 hands its O to stream 0
             // through Q's place, 32 columns at a time (both have waited for all MMAs of their own that read Q; the
             // barrier below covers the other's).
@@ -530,7 +533,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             }
         } kr{0, 0}, vr{1, 0};
         const uint32_t ring0 = RINGS == 2 ? str * RING : 0;              // first slot of the stream's ring
-        uint32_t piece = 0, ph_s = 1, ph_p = 0, at = 0;                  // s_free: phase 1 of the step before the first; tiles so far
+        uint32_t piece = 0, ph_s = 1, ph_p = 0, at = 0, buf = 0;         // s_free: phase 1 of the step before the first; tiles so far; O and P in turn
         bool s_any = false;
         auto scores = [&]() {
             wait(full + ring0 + kr.slot, kr.phase);
@@ -569,11 +572,12 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
 #pragma unroll
                     for (int ks = 0; ks < NQ * ((int)kKeys / 16); ++ks) {
                         const int n = NQ - 1 - ks / 4, c = ks & 3;
-                        mma_ts(col_o, col_p + n * 32 + c * 8, vt + (c * 2048 >> 4), instr_desc(D, 1), (NQ == 1 && v > 0) || ks > 0);
+                        mma_ts(col_o + buf * D, col_p + buf * (32 * NQ) + n * 32 + c * 8, vt + (c * 2048 >> 4), instr_desc(D, 1), (NQ == 1 && v > 0) || ks > 0);
                     }
                     mma_commit(empty + ring0 + vr.slot);
-                    mma_commit(o_done + str);
+                    mma_commit(o_done + (NQ == 1 ? str : buf));
                 }
+                if (NQ > 1) buf ^= 1;
                 vr.move(2);
             }
             at += tiles;
