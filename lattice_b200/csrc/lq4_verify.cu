@@ -12,8 +12,8 @@
 // cumulated residual exceeds u_0 times its sum; temperature 0 compares with the argmax throughout.
 //
 // One thread-block cluster per sequence walks down from the root and reads only the rows of the nodes it
-// visits (a tree of 64 nodes has few on its path); the vocabulary is cut over the cluster, 256 logits per warp
-// step.  The rows of a node are read once: a warp's share (four steps at most, as a rule) stays in registers as
+// visits (a tree of 64 nodes has few on its path); the vocabulary is cut over the cluster, 512 bytes of logits per
+// warp step.  The rows of a node are read once: a warp's share (32 logits a lane at most, as a rule) stays in registers as
 // masses relative to the warp's own maximum, (max, sum) of p and q go through distributed shared memory with one
 // cluster barrier, a refusal is a pass over the registers with another barrier, and the last token comes from the one
 // warp that the border falls into.  Longer shares are read again instead.  Every CTA takes every decision itself from the
@@ -21,7 +21,7 @@
 // barrier); the first child's rows are fetched into L2 meanwhile.
 //
 // Decisions lie next to borders.  Masses are f32 (ex2.approx of the rounded distance from the maximum: a few 2^-23, and
-// exactly 1 at the maximum; eight at a time are added in f32); all further sums are pairs of f32 (some 48 bits, any size of
+// exactly 1 at the maximum; four or eight at a time are added in f32); all further sums are pairs of f32 (some 48 bits, any size of
 // residual; sums of equal masses are exact, so that they meet a border where they should).  f64 is left to one lane: this
 // part does about two f64 operations a cycle and SM.  Code is kept short for the same reason as the loads are early: a
 // node's pass runs through it once, and instruction fetches count.
@@ -130,20 +130,20 @@ __device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) {
     return ((uint64_t)u << 32) | (uint32_t)~id;
 }
 
-// Elements [j, j + 8) of a row: fetched as they lie where a 16-byte load fits, and then read as f32, -inf outside the row and
-// for NaN.  In two steps, so that many fetches can be under way before the first value is used.  The few at a row's ends,
-// and rows of the draft that lie otherwise than the target's, come one by one.
-struct Raw {
-    uint4 a, b;
-};
-struct Eight {
-    float x[8];
+// A lane's V logits (16 bytes), from element j of a row on: fetched as they lie where the load fits, and then read as f32,
+// -inf outside the row and for NaN.  In two steps, so that many fetches can be under way before the first value is used.  The
+// few at a row's ends, and rows of the draft that lie otherwise than the target's, come one by one.
+template <typename T>
+constexpr int kLane = 16 / sizeof(T);
+template <int V>
+struct Few {
+    float x[V];
 };
 template <typename T>
-__device__ __noinline__ Eight edge8(const T* row, int32_t j, int32_t end) {
-    Eight r;
+__device__ __noinline__ Few<kLane<T>> edge(const T* row, int32_t j, int32_t end) {
+    Few<kLane<T>> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kLane<T>; ++i) {
         r.x[i] = -INFINITY;
         if (j + i >= 0 && j + i < end) {
             if constexpr (std::is_same<T, float>::value)
@@ -155,41 +155,35 @@ __device__ __noinline__ Eight edge8(const T* row, int32_t j, int32_t end) {
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void fetch8(const T* row, int32_t j, bool fits, Raw& r) {
-    if (fits) {
-        r.a = __ldg(reinterpret_cast<const uint4*>(row + j));
-        if (std::is_same<T, float>::value) r.b = __ldg(reinterpret_cast<const uint4*>(row + j) + 1);
-    }
+__device__ __forceinline__ void fetch(const T* row, int32_t j, bool fits, uint4& r) {
+    if (fits) r = __ldg(reinterpret_cast<const uint4*>(row + j));
 }
 template <typename T>
-__device__ __forceinline__ void read8(const T* row, int32_t j, int32_t end, bool fits, const Raw& r, float (&x)[8]) {
+__device__ __forceinline__ void read(const T* row, int32_t j, int32_t end, bool fits, const uint4& r, float (&x)[kLane<T>]) {
     if (fits) {
-        const uint4 a = r.a;
-        if constexpr (std::is_same<T, float>::value) {
-            const uint4 b = r.b;
-            x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
-            x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
-        } else {
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, float>::value) {
+                x[i] = __uint_as_float(w[i]);
+            } else {
                 x[2 * i] = __uint_as_float(w[i] << 16);
                 x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
             }
         }
     } else {
-        const Eight e = edge8(row, j, end);
+        const Few<kLane<T>> e = edge(row, j, end);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = e.x[i];
+        for (int i = 0; i < kLane<T>; ++i) x[i] = e.x[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = clean(x[i]);
+    for (int i = 0; i < kLane<T>; ++i) x[i] = clean(x[i]);
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int32_t j, int32_t end, bool fits, float (&x)[8]) {
-    Raw r;
-    fetch8(row, j, fits, r);
-    read8(row, j, end, fits, r, x);
+__device__ __forceinline__ void load(const T* row, int32_t j, int32_t end, bool fits, float (&x)[kLane<T>]) {
+    uint4 r;
+    fetch(row, j, fits, r);
+    read(row, j, end, fits, r, x);
 }
 
 template <typename T>
@@ -210,13 +204,18 @@ struct Row {                            // the current node's distributions, for
     uint64_t best;
 };
 
-constexpr uint32_t kHeld = 4;            // steps of a warp's share that stay in registers
+// Logits of a warp step; steps of a warp's share that stay in registers (32 logits a lane).
+template <typename T>
+constexpr uint32_t kStep = 32 * kLane<T>;
+template <typename T>
+constexpr uint32_t kHeldSteps = 32 / kLane<T>;
 
-// HELD: every warp's share is at most kHeld steps.
+// HELD: every warp's share is at most that many steps.
 template <typename T, bool HELD>
 __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_constant__ VerifyParams p) {
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    constexpr uint32_t V = kLane<T>, STEP = kStep<T>, kHeld = kHeldSteps<T>;
     const uint32_t b = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     __shared__ Exchange slots[2][kMaxCluster];
@@ -266,15 +265,15 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 
     const uint32_t all_warps = ranks * kVWarps, me = rank * kVWarps + warp;
     for (;;) {
-        // this warp's part of the row: steps of 256 logits, from the row's own 16-byte border on
+        // this warp's part of the row, in steps from the row's own 16-byte border on
         const T* prow = target_rows + cur * p.target_node;
         const T* qrow = sampled ? draft_rows + cur * p.draft_node : nullptr;
         const int32_t shift = (int32_t)((reinterpret_cast<uintptr_t>(prow) & 15) / sizeof(T));
-        const uint32_t steps = (p.vocab + shift + 255) / 256, per = (steps + all_warps - 1) / all_warps;
+        const uint32_t steps = (p.vocab + shift + STEP - 1) / STEP, per = (steps + all_warps - 1) / all_warps;
         const uint32_t c0 = min(me * per, steps), c1 = min(c0 + per, steps);
         const bool q_alike = ((reinterpret_cast<uintptr_t>(prow) ^ reinterpret_cast<uintptr_t>(qrow)) & 15) == 0;
-        auto at = [&](uint32_t c) { return (int32_t)(c * 256 + lane * 8) - shift; };      // this lane's first logit of step c
-        auto fits = [&](int32_t j, int32_t end) { return j >= 0 && j + 8 <= end; };
+        auto at = [&](uint32_t c) { return (int32_t)(c * STEP + lane * V) - shift; };      // this lane's first logit of step c
+        auto fits = [&](int32_t j, int32_t end) { return j >= 0 && j + (int32_t)V <= end; };
         uint32_t child = (uint32_t)n;                                    // the first one
         for (uint32_t c = (uint32_t)n - 1; c > cur; --c)
             if (parent[c] == (int32_t)cur) child = c;
@@ -284,22 +283,22 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         WarpSum sp{-INFINITY, {0.0f, 0.0f}}, sq = sp;                    // of this warp
         const int32_t vocab = (int32_t)p.vocab;
         uint64_t best = 0;
-        float ep[HELD ? kHeld : 1][8], eq[HELD ? kHeld : 1][8];          // masses relative to sp.m and sq.m
+        float ep[HELD ? kHeld : 1][V], eq[HELD ? kHeld : 1][V];          // masses relative to sp.m and sq.m
         if constexpr (HELD) {
-            Raw rp[kHeld], rq[kHeld];                                    // all loads are under way before the first use
+            uint4 rp[kHeld], rq[kHeld];                                  // all loads are under way before the first use
 #pragma unroll
             for (uint32_t h = 0; h < kHeld; ++h) {
                 const int32_t j = at(c0 + h);
                 const bool f = fits(j, c0 + h < c1 ? vocab : 0);
-                fetch8(prow, j, f, rp[h]);
-                fetch8(qrow, j, f && q_alike && with_q, rq[h]);
+                fetch(prow, j, f, rp[h]);
+                fetch(qrow, j, f && q_alike && with_q, rq[h]);
             }
             if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
                 const T* next_p = target_rows + child * p.target_node;
                 const T* next_q = sampled ? draft_rows + child * p.draft_node : next_p;
                 for (uint32_t h = 0; h < kHeld; ++h) {
-                    const uint32_t j = (c0 + h) * 256 + lane * 8;
-                    if (c0 + h < c1 && j < p.vocab && (lane & (sizeof(T) == 4 ? 3 : 7)) == 0) {
+                    const uint32_t j = (c0 + h) * STEP + lane * V;
+                    if (c0 + h < c1 && j < p.vocab && (lane & 7) == 0) {
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(next_p + j));
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(next_q + j));
                     }
@@ -308,8 +307,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 #pragma unroll
             for (uint32_t h = 0; h < kHeld; ++h) {
                 const int32_t j = at(c0 + h), end = c0 + h < c1 ? vocab : 0;
-                read8(prow, j, end, fits(j, end), rp[h], ep[h]);
-                if (with_q) read8(qrow, j, end, fits(j, end) && q_alike, rq[h], eq[h]);
+                read(prow, j, end, fits(j, end), rp[h], ep[h]);
+                if (with_q) read(qrow, j, end, fits(j, end) && q_alike, rq[h], eq[h]);
             }
             if (greedy) {
                 float top = -INFINITY;
@@ -317,16 +316,16 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 #pragma unroll
                 for (uint32_t h = 0; h < kHeld; ++h)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    for (int i = 0; i < (int)V; ++i)
                         if (ep[h][i] > top) top = ep[h][i], id = at(c0 + h) + i;      // (rising ids: ties stay with the lower)
                 best = rank_key(top, (uint32_t)id);
             } else {
-                auto masses = [&](float (&v)[HELD ? kHeld : 1][8], WarpSum& s) {
+                auto masses = [&](float (&v)[HELD ? kHeld : 1][V], WarpSum& s) {
                     float m = -INFINITY;
 #pragma unroll
                     for (uint32_t h = 0; h < kHeld; ++h)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) m = fmaxf(m, v[h][i]);
+                        for (int i = 0; i < (int)V; ++i) m = fmaxf(m, v[h][i]);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                     const float base = m == -INFINITY ? 0.0f : m;
@@ -336,13 +335,13 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                         float t = 0.0f;
                         if (m == INFINITY) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) v[h][i] = v[h][i] == m ? 1.0f : 0.0f;
+                            for (int i = 0; i < (int)V; ++i) v[h][i] = v[h][i] == m ? 1.0f : 0.0f;
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) v[h][i] = exp2_fast((v[h][i] - base) * it);
+                            for (int i = 0; i < (int)V; ++i) v[h][i] = exp2_fast((v[h][i] - base) * it);
                         }
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) t += v[h][i];
+                        for (int i = 0; i < (int)V; ++i) t += v[h][i];
                         sum = plus(sum, {t, 0.0f});
                     }
                     s = {m, lanes_sum(sum)};
@@ -354,21 +353,21 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             for (uint32_t c = c0; c < c1; ++c) {
                 const int32_t j = at(c);
                 const bool f = fits(j, vocab);
-                float x[8], y[8];
-                load8(prow, j, vocab, f, x);
-                if (with_q) load8(qrow, j, vocab, f && q_alike, y);
+                float x[V], y[V];
+                load(prow, j, vocab, f, x);
+                if (with_q) load(qrow, j, vocab, f && q_alike, y);
                 if (greedy) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < (int)V; ++i) {
                         const uint64_t k = rank_key(x[i], (uint32_t)(j + i));
                         best = k > best ? k : best;
                     }
                     continue;
                 }
-                auto add = [&](WarpSum& s, const float (&v)[8]) {
+                auto add = [&](WarpSum& s, const float (&v)[V]) {
                     float m = v[0];
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+                    for (int i = 1; i < (int)V; ++i) m = fmaxf(m, v[i]);
 #pragma unroll
                     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                     if (m == -INFINITY) return;                          // (one maximum for the warp)
@@ -379,7 +378,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                     }
                     float t = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) t += mass(v[i], s.m, it);
+                    for (int i = 0; i < (int)V; ++i) t += mass(v[i], s.m, it);
                     s.s = plus(s.s, {t, 0.0f});
                 };
                 add(sp, x);
@@ -442,24 +441,24 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         const float fp = mass(sp.m, pm, it), fq = mass(sq.m, qm, it);    // the warp's masses -> the row's
 
         // The residual, in units of p's masses: without a refusal its terms are those masses.  Step h of the share, at logit j.
-        auto residual = [&](uint32_t h, int32_t j, float a, uint32_t ngone, float (&w)[8]) {
+        auto residual = [&](uint32_t h, int32_t j, float a, uint32_t ngone, float (&w)[V]) {
             const float k = a * row.q_over_p;
             if constexpr (HELD) {
                 const float kq = k * fq;
                 if (a != 0.0f) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = fmaxf(fmaf(-eq[h][i], kq, ep[h][i] * fp), 0.0f);
+                    for (int i = 0; i < (int)V; ++i) w[i] = fmaxf(fmaf(-eq[h][i], kq, ep[h][i] * fp), 0.0f);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = ep[h][i] * fp;
+                    for (int i = 0; i < (int)V; ++i) w[i] = ep[h][i] * fp;
                 }
             } else {
-                float x[8], y[8];
+                float x[V], y[V];
                 const bool f = fits(j, vocab);
-                load8(prow, j, vocab, f, x);
-                if (a != 0.0f) load8(qrow, j, vocab, f && q_alike, y);
+                load(prow, j, vocab, f, x);
+                if (a != 0.0f) load(qrow, j, vocab, f && q_alike, y);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < (int)V; ++i) {
                     w[i] = mass(x[i], pm, it);
                     if (a != 0.0f && qm != -INFINITY) w[i] = fmaxf(fmaf(-mass(y[i], qm, it), k, w[i]), 0.0f);
                 }
@@ -467,7 +466,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             for (uint32_t g = 0; g < ngone; ++g) {
                 const int32_t d = (int32_t)gone[g] - j;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < (int)V; ++i)
                     if (d == i) w[i] = 0.0f;
             }
         };
@@ -476,10 +475,10 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         auto residual_pass = [&](float a, uint32_t ngone) -> Pair {
             Pair sum{0.0f, 0.0f};
             auto step = [&](uint32_t h) {
-                float w[8], t = 0.0f;
+                float w[V], t = 0.0f;
                 residual(h, at(c0 + h), a, ngone, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t += w[i];
+                for (int i = 0; i < (int)V; ++i) t += w[i];
                 sum = plus(sum, {t, 0.0f});
             };
             if constexpr (HELD) {
@@ -592,11 +591,11 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             uint32_t found = kNoToken, last = kNoToken;
             auto scan = [&](uint32_t h) {
                 const int32_t j = at(c0 + h);
-                float w[8], part[8], t = 0.0f;
+                float w[V], part[V], t = 0.0f;
                 residual(h, j, a, ngone, w);
                 uint32_t mine = kNoToken, end = kNoToken;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < (int)V; ++i) {
                     t += w[i];
                     part[i] = t;
                     if (w[i] > 0.0f) end = (uint32_t)(j + i);
@@ -605,7 +604,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                 Pair before = {__shfl_up_sync(0xffffffffu, incl.h, 1), __shfl_up_sync(0xffffffffu, incl.l, 1)};
                 if (lane == 0) before = base;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < (int)V; ++i)
                     if (mine == kNoToken && w[i] > 0.0f && above(plus(before, {part[i], 0.0f}), border)) mine = (uint32_t)(j + i);
                 const uint32_t hits = __ballot_sync(0xffffffffu, mine != kNoToken), some = __ballot_sync(0xffffffffu, end != kNoToken);
                 if (hits && found == kNoToken) found = __shfl_sync(0xffffffffu, mine, __ffs(hits) - 1);
@@ -630,8 +629,8 @@ cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl
     // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
     uint32_t ranks = kMaxCluster;
     while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
-    const uint64_t steps = ((uint64_t)p.vocab + 7 + 255) / 256;         // (a row may start up to 7 logits behind a border)
-    const bool held = (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeld;
+    const uint64_t steps = ((uint64_t)p.vocab + kLane<T> - 1 + kStep<T> - 1) / kStep<T>;      // (a row may start behind a 16-byte border)
+    const bool held = (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeldSteps<T>;
     auto fn = held ? verify_kernel<T, true> : verify_kernel<T, false>;
     static DeviceOnce once_of[2];
     DeviceOnce& once = once_of[held];
