@@ -588,7 +588,8 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args,
  *   path[b, 0 .. path_len[b])   the accepted nodes from node 0 on (rising), -1 behind them: `index` and `counts`
  *                               of lq4_kv_append
  * Sequences with node_counts[b] <= 0 get path_len 0 and next_token -1.  Exponentials are f32, sums over
- * the vocabulary pairs of f32, comparisons f64.  One launch, no workspace.  Stands behind the
+ * the vocabulary pairs of f32, comparisons f64.  One launch, or two and a small
+ * workspace where all rows together are few (make one plain call before capturing it).  Stands behind the
  * lm_head projection over all nodes' rows, where a plain step calls lq4_logits_topk. */
 typedef struct {
     const void* target_logits;        /* [batch, nodes, vocab], F32 or BF16 */

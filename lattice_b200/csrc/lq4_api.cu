@@ -58,6 +58,7 @@ struct lq4_ctx {
     uint32_t* tsync = nullptr;    // 64-bit launch counter of the decode kernels
     Buf xrot, xs, t, tmsg, partials, hx, hy, gemm, logits, topk, topk_ctr, mlp, mlp_h;   // xs: activation limb records of the dense decode kernel
     lq4_peer_buf* mlp_step = nullptr;   // step buffer of lq4_mlp_block's one-launch form (gate||up row + mailbox)
+    Buf verify;                   // lq4_verify_draft: row statistics of small calls
     Buf attend;                   // lq4_tree_attention: partials of the items that are cut between CTAs
     Buf shard_send, shard_recv;   // staging of lq4_linear_sharded: local slices, NCCL's rank-major blocks
     cudaStream_t comm_stream = nullptr;      // second stream of lq4_linear_sharded (created on first use)
@@ -350,7 +351,7 @@ void lq4_ctx_destroy(lq4_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaDeviceSynchronize();
     free_step_plan(ctx->step_plan);
-    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv, &ctx->attend})
+    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv, &ctx->attend, &ctx->verify})
         if (b->p) cudaFree(b->p);
     if (ctx->mlp_step) lq4_peer_buf_free(ctx->mlp_step);
     for (cudaEvent_t e : ctx->ev_block)
@@ -1743,8 +1744,12 @@ lq4_status lq4_verify_draft(lq4_ctx* ctx, const lq4_verify_args* a, void* stream
     if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
     if (a->batch == 0) return LQ4_OK;
     LQ4_ON_DEVICE(ctx);
-    LQ4_CUDA(launch_verify_draft(*a, ctx->status, ctx->sm_count, ctx->pdl, (cudaStream_t)stream));
-    ctx->launches += 1;
+    cudaStream_t s = (cudaStream_t)stream;
+    lq4_status st;
+    if ((st = ensure(ctx, ctx->verify, verify_workspace_bytes(*a, ctx->sm_count), false, s))) return st;
+    int launches = 0;
+    LQ4_CUDA(launch_verify_draft(*a, ctx->verify.p, ctx->status, ctx->sm_count, ctx->pdl, s, &launches));
+    ctx->launches += launches;
     return LQ4_OK;
 }
 

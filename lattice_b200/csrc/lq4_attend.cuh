@@ -47,6 +47,8 @@ cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorksp
                                   int use_pdl, cudaStream_t s);
 
 // ---- lq4_verify.cu --------------------------------------------------------------
-cudaError_t launch_verify_draft(const lq4_verify_args& a, int32_t* status, int sm_count, int use_pdl, cudaStream_t s);
+// The row statistics of a small call (0 bytes: it takes none).
+size_t verify_workspace_bytes(const lq4_verify_args& a, int sm_count);
+cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32_t* status, int sm_count, int use_pdl, cudaStream_t s, int* launches);
 
 }  // namespace lq4

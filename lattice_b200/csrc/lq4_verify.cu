@@ -17,7 +17,11 @@
 // masses relative to the warp's own maximum, (max, sum) of p and q go through distributed shared memory with one
 // cluster barrier, a refusal is a pass over the registers with another barrier, and the last token comes from the one
 // warp that the border falls into.  Longer shares are read again instead.  Every CTA takes every decision itself from the
-// same numbers, in the same order.  What bounds it is the chain of latencies per node (rows, two reductions, a
+// same numbers, in the same order.
+//
+// A cluster lives in one GPC and gets some 0.8 TB/s: two rows of 248320 f32 logits are 2.5 us and more per node, one node after
+// the other.  Where all rows together are few enough (kEagerBytes), verify_stats_kernel takes (max, sum) of every row over the
+// whole GPU first; the walk then only reads the rows of a node where a draft is refused or the last token is drawn.  What bounds it is the chain of latencies per node (rows, two reductions, a
 // barrier); the first child's rows are fetched into L2 meanwhile.
 //
 // Decisions lie next to borders.  Masses are f32 (ex2.approx of the rounded distance from the maximum: a few 2^-23, and
@@ -54,6 +58,8 @@ struct VerifyParams {
     int32_t* path_len;
     int32_t* next_token;
     int32_t* status;
+    struct Stat* stats;                 // [2: target, draft][batch * nodes][splits], or NULL
+    uint32_t batch, splits;
 };
 
 // An unevaluated sum h + l of two f32, |l| at most half a step of h.
@@ -194,6 +200,10 @@ __device__ __forceinline__ float one_logit(const T* row, uint32_t j) {
         return clean(bf16_to_f32(row[j]));
 }
 
+struct Stat {                           // of a split of a row, for the walk
+    WarpSum s;
+    uint64_t best;
+};
 struct Exchange {                       // what a CTA tells the others
     WarpSum p, q;
     uint64_t best;
@@ -284,70 +294,78 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         const int32_t vocab = (int32_t)p.vocab;
         uint64_t best = 0;
         float ep[HELD ? kHeld : 1][V], eq[HELD ? kHeld : 1][V];          // masses relative to sp.m and sq.m
-        if constexpr (HELD) {
-            uint4 rp[kHeld], rq[kHeld];                                  // all loads are under way before the first use
+        // The warp's logits of p, and of q where children need it, into ep and eq.
+        auto hold = [&]() {
+            if constexpr (HELD) {
+                uint4 rp[kHeld], rq[kHeld];                                  // all loads are under way before the first use
 #pragma unroll
-            for (uint32_t h = 0; h < kHeld; ++h) {
-                const int32_t j = at(c0 + h);
-                const bool f = fits(j, c0 + h < c1 ? vocab : 0);
-                fetch(prow, j, f, rp[h]);
-                fetch(qrow, j, f && q_alike && with_q, rq[h]);
-            }
-            if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
-                const T* next_p = target_rows + child * p.target_node;
-                const T* next_q = sampled ? draft_rows + child * p.draft_node : next_p;
                 for (uint32_t h = 0; h < kHeld; ++h) {
-                    const uint32_t j = (c0 + h) * STEP + lane * V;
-                    if (c0 + h < c1 && j < p.vocab && (lane & 7) == 0) {
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(next_p + j));
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(next_q + j));
-                    }
+                    const int32_t j = at(c0 + h);
+                    const bool f = fits(j, c0 + h < c1 ? vocab : 0);
+                    fetch(prow, j, f, rp[h]);
+                    fetch(qrow, j, f && q_alike && with_q, rq[h]);
+                }
+#pragma unroll
+                for (uint32_t h = 0; h < kHeld; ++h) {
+                    const int32_t j = at(c0 + h), end = c0 + h < c1 ? vocab : 0;
+                    read(prow, j, end, fits(j, end), rp[h], ep[h]);
+                    if (with_q) read(qrow, j, end, fits(j, end) && q_alike, rq[h], eq[h]);
                 }
             }
-#pragma unroll
-            for (uint32_t h = 0; h < kHeld; ++h) {
-                const int32_t j = at(c0 + h), end = c0 + h < c1 ? vocab : 0;
-                read(prow, j, end, fits(j, end), rp[h], ep[h]);
-                if (with_q) read(qrow, j, end, fits(j, end) && q_alike, rq[h], eq[h]);
-            }
-            if (greedy) {
-                float top = -INFINITY;
-                int32_t id = -1;
-#pragma unroll
-                for (uint32_t h = 0; h < kHeld; ++h)
-#pragma unroll
-                    for (int i = 0; i < (int)V; ++i)
-                        if (ep[h][i] > top) top = ep[h][i], id = at(c0 + h) + i;      // (rising ids: ties stay with the lower)
-                best = rank_key(top, (uint32_t)id);
-            } else {
-                auto masses = [&](float (&v)[HELD ? kHeld : 1][V], WarpSum& s) {
-                    float m = -INFINITY;
+        };
+        if constexpr (HELD) {
+            if (p.stats == nullptr) {
+                hold();
+                if (child < (uint32_t)n) {                                   // most likely the next node: its rows into L2
+                    const T* next_p = target_rows + child * p.target_node;
+                    const T* next_q = sampled ? draft_rows + child * p.draft_node : next_p;
+                    for (uint32_t h = 0; h < kHeld; ++h) {
+                        const uint32_t j = (c0 + h) * STEP + lane * V;
+                        if (c0 + h < c1 && j < p.vocab && (lane & 7) == 0) {
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(next_p + j));
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(next_q + j));
+                        }
+                    }
+                }
+                if (greedy) {
+                    float top = -INFINITY;
+                    int32_t id = -1;
 #pragma unroll
                     for (uint32_t h = 0; h < kHeld; ++h)
 #pragma unroll
-                        for (int i = 0; i < (int)V; ++i) m = fmaxf(m, v[h][i]);
+                        for (int i = 0; i < (int)V; ++i)
+                            if (ep[h][i] > top) top = ep[h][i], id = at(c0 + h) + i;      // (rising ids: ties stay with the lower)
+                    best = rank_key(top, (uint32_t)id);
+                } else {
+                    auto masses = [&](float (&v)[HELD ? kHeld : 1][V], WarpSum& s) {
+                        float m = -INFINITY;
 #pragma unroll
-                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    Pair sum{0.0f, 0.0f};
+                        for (uint32_t h = 0; h < kHeld; ++h)
 #pragma unroll
-                    for (uint32_t h = 0; h < kHeld; ++h) {
-                        float t = 0.0f;
-                        if (m == INFINITY) {
+                            for (int i = 0; i < (int)V; ++i) m = fmaxf(m, v[h][i]);
 #pragma unroll
-                            for (int i = 0; i < (int)V; ++i) v[h][i] = v[h][i] == m ? 1.0f : 0.0f;
-                        } else {
+                        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        const float base = m == -INFINITY ? 0.0f : m;
+                        Pair sum{0.0f, 0.0f};
 #pragma unroll
-                            for (int i = 0; i < (int)V; ++i) v[h][i] = exp2_fast((v[h][i] - base) * it);
+                        for (uint32_t h = 0; h < kHeld; ++h) {
+                            float t = 0.0f;
+                            if (m == INFINITY) {
+#pragma unroll
+                                for (int i = 0; i < (int)V; ++i) v[h][i] = v[h][i] == m ? 1.0f : 0.0f;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < (int)V; ++i) v[h][i] = exp2_fast((v[h][i] - base) * it);
+                            }
+#pragma unroll
+                            for (int i = 0; i < (int)V; ++i) t += v[h][i];
+                            sum = plus(sum, {t, 0.0f});
                         }
-#pragma unroll
-                        for (int i = 0; i < (int)V; ++i) t += v[h][i];
-                        sum = plus(sum, {t, 0.0f});
-                    }
-                    s = {m, lanes_sum(sum)};
-                };
-                masses(ep, sp);
-                if (with_q) masses(eq, sq);
+                        s = {m, lanes_sum(sum)};
+                    };
+                    masses(ep, sp);
+                    if (with_q) masses(eq, sq);
+                }
             }
         } else {
             for (uint32_t c = c0; c < c1; ++c) {
@@ -393,31 +411,42 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                 best = k > best ? k : best;
             }
         }
-        if (lane == 0) wp[warp] = sp, wq[warp] = sq, wbest[warp] = best;
-        __syncthreads();
-        if (warp == 0) {                                                 // the CTA's, told to all CTAs
-            Exchange e;
-            e.p = join_lanes(wp[lane & (kVWarps - 1)], kVWarps / 2, it);
-            e.q = join_lanes(wq[lane & (kVWarps - 1)], kVWarps / 2, it);
-            e.best = wbest[lane & (kVWarps - 1)];
+        if (p.stats == nullptr) {
+            if (lane == 0) wp[warp] = sp, wq[warp] = sq, wbest[warp] = best;
+            __syncthreads();
+            if (warp == 0) {                                                 // the CTA's, told to all CTAs
+                Exchange e;
+                e.p = join_lanes(wp[lane & (kVWarps - 1)], kVWarps / 2, it);
+                e.q = join_lanes(wq[lane & (kVWarps - 1)], kVWarps / 2, it);
+                e.best = wbest[lane & (kVWarps - 1)];
 #pragma unroll
-            for (int o = kVWarps / 2; o; o >>= 1) {
-                const uint64_t k = __shfl_xor_sync(0xffffffffu, e.best, o);
-                e.best = k > e.best ? k : e.best;
+                for (int o = kVWarps / 2; o; o >>= 1) {
+                    const uint64_t k = __shfl_xor_sync(0xffffffffu, e.best, o);
+                    e.best = k > e.best ? k : e.best;
+                }
+                e.total = {0.0f, 0.0f};
+                if (lane < ranks) *cluster.map_shared_rank(&slots[turn][rank], lane) = e;
             }
-            e.total = {0.0f, 0.0f};
-            if (lane < ranks) *cluster.map_shared_rank(&slots[turn][rank], lane) = e;
+            cluster.sync();
         }
-        cluster.sync();
         if (warp == 0) {
-            const uint32_t r = lane & (kMaxCluster - 1);                 // (both halves of the warp come to the same)
+            const uint32_t r = lane;                                     // (up to 16 CTAs, up to 32 splits)
             WarpSum P{-INFINITY, {0.0f, 0.0f}}, Q = P;
             best = 0;
-            if (r < ranks) P = slots[turn][r].p, Q = slots[turn][r].q, best = slots[turn][r].best;
-            P = join_lanes(P, kMaxCluster / 2, it);
-            Q = join_lanes(Q, kMaxCluster / 2, it);
+            if (p.stats != nullptr) {
+                const Stat* of = p.stats + (first + cur) * p.splits;
+                best = 0;
+                if (lane < p.splits) {
+                    P = of[lane].s, best = of[lane].best;
+                    if (with_q) Q = of[(uint64_t)p.batch * p.nodes * p.splits + lane].s;
+                }
+            } else if (r < ranks) {
+                P = slots[turn][r].p, Q = slots[turn][r].q, best = slots[turn][r].best;
+            }
+            P = join_lanes(P, 16, it);
+            Q = join_lanes(Q, 16, it);
 #pragma unroll
-            for (int o = kMaxCluster / 2; o; o >>= 1) {
+            for (int o = 16; o; o >>= 1) {
                 const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
                 best = k > best ? k : best;
             }
@@ -434,11 +463,12 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
                 child_q[c] = has_q ? mass_wide(one_logit(qrow, token[c]), Q.m, it) : 0.0;
             }
         }
-        turn ^= 1;
+        if (p.stats == nullptr) turn ^= 1;
         __syncthreads();
         const float pm = row.pm, qm = row.qm;
         best = row.best;
-        const float fp = mass(sp.m, pm, it), fq = mass(sq.m, qm, it);    // the warp's masses -> the row's
+        bool held = p.stats == nullptr;                                  // (with statistics the rows are read where they are needed)
+        float fp = mass(sp.m, pm, it), fq = mass(sq.m, qm, it);          // the warp's masses -> the row's
 
         // The residual, in units of p's masses: without a refusal its terms are those masses.  Step h of the share, at logit j.
         auto residual = [&](uint32_t h, int32_t j, float a, uint32_t ngone, float (&w)[V]) {
@@ -473,6 +503,18 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
         // Its sum over the vocabulary; every warp's share stays in wtot, every CTA's in the slots.
         uint32_t last_turn = 0;
         auto residual_pass = [&](float a, uint32_t ngone) -> Pair {
+            if (HELD && !held) {
+                held = true;
+                hold();
+#pragma unroll
+                for (uint32_t h = 0; h < (HELD ? kHeld : 1); ++h)
+#pragma unroll
+                    for (int i = 0; i < (int)V; ++i) {
+                        ep[h][i] = mass(ep[h][i], pm, it);
+                        if (with_q) eq[h][i] = mass(eq[h][i], qm, it);
+                    }
+                fp = fq = 1.0f;
+            }
             Pair sum{0.0f, 0.0f};
             auto step = [&](uint32_t h) {
                 float w[V], t = 0.0f;
@@ -624,13 +666,113 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     cluster.sync();                                                      // nobody leaves while others may still write its slots
 }
 
+// (max, sum) and the best candidate of every row that the walk may visit: one CTA per split of a row.
+constexpr uint32_t kStatThreads = 256, kMaxSplits = 32;
+constexpr uint64_t kEagerBytes = 32ull << 20;      // what this kernel may read: 5 us at HBM rate
+
 template <typename T>
-cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl, cudaStream_t s) {
+__global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
+    constexpr uint32_t V = kLane<T>, STEP = kStep<T>, WARPS = kStatThreads / 32;
+    __shared__ WarpSum ws[WARPS];
+    __shared__ uint64_t wbest[WARPS];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t split = blockIdx.x % p.splits, id = blockIdx.x / p.splits, rows = p.batch * p.nodes;
+    const bool draft = id >= rows;
+    const uint32_t at_row = draft ? id - rows : id, b = at_row / p.nodes, node = at_row - b * p.nodes;
+    pdl_wait_prior_grids();
+    pdl_launch_dependents();
+    const int32_t n = p.node_counts ? min(p.node_counts[b], (int32_t)p.nodes) : (int32_t)p.nodes;
+    if ((int32_t)node >= n) return;
+    const float tau = p.temperature ? p.temperature[b] : 1.0f;
+    const bool greedy = !(tau >= 1e-20f);
+    const float it = greedy ? 1.0f : 1.44269504088896340736f / tau;
+    if (draft) {                                                         // read for the children of a node, if it has any
+        bool inner = false;
+        for (uint32_t c = node + 1; c < (uint32_t)n && !inner; ++c) inner = (p.parents ? p.parents[(uint64_t)b * p.nodes + c] : (int32_t)c - 1) == (int32_t)node;
+        if (greedy || !inner) return;
+    }
+    const T* row = draft ? static_cast<const T*>(p.draft) + b * p.draft_batch + node * p.draft_node
+                         : static_cast<const T*>(p.target) + b * p.target_batch + node * p.target_node;
+    const int32_t vocab = (int32_t)p.vocab, shift = (int32_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const uint32_t steps = (p.vocab + shift + STEP - 1) / STEP, all = p.splits * WARPS, per = (steps + all - 1) / all;
+    const uint32_t me = split * WARPS + warp, c0 = min(me * per, steps), c1 = min(c0 + per, steps);
+    WarpSum s{-INFINITY, {0.0f, 0.0f}};
+    float top = -INFINITY;
+    int32_t top_id = -1;
+    constexpr uint32_t kAtATime = 32 / V;
+    for (uint32_t c = c0; c < c1; c += kAtATime) {
+        uint4 raw[kAtATime];
+        float x[kAtATime][V];
+#pragma unroll
+        for (uint32_t h = 0; h < kAtATime; ++h) {
+            const int32_t j = (int32_t)((c + h) * STEP + lane * V) - shift, end = c + h < c1 ? vocab : 0;
+            fetch(row, j, j >= 0 && j + (int32_t)V <= end, raw[h]);
+        }
+        float m = -INFINITY;
+#pragma unroll
+        for (uint32_t h = 0; h < kAtATime; ++h) {
+            const int32_t j = (int32_t)((c + h) * STEP + lane * V) - shift, end = c + h < c1 ? vocab : 0;
+            read(row, j, end, j >= 0 && j + (int32_t)V <= end, raw[h], x[h]);
+#pragma unroll
+            for (int i = 0; i < (int)V; ++i) {
+                m = fmaxf(m, x[h][i]);
+                if (x[h][i] > top) top = x[h][i], top_id = j + i;
+            }
+        }
+        if (greedy) continue;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m > s.m) {
+            const float f = s.m == -INFINITY ? 0.0f : mass(s.m, m, it);
+            s = {m, {s.s.h * f, s.s.l * f}};
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < kAtATime; ++h) {
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < (int)V; ++i) t += mass(x[h][i], s.m, it);
+            s.s = plus(s.s, {t, 0.0f});
+        }
+    }
+    s.s = lanes_sum(s.s);
+    uint64_t best = rank_key(top, (uint32_t)top_id);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+        best = k > best ? k : best;
+    }
+    if (lane == 0) ws[warp] = s, wbest[warp] = best;
+    __syncthreads();
+    if (warp == 0) {
+        const WarpSum all_s = join_lanes(ws[lane & (WARPS - 1)], WARPS / 2, it);
+        best = wbest[lane & (WARPS - 1)];
+#pragma unroll
+        for (int o = WARPS / 2; o; o >>= 1) {
+            const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+            best = k > best ? k : best;
+        }
+        if (lane == 0) p.stats[(uint64_t)id * p.splits + split] = {all_s, best};
+    }
+}
+
+// Splits of a row that the statistics are taken in; 0: the walk takes them itself.
+uint32_t stat_splits(const lq4_verify_args& a, int sm_count) {
+    const uint64_t rows = (uint64_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1), bytes = rows * a.vocab * (a.dtype == LQ4_DTYPE_F32 ? 4 : 2);
+    // a chain or tree of one node has nothing to walk; short rows are read by the cluster as fast as their statistics
+    if (a.nodes < 2 || bytes > kEagerBytes || (uint64_t)a.vocab * (a.dtype == LQ4_DTYPE_F32 ? 4 : 2) < (128u << 10)) return 0;
+    uint64_t splits = (4ull * sm_count + rows - 1) / rows;
+    return splits > kMaxSplits ? kMaxSplits : splits < 1 ? 1 : (uint32_t)splits;
+}
+
+template <typename T>
+cudaError_t run(VerifyParams p, int sm_count, int use_pdl, cudaStream_t s, int* launches) {
+    const uint32_t batch = p.batch;
     // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
     uint32_t ranks = kMaxCluster;
     while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
     const uint64_t steps = ((uint64_t)p.vocab + kLane<T> - 1 + kStep<T> - 1) / kStep<T>;      // (a row may start behind a 16-byte border)
     const bool held = (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeldSteps<T>;
+    if (!held) p.stats = nullptr;
     auto fn = held ? verify_kernel<T, true> : verify_kernel<T, false>;
     static DeviceOnce once_of[2];
     DeviceOnce& once = once_of[held];
@@ -653,12 +795,26 @@ cudaError_t run(const VerifyParams& p, uint32_t batch, int sm_count, int use_pdl
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = use_pdl ? 2 : 1;
+    *launches = 1;
+    if (p.stats) {
+        cudaLaunchConfig_t first = cfg;
+        first.gridDim = dim3(p.batch * p.nodes * (p.draft ? 2 : 1) * p.splits);
+        first.blockDim = dim3(kStatThreads);
+        first.attrs = attr + 1;
+        first.numAttrs = use_pdl ? 1 : 0;
+        if ((e = cudaLaunchKernelEx(&first, verify_stats_kernel<T>, p)) != cudaSuccess) return e;
+        *launches = 2;
+    }
     return cudaLaunchKernelEx(&cfg, fn, p);
 }
 
 }  // namespace
 
-cudaError_t launch_verify_draft(const lq4_verify_args& a, int32_t* status, int sm_count, int use_pdl, cudaStream_t s) {
+size_t verify_workspace_bytes(const lq4_verify_args& a, int sm_count) {
+    return (size_t)a.batch * a.nodes * 2 * stat_splits(a, sm_count) * sizeof(Stat);
+}
+
+cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32_t* status, int sm_count, int use_pdl, cudaStream_t s, int* launches) {
     VerifyParams p{};
     p.target = a.target_logits;
     p.draft = a.draft_logits;
@@ -675,7 +831,10 @@ cudaError_t launch_verify_draft(const lq4_verify_args& a, int32_t* status, int s
     p.path_len = a.path_len;
     p.next_token = a.next_token;
     p.status = status;
-    return a.dtype == LQ4_DTYPE_F32 ? run<float>(p, a.batch, sm_count, use_pdl, s) : run<uint16_t>(p, a.batch, sm_count, use_pdl, s);
+    p.batch = a.batch;
+    p.splits = stat_splits(a, sm_count);
+    p.stats = p.splits ? static_cast<Stat*>(workspace) : nullptr;
+    return a.dtype == LQ4_DTYPE_F32 ? run<float>(p, sm_count, use_pdl, s, launches) : run<uint16_t>(p, sm_count, use_pdl, s, launches);
 }
 
 }  // namespace lq4
