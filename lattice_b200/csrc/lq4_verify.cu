@@ -241,6 +241,8 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     __shared__ uint32_t gone[LQ4_MAX_TREE_NODES];
     __shared__ uint32_t s_action, s_child, s_gone;
     __shared__ double s_a, s_z;
+    __shared__ Row row_of[LQ4_MAX_TREE_NODES];                           // with statistics: every node's, known from the start
+    __shared__ double ip_of[LQ4_MAX_TREE_NODES];
 
     pdl_wait_prior_grids();
     pdl_launch_dependents();
@@ -272,6 +274,45 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     if (rank == 0 && tid < p.nodes) p.path[first + tid] = tid == 0 ? 0 : -1;
     uint32_t cur = 0, count = 1;
     __syncthreads();
+
+    // One warp: a row's shares, one per lane, to what the walk needs of it.
+    auto join_row = [&](WarpSum P, WarpSum Q, uint64_t best, bool with_q, Row& to, double& ip) {
+        P = join_lanes(P, 16, it);
+        Q = join_lanes(Q, 16, it);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+            best = k > best ? k : best;
+        }
+        const bool has_p = P.m != -INFINITY, has_q = with_q && Q.m != -INFINITY;      // (a row without mass has neither)
+        if (lane == 0) {
+            ip = has_p ? 1.0 / value(P.s) : 0.0;
+            to = {P.m, with_q ? Q.m : -INFINITY, has_q ? (float)(value(P.s) / value(Q.s)) : 0.0f, best};
+        }
+        __syncwarp();
+    };
+    auto child_masses = [&](uint32_t c, const T* prow, const T* qrow, const Row& r) {      // of a child's token behind its parent
+        if ((uint32_t)token[c] >= p.vocab) return;
+        child_p[c] = r.pm != -INFINITY ? mass_wide(one_logit(prow, token[c]), r.pm, it) : 0.0;
+        child_q[c] = r.qm != -INFINITY ? mass_wide(one_logit(qrow, token[c]), r.qm, it) : 0.0;
+    };
+    if (p.stats != nullptr) {
+        for (uint32_t node = warp; node < (uint32_t)n; node += kVWarps) {
+            bool with_q = false;
+            for (uint32_t c = node + 1; c < (uint32_t)n && sampled; ++c) with_q |= parent[c] == (int32_t)node;
+            const Stat* of = p.stats + (first + node) * p.splits;
+            Stat x{{-INFINITY, {0.0f, 0.0f}}, 0}, y = x;
+            if (lane < p.splits) {
+                x = of[lane];
+                if (with_q) y = of[(uint64_t)p.batch * p.nodes * p.splits + lane];
+            }
+            join_row(x.s, y.s, x.best, with_q, row_of[node], ip_of[node]);
+        }
+        __syncthreads();
+        if (tid < (uint32_t)n && tid > 0 && !greedy && parent[tid] >= 0 && parent[tid] < (int32_t)tid)
+            child_masses(tid, target_rows + parent[tid] * p.target_node, draft_rows + parent[tid] * p.draft_node, row_of[parent[tid]]);
+        __syncthreads();
+    }
 
     const uint32_t all_warps = ranks * kVWarps, me = rank * kVWarps + warp;
     for (;;) {
@@ -430,38 +471,18 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
             cluster.sync();
         }
         if (warp == 0) {
-            const uint32_t r = lane;                                     // (up to 16 CTAs, up to 32 splits)
-            WarpSum P{-INFINITY, {0.0f, 0.0f}}, Q = P;
-            best = 0;
             if (p.stats != nullptr) {
-                const Stat* of = p.stats + (first + cur) * p.splits;
+                if (lane == 0) row = row_of[cur], s_ip = ip_of[cur];
+            } else {
+                WarpSum P{-INFINITY, {0.0f, 0.0f}}, Q = P;
                 best = 0;
-                if (lane < p.splits) {
-                    P = of[lane].s, best = of[lane].best;
-                    if (with_q) Q = of[(uint64_t)p.batch * p.nodes * p.splits + lane].s;
-                }
-            } else if (r < ranks) {
-                P = slots[turn][r].p, Q = slots[turn][r].q, best = slots[turn][r].best;
+                if (lane < ranks) P = slots[turn][lane].p, Q = slots[turn][lane].q, best = slots[turn][lane].best;
+                join_row(P, Q, best, with_q, row, s_ip);
+                // the children's masses
+                for (uint32_t c = lane; c < (uint32_t)n && !greedy; c += 32)
+                    if (c > cur && parent[c] == (int32_t)cur) child_masses(c, prow, qrow, row);
             }
-            P = join_lanes(P, 16, it);
-            Q = join_lanes(Q, 16, it);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
-                best = k > best ? k : best;
-            }
-            const bool has_p = P.m != -INFINITY, has_q = with_q && Q.m != -INFINITY;      // (a row without mass has neither)
-            if (lane == 0) {
-                s_ip = has_p ? 1.0 / value(P.s) : 0.0;
-                row = {P.m, Q.m, has_q ? (float)(value(P.s) / value(Q.s)) : 0.0f, best};
-                s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
-            }
-            // the children's masses
-            for (uint32_t c = lane; c < (uint32_t)n; c += 32) {
-                if (greedy || c <= cur || parent[c] != (int32_t)cur || (uint32_t)token[c] >= p.vocab) continue;
-                child_p[c] = has_p ? mass_wide(one_logit(prow, token[c]), P.m, it) : 0.0;
-                child_q[c] = has_q ? mass_wide(one_logit(qrow, token[c]), Q.m, it) : 0.0;
-            }
+            if (lane == 0) s_child = cur + 1, s_gone = 0, s_a = 0.0, s_z = 1.0;
         }
         if (p.stats == nullptr) turn ^= 1;
         __syncthreads();
