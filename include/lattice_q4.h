@@ -549,7 +549,8 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* str
  * of range are not seen; they, a length above the capacity and a parent that does not come before its node (it
  * counts as a root) are reported through lq4_ctx_check.  Results depend on the lengths and the device only, not
  * on timing.  The workspace (at most 40 MB, independent of the lengths) grows on the first call with a larger
- * row count per kv head: make one plain call before capturing one into a CUDA graph.
+ * row count per kv head: make one plain call before capturing one into a CUDA graph.  An outgrown workspace is kept until
+ * the context is destroyed, so earlier graphs still replay.
  * Stands between lq4_kv_append and the o_proj call, where the reference encodes decode_attention
  * (forward/shaders/qwen35.metal:466-663). */
 #define LQ4_MAX_TREE_NODES 64
@@ -589,7 +590,8 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args,
  *                               of lq4_kv_append
  * Sequences with node_counts[b] <= 0 get path_len 0 and next_token -1.  Exponentials are f32, sums over
  * the vocabulary pairs of f32, comparisons f64.  One launch, or two and a small
- * workspace where all rows together are few (make one plain call before capturing it).  Stands behind the
+ * workspace where all rows together are few (make one plain call before capturing it; kept like
+ * lq4_tree_attention's when it is outgrown).  Stands behind the
  * lm_head projection over all nodes' rows, where a plain step calls lq4_logits_topk. */
 typedef struct {
     const void* target_logits;        /* [batch, nodes, vocab], F32 or BF16 */

@@ -60,6 +60,7 @@ struct lq4_ctx {
     lq4_peer_buf* mlp_step = nullptr;   // step buffer of lq4_mlp_block's one-launch form (gate||up row + mailbox)
     Buf verify;                   // lq4_verify_draft: row statistics of small calls
     Buf attend;                   // lq4_tree_attention: partials of the items that are cut between CTAs
+    std::vector<void*> outgrown;  // earlier allocations of these two
     Buf shard_send, shard_recv;   // staging of lq4_linear_sharded: local slices, NCCL's rank-major blocks
     cudaStream_t comm_stream = nullptr;      // second stream of lq4_linear_sharded (created on first use)
     cudaEvent_t ev_block[4] = {nullptr, nullptr, nullptr, nullptr}, ev_comm = nullptr;
@@ -99,6 +100,17 @@ lq4_status ensure(lq4_ctx* ctx, Buf& b, size_t bytes, bool zero, cudaStream_t s)
     if (zero) LQ4_CUDA(cudaMemsetAsync(b.p, 0, cap, s));      // on the caller's stream: ordered before the first launch that reads it
     b.cap = cap;
     ++ctx->alloc_gen;
+    return LQ4_OK;
+}
+
+// The same for a workspace that captured graphs hold the address of: the outgrown allocation lives as long as the
+// context, so that a graph captured before a larger call still replays.
+lq4_status ensure_kept(lq4_ctx* ctx, Buf& b, size_t bytes, cudaStream_t s) {
+    if (bytes <= b.cap) return LQ4_OK;
+    Buf next;
+    if (lq4_status st = ensure(ctx, next, bytes, false, s)) return st;
+    if (b.p) ctx->outgrown.push_back(b.p);
+    b = next;
     return LQ4_OK;
 }
 
@@ -353,6 +365,7 @@ void lq4_ctx_destroy(lq4_ctx* ctx) {
     free_step_plan(ctx->step_plan);
     for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv, &ctx->attend, &ctx->verify})
         if (b->p) cudaFree(b->p);
+    for (void* p : ctx->outgrown) cudaFree(p);
     if (ctx->mlp_step) lq4_peer_buf_free(ctx->mlp_step);
     for (cudaEvent_t e : ctx->ev_block)
         if (e) cudaEventDestroy(e);
@@ -1715,7 +1728,7 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* a, vo
     AttendWorkspace ws{ctx->attend.p, ctx->attend.cap, 0, 0};
     LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
     if (ws.need) {
-        if ((st = ensure(ctx, ctx->attend, ws.need, false, s))) return st;
+        if ((st = ensure_kept(ctx, ctx->attend, ws.need, s))) return st;
         ws = {ctx->attend.p, ctx->attend.cap, 0, 0};
         LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
     }
@@ -1746,7 +1759,7 @@ lq4_status lq4_verify_draft(lq4_ctx* ctx, const lq4_verify_args* a, void* stream
     LQ4_ON_DEVICE(ctx);
     cudaStream_t s = (cudaStream_t)stream;
     lq4_status st;
-    if ((st = ensure(ctx, ctx->verify, verify_workspace_bytes(*a, ctx->sm_count), false, s))) return st;
+    if ((st = ensure_kept(ctx, ctx->verify, verify_workspace_bytes(*a, ctx->sm_count), s))) return st;
     int launches = 0;
     LQ4_CUDA(launch_verify_draft(*a, ctx->verify.p, ctx->status, ctx->sm_count, ctx->pdl, s, &launches));
     ctx->launches += launches;

@@ -502,6 +502,29 @@ def test_attention_in_a_captured_graph(be, hq):
     be.check_device_status()
 
 
+def test_attention_graph_after_a_larger_call():
+    """A call with more rows per kv head outgrows the workspace; a graph captured before it keeps its own."""
+    from lattice_b200 import CudaQ4Backend
+    be = CudaQ4Backend(0)
+    cache = make_cache(1, 40, 64, 1, 128, seed=90)
+    lens = torch.tensor([2500], dtype=torch.int32).cuda()
+    make = lambda hq, n: [normal(91 + n, 1, n, h, 128).to(BF16).cuda() for h in (hq, 1, 1)]  # noqa: E731
+    small, large = make(4, 1), make(4, 64)
+    out = torch.empty_like(small[0])
+    eager = be.tree_attention(*small, cache, lens)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        be.tree_attention(*small, cache, lens, out=out)
+    big = be.tree_attention(*large, cache, lens)
+    out.fill_(7.0)
+    g.replay()
+    assert torch.equal(out, eager)
+    assert torch.equal(be.tree_attention(*large, cache, lens), big)
+    be.check_device_status()
+    be.close()
+
+
 def test_attention_python_refusals(be):
     cache = make_cache(2, 2, 16, 2, 64)
     q, k = normal(90, 2, 3, 4, 64).to(BF16).cuda(), normal(91, 2, 3, 2, 64).to(BF16).cuda()
@@ -637,6 +660,42 @@ def test_verify_large_batch_and_full_vocabulary(be):
     check_verify(be, target, draft, tokens, parents, None, u, None)
     target, draft, tokens, parents, u = verify_inputs(5, 2, 6, 248320, F32, True)
     check_verify(be, target, draft, tokens, parents, None, u, torch.tensor([0.9, 0.0]))
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_verify_rows_too_long_for_the_registers(be, dtype, sampled):
+    """80 sequences leave one CTA for each, and its warps' shares of a row are read again instead of being kept."""
+    target, draft, tokens, parents, u = verify_inputs(6, 80, 4, 20011, dtype, sampled)
+    tau = torch.ones(80)
+    tau[::7], tau[1::7] = 0.0, 0.6
+    check_verify(be, target, draft, tokens, parents, None, u, tau)
+
+
+@pytest.mark.parametrize("vocab", [300, 50001])
+def test_verify_in_a_captured_graph(vocab):
+    """A graph replays with other logits, tokens and uniforms, also after a call that needs a larger workspace."""
+    from lattice_b200 import CudaQ4Backend
+    be = CudaQ4Backend(0)
+    shape = (3, 5, vocab, F32, True)
+    states = [verify_inputs(seed, *shape) for seed in (12, 13, 14)]
+    target, draft, tokens, parents, u = (x.cuda() for x in states[0])
+    call = lambda: be.verify_draft(target, tokens, u, draft_logits=draft, parents=parents)  # noqa: E731
+    call()                                                                       # the workspace grows outside the capture
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    check_verify(be, *verify_inputs(15, 9, 7, 60000, F32, True)[:4], None, torch.rand(9, 7, generator=rng(16)), None)
+    for new in states:
+        for x, y in zip((target, draft, tokens, parents, u), new):
+            x.copy_(y)
+        g.replay()
+        torch.cuda.synchronize()
+        eager = check_verify(be, *new[:4], None, new[4], None)
+        for x, y in zip(out, eager):
+            assert x.cpu().numpy().tolist() == y.tolist()
+    be.close()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
