@@ -28,6 +28,10 @@
 // in tensor memory cut off below their last bit at every MMA, some 10^-5 over a few hundred of them, so P V of a tile
 // starts from zero and the softmax threads add it to O in their registers, a tile later; one stream, two buffers of P and
 // of P V.
+//
+// B200, device time: 4 trees of 64 nodes over 16384 tokens, 32 heads on 8 of 128, bf16: 115 us (0.6 PFLOP/s); 8 trees of 13
+// nodes over 2000 to 4000, 40 heads on 8 of 128, f32: 83 us.  Neither HBM nor the tensor cores are busy (23 % and 26 % at
+// half the first one's length): a stream waits for its own scores, exponentials and products in turn.
 #include "lq4_attend_dev.cuh"
 
 namespace lq4 {

@@ -21,8 +21,10 @@
 //
 // A cluster lives in one GPC and gets some 0.8 TB/s: two rows of 248320 f32 logits are 2.5 us and more per node, one node after
 // the other.  Where all rows together are few enough (kEagerBytes), verify_stats_kernel takes (max, sum) of every row over the
-// whole GPU first; the walk then only reads the rows of a node where a draft is refused or the last token is drawn.  What bounds it is the chain of latencies per node (rows, two reductions, a
-// barrier); the first child's rows are fetched into L2 meanwhile.
+// whole GPU first; the walk then only reads the rows of a node where a draft is refused or the last token is drawn.  What
+// bounds it is the chain of latencies per node (rows, two reductions, a barrier); without statistics the first child's rows
+// are fetched into L2 meanwhile.  B200, device time: a chain of 5 over 248320 f32 logits, all accepted, 31 us (10 MB of rows:
+// 1.5 us at HBM rate); 16 trees of 24 over 100003 bf16 logits 55 to 101 us with the data.
 //
 // Decisions lie next to borders.  Masses are f32 (ex2.approx of the rounded distance from the maximum: a few 2^-23, and
 // exactly 1 at the maximum; four or eight at a time are added in f32); all further sums are pairs of f32 (some 48 bits, any size of
@@ -689,9 +691,11 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 
 // (max, sum) and the best candidate of every row that the walk may visit: one CTA per split of a row.
 constexpr uint32_t kStatThreads = 256, kMaxSplits = 32;
-// What this kernel may read: 5 us at HBM rate.  A chain of 5 nodes over 248320 f32 logits (10 MB) takes 31 us with it; before the
-// nodes' rows were joined ahead of the walk it took 52 us.
-constexpr uint64_t kEagerBytes = 32ull << 20;
+// What this kernel may read.  It costs the rows of nodes that the walk never visits and saves a row's pass per visited one.
+// Without and with it, means of six inputs on a B200 (what a walk costs depends on how far it gets): f32, chains of 5 over
+// 248320: 1 sequence (10 MB) 51 and 28 us, 4 (40 MB) 66 and 41, 8 (79 MB) 87 and 71; bf16, trees of 24 over 100003: 1
+// (10 MB) 44 and 31, 8 (77 MB) 89 and 77, 16 (154 MB) 79 and 111.  A walk that ends at the root loses 2 to 7 us by it.
+constexpr uint64_t kEagerBytes = 80ull << 20;
 
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
