@@ -129,6 +129,11 @@ __device__ __forceinline__ WarpSum join_lanes(WarpSum a, int first, float c) {
 }
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }      // NaN carries no mass
 
+// A cluster's start: another CTA's shared memory may be touched once all of them are known to run.  In two halves, so that the
+// way between them hides behind a load.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // Order of candidates: higher logit first, ties to the lower id (0: nothing that ranks).
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) {
     if (v == -INFINITY) return 0;
@@ -246,9 +251,11 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     __shared__ Row row_of[LQ4_MAX_TREE_NODES];                           // with statistics: every node's, known from the start
     __shared__ double ip_of[LQ4_MAX_TREE_NODES];
 
+    cluster_arrive();
     pdl_wait_prior_grids();
     pdl_launch_dependents();
     int32_t n = p.node_counts ? p.node_counts[b] : (int32_t)p.nodes;
+    cluster_wait();                                                      // the other CTAs' slots exist from here on
     if (n > (int32_t)p.nodes) {
         n = (int32_t)p.nodes;
         if (tid == 0 && rank == 0) atomicOr(p.status, kDevErrBadIndex);
