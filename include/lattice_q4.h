@@ -490,8 +490,9 @@ lq4_status lq4_rope_rows(lq4_ctx* ctx, const lq4_rope_args* args, void* stream);
  *   LINEAR  the same over `factor` (positions interpolated)
  *   NTK     theta replaced by theta * factor^(rot_dim / (rot_dim - 2)): the slowest pair as LINEAR, the fastest unchanged
  *   YARN    pairs that turn at least beta_fast times in original_len positions keep their frequency, pairs that
- *           turn at most beta_slow times get it over factor, a linear ramp over the pair index between;
- *           scale = 0.1 ln(factor) + 1 (Peng et al. 2023)
+ *           turn at most beta_slow times get it over factor, a linear ramp over the pair index between (its ends are
+ *           rounded outwards to whole pairs and lie in [0, rot_dim - 1], so behind the last pair where even that one
+ *           turns more than beta_slow times);  scale = 0.1 ln(factor) + 1 (Peng et al. 2023)
  *   BANDS   as YARN, but the ramp runs over the number of turns in original_len, from beta_slow to beta_fast; scale 1
  * LQ4_ERR_ROT for an odd or zero rot_dim (NTK: rot_dim 2 too), theta <= 1 or a factor below 1, or unordered betas. */
 typedef struct {

@@ -1660,7 +1660,7 @@ lq4_status lq4_rope_frequencies(const lq4_rope_scaling* c, double* h_freq, float
     double low = 0, high = 0;
     if (c->kind == LQ4_ROPE_YARN) {
         low = std::fmax(std::floor(pair_of(c->beta_fast)), 0.0);
-        high = std::fmin(std::ceil(pair_of(c->beta_slow)), half - 1.0);
+        high = std::fmin(std::ceil(pair_of(c->beta_slow)), c->rot_dim - 1.0);      // (it may lie behind the last pair)
     }
     *h_scale = c->kind == LQ4_ROPE_YARN ? (float)(0.1 * std::log(c->factor) + 1.0) : 1.0f;
     for (uint32_t i = 0; i < half; ++i) {

@@ -1,0 +1,34 @@
+"""No-GPU checks at the edges of the attention half of a step: ramps of rotary frequencies over long trained contexts."""
+import math
+
+import numpy as np
+import pytest
+
+from lattice_b200 import rope_frequencies
+
+
+def yarn_by_definition(rot, theta, factor, original_len, fast, slow):
+    """Peng et al. 2023: a ramp over the pair index between the pairs that turn `fast` and `slow` times in original_len
+    positions, rounded outwards to whole pairs and kept within the channels of a head."""
+    pair = lambda turns: rot * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+    low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+    out = []
+    for i in range(rot // 2):
+        f = theta ** (-2 * i / rot)
+        share = 1 - min(max((i - low) / (high - low), 0), 1)                  # of the unscaled frequency
+        out.append(f / factor * (1 - share) + f * share)
+    return np.array(out)
+
+
+@pytest.mark.parametrize("rot, theta, original_len, slow", [
+    (128, 1e4, 4096, 1.0), (128, 1e4, 65536, 1.0), (128, 1e4, 131072, 1.0), (64, 1e4, 1 << 20, 1.0), (64, 1e4, 131072, 4.0), (2, 1e4, 131072, 1.0),
+    (96, 500000.0, 1 << 24, 1.0), (128, 10.0, 100.0, 1.0),
+])
+def test_yarn_where_the_slowest_pair_still_turns(rot, theta, original_len, slow):
+    """Beyond about 2 pi theta trained positions the pair that turns `slow` times lies behind the last one: the last pairs
+    are on the ramp, not at its end."""
+    f, _ = rope_frequencies(rot, theta, "yarn", factor=4.0, original_len=original_len, beta_fast=32.0, beta_slow=slow)
+    np.testing.assert_allclose(f, yarn_by_definition(rot, theta, 4.0, original_len, 32.0, slow), rtol=1e-12)
+    plain = np.array([theta ** (-2 * i / rot) for i in range(rot // 2)])
+    turns = plain * original_len / (2 * math.pi)
+    assert np.all(f[turns > slow] > plain[turns > slow] / 4 * (1 + 1e-9))     # what turns more often keeps a share
