@@ -1667,7 +1667,7 @@ lq4_status lq4_rope_frequencies(const lq4_rope_scaling* c, double* h_freq, float
         const double f = std::pow(theta, -(double)i / half);
         double keep = 1.0;                      // share of the unscaled frequency
         if (c->kind == LQ4_ROPE_LINEAR) keep = 0.0;
-        if (c->kind == LQ4_ROPE_YARN) keep = 1.0 - std::fmin(std::fmax((i - low) / std::fmax(high - low, 0.001), 0.0), 1.0);
+        if (c->kind == LQ4_ROPE_YARN) keep = high > 0.0 ? 1.0 - std::fmin(std::fmax((i - low) / std::fmax(high - low, 0.001), 0.0), 1.0) : 0.0;
         if (c->kind == LQ4_ROPE_BANDS) keep = std::fmin(std::fmax((c->original_len * f / (2 * pi) - c->beta_slow) / (c->beta_fast - c->beta_slow), 0.0), 1.0);
         h_freq[i] = c->kind == LQ4_ROPE_PLAIN || c->kind == LQ4_ROPE_NTK ? f : f / c->factor * (1.0 - keep) + f * keep;
     }

@@ -32,3 +32,10 @@ def test_yarn_where_the_slowest_pair_still_turns(rot, theta, original_len, slow)
     plain = np.array([theta ** (-2 * i / rot) for i in range(rot // 2)])
     turns = plain * original_len / (2 * math.pi)
     assert np.all(f[turns > slow] > plain[turns > slow] / 4 * (1 + 1e-9))     # what turns more often keeps a share
+
+
+@pytest.mark.parametrize("original_len", [1.0, 4.0, 6.0])
+def test_yarn_where_no_pair_turns(original_len):
+    """A context so short that even the fastest pair turns less than beta_slow times: all of them are interpolated."""
+    f, _ = rope_frequencies(64, 1e4, "yarn", factor=4.0, original_len=original_len)
+    np.testing.assert_allclose(f, [1e4 ** (-2 * i / 64) / 4 for i in range(32)], rtol=1e-12)
