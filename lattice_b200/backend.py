@@ -606,8 +606,6 @@ class CudaQ4Backend:
         status = self._lib.lq4_kv_append(self._ctx, self._args_at, _raw_stream(self.device))
         if status:
             check(status)
-        if rows == 0:
-            new_lens.copy_(kv_lens)
         return new_lens
 
     def tree_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KvCache, kv_lens: torch.Tensor, *,

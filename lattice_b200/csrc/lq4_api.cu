@@ -1680,18 +1680,21 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* a, void* stream
     if ((st = check_cache(a->cache))) return st;
     if (!act_dtype(a->dtype)) return fail(LQ4_ERR_DTYPE, "rows must be F32 or BF16");
     if (a->rows > 0x7fffffffu || (uint64_t)a->cache->batch * a->rows > 0x7fffffffull * 8) return fail(LQ4_ERR_OVERFLOW, "batch * rows does not fit");
-    if (a->cache->batch && a->rows) {
-        if (!a->k || !a->v || !a->kv_lens) return fail(LQ4_ERR_NULL, "k, v and kv_lens must be non-NULL");
-        if (!aligned(a->k, 16) || !aligned(a->v, 16)) return fail(LQ4_ERR_ALIGN, "k and v must be 16-byte aligned");
-        if (a->batch_stride % 8 || a->row_stride % 8 || a->head_stride % 8) return fail(LQ4_ERR_ALIGN, "row strides must be multiples of 8 elements");
+    if (a->cache->batch && (a->rows || a->new_lens)) {
+        if (!a->kv_lens) return fail(LQ4_ERR_NULL, "kv_lens must be non-NULL");
         if (!aligned(a->kv_lens, 4) || !aligned(a->counts, 4) || !aligned(a->index, 4) || !aligned(a->new_lens, 4))
             return fail(LQ4_ERR_ALIGN, "an int32 array is misaligned");
+    }
+    if (a->cache->batch && a->rows) {
+        if (!a->k || !a->v) return fail(LQ4_ERR_NULL, "k and v must be non-NULL");
+        if (!aligned(a->k, 16) || !aligned(a->v, 16)) return fail(LQ4_ERR_ALIGN, "k and v must be 16-byte aligned");
+        if (a->batch_stride % 8 || a->row_stride % 8 || a->head_stride % 8) return fail(LQ4_ERR_ALIGN, "row strides must be multiples of 8 elements");
         if (a->new_lens && a->new_lens == a->kv_lens) return fail(LQ4_ERR_SHAPE, "new_lens must not be kv_lens: the lengths are read while it is written");
         if (mul_overflows(a->batch_stride, a->cache->batch, 1ull << 60) || mul_overflows(a->row_stride, a->rows, 1ull << 60))
             return fail(LQ4_ERR_OVERFLOW, "row strides do not fit");
     }
     if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
-    if (a->cache->batch == 0 || a->rows == 0) return LQ4_OK;
+    if (a->cache->batch == 0 || (a->rows == 0 && !a->new_lens)) return LQ4_OK;
     LQ4_ON_DEVICE(ctx);
     LQ4_CUDA(launch_kv_append(*a, ctx->status, ctx->pdl, (cudaStream_t)stream));
     ctx->launches += 1;

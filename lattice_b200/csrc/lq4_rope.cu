@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     pdl_launch_dependents();
 }
 
-// One warp per (sequence, row): the page is looked up once, the lanes move K then V in 8-element pieces.
+// One warp per (sequence, row), and per sequence where there are no rows (for the lengths): the page is looked up once, the lanes
+// move K then V in 8-element pieces.
 struct AppendParams {
     CacheView c;
     const void* k;
@@ -227,8 +228,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     const uint64_t item = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    if (item >= (uint64_t)p.batch * p.rows) return;
-    const uint32_t b = (uint32_t)(item / p.rows), j = (uint32_t)(item - (uint64_t)b * p.rows);
+    const uint32_t per = max(p.rows, 1u);
+    if (item >= (uint64_t)p.batch * per) return;
+    const uint32_t b = (uint32_t)(item / per), j = (uint32_t)(item - (uint64_t)b * per);
     const int32_t len = p.kv_lens[b];
     int32_t count = p.counts ? p.counts[b] : (int32_t)p.rows;
     const int64_t capacity = (int64_t)p.c.max_pages * p.c.page_size;
@@ -354,7 +356,7 @@ cudaError_t launch_kv_append(const lq4_kv_append_args& a, int32_t* status, int u
     p.index = a.index;
     p.new_lens = a.new_lens;
     p.status = status;
-    const uint64_t items = (uint64_t)p.batch * p.rows;
+    const uint64_t items = (uint64_t)p.batch * (p.rows ? p.rows : 1);
     return launch(kv_append_kernel, dim3((unsigned)((items + 7) / 8)), 256, 0, use_pdl, s, p);
 }
 

@@ -1,10 +1,12 @@
-"""No-GPU checks at the edges of the attention half of a step: ramps of rotary frequencies over long trained contexts."""
+"""No-GPU checks at the edges of the attention half of a step: frequencies over long trained contexts, refusals."""
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
 
-from lattice_b200 import rope_frequencies
+from lattice_b200 import _lib, rope_frequencies
+from lattice_b200._lib import KvAppendArgs, KvCacheDesc
 
 
 def yarn_by_definition(rot, theta, factor, original_len, fast, slow):
@@ -39,3 +41,32 @@ def test_yarn_where_no_pair_turns(original_len):
     """A context so short that even the fastest pair turns less than beta_slow times: all of them are interpolated."""
     f, _ = rope_frequencies(64, 1e4, "yarn", factor=4.0, original_len=original_len)
     np.testing.assert_allclose(f, [1e4 ** (-2 * i / 64) / 4 for i in range(32)], rtol=1e-12)
+
+
+# ---- arguments -----------------------------------------------------------------------------------------------------
+
+P = 0x10000          # a made-up device address, 16-byte aligned: refused calls never touch it
+
+
+@pytest.fixture(scope="module")
+def L():
+    from lattice_b200 import build as lq4_build
+    lq4_build.build()
+    return _lib.lib()
+
+
+def cache_desc():
+    return KvCacheDesc(k=P, v=P, pages=8, page_size=16, kv_heads=2, head_dim=64, page_table=P, batch=2, max_pages=4)
+
+
+def test_append_of_no_rows_checks_what_it_reads(L):
+    """Without rows k and v are not read, the lengths are where new_lens is asked for."""
+    def call(**change):
+        fields = dict(cache=C.pointer(cache_desc()), k=None, v=None, dtype=1, rows=0, kv_lens=P, new_lens=2 * P)
+        fields.update(change)
+        return L.lq4_kv_append(None, C.byref(KvAppendArgs(**fields)), None), L.lq4_last_error()
+    assert call() == (_lib.ERR_NULL, b"ctx is NULL")
+    assert call(kv_lens=None, new_lens=None) == (_lib.ERR_NULL, b"ctx is NULL")
+    status, text = call(kv_lens=None)
+    assert status == _lib.ERR_NULL and b"kv_lens" in text
+    assert call(new_lens=P + 2)[0] == _lib.ERR_ALIGN

@@ -1,0 +1,56 @@
+"""The attention half of a step at the edges of what its calls allow, on the GPU."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def be():
+    from lattice_b200 import CudaQ4Backend
+    b = CudaQ4Backend(0)
+    yield b
+    b.close()
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+def i32(x):
+    return torch.as_tensor(x, dtype=torch.int32).cuda()
+
+
+def dense_cache(batch, max_pages, page, heads, dim, seed=1):
+    """A cache of known contents whose pages lie in order."""
+    from lattice_b200 import KvCache
+    shape = (batch * max_pages, page, heads, dim)
+    k, v = (normal(seed + i, *shape).to(BF16).cuda() for i in range(2))
+    return KvCache(k, v, torch.arange(batch * max_pages, dtype=torch.int32).view(batch, max_pages).cuda())
+
+
+# ---- cache append --------------------------------------------------------------------------------------------------
+
+def append_by_c(be, cache, rows, kv_lens, new_lens, counts=None):
+    """lq4_kv_append as a C caller makes it, without rows to read."""
+    from lattice_b200 import _lib
+    args = _lib.KvAppendArgs(C.pointer(cache.desc), None, None, _lib.DTYPE_BF16, rows, 0, 0, 0, kv_lens.data_ptr(),
+                             None if counts is None else counts.data_ptr(), None, None if new_lens is None else new_lens.data_ptr())
+    return _lib.lib().lq4_kv_append(be._ctx, C.byref(args), torch.cuda.current_stream().cuda_stream)
+
+
+def test_append_of_no_rows_writes_the_lengths(be):
+    cache = dense_cache(4, 2, 8, 1, 16)
+    lens, new = i32([5, 0, -3, 16]), i32([99, 99, 99, 99])
+    assert append_by_c(be, cache, 0, lens, new) == 0
+    assert new.tolist() == [5, 0, -3, 16]
+    assert append_by_c(be, cache, 0, lens, None) == 0
+    empty = torch.empty(4, 0, 1, 16, dtype=BF16).cuda()
+    assert be.kv_append(cache, empty, empty, lens).tolist() == [5, 0, -3, 16]
+    assert be.kv_append(cache, empty, empty, lens, new_lens=lens).tolist() == [5, 0, -3, 16]
+    be.check_device_status()
