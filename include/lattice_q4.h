@@ -519,8 +519,10 @@ typedef struct {
  * kv_lens[b] + j, for j < counts[b] (counts NULL: all `rows`); f32 rows are rounded to bf16 once.  Slots
  * that are not written keep what they held.  kv_lens[b] < 0 marks a sequence to leave alone.  new_lens[b]
  * (may be NULL; must not be kv_lens unless rows is 0) receives kv_lens[b] + counts[b], or the capacity max_pages *
- * page_size where that is less (the rows beyond it are skipped and reported); rows == 0 writes it too.  With `index` = the path and `counts` = the
- * path length of lq4_verify_draft the call commits what a verification accepted; without, a prompt's rows or
+ * page_size where that is less (the rows beyond it are skipped and reported); rows == 0 writes it too.  Counts outside
+ * 0..rows and lengths above the capacity are reported as well, but nothing is for a sequence to leave alone.  With
+ * `index` = the path and `counts` = the path length of lq4_verify_draft the call commits what a verification
+ * accepted; without, a prompt's rows or
  * the one row of a plain decode step.  The reference's counterpart is copy_kv_cache_batch
  * (forward/shaders/qwen35.metal:2493). */
 typedef struct {

@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     const int32_t len = p.kv_lens[b];
     int32_t count = p.counts ? p.counts[b] : (int32_t)p.rows;
     const int64_t capacity = (int64_t)p.c.max_pages * p.c.page_size;
-    bool bad = false;
-    if (count > (int32_t)p.rows) count = (int32_t)p.rows, bad = true;
-    if (count < 0 || len < 0) count = 0;
+    // what the lengths and counts hold out of range is reported, but for a sequence to leave alone
+    bool bad = len >= 0 && (len > capacity || count < 0 || count > (int32_t)p.rows);
+    count = len < 0 ? 0 : min(max(count, 0), (int32_t)p.rows);
     if (j == 0 && lane == 0 && p.new_lens)
         p.new_lens[b] = len < 0 ? len : (int32_t)min((int64_t)len + count, min(capacity, (int64_t)0x7fffffff));
     if ((int32_t)j < count) {

@@ -54,3 +54,27 @@ def test_append_of_no_rows_writes_the_lengths(be):
     assert be.kv_append(cache, empty, empty, lens).tolist() == [5, 0, -3, 16]
     assert be.kv_append(cache, empty, empty, lens, new_lens=lens).tolist() == [5, 0, -3, 16]
     be.check_device_status()
+
+
+@pytest.mark.parametrize("lens, counts, rows, want", [
+    ([5], [-1], 3, [5]),                     # a negative count
+    ([17], [0], 3, [16]),                    # a length above the capacity, nothing to add
+    ([17], None, 0, [16]),                   # the same without any rows
+    ([5], [1], 0, [5]),                      # a count above the rows there are
+])
+def test_append_reports_every_value_out_of_range(be, lens, counts, rows, want):
+    from lattice_b200 import Lq4Error
+    cache = dense_cache(1, 2, 8, 1, 16)
+    before = cache.k.clone()
+    x = normal(3, 1, rows, 1, 16).to(BF16).cuda()
+    assert be.kv_append(cache, x, x, i32(lens), counts=None if counts is None else i32(counts)).tolist() == want
+    with pytest.raises(Lq4Error):
+        be.check_device_status()
+    assert torch.equal(cache.k, before)
+
+
+def test_append_reports_nothing_of_sequences_to_leave_alone(be):
+    cache = dense_cache(2, 2, 8, 1, 16)
+    x = normal(4, 2, 3, 1, 16).to(BF16).cuda()
+    assert be.kv_append(cache, x, x, i32([-1, 16]), counts=i32([9, 0]), index=i32([[7, 7, 7], [-1, -1, -1]])).tolist() == [-1, 16]
+    be.check_device_status()
