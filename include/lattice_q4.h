@@ -585,7 +585,8 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args,
  * node; when none is, or there are none, the next token is drawn from what is left:
  *   accepted          iff  u q(t) < p'(t), u = uniforms[b, child], p' the current residual (certain: u < p'(t))
  *   next_token[b]     the smallest j with  sum(p'[0..j]) > uniforms[b, 0] * sum(p')
- *   temperature 0     (below 1e-20) accepts the argmax (ties to the lower id) and returns it
+ *   temperature 0     (below 1e-20, and NaN) accepts the argmax (ties to the lower id) and returns it
+ *   temperature +inf  the limit: every logit above -inf has the same mass
  * NaN and -inf logits carry no mass; +inf takes all of it; a row without mass accepts nothing and gives next_token -1.
  * A drafted token outside the vocabulary is never accepted and changes nothing.  If nothing is left of p after
  * the refusals (by rounding), the token comes from p.  Uniforms lie in [0, 1).

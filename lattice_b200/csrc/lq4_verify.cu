@@ -104,7 +104,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// exp((x - m) / tau), c = log2(e) / tau; a row whose maximum is +inf has all its mass on the entries that are.
+// log2(e) / tau.  Above zero for an infinite temperature too: that is the limit in which everything above -inf weighs the same,
+// and 0 * -inf would be NaN.
+__device__ __forceinline__ float per_tau(float tau) { return fmaxf(1.44269504088896340736f / tau, 1.4e-45f); }
+// exp((x - m) / tau), c = per_tau(tau); a row whose maximum is +inf has all its mass on the entries that are.
 __device__ __forceinline__ float mass(float x, float m, float c) {
     if (m == INFINITY) return x == m ? 1.0f : 0.0f;
     return exp2_fast((x - (m == -INFINITY ? 0.0f : m)) * c);
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
     }
     const float tau = p.temperature ? p.temperature[b] : 1.0f;
     const bool greedy = !(tau >= 1e-20f);
-    const float it = greedy ? 1.0f : 1.44269504088896340736f / tau;      // log2(e) / tau
+    const float it = greedy ? 1.0f : per_tau(tau);
     const bool sampled = p.draft != nullptr && !greedy;
     const T* target_rows = static_cast<const T*>(p.target) + b * p.target_batch;
     const T* draft_rows = static_cast<const T*>(p.draft) + b * p.draft_batch;
@@ -719,7 +722,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
     if ((int32_t)node >= n) return;
     const float tau = p.temperature ? p.temperature[b] : 1.0f;
     const bool greedy = !(tau >= 1e-20f);
-    const float it = greedy ? 1.0f : 1.44269504088896340736f / tau;
+    const float it = greedy ? 1.0f : per_tau(tau);
     if (draft) {                                                         // read for the children of a node, if it has any
         bool inner = false;
         for (uint32_t c = node + 1; c < (uint32_t)n && !inner; ++c) inner = (p.parents ? p.parents[(uint64_t)b * p.nodes + c] : (int32_t)c - 1) == (int32_t)node;

@@ -78,3 +78,31 @@ def test_append_reports_nothing_of_sequences_to_leave_alone(be):
     x = normal(4, 2, 3, 1, 16).to(BF16).cuda()
     assert be.kv_append(cache, x, x, i32([-1, 16]), counts=i32([9, 0]), index=i32([[7, 7, 7], [-1, -1, -1]])).tolist() == [-1, 16]
     be.check_device_status()
+
+
+# ---- verification of drafted tokens --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("batch, vocab", [(3, 40), (3, 300), (80, 20011), (3, 70000)])      # (the last: row statistics first)
+def test_verify_at_an_infinite_temperature(be, batch, vocab, sampled, dtype):
+    """All logits above -inf weigh the same: one of n is accepted below 1 / n, and the last token is the one that the uniform
+    points at.  The logits' size no longer counts, and the rows' padding has no mass."""
+    g = torch.Generator().manual_seed(5)
+    target = (30 * torch.randn(batch, 3, vocab, generator=g)).to(dtype)
+    target[:, :, ::4] = -math.inf                                            # a quarter (rounded up) is masked out
+    n = vocab - (vocab + 3) // 4
+    draft = torch.randn(batch, 3, vocab, generator=g).to(dtype) if sampled else None      # all of them: 1 / vocab each
+    tokens = torch.full((batch, 3), 1, dtype=torch.int32)
+    u = torch.full((batch, 3), 0.5)
+    u[:, 0] = (n // 2 + 0.5) / n                                             # in the middle of an entry
+    u[:, 1] = 0.999 if sampled else 0.5 / n                                  # accepted: u / vocab < 1 / n, or u < 1 / n
+    u[::2, 2] = 0.5 if sampled else 1.5 / n
+    tokens[:, 2] = 4                                                         # masked: refused
+    tau = torch.full((batch,), math.inf)
+    path, count, token = be.verify_draft(target.cuda(), tokens.cuda(), u.cuda(), draft_logits=None if draft is None else draft.cuda(), temperature=tau.cuda())
+    assert path.tolist() == [[0, 1, -1]] * batch and count.tolist() == [2] * batch
+    # behind the refusal: max(p - q, 0) is 1/n - 1/vocab on the unmasked ones, and without a draft token 4 had no mass either
+    live = [j for j in range(vocab) if j % 4]
+    assert token.tolist() == [live[n // 2]] * batch
+    be.check_device_status()
