@@ -546,7 +546,9 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* str
  * lq4_kv_append then adds.  Query head h reads kv head h / (q_heads / kv_heads).
  *   q and out   [batch, nodes, q_heads, head_dim] of one type, F32 or BF16
  *   k and v     [batch, nodes, kv_heads, head_dim] bf16
- * A key that a node may not see contributes nothing whatever it holds (NaN and infinities included).  Nodes from
+ * A key that a node may not see contributes nothing whatever it holds (NaN and infinities included).  In a V row that
+ * it sees, an infinity makes that column infinite and a NaN, or two infinities of different signs, make it NaN, however
+ * small the key's weight; with f32 activations a K row with an infinity or a NaN makes NaN of the node's row.  Nodes from
  * node_counts[b] on (NULL: all live) and sequences with kv_lens[b] < 0 or no live node are left as they were in
  * `out`.  Softmax and sums are f32; with f32 activations the products are too (three bf16 terms each).  Pages out
  * of range are not seen; they, a length above the capacity and a parent that does not come before its node (it

@@ -27,7 +27,8 @@
 //
 // A key that a row may not see contributes nothing whatever it holds: its score is replaced by -inf, and a
 // non-finite V entry of a node (0 * inf would reach the rows that do not see it) is cleared in shared memory
-// and added back at the end for the rows that do see it.
+// and added back at the end for the rows that do see it.  A cached one is seen by all rows of its sequence; what a weight of
+// zero makes NaN of it is put right by the join (kMark).
 #include "lq4_attend_dev.cuh"
 
 namespace lq4 {
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
                         else
                             static_cast<float*>(p.out)[at + e] = y[e] * inv;
                     }
+                    if (d == 0 && !(sum > 0.0f)) mark(p, NQ == 1, at);
                 } else {
                     *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(y[0], y[1], y[2], y[3]);
                     if (d == 0) p.part_ml[(uint64_t)slot * BM + r] = make_float2(top, sum);
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
 }
 
 // Joins the partials of the items that a CTA border cut, the CTAs in order: W warps per row, which take every W-th of them and
-// meet in shared memory (one row's partials may come from every CTA of the grid).
+// meet in shared memory (one row's partials may come from every CTA of the grid).  Then looks at every row's result (kMark).
 template <int D, int W>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendParams p, uint32_t BM, int bf16_out) {
     constexpr int V = D / 32;
@@ -390,48 +392,81 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const uint64_t share = cta_share(total, p.grid);
     const uint64_t first = before + ((uint64_t)h * p.row_tiles + rt) * sq.tiles;
     const uint32_t c0 = (uint32_t)(first / share), c1 = (uint32_t)((first + sq.tiles - 1) / share);
-    if (c0 == c1) return;                                                // one CTA had it all and wrote it
-    // the CTA that has the item's first tile keeps it in its slot 1, the others in slot 0
-    float top = -INFINITY;
-    for (uint32_t c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(uint64_t)(2 * c + (c == c0)) * BM + r].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float safe = top == -INFINITY ? 0.0f : top;
-    float acc[V], sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (uint32_t c = c0 + w; c <= c1; c += W) {
-        const uint64_t slot = (uint64_t)(2 * c + (c == c0)) * BM + r;
-        const float2 e = p.part_ml[slot];
-        const float f = exp2_fast(e.x - safe);
-        sum += e.y * f;
-        const float* src = p.part_o + slot * D + lane * V;
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += src[k] * f;
-    }
-    if constexpr (W > 1) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) part[w][lane * V + k] = acc[k];
-        if (lane == 0) part[w][D] = sum;
-        __syncthreads();
+    const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + lane * V;
+    uint32_t nans = 0;                                                   // this lane's columns that hold a NaN
+    auto is_nan = [](uint32_t bits) { return (bits & 0x7fffffffu) > 0x7f800000u; };
+    if (c0 == c1) {                                                      // one CTA had it all and wrote it
         if (w > 0) return;
+        uint32_t got[V];
 #pragma unroll
-        for (int i = 1; i < W; ++i) {
-            sum += part[i][D];
+        for (int k = 0; k < V; ++k) {
+            got[k] = 0;
+            if (lane * V + k < p.head_dim) got[k] = bf16_out ? (uint32_t)static_cast<const uint16_t*>(p.out)[at + k] << 16 : static_cast<const uint32_t*>(p.out)[at + k];
+        }
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += part[i][lane * V + k];
+        for (int k = 0; k < V; ++k) nans |= (uint32_t)is_nan(got[k]) << k;
+        if (__shfl_sync(0xffffffffu, got[0], 0) == kMark) {
+            if (lane > 0) return;
+            if (bf16_out)
+                static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(NAN);
+            else
+                static_cast<float*>(p.out)[at] = NAN;
+            return;
+        }
+    } else {
+        // the CTA that has the item's first tile keeps it in its slot 1, the others in slot 0
+        float top = -INFINITY;
+        for (uint32_t c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.part_ml[(uint64_t)(2 * c + (c == c0)) * BM + r].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float safe = top == -INFINITY ? 0.0f : top;
+        float acc[V], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+        for (uint32_t c = c0 + w; c <= c1; c += W) {
+            const uint64_t slot = (uint64_t)(2 * c + (c == c0)) * BM + r;
+            const float2 e = p.part_ml[slot];
+            const float f = exp2_fast(e.x - safe);
+            sum += e.y * f;
+            const float* src = p.part_o + slot * D + lane * V;
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] += src[k] * f;
+        }
+        if constexpr (W > 1) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) part[w][lane * V + k] = acc[k];
+            if (lane == 0) part[w][D] = sum;
+            __syncthreads();
+            if (w > 0) return;
+#pragma unroll
+            for (int i = 1; i < W; ++i) {
+                sum += part[i][D];
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc[k] += part[i][lane * V + k];
+            }
+        }
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (lane * V + k >= p.head_dim) break;
+            if (bf16_out)
+                static_cast<__nv_bfloat16*>(p.out)[at + k] = __float2bfloat16_rn(acc[k] * inv);
+            else
+                static_cast<float*>(p.out)[at + k] = acc[k] * inv;
+            nans |= (uint32_t)(acc[k] != acc[k] && sum > 0.0f) << k;
         }
     }
-    const float inv = 1.0f / sum;
-    const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + lane * V;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        if (lane * V + k >= p.head_dim) break;
+    for (; nans; nans &= nans - 1) {
+        const uint32_t k = __ffs(nans) - 1;
+        Piece x;
+        x.sq = sq, x.b = b, x.h = h;
+        const float y = nonfinite_total(p, x, t, lane * V + k);
+        if (y == 0.0f) continue;
         if (bf16_out)
-            static_cast<__nv_bfloat16*>(p.out)[at + k] = __float2bfloat16_rn(acc[k] * inv);
+            static_cast<__nv_bfloat16*>(p.out)[at + k] = __float2bfloat16_rn(y);
         else
-            static_cast<float*>(p.out)[at + k] = acc[k] * inv;
+            static_cast<float*>(p.out)[at + k] = y;
     }
 }
 

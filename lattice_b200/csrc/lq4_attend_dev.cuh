@@ -207,6 +207,39 @@ static __device__ __noinline__ float nonfinite_sum(const AttendParams& p, const 
     return sum;
 }
 
+// The infinities of cached V.  A weight that is zero in f32 (or in one of the bf16 terms it is split into) makes NaN of an
+// infinity that the definition keeps.  attend_join_kernel looks at every result once more and writes what the column has in
+// memory where a NaN came out.  A row whose weights are NaN themselves keeps its NaNs: the attention kernels, which write such a
+// row whole, mark its first entry with a -NaN that no arithmetic gives.  (Nothing of this is in the loops over the keys.)
+constexpr uint32_t kMark = 0xffc10000u;
+__device__ __forceinline__ void mark(const AttendParams& p, bool bf16_out, uint64_t at) {
+    if (bf16_out)
+        static_cast<uint16_t*>(p.out)[at] = kMark >> 16;
+    else
+        static_cast<uint32_t*>(p.out)[at] = kMark;
+}
+// What the non-finite entries of column d come to for node t, over all keys that it sees: their sum, or 0 if there are none.
+static __device__ __noinline__ float nonfinite_total(const AttendParams& p, const Piece& x, uint32_t t, uint32_t d) {
+    constexpr uint32_t kAtATime = 8;
+    bool bad = false;
+    float sum = nonfinite_sum(p, x, node_path(p, x.b, t, bad), d);
+    for (uint32_t key = 0; key < (uint32_t)x.sq.len && sum == sum; key += kAtATime) {
+        float y[kAtATime];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtATime; ++i) {
+            const uint32_t k = key + i, entry = k / p.c.page_size;
+            const int32_t page = k < (uint32_t)x.sq.len ? p.c.table[(uint64_t)x.b * p.c.max_pages + entry] : -1;
+            y[i] = 0.0f;
+            if ((uint32_t)page < p.c.pages)
+                y[i] = bf16_to_f32(p.c.v[(uint32_t)page * p.c.page_stride + (k - entry * p.c.page_size) * p.c.slot_stride + x.h * p.c.head_stride + d]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAtATime; ++i)
+            if (!isfinite(y[i])) sum += y[i];
+    }
+    return sum;
+}
+
 // ---- loaders --------------------------------------------------------------------
 // The K and V rows of all tiles of a CTA's range, through cp.async into RINGS rings of RING slots (K and V of a tile in turn;
 // tile n goes to ring n % RINGS), by TEAMS teams of TEAM warps that take the tiles in turn; warp `w` of them.  A lone warp

@@ -505,12 +505,13 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                 if constexpr (kMeets) {
                     named_bar_sync(3, 256);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = o[e] * f + (f_other == 0.0f ? 0.0f : pass[e * 128] * f_other);
+                    for (int e = 0; e < 32; ++e) o[e] = o[e] * f + pass[e * 128] * f_other;      // (0 of a stream without tiles)
                     named_bar_sync(4, 256);
                 }
                 if (live) put(d, o);
             }
             }
+            if (live && whole && (!kMeets || str == 0) && !(l > 0.0f)) mark(p, NQ == 1, to);
             __syncwarp();
             tc_fence_before();
             named_bar_sync(2, kSoftmax);                                 // everybody has read anc, meet and O

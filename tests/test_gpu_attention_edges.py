@@ -80,6 +80,66 @@ def test_append_reports_nothing_of_sequences_to_leave_alone(be):
     be.check_device_status()
 
 
+# ---- attention -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("length", [50, 5000])
+@pytest.mark.parametrize("hq, d", [(2, 64), (10, 64), (32, 64), (2, 128), (9, 128), (80, 128), (3, 256), (12, 256), (3, 192), (12, 192)])
+def test_attention_over_a_cache_with_infinities(be, hq, d, length, dtype):
+    """The weights of a softmax are positive: an infinity in a cached V row makes its column infinite for every row that sees
+    it, two of different signs or a NaN make it NaN, and no other column changes, however light the key is."""
+    b, t = 2, 4
+    light, lens = 37, [length, length // 2]
+    cache = dense_cache(b, -(-length // 16) + 1, 16, 1, d, seed=30)
+    q = normal(31, b, t, hq, d).abs().to(dtype).cuda()
+    k, v = normal(32, b, t, 1, d).to(BF16).cuda(), normal(33, b, t, 1, d).to(BF16).cuda()
+    par = i32([[-1, 0, 0, 1]] * b)
+    rows = lambda x: x.view(b, -1, 1, d)  # noqa: E731
+    rows(cache.k)[:, light] = -30.0                                          # its weight underflows: below e^-100 of the others'
+    clean = be.tree_attention(q, k, v, cache, i32(lens), parents=par).cpu()
+    inf, nan = math.inf, math.nan
+    c = rows(cache.v)
+    c[0, 3, 0, 0], c[0, 11, 0, 1], c[0, 20, 0, 2] = inf, -inf, nan
+    c[0, 5, 0, 3], c[0, 45, 0, 3] = inf, -inf
+    c[0, light, 0, d - 1] = inf
+    c[0, lens[0] - 1, 0, 9], c[0, light, 0, 9] = -inf, -inf
+    c[0, 3, 0, 10] = inf
+    v[0, 2, 0, 10] = -inf                                                    # node 2 sees both
+    c[0, lens[0]:] = nan                                                     # nobody sees these
+    got = be.tree_attention(q, k, v, cache, i32(lens), parents=par).cpu()
+    want = clean.clone()
+    for col, x in ((0, inf), (1, -inf), (2, nan), (3, nan), (d - 1, inf), (9, -inf), (10, inf)):
+        want[0, :, :, col] = x
+    want[0, 2, :, 10] = nan
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+    be.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq, d", [(2, 64), (10, 64), (80, 64), (2, 128), (9, 128), (80, 128), (3, 256), (12, 256), (12, 192)])
+def test_attention_over_many_caches_with_infinities(be, hq, d, dtype):
+    """The same where a CTA has whole sequences, not parts of them; and a row whose weights are NaN stays NaN everywhere."""
+    b, t, length = 500, 2, 100
+    cache = dense_cache(b, 7, 16, 1, d, seed=40)
+    q = normal(41, b, t, hq, d).to(dtype).cuda()
+    k, v = normal(42, b, t, 1, d).to(BF16).cuda(), normal(43, b, t, 1, d).to(BF16).cuda()
+    q[7::50, 1, 0, 5] = math.nan
+    lens = i32([length - i % 3 for i in range(b)])
+    clean = be.tree_attention(q, k, v, cache, lens).cpu()
+    c = cache.v.view(b, -1, 1, d)
+    c[::2, 31, 0, 3], c[::2, 64, 0, 4] = math.inf, -math.inf
+    c[::3, 90, 0, 5], c[::3, 2, 0, 5] = math.inf, -math.inf
+    got = be.tree_attention(q, k, v, cache, lens).cpu()
+    want = clean.clone()
+    want[::2, ..., 3], want[::2, ..., 4], want[::3, ..., 5] = math.inf, -math.inf, math.nan
+    want[7::50, 1, 0] = math.nan
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+    bits = got.view(torch.int16 if dtype == BF16 else torch.int32)
+    assert not bool(((bits < 0) & got.isnan()).any())                        # no mark is left
+
+
 # ---- verification of drafted tokens --------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
