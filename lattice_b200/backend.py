@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+import threading
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Tuple
 
@@ -41,6 +42,14 @@ def _raw_stream(device: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+class _ArgumentBuffer(threading.local):
+    """Where a thread packs the arguments of an attention call (the library reads them after the GIL is released)."""
+
+    def __init__(self):
+        self.buf = C.create_string_buffer(64 * (1 + _lib.MAX_ROPE_PARTS))
+        self.at = C.addressof(self.buf)
 
 
 class Q4WeightBuf:
@@ -161,8 +170,7 @@ class CudaQ4Backend:
         check(_lib.lib().lq4_ctx_create(device, C.byref(h)))
         self._ctx = h.value
         self._lib = _lib.lib()
-        self._args = C.create_string_buffer(64 * (1 + _lib.MAX_ROPE_PARTS))      # arguments of the attention calls
-        self._args_at = C.addressof(self._args)
+        self._args = _ArgumentBuffer()
         self.num_hidden_layers = num_hidden_layers
         # module name -> (d_in, d_out); None disables the model-shape check of load_lora_adapter
         self.projection_shapes = projection_shapes
@@ -511,7 +519,7 @@ class CudaQ4Backend:
 
     # ---- rotary positions and the key/value cache --------------------------------------------
     # One decode step makes these calls once per layer on tiny inputs, so the host side counts: arguments are packed
-    # into a buffer of this backend (the library reads it before a call returns), checks are single comparisons.
+    # into a buffer of the calling thread (the library reads it before a call returns), checks are single comparisons.
     _ROPE_PART = struct.Struct("@PPiiIiQQQQ")
     _ROPE_ARGS = struct.Struct("@PIIIPP")
     _APPEND_ARGS = struct.Struct("@PPPiIQQQPPPP")
@@ -536,7 +544,7 @@ class CudaQ4Backend:
             return []
         if n > _lib.MAX_ROPE_PARTS:
             raise ValueError(f"rope_rows takes at most {_lib.MAX_ROPE_PARTS} tensors, got {n}")
-        dev, buf, at, types = self.device, self._args, self._args_at, self._ACT_DTYPES
+        dev, buf, at, types = self.device, self._args.buf, self._args.at, self._ACT_DTYPES
         rows, _, dim = parts[0][0].shape
         ys = []
         for i, (x, turn) in enumerate(parts):
@@ -600,10 +608,10 @@ class CudaQ4Backend:
         if new_lens is None:
             new_lens = torch.empty_like(kv_lens)
         s0, s1, s2, _ = k.stride()
-        self._APPEND_ARGS.pack_into(self._args, 0, cache.address, k.data_ptr(), v.data_ptr(), self._ACT_DTYPES[k.dtype], rows, s0, s1, s2, lens_at,
+        self._APPEND_ARGS.pack_into(self._args.buf, 0, cache.address, k.data_ptr(), v.data_ptr(), self._ACT_DTYPES[k.dtype], rows, s0, s1, s2, lens_at,
                                     0 if counts is None else self._int32("counts", counts, (b,)),
                                     0 if index is None else self._int32("index", index, (b, rows)), self._int32("new_lens", new_lens, (b,)))
-        status = self._lib.lq4_kv_append(self._ctx, self._args_at, _raw_stream(self.device))
+        status = self._lib.lq4_kv_append(self._ctx, self._args.at, _raw_stream(self.device))
         if status:
             check(status)
         return new_lens
@@ -636,11 +644,11 @@ class CudaQ4Backend:
         if o3 != 1:
             raise ValueError("tree_attention: out must have unit stride along head_dim")
         k0, k1, k2, _ = k.stride()
-        self._TREE_ARGS.pack_into(self._args, 0, q.data_ptr(), out.data_ptr(), self._ACT_DTYPES[q.dtype], k.data_ptr(), v.data_ptr(), cache.address,
+        self._TREE_ARGS.pack_into(self._args.buf, 0, q.data_ptr(), out.data_ptr(), self._ACT_DTYPES[q.dtype], k.data_ptr(), v.data_ptr(), cache.address,
                                   t, heads, q0, q1, q2, o0, o1, o2, k0, k1, k2, self._int32("kv_lens", kv_lens, (b,)),
                                   0 if node_counts is None else self._int32("node_counts", node_counts, (b,)),
                                   0 if parents is None else self._int32("parents", parents, (b, t)), dim ** -0.5 if scale is None else scale)
-        status = self._lib.lq4_tree_attention(self._ctx, self._args_at, _raw_stream(self.device))
+        status = self._lib.lq4_tree_attention(self._ctx, self._args.at, _raw_stream(self.device))
         if status:
             check(status)
         return out
@@ -722,11 +730,11 @@ class CudaQ4Backend:
                 raise ValueError(f"verify_draft: {name} must be a contiguous float32 tensor of shape {list(shape)} on cuda:{dev}")
         path = torch.empty_like(tokens)
         path_len, token = tokens.new_empty((2, b)).unbind()
-        self._VERIFY_ARGS.pack_into(self._args, 0, target_logits.data_ptr(), draft_at, self._ACT_DTYPES[target_logits.dtype], b, t, vocab, s0, s1, d0, d1,
+        self._VERIFY_ARGS.pack_into(self._args.buf, 0, target_logits.data_ptr(), draft_at, self._ACT_DTYPES[target_logits.dtype], b, t, vocab, s0, s1, d0, d1,
                                     self._int32("tokens", tokens, (b, t)), 0 if parents is None else self._int32("parents", parents, (b, t)),
                                     0 if node_counts is None else self._int32("node_counts", node_counts, (b,)), f32[0], f32[1], path.data_ptr(),
                                     path_len.data_ptr(), token.data_ptr())
-        status = self._lib.lq4_verify_draft(self._ctx, self._args_at, _raw_stream(dev))
+        status = self._lib.lq4_verify_draft(self._ctx, self._args.at, _raw_stream(dev))
         if status:
             check(status)
         return path, path_len, token

@@ -70,3 +70,15 @@ def test_append_of_no_rows_checks_what_it_reads(L):
     status, text = call(kv_lens=None)
     assert status == _lib.ERR_NULL and b"kv_lens" in text
     assert call(new_lens=P + 2)[0] == _lib.ERR_ALIGN
+
+
+def test_every_thread_packs_its_own_arguments():
+    """The library reads packed arguments while another thread may run, and pack its own."""
+    from concurrent.futures import ThreadPoolExecutor
+    from lattice_b200.backend import _ArgumentBuffer
+    args = _ArgumentBuffer()
+    args.buf[0:4] = b"here"
+    with ThreadPoolExecutor(1) as pool:
+        there = pool.submit(lambda: (args.at, args.buf[0:4])).result()
+    assert there[0] != args.at and there[1] == bytes(4)
+    assert args.buf[0:4] == b"here" and args.at == C.addressof(args.buf)
