@@ -440,8 +440,13 @@ lq4_status lq4_rot_signs_from_seed(uint64_t seed, uint32_t dim, float* signs, vo
 
 /* What lies between the q/k/v projections and o_proj of a decode or prefill step.  The calls below take a
  * context like the projections do, run on the context's device whichever one is current, and are
- * asynchronous on `stream` (a stream of that device).  None of them synchronises; where a workspace has to
- * grow the call that grows it does, as lq4_ctx_reserve describes.  Values that the host cannot see (page
+ * asynchronous on `stream` (a stream of that device).  None of them synchronises.  They may be made on several
+ * streams and from several threads at once, and captured into several CUDA graphs: the workspaces of
+ * lq4_tree_attention and lq4_verify_draft belong to one stream or to one graph at a time (further streams than
+ * the first share four of them, in turn).  A workspace that is too small is allocated anew, in a
+ * capture too, and what it replaces lives as long as the context, so that earlier graphs still replay.  With
+ * LQ4_OPT_ALLOW_GROW 0 all streams and graphs take the first stream's workspace as it is, so that their calls have to be
+ * ordered; where it is too small lq4_tree_attention returns LQ4_ERR_NOSPACE.  Values that the host cannot see (page
  * ids, lengths, parents, path entries) are checked by the kernels: what is out of range is skipped, and
  * lq4_ctx_check reports it as LQ4_ERR_DEVICE with bit 8 of the status set. */
 
@@ -554,8 +559,7 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* str
  * of range are not seen; they, a length above the capacity and a parent that does not come before its node (it
  * counts as a root) are reported through lq4_ctx_check.  Results depend on the lengths and the device only, not
  * on timing.  The workspace (at most 40 MB, independent of the lengths) grows on the first call with a larger
- * row count per kv head: make one plain call before capturing one into a CUDA graph.  An outgrown workspace is kept until
- * the context is destroyed, so earlier graphs still replay.
+ * row count per kv head.
  * Stands between lq4_kv_append and the o_proj call, where the reference encodes decode_attention
  * (forward/shaders/qwen35.metal:466-663). */
 #define LQ4_MAX_TREE_NODES 64
@@ -595,9 +599,8 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args,
  *   path[b, 0 .. path_len[b])   the accepted nodes from node 0 on (rising), -1 behind them: `index` and `counts`
  *                               of lq4_kv_append
  * Sequences with node_counts[b] <= 0 get path_len 0 and next_token -1.  Exponentials are f32, sums over
- * the vocabulary pairs of f32, comparisons f64.  One launch, or two and a small
- * workspace where all rows together are few (make one plain call before capturing it; kept like
- * lq4_tree_attention's when it is outgrown).  Stands behind the
+ * the vocabulary pairs of f32, comparisons f64.  One launch, or two and a small workspace (64 KB; one launch where it
+ * cannot be had) where all rows together are few.  Stands behind the
  * lm_head projection over all nodes' rows, where a plain step calls lq4_logits_topk. */
 typedef struct {
     const void* target_logits;        /* [batch, nodes, vocab], F32 or BF16 */

@@ -17,6 +17,7 @@
 #include "lq4_attend.cuh"
 #include "lq4_gemm.cuh"
 #include "lq4_kernels.cuh"
+#include "lq4_scratch.h"
 #include "lq4_step.cuh"
 #include "lq4_decode_common.cuh"
 
@@ -53,14 +54,12 @@ void set_last_error(const char* msg) { g_last_error = msg ? msg : ""; }
 struct lq4_ctx {
     int device = 0;
     int sm_count = 0;
-    uint64_t launches = 0;
+    std::atomic<uint64_t> launches{0};
     int32_t* status = nullptr;    // device status word
     uint32_t* tsync = nullptr;    // 64-bit launch counter of the decode kernels
     Buf xrot, xs, t, tmsg, partials, hx, hy, gemm, logits, topk, topk_ctr, mlp, mlp_h;   // xs: activation limb records of the dense decode kernel
     lq4_peer_buf* mlp_step = nullptr;   // step buffer of lq4_mlp_block's one-launch form (gate||up row + mailbox)
-    Buf verify;                   // lq4_verify_draft: row statistics of small calls
-    Buf attend;                   // lq4_tree_attention: partials of the items that are cut between CTAs
-    std::vector<void*> outgrown;  // earlier allocations of these two
+    ScratchPool scratch;          // partials of lq4_tree_attention's items, row statistics of lq4_verify_draft
     Buf shard_send, shard_recv;   // staging of lq4_linear_sharded: local slices, NCCL's rank-major blocks
     cudaStream_t comm_stream = nullptr;      // second stream of lq4_linear_sharded (created on first use)
     cudaEvent_t ev_block[4] = {nullptr, nullptr, nullptr, nullptr}, ev_comm = nullptr;
@@ -100,17 +99,6 @@ lq4_status ensure(lq4_ctx* ctx, Buf& b, size_t bytes, bool zero, cudaStream_t s)
     if (zero) LQ4_CUDA(cudaMemsetAsync(b.p, 0, cap, s));      // on the caller's stream: ordered before the first launch that reads it
     b.cap = cap;
     ++ctx->alloc_gen;
-    return LQ4_OK;
-}
-
-// The same for a workspace that captured graphs hold the address of: the outgrown allocation lives as long as the
-// context, so that a graph captured before a larger call still replays.
-lq4_status ensure_kept(lq4_ctx* ctx, Buf& b, size_t bytes, cudaStream_t s) {
-    if (bytes <= b.cap) return LQ4_OK;
-    Buf next;
-    if (lq4_status st = ensure(ctx, next, bytes, false, s)) return st;
-    if (b.p) ctx->outgrown.push_back(b.p);
-    b = next;
     return LQ4_OK;
 }
 
@@ -363,9 +351,9 @@ void lq4_ctx_destroy(lq4_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaDeviceSynchronize();
     free_step_plan(ctx->step_plan);
-    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv, &ctx->attend, &ctx->verify})
+    for (Buf* b : {&ctx->xrot, &ctx->xs, &ctx->t, &ctx->tmsg, &ctx->partials, &ctx->hx, &ctx->hy, &ctx->gemm, &ctx->logits, &ctx->topk, &ctx->topk_ctr, &ctx->mlp, &ctx->mlp_h, &ctx->shard_send, &ctx->shard_recv})
         if (b->p) cudaFree(b->p);
-    for (void* p : ctx->outgrown) cudaFree(p);
+    ctx->scratch.free_all();
     if (ctx->mlp_step) lq4_peer_buf_free(ctx->mlp_step);
     for (cudaEvent_t e : ctx->ev_block)
         if (e) cudaEventDestroy(e);
@@ -416,7 +404,7 @@ lq4_status lq4_ctx_check(lq4_ctx* ctx, void* stream) {
     return LQ4_OK;
 }
 
-uint64_t lq4_ctx_launch_count(const lq4_ctx* ctx) { return ctx ? ctx->launches : 0; }
+uint64_t lq4_ctx_launch_count(const lq4_ctx* ctx) { return ctx ? ctx->launches.load() : 0; }
 
 lq4_status lq4_ctx_set_option(lq4_ctx* ctx, int32_t option, int32_t value) {
     if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
@@ -1728,13 +1716,18 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* a, vo
     if (c.batch == 0 || a->nodes == 0) return LQ4_OK;
     LQ4_ON_DEVICE(ctx);
     cudaStream_t s = (cudaStream_t)stream;
-    AttendWorkspace ws{ctx->attend.p, ctx->attend.cap, 0, 0};
+    std::lock_guard<std::mutex> lock(ctx->scratch.mu);
+    Scratch* w = nullptr;
+    LQ4_CUDA(ctx->scratch.pick(s, ctx->allow_grow, &w));
+    AttendWorkspace ws{w->p[kScratchAttend], w->cap[kScratchAttend], 0, 0};
     LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
     if (ws.need) {
-        if ((st = ensure_kept(ctx, ctx->attend, ws.need, s))) return st;
-        ws = {ctx->attend.p, ctx->attend.cap, 0, 0};
+        if (!ctx->allow_grow) return fail(LQ4_ERR_NOSPACE, "workspace too small and growth is disabled");
+        LQ4_CUDA(ctx->scratch.grow(*w, kScratchAttend, ws.need));
+        ws = {w->p[kScratchAttend], w->cap[kScratchAttend], 0, 0};
         LQ4_CUDA(launch_tree_attention(*a, ws, ctx->status, ctx->sm_count, ctx->pdl, s));
     }
+    LQ4_CUDA(ctx->scratch.done(*w, s));
     ctx->launches += ws.launches;
     return LQ4_OK;
 }
@@ -1761,10 +1754,17 @@ lq4_status lq4_verify_draft(lq4_ctx* ctx, const lq4_verify_args* a, void* stream
     if (a->batch == 0) return LQ4_OK;
     LQ4_ON_DEVICE(ctx);
     cudaStream_t s = (cudaStream_t)stream;
-    lq4_status st;
-    if ((st = ensure_kept(ctx, ctx->verify, verify_workspace_bytes(*a, ctx->sm_count), s))) return st;
+    std::lock_guard<std::mutex> lock(ctx->scratch.mu);
+    Scratch* w = nullptr;
+    void* stats = nullptr;                     // without room for statistics the walk takes its own
+    if (const size_t need = verify_workspace_bytes(*a, ctx->sm_count)) {
+        LQ4_CUDA(ctx->scratch.pick(s, ctx->allow_grow, &w));
+        if (need <= w->cap[kScratchVerify] || (ctx->allow_grow && ctx->scratch.grow(*w, kScratchVerify, need > 65536 ? need : 65536) == cudaSuccess))
+            stats = w->p[kScratchVerify];
+    }
     int launches = 0;
-    LQ4_CUDA(launch_verify_draft(*a, ctx->verify.p, ctx->status, ctx->sm_count, ctx->pdl, s, &launches));
+    LQ4_CUDA(launch_verify_draft(*a, stats, ctx->status, ctx->sm_count, ctx->pdl, s, &launches));
+    if (stats) LQ4_CUDA(ctx->scratch.done(*w, s));
     ctx->launches += launches;
     return LQ4_OK;
 }

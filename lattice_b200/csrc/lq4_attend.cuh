@@ -47,7 +47,7 @@ cudaError_t launch_tree_attention(const lq4_tree_attention_args& a, AttendWorksp
                                   int use_pdl, cudaStream_t s);
 
 // ---- lq4_verify.cu --------------------------------------------------------------
-// The row statistics of a small call (0 bytes: it takes none).
+// The row statistics of a small call (0 bytes: it takes none); `workspace` may be NULL where there is no room for them.
 size_t verify_workspace_bytes(const lq4_verify_args& a, int sm_count);
 cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32_t* status, int sm_count, int use_pdl, cudaStream_t s, int* launches);
 

@@ -849,7 +849,7 @@ cudaError_t run(VerifyParams p, int sm_count, int use_pdl, cudaStream_t s, int* 
 }  // namespace
 
 size_t verify_workspace_bytes(const lq4_verify_args& a, int sm_count) {
-    return (size_t)a.batch * a.nodes * 2 * stat_splits(a, sm_count) * sizeof(Stat);
+    return (size_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1) * stat_splits(a, sm_count) * sizeof(Stat);      // (30 KB at most)
 }
 
 cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32_t* status, int sm_count, int use_pdl, cudaStream_t s, int* launches) {
@@ -871,7 +871,7 @@ cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32
     p.status = status;
     p.batch = a.batch;
     p.splits = stat_splits(a, sm_count);
-    p.stats = p.splits ? static_cast<Stat*>(workspace) : nullptr;
+    p.stats = static_cast<Stat*>(workspace);
     return a.dtype == LQ4_DTYPE_F32 ? run<float>(p, sm_count, use_pdl, s, launches) : run<uint16_t>(p, sm_count, use_pdl, s, launches);
 }
 

@@ -166,3 +166,171 @@ def test_verify_at_an_infinite_temperature(be, batch, vocab, sampled, dtype):
     live = [j for j in range(vocab) if j % 4]
     assert token.tolist() == [live[n // 2]] * batch
     be.check_device_status()
+
+
+# ---- streams, threads and graphs -----------------------------------------------------------------------------------
+
+def attention_job(seed, nodes, hq, dtype=BF16, batch=2, length=3000):
+    """A call that needs partials of its own, and what it gives when nothing else runs."""
+    cache = dense_cache(batch, -(-length // 32) + 1, 32, 2, 128, seed=seed)
+    q = normal(seed + 5, batch, nodes, hq, 128).to(dtype).cuda()
+    k, v = normal(seed + 6, batch, nodes, 2, 128).to(BF16).cuda(), normal(seed + 7, batch, nodes, 2, 128).to(BF16).cuda()
+    lens = i32([length - 7 * i for i in range(batch)])
+    return lambda be, out=None: be.tree_attention(q, k, v, cache, lens, out=out)
+
+
+def verify_job(seed, vocab=70000):
+    """A chain whose row statistics come first."""
+    g = torch.Generator().manual_seed(seed)
+    target = (2 * torch.randn(2, 5, vocab, generator=g)).cuda()
+    draft = target + 0.3 * torch.randn(2, 5, vocab, generator=g).cuda()
+    tokens, u = draft.argmax(-1).roll(1, 1).to(torch.int32), torch.rand(2, 5, generator=g).cuda()
+    return lambda be: torch.cat([x.flatten() for x in be.verify_draft(target, tokens, u, draft_logits=draft)])
+
+
+JOBS = [lambda s=s, shape=shape: attention_job(10 * s, *shape) for s, shape in enumerate([(1, 8), (16, 8), (5, 6, F32), (64, 8), (1, 24, F32)])] + \
+       [lambda s=s: verify_job(100 + s) for s in range(3)]
+
+
+@pytest.mark.parametrize("n_streams", [2, 8])
+def test_one_backend_on_several_streams(n_streams):
+    """Calls that run side by side do not disturb one another's workspaces, however many streams there are."""
+    from lattice_b200 import CudaQ4Backend
+    be = CudaQ4Backend(0)
+    jobs = [make() for make in JOBS][:n_streams] if n_streams > 2 else [JOBS[0](), JOBS[1]()]
+    want = [job(be).clone() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for turn in range(30):
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[(i + turn // 10) % len(streams)]):
+                got[i].append(job(be))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+    be.check_device_status()
+    be.close()
+
+
+def test_one_backend_on_several_threads():
+    """Each thread has its own stream and its own packed arguments."""
+    import threading
+    from lattice_b200 import CudaQ4Backend
+    be = CudaQ4Backend(0)
+    jobs = [make() for make in JOBS]
+    want = [job(be).clone() for job in jobs]
+    torch.cuda.synchronize()
+    wrong, failed = [], []
+
+    def work(job, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                outs = [job(be) for _ in range(60)]
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(o for o in outs if not torch.equal(o, w))
+        except Exception as e:                                               # (an exception in a thread does not end the test)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and not wrong
+    be.check_device_status()
+    be.close()
+
+
+def test_two_graphs_of_one_backend_side_by_side():
+    """Graphs captured from one backend, without a plain call before, replay on two streams at once beside eager calls."""
+    from lattice_b200 import CudaQ4Backend
+    be, other = CudaQ4Backend(0), CudaQ4Backend(0)
+    jobs = [make() for make in JOBS]
+    want = [job(other).clone() for job in jobs]
+    graphs, outs = [], []
+    for job in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([job(be), job(be)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = [job(be) for job in jobs]
+    torch.cuda.synchronize()
+    for w, pair, e in zip(want, outs, eager):
+        assert torch.equal(w, pair[0]) and torch.equal(w, pair[1]) and torch.equal(w, e)
+    be.check_device_status()
+    be.close()
+    other.close()
+
+
+def test_a_graph_that_grows_inside_its_capture():
+    """A wider call later in a capture takes a larger workspace; the calls before it keep theirs."""
+    from lattice_b200 import CudaQ4Backend
+    be, other = CudaQ4Backend(0), CudaQ4Backend(0)
+    small, large = JOBS[0](), JOBS[3]()
+    want = small(other).clone(), large(other).clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [small(be), large(be), small(be)]
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(outs[2], want[0])
+    be.close()
+    other.close()
+
+
+def test_workspaces_of_dropped_graphs_are_taken_over():
+    import gc
+    from lattice_b200 import CudaQ4Backend
+    be = CudaQ4Backend(0)
+    job = JOBS[3]()
+    want = job(be).clone()
+    room = []
+    for _ in range(24):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = job(be)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del g, out
+        gc.collect()
+        room.append(torch.cuda.mem_get_info()[0])
+    assert room[3] - room[-1] < 64 << 20                                     # (a workspace of this call takes 39 MB)
+    be.close()
+
+
+def test_no_growth():
+    """Without growth: attention takes what the first stream has or refuses, verification does without statistics."""
+    from lattice_b200 import CudaQ4Backend, Lq4Error, _lib
+    be = CudaQ4Backend(0)
+    small, large, verify = JOBS[0](), JOBS[3](), JOBS[5]()
+    with_stats = verify(CudaQ4Backend(0))
+    want = small(be).clone()
+    be.set_option(_lib.OPT_ALLOW_GROW, 0)
+    with pytest.raises(Lq4Error, match="growth"):
+        large(be)
+    before = be.launch_count
+    assert torch.equal(verify(be), with_stats) and be.launch_count == before + 1
+    assert torch.equal(small(be), want)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        assert torch.equal(small(be), want)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = small(be)
+    g.replay()
+    assert torch.equal(out, want)
+    fresh = CudaQ4Backend(0)
+    fresh.set_option(_lib.OPT_ALLOW_GROW, 0)
+    with pytest.raises(Lq4Error, match="growth"):
+        small(fresh)
+    be.close()
+    fresh.close()
