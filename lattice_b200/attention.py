@@ -65,6 +65,8 @@ class KvCache:
             raise TypeError(f"the cache holds bfloat16, got {k.dtype} and {v.dtype}")
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v must be [pages, page_size, kv_heads, head_dim] with equal strides, the innermost 1")
+        if any(n > 1 and s == 0 for n, s in zip(k.shape, k.stride())):      # (0 means dense to the library)
+            raise ValueError("k and v must not be expanded tensors")
         if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
             raise TypeError("page_table must be a contiguous [batch, max_pages] int32 tensor")
         self.device = k.get_device()
@@ -72,7 +74,7 @@ class KvCache:
             raise ValueError("k, v and page_table must lie on one CUDA device")
         self.k, self.v, self.page_table = k, v, page_table
         pages, size, heads, dim = k.shape
-        s0, s1, s2, _ = k.stride()
+        s0, s1, s2 = (s if n > 1 else 0 for n, s in zip(k.shape[:3], k.stride()))      # (of one entry it may be anything)
         batch, max_pages = page_table.shape
         self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, s0, s1, s2, page_table.data_ptr(), batch, max_pages)
         self.address = C.addressof(self.desc)

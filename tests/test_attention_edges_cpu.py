@@ -4,8 +4,9 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
-from lattice_b200 import _lib, rope_frequencies
+from lattice_b200 import KvCache, _lib, rope_frequencies
 from lattice_b200._lib import KvAppendArgs, KvCacheDesc
 
 
@@ -82,3 +83,22 @@ def test_every_thread_packs_its_own_arguments():
         there = pool.submit(lambda: (args.at, args.buf[0:4])).result()
     assert there[0] != args.at and there[1] == bytes(4)
     assert args.buf[0:4] == b"here" and args.at == C.addressof(args.buf)
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_a_cache_of_expanded_tensors_is_refused(dim):
+    """A stride of 0 means dense to the library, which would then read and write behind an expanded tensor."""
+    shape, small = [4, 8, 2, 16], [4, 8, 2, 16]
+    small[dim] = 1
+    k = torch.zeros(small, dtype=torch.bfloat16).expand(shape)
+    with pytest.raises(ValueError, match="expanded"):
+        KvCache(k, k.clone().as_strided(shape, k.stride()), torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_strides_of_single_entries_do_not_count(monkeypatch):
+    """The stride of a dimension of one entry may be anything."""
+    x = torch.zeros(1000, dtype=torch.bfloat16).as_strided((1, 4, 1, 16), (3, 16, 5, 1))
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)          # as if they lay on a GPU; nothing is launched
+    cache = KvCache(x, x, table)
+    assert (cache.desc.page_stride, cache.desc.slot_stride, cache.desc.head_stride) == (0, 16, 0)
