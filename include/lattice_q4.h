@@ -577,7 +577,7 @@ typedef struct {
     const int32_t* kv_lens;           /* [batch] */
     const int32_t* node_counts;       /* [batch] or NULL */
     const int32_t* parents;           /* [batch, nodes] or NULL */
-    float scale;                      /* finite; 1 / sqrt(head_dim) as a rule */
+    float scale;                      /* finite, times log2(e) too; 1 / sqrt(head_dim) as a rule */
 } lq4_tree_attention_args;
 lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args, void* stream);
 

@@ -1698,7 +1698,7 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* a, vo
     if (a->nodes > LQ4_MAX_TREE_NODES) return fail(LQ4_ERR_SHAPE, "at most 64 nodes");
     if (a->q_heads == 0 || a->q_heads % c.kv_heads) return fail(LQ4_ERR_SHAPE, "q_heads must be a multiple of kv_heads");
     if (a->q_heads / c.kv_heads > 1024) return fail(LQ4_ERR_SHAPE, "more than 1024 query heads per kv head");
-    if (!std::isfinite(a->scale)) return fail(LQ4_ERR_SHAPE, "scale must be finite");
+    if (!std::isfinite(a->scale * 1.44269504088896340736f)) return fail(LQ4_ERR_SHAPE, "scale (times log2 e) must be finite");
     if ((uint64_t)c.batch * a->q_heads * a->nodes > 0x7fffffffull) return fail(LQ4_ERR_OVERFLOW, "batch * nodes * q_heads does not fit");
     if (c.batch && a->nodes) {
         if (!a->q || !a->out || !a->k || !a->v || !a->kv_lens) return fail(LQ4_ERR_NULL, "q, out, k, v and kv_lens must be non-NULL");

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from lattice_b200 import KvCache, _lib, rope_frequencies
-from lattice_b200._lib import KvAppendArgs, KvCacheDesc
+from lattice_b200._lib import KvAppendArgs, KvCacheDesc, TreeAttentionArgs
 
 
 def yarn_by_definition(rot, theta, factor, original_len, fast, slow):
@@ -102,3 +102,11 @@ def test_strides_of_single_entries_do_not_count(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)          # as if they lay on a GPU; nothing is launched
     cache = KvCache(x, x, table)
     assert (cache.desc.page_stride, cache.desc.slot_stride, cache.desc.head_stride) == (0, 16, 0)
+
+
+@pytest.mark.parametrize("scale, ok", [(3e38, False), (-3e38, False), (2.3e38, True), (-2.3e38, True), (0.0, True)])
+def test_attention_refuses_scales_that_overflow(L, scale, ok):
+    """The kernels work in units of log2: scale times log2(e) has to be finite as well."""
+    a = TreeAttentionArgs(q=P, out=2 * P, dtype=1, k=P, v=P, nodes=3, q_heads=4, q_batch=768, q_node=256, q_head=64, out_batch=768, out_node=256,
+                          out_head=64, kv_batch=384, kv_node=128, kv_head=64, kv_lens=P, scale=scale, cache=C.pointer(cache_desc()))
+    assert L.lq4_tree_attention(None, C.byref(a), None) == (_lib.ERR_NULL if ok else _lib.ERR_SHAPE)      # (in order: only the context is missing)
