@@ -47,7 +47,7 @@ enum {
     LQ4_ERR_BAD_BLOCK = 8,     /* a block's scale is not finite-positive or its bias not finite */
     LQ4_ERR_CUDA = 9,          /* a CUDA runtime call failed; see lq4_last_error() */
     LQ4_ERR_UNSUPPORTED = 10,  /* shape outside what this build handles */
-    LQ4_ERR_DEVICE = 11,       /* a kernel reported a failed bounded wait */
+    LQ4_ERR_DEVICE = 11,       /* a kernel reported a failed bounded wait or an index out of range */
     LQ4_ERR_FORMAT = 12,       /* malformed .q4 image */
     LQ4_ERR_IO = 13,
     LQ4_ERR_SHAPE = 14,        /* shape / length mismatch */
@@ -135,8 +135,8 @@ lq4_status lq4_ctx_create(int32_t device, lq4_ctx** out);
 void lq4_ctx_destroy(lq4_ctx* ctx);
 /* Grows the workspace so that a later lq4_linear of this shape allocates nothing. */
 lq4_status lq4_ctx_reserve(lq4_ctx* ctx, uint32_t m, uint32_t n, uint32_t k, uint32_t rank);
-/* Synchronises `stream` and returns LQ4_ERR_DEVICE if any kernel launched through
- * this context gave up on a bounded wait since the last call; clears the flag. */
+/* Synchronises `stream` (of the context's device) and returns LQ4_ERR_DEVICE if any kernel launched through
+ * this context gave up on a bounded wait, or skipped an index out of range, since the last call; clears the flag. */
 lq4_status lq4_ctx_check(lq4_ctx* ctx, void* stream);
 /* Per-context switches.  LQ4_OPT_MLP_ONE_LAUNCH (default 1): lq4_mlp_block runs a one-token block whose
  * gate||up row lives in the library's workspace as ONE lq4_decode_step launch instead of two launches (measured

@@ -194,8 +194,9 @@ class CudaQ4Backend:
         return int(_lib.lib().lq4_ctx_launch_count(self._ctx))
 
     def check_device_status(self) -> None:
-        """Synchronises the current stream and raises if a kernel gave up on a bounded wait."""
-        check(_lib.lib().lq4_ctx_check(self._ctx, _stream()))
+        """Synchronises the current stream of this backend's device and raises if a kernel gave up on a bounded wait
+        or skipped an index out of range."""
+        check(_lib.lib().lq4_ctx_check(self._ctx, _raw_stream(self.device)))
 
     def set_option(self, option: int, value: int) -> None:
         """Per-context switches of the library (``_lib.OPT_*``)."""

@@ -102,6 +102,26 @@ lq4_status ensure(lq4_ctx* ctx, Buf& b, size_t bytes, bool zero, cudaStream_t s)
     return LQ4_OK;
 }
 
+// Makes the context's device current for one call and puts the caller's back.
+struct DeviceScope {
+    int prev = -1;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceScope(int device) {
+        int cur = 0;
+        err = cudaGetDevice(&cur);
+        if (err == cudaSuccess && cur != device) {
+            err = cudaSetDevice(device);
+            if (err == cudaSuccess) prev = cur;
+        }
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+#define LQ4_ON_DEVICE(ctx)             \
+    DeviceScope on_device((ctx)->device); \
+    if (on_device.err != cudaSuccess) return cuda_fail(on_device.err, "selecting the context's device")
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline bool is_pow2(uint64_t v) { return v && !(v & (v - 1)); }
 
@@ -390,6 +410,7 @@ lq4_status lq4_ctx_reserve(lq4_ctx* ctx, uint32_t m, uint32_t n, uint32_t k, uin
 
 lq4_status lq4_ctx_check(lq4_ctx* ctx, void* stream) {
     if (!ctx) return fail(LQ4_ERR_NULL, "ctx is NULL");
+    LQ4_ON_DEVICE(ctx);
     cudaStream_t s = (cudaStream_t)stream;
     int32_t h = 0;
     LQ4_CUDA(cudaMemcpyAsync(&h, ctx->status, 4, cudaMemcpyDeviceToHost, s));
@@ -1547,26 +1568,6 @@ lq4_status lq4_rot_signs_from_seed(uint64_t seed, uint32_t dim, float* signs, vo
 // ---- rotary positions, cache append -----------------------------------------------------------------
 
 namespace {
-
-// Makes the context's device current for one call and puts the caller's back.
-struct DeviceScope {
-    int prev = -1;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceScope(int device) {
-        int cur = 0;
-        err = cudaGetDevice(&cur);
-        if (err == cudaSuccess && cur != device) {
-            err = cudaSetDevice(device);
-            if (err == cudaSuccess) prev = cur;
-        }
-    }
-    ~DeviceScope() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
-#define LQ4_ON_DEVICE(ctx)             \
-    DeviceScope on_device((ctx)->device); \
-    if (on_device.err != cudaSuccess) return cuda_fail(on_device.err, "selecting the context's device")
 
 bool act_dtype(int32_t t) { return t == LQ4_DTYPE_F32 || t == LQ4_DTYPE_BF16; }
 size_t act_size(int32_t t) { return t == LQ4_DTYPE_F32 ? 4 : 2; }

@@ -110,3 +110,18 @@ def test_attention_refuses_scales_that_overflow(L, scale, ok):
     a = TreeAttentionArgs(q=P, out=2 * P, dtype=1, k=P, v=P, nodes=3, q_heads=4, q_batch=768, q_node=256, q_head=64, out_batch=768, out_node=256,
                           out_head=64, kv_batch=384, kv_node=128, kv_head=64, kv_lens=P, scale=scale, cache=C.pointer(cache_desc()))
     assert L.lq4_tree_attention(None, C.byref(a), None) == (_lib.ERR_NULL if ok else _lib.ERR_SHAPE)      # (in order: only the context is missing)
+
+
+def test_the_status_is_read_on_the_backends_device(monkeypatch):
+    """Whichever device is current: the calls ran on the current stream of the backend's."""
+    from types import SimpleNamespace
+    from lattice_b200 import backend
+    seen = []
+    monkeypatch.setattr(backend, "_raw_stream", lambda device: 1000 + device)
+    monkeypatch.setattr(backend, "_stream", lambda: 1)
+    monkeypatch.setattr(backend._lib, "lib", lambda: SimpleNamespace(lq4_ctx_check=lambda ctx, stream: seen.append((ctx, stream)) or 0))
+    be = backend.CudaQ4Backend.__new__(backend.CudaQ4Backend)
+    be._ctx, be.device = 77, 3
+    be.check_device_status()
+    be._ctx = None                                                           # (nothing to destroy)
+    assert seen == [(77, 1003)]
