@@ -99,6 +99,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
         }
         for (int i = 0; i < 16; ++i) mbar_init(info + i, S::kTeam);
         mbar_fence_init();
+        ctl[2] = range.begin;
     }
     __syncthreads();
     uint64_t u = range.begin, seq_first = range.seq_first;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
     };
 
     if (tid >= S::kMath) {
-        load_stream<D, RING, 1, S::kTeams, S::kTeam>(p, u, u_end, b, seq_first, warp - S::kMath / 32, smem, full, empty, info, valid, fixes, ok,
+        load_stream<D, RING, 1, S::kTeams, S::kTeam, kPieceTiles<NQ>>(p, u, u_end, b, seq_first, warp - S::kMath / 32, smem, full, empty, info, valid, fixes, ok,
                                                      [](uint32_t r, uint32_t c) { return tile_at<D>(r, c); });
         if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);
         return;
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
     const uint32_t wm = warp / WN, wn = warp % WN, quad = lane >> 2, qc = (lane & 3) * 2;
     uint32_t tile = 0, kslot = 0, phase = 0;                             // tiles so far, their K's slot (V: the next) and its phase
     while (u < u_end) {
-        const Piece x = next_piece(p, u, u_end, b, seq_first);
+        const Piece x = next_piece<kPieceTiles<NQ>>(p, u, u_end, b, seq_first);
         const Seq& sq = x.sq;
         const uint32_t h = x.h, rt = x.rt, t0 = x.t0, n_tiles = x.n_tiles;
         const uint32_t rows = p.nodes * p.group;
@@ -318,8 +319,7 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
             for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + wm * 16 + quad + 8 * r].x);
             f[r] = exp2_fast(m[r] - (top == -INFINITY ? 0.0f : top));
         }
-        const bool whole = t0 == 0 && x.has_nodes;
-        const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+        const Fate to = fate<NQ>(x, u, ctl[2]);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
@@ -344,9 +344,18 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
                     const float4 v = *reinterpret_cast<const float4*>(os + (w * BM + r) * 36 + (i & 7) * 4);
                     y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
                 }
+                float4* const part = reinterpret_cast<float4*>(p.part_o + ((uint64_t)to.slot * BM + r) * D + d);
+                if (NQ == 1 && to.goes_on) {                             // (the same thread wrote it)
+                    const float2 e = p.part_ml[(uint64_t)to.slot * BM + r];
+                    const float all = fmaxf(top, e.x), base = all == -INFINITY ? 0.0f : all, f0 = exp2_fast(top - base), f1 = exp2_fast(e.x - base);
+                    const float4 v = *part;
+                    y[0] = y[0] * f0 + v.x * f1, y[1] = y[1] * f0 + v.y * f1, y[2] = y[2] * f0 + v.z * f1, y[3] = y[3] * f0 + v.w * f1;
+                    sum = sum * f0 + e.y * f1;
+                    top = all;
+                }
                 if (fix)
                     for (int e = 0; e < 4; ++e) y[e] += nonfinite_sum(p, x, anc[t], d + e);
-                if (whole) {
+                if (to.whole) {
                     const float inv = 1.0f / sum;
                     const uint64_t at = b * p.out_batch + t * p.out_node + (uint64_t)(h * p.group + g) * p.out_head + d;
 #pragma unroll
@@ -358,11 +367,23 @@ __global__ void __launch_bounds__((Shape<D, WM, NQ>::NT), (Shape<D, WM, NQ>::kPe
                     }
                     if (d == 0 && !(sum > 0.0f)) mark(p, NQ == 1, at);
                 } else {
-                    *reinterpret_cast<float4*>(p.part_o + ((uint64_t)slot * BM + r) * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-                    if (d == 0) p.part_ml[(uint64_t)slot * BM + r] = make_float2(top, sum);
+                    *part = make_float4(y[0], y[1], y[2], y[3]);
+                    if (NQ > 1 && d == 0) p.part_ml[(uint64_t)to.slot * BM + r] = make_float2(top, sum);
                 }
             }
             named_bar_sync(1, S::kMath);                                 // the columns are read (at last: anc and ml, too)
+        }
+        if (NQ == 1 && !to.whole && tid < BM) {                          // (behind the last use of what pieces before have left)
+            float2* const at = p.part_ml + (uint64_t)to.slot * BM + tid;
+            const float2 before = to.goes_on ? *at : make_float2(-INFINITY, 0.0f);
+            float top = before.x;
+#pragma unroll
+            for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * BM + tid].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float sum = before.y * exp2_fast(before.x - base);
+#pragma unroll
+            for (int w = 0; w < WN; ++w) sum += ml[w * BM + tid].y * exp2_fast(ml[w * BM + tid].x - base);
+            *at = make_float2(top, sum);
         }
         u += n_tiles;
     }

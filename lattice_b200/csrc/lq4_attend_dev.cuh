@@ -10,6 +10,13 @@ namespace lq4 {
 
 constexpr uint32_t kKeys = 64;                 // keys per tile
 constexpr uint32_t kMaxNodes = LQ4_MAX_TREE_NODES;
+// Tiles of a piece, with bf16 activations.  Every MMA cuts off what falls below its accumulator's last bit, always towards zero:
+// some 3e-7 of the sum a tile.  Left to one accumulator, O was 1.1e-3 low after 4096 tiles of tcgen05 and 3.2e-3 after 8192,
+// more than the rounding of a bf16 result.  So the sum over a longer run of tiles is taken up in f32, where partials lie
+// anyway.  (With f32 activations every tile's product is added up in f32.)
+constexpr uint32_t kMaxPiece = 512;
+template <int NQ>
+constexpr uint32_t kPieceTiles = NQ == 1 ? kMaxPiece : 0xffffffffu;
 
 struct AttendParams {
     CacheView c;
@@ -146,13 +153,26 @@ __device__ __forceinline__ Range cta_range(const AttendParams& p, uint64_t* word
     return r;
 }
 
-// One piece of a CTA's range: consecutive tiles of one item.
+// One piece of a CTA's range: at most kPieceTiles consecutive tiles of one item.
 struct Piece {
     Seq sq;
     uint32_t b, h, rt, t0, n_tiles;
     bool has_nodes;                            // it ends with the nodes' own tile
 };
+// What becomes of a piece that starts at unit u, in the range that starts at unit `begin`.
+struct Fate {
+    bool whole;                                // the CTA has all of the item, and this is its end: the result
+    bool goes_on;                              // the item's pieces before it lie in the slot as a partial
+    uint32_t slot;                             // of the CTA's partials: 1 for an item whose first tile it has, else 0
+};
+template <int NQ>
+__device__ __forceinline__ Fate fate(const Piece& x, uint64_t u, uint64_t begin) {
+    if (NQ > 1) return {x.t0 == 0 && x.has_nodes, false, 2 * blockIdx.x + (x.t0 == 0 ? 1 : 0)};
+    const bool from_first = u - x.t0 >= begin;                           // (the unit of the item's first tile)
+    return {from_first && x.has_nodes, x.t0 > 0 && u > begin, 2 * blockIdx.x + (from_first ? 1 : 0)};
+}
 // The piece that unit `u` starts; moves the sequence cursor (b, seq_first) on to it.
+template <uint32_t MOST>
 __device__ __forceinline__ Piece next_piece(const AttendParams& p, uint64_t u, uint64_t u_end, uint32_t& b, uint64_t& seq_first) {
     const uint64_t items = (uint64_t)p.kv_heads * p.row_tiles;
     Piece x;
@@ -166,7 +186,7 @@ __device__ __forceinline__ Piece next_piece(const AttendParams& p, uint64_t u, u
     x.b = b;
     x.h = item / p.row_tiles;
     x.rt = item - x.h * p.row_tiles;
-    x.n_tiles = (uint32_t)min((uint64_t)(x.sq.tiles - x.t0), u_end - u);
+    x.n_tiles = (uint32_t)min((uint64_t)min(x.sq.tiles - x.t0, MOST), u_end - u);
     x.has_nodes = x.t0 + x.n_tiles == x.sq.tiles;
     return x;
 }
@@ -251,7 +271,7 @@ static __device__ __noinline__ float nonfinite_total(const AttendParams& p, cons
 //   info          [16] by tile: TEAM arrivals when `valid` is there (which of the 64 keys there are, [16][2])
 //   fixes         [16][2]: non-finite V entries of the nodes' tile were cleared; there when its V is
 //   place(r, c)   byte offset of 16-byte chunk c of row r in a slot
-template <int D, uint32_t RING, uint32_t RINGS, uint32_t TEAMS, uint32_t TEAM, typename Place>
+template <int D, uint32_t RING, uint32_t RINGS, uint32_t TEAMS, uint32_t TEAM, uint32_t MOST, typename Place>
 __device__ __forceinline__ void load_stream(const AttendParams& p, uint64_t u, uint64_t u_end, uint32_t b, uint64_t seq_first, uint32_t w, unsigned char* smem,
                                             uint64_t* full, uint64_t* empty, uint64_t* info, volatile uint32_t* valid, volatile uint32_t* fixes, bool& ok, Place place) {
     constexpr uint32_t CPR = D / 8, kWarps = TEAMS, kOn = kWarps * kKeys, kHold = 2 / TEAM, kCopies = kHold * CPR;
@@ -274,7 +294,7 @@ __device__ __forceinline__ void load_stream(const AttendParams& p, uint64_t u, u
     const uint32_t ring0 = RINGS == 2 ? (lw & 1) * RING : 0;         // (a team's tiles are all even or all odd)
     const uint32_t page_size = p.c.page_size, pages_on = kOn / page_size, slots_on = kOn - pages_on * page_size;
     while (u < u_end) {
-        const Piece x = next_piece(p, u, u_end, b, seq_first);
+        const Piece x = next_piece<MOST>(p, u, u_end, b, seq_first);
         const int32_t* const table = p.c.table + (uint64_t)x.b * p.c.max_pages;
         const uint32_t plain = x.n_tiles - x.has_nodes;              // tiles of cached keys in this piece
         uint32_t i = (lw - tile) & (kWarps - 1);

@@ -126,6 +126,31 @@ __device__ __forceinline__ uint32_t swz(uint32_t rows, uint32_t r, uint32_t c) {
     return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+// Adds what the item's pieces before have left of a row (ml, and D floats at `from`) to the row's O in tensor memory, maximum and sum;
+// none: there is no O yet.  A call of its own: the end of a piece runs once or twice per CTA, and what it has to fetch of the
+// program counts (inline this cost 6 us of 126 where no item had several pieces).
+template <int D>
+__device__ __noinline__ float2 resume(uint32_t col_o, bool none, float m, float l, float2 ml, const float* from) {
+    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.0f : top, f = exp2_fast(m - base), g = exp2_fast(ml.x - base);
+    __syncwarp();
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+        float o[32];
+        tmem_ld32<0>(col_o + d, o);
+        tmem_ld_wait();
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float4 v = reinterpret_cast<const float4*>(from + d)[e];
+            w[4 * e] = __float_as_uint((none ? 0.0f : o[4 * e] * f) + v.x * g), w[4 * e + 1] = __float_as_uint((none ? 0.0f : o[4 * e + 1] * f) + v.y * g);
+            w[4 * e + 2] = __float_as_uint((none ? 0.0f : o[4 * e + 2] * f) + v.z * g), w[4 * e + 3] = __float_as_uint((none ? 0.0f : o[4 * e + 3] * f) + v.w * g);
+        }
+        tmem_st32(col_o + d, w);
+    }
+    tmem_st_wait();
+    return make_float2(top, l * f + ml.y * g);
+}
+
 // NS streams; WIDE: items of 256 rows; NQ bf16 terms of q and P: 1 for bf16 activations, 3 for f32.
 template <int D, int NS, bool WIDE, int NQ>
 struct TcShape {
@@ -161,7 +186,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
     uint64_t* anc = reinterpret_cast<uint64_t*>(smem + S::kAnc);        // [nodes] of the piece's sequence
     float2* meet = reinterpret_cast<float2*>(smem + S::kMeet);          // [128] (max, sum) of stream 1's rows
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..15: warp sums; 16: tensor memory
+    uint64_t* ctl = reinterpret_cast<uint64_t*>(smem + S::kCtl);        // 0, 1: cursor; 2..15: warp sums, then 2: the range's first unit; 16: tensor memory
     uint64_t *full = bars, *empty = bars + SL, *s_full = bars + 2 * SL, *s_free = s_full + 2, *p_full = s_full + 4, *o_done = s_full + 6;
     uint64_t *q_full = s_full + 8, *drained = s_full + 9, *info = s_full + 10;      // info: [16], the loaders are at most 7 tiles ahead
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16);
@@ -189,6 +214,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             mbar_init(drained, NS);
             for (int i = 0; i < 16; ++i) mbar_init(info + i, S::kTeam);
             mbar_fence_init();
+            ctl[2] = range.begin;
         }
     }
     tc_fence_before();
@@ -217,7 +243,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
         const uint32_t rows = p.nodes * p.group;
         uint32_t used = 0;                                               // steps of this stream so far
         while (u < u_end) {
-            const Piece x = next_piece(p, u, u_end, b, seq_first);
+            const Piece x = next_piece<kPieceTiles<NQ>>(p, u, u_end, b, seq_first);
             if (x.sq.bad && tid == 0) atomicOr(p.status, kDevErrBadIndex);
             const uint32_t row = x.rt * S::kItemRows + (WIDE ? tid : r), t = row / p.group, g = row - t * p.group;
             const bool live = row < rows && (int32_t)t < x.sq.nodes;
@@ -414,6 +440,14 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             // through Q's place, 32 columns at a time (both have waited for all MMAs of their own that read Q; the
             // barrier below covers the other's).
             constexpr bool kMeets = NS == 2 && !WIDE;
+            const Fate fates = fate<NQ>(x, u, ctl[2]);
+            const bool whole = fates.whole;
+            const uint64_t slot = (uint64_t)fates.slot * S::kItemRows + (WIDE ? tid : r);
+            if (NQ == 1 && fates.goes_on && (!kMeets || str == 0)) {
+                const float2 ml = resume<D>(col_o, first, m, l, p.part_ml[slot], p.part_o + slot * D);
+                m = ml.x, l = ml.y;
+                first = false;
+            }
             float f = 1.0f, f_other = 0.0f;
             if constexpr (kMeets) {
                 if (str == 1) meet[r] = make_float2(m, l);
@@ -427,8 +461,6 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                     m = top;
                 }
             }
-            const bool whole = x.t0 == 0 && x.has_nodes;
-            const uint64_t slot = ((uint64_t)2 * blockIdx.x + (x.t0 == 0 ? 1 : 0)) * S::kItemRows + (WIDE ? tid : r);
             const bool fix = x.has_nodes && (fixes[((tile + x.n_tiles - 1) & 15) * 2] | (S::kTeam == 2 ? fixes[((tile + x.n_tiles - 1) & 15) * 2 + 1] : 0));      // (the nodes' tile is a piece's last one)
             const float inv = 1.0f / l;
             if (!whole && live && (!kMeets || str == 0)) p.part_ml[slot] = make_float2(m, l);
@@ -560,7 +592,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             kr.move(2);
         };
         while (u < u_end) {
-            const Piece x = next_piece(p, u, u_end, b, seq_first);
+            const Piece x = next_piece<kPieceTiles<NQ>>(p, u, u_end, b, seq_first);
             const uint32_t tiles = uniform(x.n_tiles);
             const uint32_t steps = RINGS == 2 ? (tiles + 1 - ((str - at) & 1)) / 2 : tiles;      // of this stream
             wait(q_full, piece & 1);
@@ -594,7 +626,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
         __syncwarp();
     } else {
         // ---- loaders -----------------------------------------------------------------------------------------
-        load_stream<D, RING, RINGS, S::kTeams, S::kTeam>(p, u, u_end, b, seq_first, warp - (S::kThreads - S::kLoaders) / 32, smem, full, empty, info, valid, fixes, ok,
+        load_stream<D, RING, RINGS, S::kTeams, S::kTeam, kPieceTiles<NQ>>(p, u, u_end, b, seq_first, warp - (S::kThreads - S::kLoaders) / 32, smem, full, empty, info, valid, fixes, ok,
                                                          [](uint32_t r, uint32_t c) { return swz(kKeys, r, c); });
     }
     if (!ok) atomicOr(p.status, kDevErrBarrierTimeout);

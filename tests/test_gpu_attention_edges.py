@@ -140,6 +140,70 @@ def test_attention_over_many_caches_with_infinities(be, hq, d, dtype):
     assert not bool(((bits < 0) & got.isnan()).any())                        # no mark is left
 
 
+@pytest.mark.parametrize("hq, d, keys", [(4, 128, 1 << 19), (40, 128, 1 << 19), (80, 128, 1 << 18), (200, 64, 1 << 18), (4, 256, 1 << 19), (24, 256, 1 << 19), (24, 192, 100032)])
+def test_attention_over_long_pieces_has_no_bias(be, hq, d, keys):
+    """One CTA sums thousands of tiles of values of one sign: a sum that cuts off its last bits is low by more the longer it
+    gets.  148 sequences share one set of pages, so that each CTA has whole items; the columns' means are spread over two
+    binades, so that the roundings of the results do not add up."""
+    from lattice_b200 import KvCache
+    b, page = 148, 64
+    g = torch.Generator(device="cuda").manual_seed(50)
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    mean = 0.5 + 1.5 * (torch.arange(d, device="cuda") + 0.5) / d
+    k = draw(keys // page, page, 1, d).to(BF16)
+    v = (mean * (1 + 0.3 * draw(keys // page, page, 1, d))).to(BF16)
+    table = torch.arange(keys // page, dtype=torch.int32, device="cuda").expand(b, -1).contiguous()
+    q, kn, vn = draw(b, 1, hq, d).to(BF16), draw(b, 1, 1, d).to(BF16), mean.to(BF16).expand(b, 1, 1, d)
+    lens = torch.full((b,), keys, dtype=torch.int32, device="cuda")
+    got = be.tree_attention(q, kn, vn, KvCache(k, v, table), lens)
+    be.check_device_status()
+    off = []
+    for i in (0, 77, 147):
+        kk, vv = torch.cat([k.view(keys, d), kn[i, 0]]).double(), torch.cat([v.view(keys, d), vn[i, 0]]).double()
+        ref = torch.softmax(q[i, 0].double() @ kk.T * d ** -0.5, -1) @ vv
+        err = (got[i, 0].double() - ref) / ref
+        # half a step of the result, and half a step of each weight (their sum's errors average out: 0.3 of it at most)
+        assert float(err.abs().max()) <= 2.0 ** -8 + 0.3 * 2.0 ** -8
+        off.append(float(err.mean()))
+    # The results' roundings: uniform within half a step, an rms of 2^-8 / 3^0.5, one of its own per column and five standard
+    # deviations of their mean.  A cut-off of half a last bit (2^-24) on average at each of the MMAs that one sum goes through:
+    # at most four a tile for 512 tiles, which are then summed up in f32.
+    assert abs(sum(off)) / 3 <= 5 * 2.0 ** -8 / (3 * d) ** 0.5 + 4 * 512 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hq, d", [(4, 64), (9, 128), (24, 128), (40, 128), (200, 128), (140, 64), (3, 256), (24, 256), (12, 192)])
+def test_attention_of_items_in_several_pieces(be, hq, d, dtype):
+    """Sequences of 500 to 1600 tiles, whose pieces end at 512 tiles, at the items' and at the CTAs' borders."""
+    from lattice_b200 import KvCache
+    b, page, most = 151, 48, 102400
+    g = torch.Generator(device="cuda").manual_seed(60)
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    k, v = draw(-(-most // page), page, 1, d).to(BF16), draw(-(-most // page), page, 1, d).to(BF16)
+    table = torch.arange(k.shape[0], dtype=torch.int32, device="cuda").expand(b, -1).contiguous()
+    q, kn, vn = draw(b, 1, hq, d).to(dtype), draw(b, 1, 1, d).to(BF16), draw(b, 1, 1, d).to(BF16)
+    lens = [32000 + (i * 7919) % 70000 for i in range(b)]
+    lens[0], lens[1], lens[2], lens[3] = 511 * 64, 511 * 64 + 1, 512 * 64 + 1, 0
+    q[1] *= 30.0 / d ** 0.5                                                  # sharp weights too: the maximum moves late
+    got = be.tree_attention(q, kn, vn, KvCache(k, v, table), i32(lens))
+    assert torch.equal(got, be.tree_attention(q, kn, vn, KvCache(k, v, table), i32(lens)))
+    be.check_device_status()
+    for i in (0, 1, 2, 3, 50, 77, 149, 150):
+        n = lens[i]
+        kk, vv = torch.cat([k.view(-1, d)[:n], kn[i, 0]]).double(), torch.cat([v.view(-1, d)[:n], vn[i, 0]]).double()
+        x = q[i, 0].double()
+        w = torch.softmax(x @ kk.T * d ** -0.5, -1)
+        ref, mag, size = w @ vv, w @ vv.abs(), (x.norm(dim=-1) * kk.norm(dim=-1).amax() * d ** -0.5)[:, None]
+        # products are exact, about 16 roundings of 2^-23 of at most |q| |k| scale lie in a score, two more in the exponent and
+        # 2^-22 in exp2, each counts twice; four cut-offs of 2^-23 a tile for 512 tiles with bf16 activations, else one a
+        # tile, and the joins; half a step for bf16 weights, and of the result
+        e = 2 * (16 * 2.0 ** -23 * size + 2.0 ** -21) + (4 * 512 if dtype == BF16 else n / 64 + 200) * 2.0 ** -23
+        half = 2.0 ** -8 if dtype == BF16 else 2.0 ** -24
+        tol = mag * (e + (half if dtype == BF16 else 0.0)) + half * ref.abs() * 1.01
+        err = (got[i, 0].double() - ref).abs()
+        assert bool((err <= tol).all()), (i, float((err / tol).max()))
+
+
 # ---- verification of drafted tokens --------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
