@@ -20,7 +20,7 @@
 // same numbers, in the same order.
 //
 // A cluster lives in one GPC and gets some 0.8 TB/s: two rows of 248320 f32 logits are 2.5 us and more per node, one node after
-// the other.  Where all rows together are few enough (kEagerBytes), verify_stats_kernel takes (max, sum) of every row over the
+// the other.  Where there are few enough rows (stat_splits), verify_stats_kernel takes (max, sum) of every row over the
 // whole GPU first; the walk then only reads the rows of a node where a draft is refused or the last token is drawn.  What
 // bounds it is the chain of latencies per node (rows, two reductions, a barrier); without statistics the first child's rows
 // are fetched into L2 meanwhile.  B200, device time: a chain of 5 over 248320 f32 logits, all accepted, 31 us (10 MB of rows:
@@ -701,11 +701,15 @@ __global__ void __launch_bounds__(kVThreads, 1) verify_kernel(const __grid_const
 
 // (max, sum) and the best candidate of every row that the walk may visit: one CTA per split of a row.
 constexpr uint32_t kStatThreads = 256, kMaxSplits = 32;
-// What this kernel may read.  It costs the rows of nodes that the walk never visits and saves a row's pass per visited one.
-// Without and with it, means of six inputs on a B200 (what a walk costs depends on how far it gets): f32, chains of 5 over
-// 248320: 1 sequence (10 MB) 51 and 28 us, 4 (40 MB) 66 and 41, 8 (79 MB) 87 and 71; bf16, trees of 24 over 100003: 1
-// (10 MB) 44 and 31, 8 (77 MB) 89 and 77, 16 (154 MB) 79 and 111.  A walk that ends at the root loses 2 to 7 us by it.
-constexpr uint64_t kEagerBytes = 80ull << 20;
+// When the statistics come first.  They cost the rows of nodes that the walk never visits, and save it a pass over a row per
+// visited one.  Without and with them, us on a B200, means of six inputs that get differently far:
+//   rows       chains of 5, f32: 1 over 2048 (10 rows) 54 and 29, 64 over 2048 (640) 66 and 34, 64 over 8192 68 and 33, 1 over
+//              32000 56 and 31; trees of 24 over 32000, bf16: 16 (768 rows) 73 and 63; trees of 64 over 2048, bf16: 64 (8192
+//              rows, of which few are visited) 77 and 110
+//   bytes      trees of 24 over 100003, bf16: 8 (77 MB) 89 and 77, 10 (96 MB) 58 and 67, 16 (154 MB) 80 and 109; a chain's rows are
+//              more likely to be visited: 9 of 5 over 248320, f32 (89 MB) 94 and 77, 9 of 8 (143 MB) 147 and 107
+// With one node there is nothing to walk.
+constexpr uint64_t kMaxStatRows = 2048, kTreeBytes = 80ull << 20, kChainBytes = 144ull << 20;
 
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
@@ -795,9 +799,8 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
 // Splits of a row that the statistics are taken in; 0: the walk takes them itself.
 uint32_t stat_splits(const lq4_verify_args& a, int sm_count) {
     const uint64_t rows = (uint64_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1), row = (uint64_t)a.vocab * (a.dtype == LQ4_DTYPE_F32 ? 4 : 2);
-    // a chain or tree of one node has nothing to walk; short rows are read by the cluster as fast as their statistics
     // (a division: rows * row may pass 64 bits where rows are broadcast)
-    if (a.nodes < 2 || rows > kEagerBytes / row || row < (128u << 10)) return 0;
+    if (a.nodes < 2 || rows > kMaxStatRows || rows > (a.parents ? kTreeBytes : kChainBytes) / row) return 0;
     uint64_t splits = (4ull * sm_count + rows - 1) / rows;
     return splits > kMaxSplits ? kMaxSplits : splits < 1 ? 1 : (uint32_t)splits;
 }
@@ -849,7 +852,7 @@ cudaError_t run(VerifyParams p, int sm_count, int use_pdl, cudaStream_t s, int* 
 }  // namespace
 
 size_t verify_workspace_bytes(const lq4_verify_args& a, int sm_count) {
-    return (size_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1) * stat_splits(a, sm_count) * sizeof(Stat);      // (30 KB at most)
+    return (size_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1) * stat_splits(a, sm_count) * sizeof(Stat);      // (64 KB at most)
 }
 
 cudaError_t launch_verify_draft(const lq4_verify_args& a, void* workspace, int32_t* status, int sm_count, int use_pdl, cudaStream_t s, int* launches) {
