@@ -65,7 +65,9 @@ class KvCache:
             raise TypeError(f"the cache holds bfloat16, got {k.dtype} and {v.dtype}")
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v must be [pages, page_size, kv_heads, head_dim] with equal strides, the innermost 1")
-        if any(n > 1 and s == 0 for n, s in zip(k.shape, k.stride())):      # (0 means dense to the library)
+        pages, size, heads, dim = k.shape
+        s0, s1, s2, _ = k.stride()
+        if (not s0 and pages > 1) or (not s1 and size > 1) or (not s2 and heads > 1):      # (0 means dense to the library)
             raise ValueError("k and v must not be expanded tensors")
         if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
             raise TypeError("page_table must be a contiguous [batch, max_pages] int32 tensor")
@@ -73,10 +75,9 @@ class KvCache:
         if self.device < 0 or v.get_device() != self.device or page_table.get_device() != self.device:
             raise ValueError("k, v and page_table must lie on one CUDA device")
         self.k, self.v, self.page_table = k, v, page_table
-        pages, size, heads, dim = k.shape
-        s0, s1, s2 = (s if n > 1 else 0 for n, s in zip(k.shape[:3], k.stride()))      # (of one entry it may be anything)
         batch, max_pages = page_table.shape
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, s0, s1, s2, page_table.data_ptr(), batch, max_pages)
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), pages, size, heads, dim, s0 if pages > 1 else 0, s1 if size > 1 else 0,
+                                s2 if heads > 1 else 0, page_table.data_ptr(), batch, max_pages)      # (of one entry a stride may be anything)
         self.address = C.addressof(self.desc)
         self.rows_shape = (batch, heads, dim)                            # of rows to append or attend with, but for their number
 
