@@ -448,7 +448,8 @@ lq4_status lq4_rot_signs_from_seed(uint64_t seed, uint32_t dim, float* signs, vo
  * LQ4_OPT_ALLOW_GROW 0 all streams and graphs take the first stream's workspace as it is, so that their calls have to be
  * ordered; where it is too small lq4_tree_attention returns LQ4_ERR_NOSPACE.  Values that the host cannot see (page
  * ids, lengths, parents, path entries) are checked by the kernels: what is out of range is skipped, and
- * lq4_ctx_check reports it as LQ4_ERR_DEVICE with bit 8 of the status set. */
+ * lq4_ctx_check reports it as LQ4_ERR_DEVICE with the value 8 in the status (tokens and parents of lq4_verify_draft
+ * excepted: what they name out of range is never accepted or visited). */
 
 enum { LQ4_ROPE_HALF = 0, LQ4_ROPE_INTERLEAVED = 1 };
 enum { LQ4_ROPE_PLAIN = 0, LQ4_ROPE_LINEAR = 1, LQ4_ROPE_NTK = 2, LQ4_ROPE_YARN = 3, LQ4_ROPE_BANDS = 4 };
@@ -555,7 +556,8 @@ lq4_status lq4_kv_append(lq4_ctx* ctx, const lq4_kv_append_args* args, void* str
  * it sees, an infinity makes that column infinite and a NaN, or two infinities of different signs, make it NaN, however
  * small the key's weight; with f32 activations a K row with an infinity or a NaN makes NaN of the node's row.  Nodes from
  * node_counts[b] on (NULL: all live) and sequences with kv_lens[b] < 0 or no live node are left as they were in
- * `out`.  Softmax and sums are f32; with f32 activations the products are too (three bf16 terms each).  Pages out
+ * `out`.  Scores, softmax and sums are f32.  The products are bf16 with bf16 activations: q as it is, each weight rounded
+ * once (half a step of 2^-8, of the size of the result's own rounding); with f32 activations they are f32 (three bf16 terms each).  Pages out
  * of range are not seen; they, a length above the capacity and a parent that does not come before its node (it
  * counts as a root) are reported through lq4_ctx_check.  Results depend on the lengths and the device only, not
  * on timing.  The workspace (at most 40 MB, independent of the lengths) grows on the first call with a larger

@@ -17,13 +17,17 @@
 //   loads      four warps of their own (load_stream): cp.async, 16 bytes a lane, into a ring of K and V tiles.  Every
 //              key's address is looked up on its own (slot -> page), so pages of any size may end anywhere inside a tile.
 //   math       mma.sync m16n8k16 on bf16.  K and V are bf16 in memory and exact.  q and the probabilities are one
-//              bf16 term each for bf16 activations (both roundings are of the size of the output's own), and three
-//              terms each (24 bits) for f32 ones, so that an f32 result keeps 32-bit accuracy.
+//              bf16 term each for bf16 activations (q is one; the weights' rounding is of the size of the output's own), and
+//              three terms each (24 bits) for f32 ones, so that an f32 result keeps 32-bit accuracy.  A second term of the
+//              weights would take the error of the batch below from 1.83e-3 to 1.67e-3 (2-norm; what the result's own rounding
+//              leaves) for 154 -> 164 us a call, and with tcgen05 that of large trees from 2.27e-3 to 1.67e-3 for 126 -> 162 us.
 //   warps      four for the math, WM x WN: WM bands of 16 rows, WN shares of the 64 keys.  Each warp keeps its own running
 //              maximum, sum and O over its keys; they meet in shared memory once per piece.
 //
-// B200, device time: 32 sequences of 4096 to 8191 tokens, 40 heads on 8 of 128, bf16: 141 us (5.8 TB/s; every key is read
-// once).  One of 120001, 24 heads on 4 of 256, f32: 148 us (3.3 TB/s; 6 rows fill 16, and each product is three).
+// B200, device time: 32 sequences of 4096 to 8191 tokens, 40 heads on 8 of 128, bf16: 144 us (5.7 TB/s; every key is read
+// once).  One of 120001, 24 heads on 4 of 256, f32: 148 us (3.3 TB/s; 6 rows fill 16, and each product is three: tensor pipe 34 %,
+// issue active 30 %, and one math warp a scheduler has nobody to hide its waits).  f32 above a head_dim of 128 is at the limit of
+// 255 registers and spills: 120 bytes of loads at 256 with up to 16 rows, 272 with 32.
 //
 // A key that a row may not see contributes nothing whatever it holds: its score is replaced by -inf, and a
 // non-finite V entry of a node (0 * inf would reach the rows that do not see it) is cleared in shared memory

@@ -29,9 +29,10 @@
 // starts from zero and the softmax threads add it to O in their registers, a tile later; one stream, two buffers of P and
 // of P V.
 //
-// B200, device time: 4 trees of 64 nodes over 16384 tokens, 32 heads on 8 of 128, bf16: 115 us (0.6 PFLOP/s); 8 trees of 13
-// nodes over 2000 to 4000, 40 heads on 8 of 128, f32: 83 us.  Neither HBM nor the tensor cores are busy (23 % and 26 % at
-// half the first one's length): a stream waits for its own scores, exponentials and products in turn.
+// B200, device time: 4 trees of 64 nodes over 16384 tokens, 32 heads on 8 of 128, bf16: 119 us (0.6 PFLOP/s); 8 trees of 13
+// nodes over 2000 to 4000, 40 heads on 8 of 128, f32: 86 us.  Neither HBM nor the tensor cores are busy (22 % and 26 % at
+// half the first one's length, 16 % and 27 % in the second): a stream waits for its own scores, exponentials and products in
+// turn, and with f32 activations, where a scheduler has one softmax warp, most of all for its instructions.
 #include "lq4_attend_dev.cuh"
 
 namespace lq4 {

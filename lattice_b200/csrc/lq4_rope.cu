@@ -3,13 +3,15 @@
 // Both are passes over memory: every element is read once and written once.
 //
 // rope_kernel: pair i of a head is a complex number turned by the angle pos * freq[i].  The angle of a far
-// position does not fit f32 (10^6 radians leave 2^-4 of a turn), so it is formed in f64 as a number of
+// position does not fit f32 (at 10^6 radians its step is 2^-4 of a radian), so it is formed in f64 as a number of
 // TURNS, its whole part is dropped there, and only the remainder in [-1/2, 1/2] goes to f32 and sincospi:
 // three f64 operations per (row, pair), shared by the heads of a CTA through shared memory.  A CTA takes a
 // few rows (256 angles, one per thread) and the heads of one tensor, or a slice of them when the rows alone would not
 // fill the GPU; a thread keeps its place in the head and has 64 to 128 bytes of several heads under way at a time (V
 // pairs per step: both halves are in its registers before it stores, so the call may work in place).  B200, device time: 4099
-// rows of 32 heads of 256, bf16, 64 channels turned: 33 us (4.0 TB/s); 2047 rows of 56 heads of 128, f32: 27 us (4.3 TB/s).
+// rows of 32 heads of 256, bf16, 64 channels turned: 33 us (4.0 TB/s); 2047 rows of 56 heads of 128, f32: 27 us (4.3 TB/s).  What
+// bounds it is latency at low occupancy: three CTAs an SM (78 registers, 35 % of the warps), issue active 66 and 40 %, the
+// waits for loads and for the instruction before as large as one another, or the loads' alone.
 //
 // kv_append_kernel: 3 x 4001 rows of 4 heads of 256, f32 to a bf16 cache: 23 us (6.4 TB/s).
 #include "lq4_attend.cuh"

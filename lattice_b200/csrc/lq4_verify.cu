@@ -23,8 +23,10 @@
 // the other.  Where there are few enough rows (stat_splits), verify_stats_kernel takes (max, sum) of every row over the
 // whole GPU first; the walk then only reads the rows of a node where a draft is refused or the last token is drawn.  What
 // bounds it is the chain of latencies per node (rows, two reductions, a barrier); without statistics the first child's rows
-// are fetched into L2 meanwhile.  B200, device time: a chain of 5 over 248320 f32 logits, all accepted, 31 us (10 MB of rows:
-// 1.5 us at HBM rate); 16 trees of 24 over 100003 bf16 logits 55 to 101 us with the data.
+// are fetched into L2 meanwhile.  B200, device time: a chain of 5 over 248320 f32 logits 26 to 31 us with the data (10 MB of rows:
+// 1.5 us at HBM rate); 16 trees of 24 over 100003 bf16 logits 49 to 101 us.  Under ncu the chain waits at barriers most of
+// all, then for instructions and loads.  The held form does not fit 128 registers: 1012 bytes of spill loads with f32
+// logits, 236 with bf16, none in the form that reads long shares again.
 //
 // Decisions lie next to borders.  Masses are f32 (ex2.approx of the rounded distance from the maximum: a few 2^-23, and
 // exactly 1 at the maximum; four or eight at a time are added in f32); all further sums are pairs of f32 (some 48 bits, any size of
