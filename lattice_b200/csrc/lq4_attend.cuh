@@ -8,6 +8,28 @@ namespace lq4 {
 
 constexpr int kDevErrBadIndex = 8;      // a page id, length, count, parent or path entry outside its range
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Launches a kernel, with programmatic dependent launch if asked for.
+template <typename... Args>
+cudaError_t attend_launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size_t smem, int use_pdl, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = use_pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 // ---- lq4_rope.cu ----------------------------------------------------------------
 // Arguments are validated by the caller (lq4_api.cu).
 cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, cudaStream_t s);

@@ -87,11 +87,6 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // (a, b) -> one word of bf16 and what the rounding left of each.
 __device__ __forceinline__ uint32_t split_pair(float& a, float& b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
@@ -395,20 +390,6 @@ inline bool attend_workspace(AttendParams& p, AttendWorkspace& ws, uint32_t rows
     p.part_ml = static_cast<float2*>(ws.p);
     p.part_o = reinterpret_cast<float*>(p.part_ml + slots);
     return true;
-}
-template <typename... Args>
-cudaError_t attend_launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size_t smem, int use_pdl, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = use_pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 // lq4_attend.cu: joins the partials of a launch with items of `rows` rows and D channels; completes ws.launches.
 cudaError_t launch_attend_join(const AttendParams& p, uint32_t rows, uint32_t D, bool bf16_out, AttendWorkspace& ws, int use_pdl, cudaStream_t s);

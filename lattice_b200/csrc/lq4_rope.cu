@@ -266,23 +266,6 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     if (bad && lane == 0) atomicOr(p.status, kDevErrBadIndex);
 }
 
-template <typename... Args>
-cudaError_t launch(void (*fn)(Args...), dim3 grid, uint32_t threads, size_t smem, int use_pdl, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    if (use_pdl) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, fn, args...);
-}
-
 // Whether every part can be moved `vec` elements at a time.
 bool vec_fits(const lq4_rope_args& a, uint32_t half, uint32_t vec) {
     if (half % vec || (a.head_dim - 2 * half) % vec || a.head_dim % vec) return false;
@@ -337,7 +320,7 @@ cudaError_t launch_rope_rows(const lq4_rope_args& a, int sm_count, int use_pdl, 
     const dim3 grid(row_ctas, ctas);
     const size_t smem = (size_t)p.rows_per_cta * p.half * sizeof(float2);
     auto fn = vec == 8 ? rope_kernel<8> : vec == 4 ? rope_kernel<4> : rope_kernel<1>;
-    return launch(fn, grid, kRopeThreads, smem, use_pdl, s, p);
+    return attend_launch(fn, grid, kRopeThreads, smem, use_pdl, s, p);
 }
 
 cudaError_t launch_kv_append(const lq4_kv_append_args& a, int32_t* status, int use_pdl, cudaStream_t s) {
@@ -359,7 +342,7 @@ cudaError_t launch_kv_append(const lq4_kv_append_args& a, int32_t* status, int u
     p.new_lens = a.new_lens;
     p.status = status;
     const uint64_t items = (uint64_t)p.batch * (p.rows ? p.rows : 1);
-    return launch(kv_append_kernel, dim3((unsigned)((items + 7) / 8)), 256, 0, use_pdl, s, p);
+    return attend_launch(kv_append_kernel, dim3((unsigned)((items + 7) / 8)), 256, 0, use_pdl, s, p);
 }
 
 }  // namespace lq4

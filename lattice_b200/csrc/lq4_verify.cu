@@ -101,11 +101,6 @@ struct WarpSum {
     Pair s;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // log2(e) / tau.  Above zero for an infinite temperature too: that is the limit in which everything above -inf weighs the same,
 // and 0 * -inf would be NaN.
 __device__ __forceinline__ float per_tau(float tau) { return fmaxf(1.44269504088896340736f / tau, 1.4e-45f); }
