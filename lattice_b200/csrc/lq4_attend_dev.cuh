@@ -3,6 +3,7 @@
 #pragma once
 
 #include "lq4_attend.cuh"
+#include "lq4_tc.cuh"
 
 #include <cuda_bf16.h>
 
@@ -82,7 +83,6 @@ __device__ __forceinline__ uint64_t cta_share(uint64_t total, uint32_t grid) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

@@ -42,25 +42,7 @@ namespace {
 constexpr int kTcRows = 128;
 constexpr float kLazy = 8.0f;                  // how far (log2) a row's maximum may outgrow its base
 
-__device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// D[tmem] (+)= A[smem] B[smem]; bf16, f32 accumulation; one thread issues.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// The same with A in tensor memory (a lane per row, two consecutive k per column).
+// D[tmem] (+)= A[tmem] B[smem]: A has a lane per row and two consecutive k per column; one thread issues.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -74,21 +56,10 @@ __device__ __forceinline__ bool elect_lane() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
     return is != 0;
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 template <int AT, int N>
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[N]) {      // 32 columns -> r[AT .. AT + 32)
     uint32_t u[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
-          "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
-          "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-        : "r"(taddr)
-        : "memory");
+    tmem_ld_32x32(taddr, u);
 #pragma unroll
     for (int i = 0; i < 32; ++i) r[AT + i] = __uint_as_float(u[i]);
 }
@@ -106,7 +77,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&u)[8])
                  "r"(u[6]), "r"(u[7]), "r"(taddr)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptors, 128-byte swizzle (version 1 at bits 46-47, swizzle mode 2 at 61-63); a tile is
@@ -585,10 +555,10 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
 #pragma unroll
                 for (int ks = 0; ks < NQ * (D / 16); ++ks) {             // the smallest term first
                     const int n = NQ - 1 - ks / (D / 16), c = ks % (D / 16) >> 2, in = (ks & 3) * 32;
-                    mma_ss(col_s, q + (n * S::kQTerm + c * (kTcRows * 128) + in >> 4), k + (c * (kKeys * 128) + in >> 4), instr_desc(kKeys, 0), ks > 0);
+                    umma_f16(col_s, q + (n * S::kQTerm + c * (kTcRows * 128) + in >> 4), k + (c * (kKeys * 128) + in >> 4), instr_desc(kKeys, 0), ks > 0);
                 }
-                mma_commit(empty + ring0 + kr.slot);
-                mma_commit(s_full + str);
+                umma_commit(empty + ring0 + kr.slot);
+                umma_commit(s_full + str);
             }
             kr.move(2);
         };
@@ -612,8 +582,8 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
                         const int n = NQ - 1 - ks / 4, c = ks & 3;
                         mma_ts(col_o + buf * D, col_p + buf * (32 * NQ) + n * 32 + c * 8, vt + (c * 2048 >> 4), instr_desc(D, 1), (NQ == 1 && v > 0) || ks > 0);
                     }
-                    mma_commit(empty + ring0 + vr.slot);
-                    mma_commit(o_done + (NQ == 1 ? str : buf));
+                    umma_commit(empty + ring0 + vr.slot);
+                    umma_commit(o_done + (NQ == 1 ? str : buf));
                 }
                 if (NQ > 1) buf ^= 1;
                 vr.move(2);
@@ -622,7 +592,7 @@ __global__ void __launch_bounds__((TcShape<D, NS, WIDE, NQ>::kThreads), 1) atten
             ++piece;
             u += tiles;
         }
-        if (leader) mma_commit(drained);                                 // tensor memory is freed behind the last MMA
+        if (leader) umma_commit(drained);                                 // tensor memory is freed behind the last MMA
         if (!mbar_wait(drained, 0)) ok = false;
         __syncwarp();
     } else {
