@@ -601,7 +601,9 @@ lq4_status lq4_tree_attention(lq4_ctx* ctx, const lq4_tree_attention_args* args,
  *   path[b, 0 .. path_len[b])   the accepted nodes from node 0 on (rising), -1 behind them: `index` and `counts`
  *                               of lq4_kv_append
  * Sequences with node_counts[b] <= 0 get path_len 0 and next_token -1.  Exponentials are f32, sums over
- * the vocabulary pairs of f32, comparisons f64.  One launch, or two and a small workspace (64 KB; one launch where it
+ * the vocabulary pairs of f32, comparisons f64: a residual is known to some 2^-22 of p, so where draft and target agree to
+ * that, what is left after a refusal (which then has that probability) is decided by rounding, and logits whose share is
+ * below 2^-126 carry no mass.  One launch, or two and a small workspace (64 KB; one launch where it
  * cannot be had) where all rows together are few.  Stands behind the
  * lm_head projection over all nodes' rows, where a plain step calls lq4_logits_topk. */
 typedef struct {
