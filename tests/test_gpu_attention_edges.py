@@ -332,6 +332,37 @@ def test_two_graphs_of_one_backend_side_by_side():
     other.close()
 
 
+@pytest.mark.parametrize("known", [True, False])
+def test_an_eager_call_beside_a_capture(known):
+    """While one stream captures, another one may call, also for the first time, and take or grow a workspace."""
+    from lattice_b200 import CudaQ4Backend
+    be, other = CudaQ4Backend(0), CudaQ4Backend(0)
+    cache, lens = dense_cache(2, 60, 32, 2, 128, seed=70), i32([1800, 1700])
+    q, k, v = (normal(71 + i, 2, 3, h, 128).to(BF16).cuda() for i, h in enumerate((16, 2, 2)))
+    want = other.tree_attention(q, k, v, cache, lens)
+    side, outs = torch.cuda.Stream(), [torch.zeros_like(q) for _ in range(2)]
+    torch.cuda.synchronize()
+    if known:
+        with torch.cuda.stream(side):
+            be.tree_attention(q, k, v, cache, lens, out=outs[1])
+        torch.cuda.synchronize()
+        outs[1].zero_()
+        torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        be.tree_attention(q, k, v, cache, lens, out=outs[0])
+        with torch.cuda.stream(side):
+            be.tree_attention(q, k, v, cache, lens, out=outs[1])
+    side.synchronize()
+    assert torch.equal(outs[1], want)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want)
+    be.check_device_status()
+    be.close()
+    other.close()
+
+
 def test_a_graph_that_grows_inside_its_capture():
     """A wider call later in a capture takes a larger workspace; the calls before it keep theirs."""
     from lattice_b200 import CudaQ4Backend
