@@ -27,7 +27,7 @@
 // B200, device time: 32 sequences of 4096 to 8191 tokens, 40 heads on 8 of 128, bf16: 144 us (5.7 TB/s; every key is read
 // once).  One of 120001, 24 heads on 4 of 256, f32: 148 us (3.3 TB/s; 6 rows fill 16, and each product is three: tensor pipe 34 %,
 // issue active 30 %, and one math warp a scheduler has nobody to hide its waits).  f32 above a head_dim of 128 is at the limit of
-// 255 registers and spills: 120 bytes of loads at 256 with up to 16 rows, 272 with 32.
+// 255 registers and spills: 120 bytes of loads at 256 with up to 16 rows and 272 with 32, 68 and 160 at 192.
 //
 // A key that a row may not see contributes nothing whatever it holds: its score is replaced by -inf, and a
 // non-finite V entry of a node (0 * inf would reach the rows that do not see it) is cleared in shared memory

@@ -793,11 +793,29 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const __grid
     }
 }
 
-// Splits of a row that the statistics are taken in; 0: the walk takes them itself.
+// CTAs per sequence, and whether a warp's share of a row stays in its registers.
+struct WalkShape {
+    uint32_t ranks;
+    bool held;
+};
+template <typename T>
+WalkShape walk_shape(uint32_t batch, uint32_t vocab, int sm_count) {
+    // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
+    uint32_t ranks = kMaxCluster;
+    while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || vocab / ranks < 2048)) ranks >>= 1;
+    const uint64_t steps = ((uint64_t)vocab + kLane<T> - 1 + kStep<T> - 1) / kStep<T>;      // (a row may start behind a 16-byte border)
+    return {ranks, (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeldSteps<T>};
+}
+
+// Splits of a row that the statistics are taken in; 0: the walk takes them itself.  Only the form that holds its share works with
+// them; beyond it the time goes up in a step: chains of 5 over 248320 logits, f32, 9 sequences 78 us and 10 (8 CTAs each) 92; bf16,
+// 18 sequences 92 us and 19 (4 CTAs each) 119.
 uint32_t stat_splits(const lq4_verify_args& a, int sm_count) {
-    const uint64_t rows = (uint64_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1), row = (uint64_t)a.vocab * (a.dtype == LQ4_DTYPE_F32 ? 4 : 2);
+    const bool f32 = a.dtype == LQ4_DTYPE_F32;
+    const uint64_t rows = (uint64_t)a.batch * a.nodes * (a.draft_logits ? 2 : 1), row = (uint64_t)a.vocab * (f32 ? 4 : 2);
     // (a division: rows * row may pass 64 bits where rows are broadcast)
     if (a.nodes < 2 || rows > kMaxStatRows || rows > (a.parents ? kTreeBytes : kChainBytes) / row) return 0;
+    if (!(f32 ? walk_shape<float>(a.batch, a.vocab, sm_count) : walk_shape<uint16_t>(a.batch, a.vocab, sm_count)).held) return 0;
     uint64_t splits = (4ull * sm_count + rows - 1) / rows;
     return splits > kMaxSplits ? kMaxSplits : splits < 1 ? 1 : (uint32_t)splits;
 }
@@ -805,12 +823,9 @@ uint32_t stat_splits(const lq4_verify_args& a, int sm_count) {
 template <typename T>
 cudaError_t run(VerifyParams p, int sm_count, int use_pdl, cudaStream_t s, int* launches) {
     const uint32_t batch = p.batch;
-    // as many CTAs per sequence as keep every SM at one CTA, and at least 2048 logits for each of them
-    uint32_t ranks = kMaxCluster;
-    while (ranks > 1 && ((uint64_t)batch * ranks > (uint64_t)sm_count || p.vocab / ranks < 2048)) ranks >>= 1;
-    const uint64_t steps = ((uint64_t)p.vocab + kLane<T> - 1 + kStep<T> - 1) / kStep<T>;      // (a row may start behind a 16-byte border)
-    const bool held = (steps + ranks * kVWarps - 1) / (ranks * kVWarps) <= kHeldSteps<T>;
-    if (!held) p.stats = nullptr;
+    const WalkShape shape = walk_shape<T>(batch, p.vocab, sm_count);
+    const uint32_t ranks = shape.ranks;
+    const bool held = shape.held;
     auto fn = held ? verify_kernel<T, true> : verify_kernel<T, false>;
     static DeviceOnce once_of[2];
     DeviceOnce& once = once_of[held];
